@@ -33,7 +33,8 @@ NATIVE = PKG / "_native"
 BUILD = NATIVE / "build"
 INCLUDE = PKG.parent / "include"
 
-KERNEL_MODULES = ("copy", "elementwise", "map", "imap", "fmap", "distance", "gather", "softmax", "quantize", "gemm")
+KERNEL_MODULES = ("copy", "elementwise", "map", "imap", "fmap", "distance", "gather", "softmax", "quantize", "gemm",
+                  "rmsnorm", "ffn", "xent", "clip")
 ARCH = "gfx950"
 
 # Packed fp32 VALU forms are kept out of every kernel.
@@ -114,7 +115,7 @@ def build_runtime() -> Path:
     _run([cxx, "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", *_defines(),
           "-D__HIP_PLATFORM_AMD__", "-I", str(rocm / "include"),
           "-I", str(INCLUDE), "-I", str(CSRC), f"-Wa,-I{BUILD}",
-          str(CSRC / "runtime.cpp"), str(CSRC / "blobs.S"), str(scratch),
+          str(CSRC / "runtime.cpp"), str(CSRC / "operators.cpp"), str(CSRC / "blobs.S"), str(scratch),
           "-o", str(out),
           f"-L{rocm / 'lib'}", f"-Wl,-rpath,{rocm / 'lib'}", "-lamdhip64"])
     return out

@@ -25,5 +25,9 @@ hcamd_blob_\name\()_end:
         hcamd_blob softmax
         hcamd_blob quantize
         hcamd_blob gemm
+        hcamd_blob rmsnorm
+        hcamd_blob ffn
+        hcamd_blob xent
+        hcamd_blob clip
 
         .section .note.GNU-stack, "", @progbits

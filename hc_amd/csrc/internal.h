@@ -17,6 +17,14 @@ HCAMD_HIDDEN void hcamdInternalReport(OlQueue q, const char *fmt, ...) noexcept
 // resolved when the device was created (a launch then loads nothing).
 HCAMD_HIDDEN int hcamdInternalColsKernelsReady(OlQueue q) noexcept;
 
+// runtime.cpp, for the launchers of operators.cpp: enqueues a built-in kernel on the
+// queue (with the queue's device current, restored afterwards; nothing throws), the
+// number of compute units of the queue's device, the selected variant of a family.
+HCAMD_HIDDEN int hcamdInternalLaunch(OlQueue q, const char *module, const char *kernel, size_t gridX, size_t gridY,
+                                     size_t gridZ, size_t threads, void **args) noexcept;
+HCAMD_HIDDEN int hcamdInternalComputeUnits(OlQueue q) noexcept;
+HCAMD_HIDDEN int hcamdInternalVariant(const char *family) noexcept;
+
 // scratch.hip: looks up the address of the library's static device scratch
 // array on `device`, which must be current; 0 on success, else the HIP error
 // name in `err`.  Called once per device by olCreateDevice.

@@ -1,0 +1,116 @@
+// Argument blocks of the language-model kernels, passed by value and shared by
+// the launchers (operators.cpp) and the kernels.  Pointers are device pointers,
+// leading dimensions are in elements.
+#pragma once
+#include <stddef.h>
+#include <stdint.h>
+
+namespace hcamd {
+
+// h = x + residual, y = h / rms(h) * weight (rmsnorm.hip)
+struct NormArgs {
+  const void *x, *residual, *weight; // residual, weight may be null
+  void *summed, *out;                // summed may be null
+  float *scale, *rstd;               // scale: 8-bit output only; rstd may be null
+  size_t ldx, ldr, lds, ldo;
+  uint32_t rows, cols;
+  float eps;
+  int weight_f32; // weight is fp32 (else the element type)
+};
+struct NormBackArgs {
+  const void *grad_out, *summed, *weight, *grad_summed; // weight, grad_summed may be null
+  const float *rstd;
+  void *grad_in, *grad_weight; // grad_weight may be null
+  float *partial;              // [bands][cols]
+  size_t ldg, ldh, ldgs, ldgi;
+  uint32_t rows, cols, band, bands; // rows to a band, bands
+  int weight_f32;
+};
+
+// One tiled product C[M,N] = sum_k A(m,k) B(n,k) (mma.h).  A second pair
+// continues the sum over k where `segments` is 2; a second B alone interleaves
+// its rows with the first's (the gated block).
+struct MmaArgs {
+  const void *a[2], *b[2];
+  size_t lda[2], ldb[2];
+  int M, N, K;
+  int segments;   // 1, or 2: k runs through (a[0], b[0]), then (a[1], b[1])
+  int splits;     // k tiles are dealt to this many workgroups (grid y)
+};
+
+struct GatedArgs {
+  MmaArgs mma; // a[0] = x [T,D], b = {gate, up} [F,D]; N = F
+  const float *x_scale, *gate_scale, *up_scale; // 8-bit operands only
+  void *out, *gate, *up;                        // gate, up may be null
+  size_t ldo, ldgate, ldup;
+  int activation;
+  int out_f16; // 8-bit operands: the output is fp16 (else bf16)
+};
+struct GatedBackArgs { // pre-activation gradients, element by element
+  const void *grad_out, *gate, *up;
+  void *dgate, *dup;
+  size_t ldg, ldgate, ldup, ldd;
+  uint32_t rows, cols;
+  int activation;
+};
+
+// a product whose result is stored: in the element type (`out`), or as fp32
+// partial sums (`partial`: [splits][M][ldp]) that a second kernel adds up
+struct StoreArgs {
+  MmaArgs mma;
+  void *out;
+  float *partial;
+  size_t ldo, ldp;
+  const float *undo; // when not null: *undo multiplies what goes to `out`
+  int accumulate;      // add to `partial` instead of replacing it
+};
+struct PairStoreArgs { // two products of one shape, selected by grid z
+  StoreArgs p[2];
+};
+struct FoldArgs { // out = sum over splits of partial (* *undo)
+  const float *partial;
+  void *out;
+  size_t ldp, ldo;
+  uint32_t rows, cols, splits;
+  const float *undo;
+};
+
+struct XentArgs {
+  MmaArgs mma; // a = x [T,D], b = weight rows of this piece; N = rows of the piece
+  const void *targets;
+  int target_i64;
+  int v0;            // first vocabulary row of the piece
+  int vocab;         // rows of the whole weight matrix
+  // forward: per row and column tile (max, sum of exp(z - max)), target logit
+  float *stats;      // [T][tiles][2]
+  float *zt;         // [T]
+  int tiles;
+  // backward
+  const float *lse, *grad_loss, *factor;
+  void *p;           // [T][ldp] (softmax - onehot) * grad_loss * *factor
+  size_t ldp;
+};
+struct XentRowsArgs {
+  const float *stats, *zt;
+  const void *targets;
+  int target_i64;
+  float *loss, *lse;
+  uint32_t rows, vocab, tiles;
+};
+
+// Clipping by the global norm (clip.hip): the tensors of one launch.
+constexpr int kClipTensors = 64;
+struct ClipArgs {
+  const void *in[kClipTensors];
+  void *out[kClipTensors];
+  uint64_t count[kClipTensors];
+  uint32_t first_chunk[kClipTensors + 1]; // chunks before this tensor
+  uint8_t type[kClipTensors];
+  uint32_t tensors;
+  double *partial;       // one cell per workgroup of every launch of the call
+  uint32_t first_cell, cells;
+  float max_norm;
+  float *norm;
+};
+
+} // namespace hcamd

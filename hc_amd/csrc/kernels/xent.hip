@@ -1,0 +1,194 @@
+// Softmax cross entropy of the product z = x W' against target columns, and its
+// gradients, without the logits ever being stored.  x [T,D], W [V,D].
+//
+// Forward: the product's tiles end in per-row statistics (maximum, sum of
+// exp(z - maximum)) and the target's logit; a second kernel joins the tiles of a
+// row: lse = log sum exp z, loss = lse - z[target].
+// Backward, vocabulary piece by piece: the product again with
+// p = (exp(z - lse) - onehot) * grad_loss as its epilogue, then
+//   dx += p W   (fp32 partial sums, folded once at the end)    dW = p' x
+// p is rounded to the element type because it is a matrix operand.
+//
+// A target below 0 takes its row out: loss 0, no gradient.  A target of V or more
+// is an error of the caller's: loss NaN, no gradient.
+#include "mma.h"
+
+using namespace hcamd;
+
+namespace {
+
+__device__ __forceinline__ int64_t target_of(const void *targets, int is64, size_t row) {
+  return is64 ? static_cast<const int64_t *>(targets)[row] : (int64_t)static_cast<const int32_t *>(targets)[row];
+}
+
+// per-row statistics of a tile: lanes l, l + 16, l + 32, l + 48 hold one row's
+// columns; WN waves share the row and meet in LDS
+template <int MI, int NI, int WN, int BM, int BN>
+__device__ __forceinline__ void tile_stats(const XentArgs &a, f32x4 (&acc)[MI][NI], int tile_m0, int wave_m, int tn,
+                                           int wave_n, int lane, float *lds) {
+  const int M = a.mma.M, N = a.mma.N;
+  const int wn = wave_n / (NI * 16);
+  float *slot_m = lds, *slot_s = lds + WN * BM; // [WN][BM] each
+  const int n0 = tn * BN + wave_n + lane / 16 * 4;
+#pragma unroll
+  for (int i = 0; i < MI; ++i) {
+    const int in_tile = wave_m + i * 16 + lane % 16, m = tile_m0 + in_tile;
+    float most = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < NI; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (n0 + j * 16 + e < N)
+          most = fmaxf(most, acc[i][j][e]);
+    most = fmaxf(most, __shfl_xor(most, 16));
+    most = fmaxf(most, __shfl_xor(most, 32));
+    // a row of -infinities: subtract 0, every term is then 0
+    const float from = most == -INFINITY ? 0.0f : most;
+    float sum = 0.0f;
+#pragma unroll
+    for (int j = 0; j < NI; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (n0 + j * 16 + e < N)
+          sum += __expf(acc[i][j][e] - from);
+    sum += __shfl_xor(sum, 16);
+    sum += __shfl_xor(sum, 32);
+    if (m < M) {
+      const int64_t at = target_of(a.targets, a.target_i64, m) - n0;
+#pragma unroll
+      for (int j = 0; j < NI; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (at == j * 16 + e && n0 + j * 16 + e < N)
+            a.zt[m] = acc[i][j][e];
+    }
+    if (lane < 16) {
+      slot_m[wn * BM + in_tile] = most;
+      slot_s[wn * BM + in_tile] = sum;
+    }
+  }
+  __syncthreads();
+  for (int r = threadIdx.x; r < BM; r += blockDim.x) {
+    const int m = tile_m0 + r;
+    if (m >= M)
+      continue;
+    float most = slot_m[r];
+#pragma unroll
+    for (int w = 1; w < WN; ++w)
+      most = fmaxf(most, slot_m[w * BM + r]);
+    const float from = most == -INFINITY ? 0.0f : most;
+    float sum = 0.0f;
+#pragma unroll
+    for (int w = 0; w < WN; ++w)
+      sum += slot_s[w * BM + r] * __expf(slot_m[w * BM + r] - from);
+    float *cell = a.stats + ((size_t)m * a.tiles + tn) * 2;
+    cell[0] = most;
+    cell[1] = sum;
+  }
+}
+
+template <class E> __device__ __forceinline__ void stats_general(const XentArgs &a) {
+  __shared__ __attribute__((aligned(1024))) unsigned char lds[4 * 128 * 128];
+  mma_general<E, kKFast, kKFast, false>(
+      a.mma, lds, [&](auto &acc, int m0, int wave_m, int tn, int wave_n, int lane, unsigned char *l) {
+        // (the main loop ends with a barrier: its stages are free)
+        tile_stats<4, 4, 2, 128, 128>(a, acc, m0, wave_m, tn, wave_n, lane, reinterpret_cast<float *>(l));
+      });
+}
+
+// p of a tile, from registers
+template <class E, int MI, int NI>
+__device__ __forceinline__ void tile_p(const XentArgs &a, f32x4 (&acc)[MI][NI], int m0, int n0, int lane) {
+  const int M = a.mma.M, N = a.mma.N;
+  const float factor = *a.factor;
+  const bool vec = can_store4<E>(a.p, a.ldp);
+#pragma unroll
+  for (int i = 0; i < MI; ++i) {
+    const int m = m0 + i * 16 + lane % 16;
+    if (m >= M)
+      continue;
+    const int64_t t = target_of(a.targets, a.target_i64, m);
+    const bool live = t >= 0 && t < a.vocab;
+    const float g = live ? a.grad_loss[m] * factor : 0.0f, lse = a.lse[m];
+#pragma unroll
+    for (int j = 0; j < NI; ++j) {
+      const int n = n0 + j * 16 + lane / 16 * 4;
+      f32x4 p;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float hot = t - a.v0 == n + e ? 1.0f : 0.0f;
+        // a row without a target: 0, whatever its logits are
+        p[e] = live ? (__expf(acc[i][j][e] - lse) - hot) * g : 0.0f;
+      }
+      store4<E>(static_cast<E *>(a.p) + (size_t)m * a.ldp, n, N, vec, p);
+    }
+  }
+}
+
+template <class E> __device__ __forceinline__ void p_general(const XentArgs &a) {
+  __shared__ __attribute__((aligned(1024))) unsigned char lds[4 * 128 * 128];
+  mma_general<E, kKFast, kKFast, false>(
+      a.mma, lds, [&](auto &acc, int m0, int wave_m, int tn, int wave_n, int lane, unsigned char *) {
+        tile_p<E, 4, 4>(a, acc, m0 + wave_m, tn * 128 + wave_n, lane);
+      });
+}
+
+// one wave per row joins the tiles' statistics
+__device__ __forceinline__ void rows_join(const XentRowsArgs &a) {
+  const int lane = threadIdx.x % kWave;
+  const size_t row = (size_t)blockIdx.x * (blockDim.x / kWave) + threadIdx.x / kWave;
+  if (row >= a.rows)
+    return;
+  const f32x2 *cells = reinterpret_cast<const f32x2 *>(a.stats) + row * a.tiles;
+  float most = -INFINITY;
+  for (uint32_t t = lane; t < a.tiles; t += kWave)
+    most = fmaxf(most, cells[t][0]);
+  most = wave_reduce<MaxOp>(most);
+  const float from = most == -INFINITY ? 0.0f : most;
+  float sum = 0.0f;
+  for (uint32_t t = lane; t < a.tiles; t += kWave)
+    sum += cells[t][1] * __expf(cells[t][0] - from);
+  sum = wave_reduce<SumOp>(sum);
+  if (lane == 0) {
+    const float lse = most + logf(sum);
+    const int64_t t = target_of(a.targets, a.target_i64, row);
+    a.lse[row] = lse;
+    a.loss[row] = t < 0 ? 0.0f : t >= a.vocab ? __builtin_nanf("") : lse - a.zt[row];
+  }
+}
+
+// What p is multiplied by before it is rounded, factor[0], and what undoes it in the
+// products, factor[1]: the largest |grad_loss| becomes 1 (bf16) or 2^15 (fp16).  With
+// the usual grad_loss, one value for every live row, the -1 at a target is then
+// represented exactly, where -grad_loss itself would carry one and the same rounding
+// error into every row's largest entry; and fp16 keeps the small p of a large
+// vocabulary above its subnormals.  One workgroup.
+__device__ __forceinline__ void p_factor(const float *grad_loss, uint32_t rows, float top, float *factor) {
+  __shared__ float slots[16];
+  float most = 0.0f;
+  for (uint32_t r = threadIdx.x; r < rows; r += blockDim.x)
+    most = fmaxf(most, fabsf(grad_loss[r]));
+  most = group_reduce<MaxOp, 16>(most, slots);
+  if (threadIdx.x == 0) {
+    const bool usable = most > 0x1p-100f && most < 0x1p100f;
+    factor[0] = usable ? top / most : 1.0f;
+    factor[1] = usable ? most / top : 1.0f;
+  }
+}
+
+} // namespace
+
+#define HCAMD_XENT(SUFFIX, E)                                                                             \
+  extern "C" __global__ __launch_bounds__(256) void hcamd_xent_stats_##SUFFIX##_general(XentArgs a) {     \
+    stats_general<E>(a);                                                                                  \
+  }                                                                                                       \
+  extern "C" __global__ __launch_bounds__(256) void hcamd_xent_p_##SUFFIX##_general(XentArgs a) {         \
+    p_general<E>(a);                                                                                      \
+  }
+HCAMD_XENT(bf16, __bf16)
+HCAMD_XENT(f16, _Float16)
+extern "C" __global__ __launch_bounds__(256) void hcamd_xent_rows(XentRowsArgs a) { rows_join(a); }
+extern "C" __global__ __launch_bounds__(1024) void hcamd_xent_factor(const float *grad_loss, uint32_t rows,
+                                                                      float top, float *factor) {
+  p_factor(grad_loss, rows, top, factor);
+}

@@ -1,0 +1,624 @@
+// Launchers of the language-model operators (rmsnorm.hip, ffn.hip, xent.hip,
+// clip.hip): checks of arguments, choice of kernel and geometry, workspaces.  The
+// entry points are documented in include/hc_amd_runtime.h.
+#include "hc_amd_runtime.h"
+#include "internal.h"
+#include "kernels/op_args.h"
+
+#include <algorithm>
+#include <cstdarg>
+#include <cstdio>
+#include <cstring>
+
+using namespace hcamd;
+
+namespace {
+
+constexpr size_t kMaxDim = 0x7fffff00; // sizes are held in 32 bits, tiles may run past an edge
+
+inline size_t ceilDiv(size_t a, size_t b) { return (a + b - 1) / b; }
+inline size_t alignUp(size_t a, size_t b) { return ceilDiv(a, b) * b; }
+inline size_t elemBytes(int type) { return type == HCAMD_F32 ? 4 : type == HCAMD_I8 ? 1 : 2; }
+inline const char *typeName(int type) {
+  return type == HCAMD_F32 ? "f32" : type == HCAMD_F16 ? "f16" : type == HCAMD_BF16 ? "bf16" : "i8";
+}
+inline bool half16(int type) { return type == HCAMD_F16 || type == HCAMD_BF16; }
+
+// One operand of a call: what the checks look at.
+struct Arg {
+  const char *name;
+  const void *p;
+  size_t ld, rows, cols, bytes; // bytes: of an element
+};
+
+struct Call {
+  OlQueue q;
+  const char *who;
+
+  int fail(const char *fmt, ...) const __attribute__((format(printf, 2, 3))) {
+    char text[200];
+    va_list ap;
+    va_start(ap, fmt);
+    std::vsnprintf(text, sizeof(text), fmt, ap);
+    va_end(ap);
+    hcamdInternalReport(q, "%s: %s", who, text);
+    return 1;
+  }
+  int check(const Arg &a) const {
+    if (!a.p)
+      return fail("%s is null", a.name);
+    if (reinterpret_cast<uintptr_t>(a.p) % a.bytes)
+      return fail("%s is not aligned to its elements", a.name);
+    if (a.rows > 1 && a.ld < a.cols)
+      return fail("%s: leading dimension smaller than a row", a.name);
+    if (a.ld > ((size_t)1 << 40) || (a.rows > 1 && a.ld > ((size_t)1 << 46) / a.rows))
+      return fail("%s: leading dimension out of range", a.name);
+    return 0;
+  }
+  int checkAll(std::initializer_list<Arg> all) const {
+    for (const Arg &a : all)
+      if (check(a))
+        return 1;
+    return 0;
+  }
+  int work(const void *work, size_t have, size_t need) const {
+    if (need == 0)
+      return 0;
+    if (!work || have < need)
+      return fail("workspace of %zu bytes, %zu needed", work ? have : 0, need);
+    if (reinterpret_cast<uintptr_t>(work) % 256)
+      return fail("the workspace is not aligned to 256 bytes");
+    return 0;
+  }
+  template <class T>
+  int launch(const char *module, const char *kernel, T &args, size_t x, size_t y = 1, size_t z = 1,
+             size_t threads = 256) const {
+    if (x > 0x7fffff || y > 65535 || z > 65535)
+      return fail("%zu x %zu x %zu workgroups", x, y, z);
+    void *ptrs[] = {&args};
+    return hcamdInternalLaunch(q, module, kernel, x, y, z, threads, ptrs);
+  }
+};
+
+// ---- tiled products -----------------------------------------------------------
+// How many workgroups share the k tiles of an output tile: as many as bring the
+// launch to about one workgroup per compute unit, each with at least 8 k tiles, and
+// no more than 64 MiB of fp32 partial sums.
+struct Product {
+  size_t tilesM, tilesN;
+  int splits;
+};
+size_t padCols(size_t n) { return alignUp(n, 8); }
+Product productOf(size_t m, size_t n, size_t k, int segments) {
+  Product p;
+  p.tilesM = ceilDiv(m, (size_t)128);
+  p.tilesN = ceilDiv(n, (size_t)128);
+  const size_t tiles = p.tilesM * p.tilesN, kTiles = ceilDiv(k, (size_t)64) * segments;
+  size_t s = std::min<size_t>(256 / std::max<size_t>(tiles, 1), kTiles / 8);
+  s = std::min(s, ((size_t)64 << 20) / std::max<size_t>(m * padCols(n) * 4, 1));
+  p.splits = (int)std::max<size_t>(s, 1);
+  return p;
+}
+size_t partialBytes(const Product &p, size_t m, size_t n) {
+  return p.splits > 1 ? alignUp((size_t)p.splits * m * padCols(n) * 4, 256) : 0;
+}
+
+int launchFold(const Call &c, int type, const FoldArgs &f) {
+  FoldArgs a = f;
+  char name[64];
+  std::snprintf(name, sizeof(name), "hcamd_fold_%s", typeName(type));
+  return c.launch("ffn", name, a, std::min<size_t>(ceilDiv((size_t)a.rows * a.cols, (size_t)256), 4096));
+}
+
+bool dimsOk(const Call &c, size_t a, size_t b, size_t d) {
+  if (a > kMaxDim || b > kMaxDim || d > kMaxDim) {
+    c.fail("a dimension exceeds 2^31 - 256");
+    return false;
+  }
+  return true;
+}
+
+} // namespace
+
+extern "C" {
+
+// ===========================================================================
+// add + RMS norm
+// ===========================================================================
+int hcamdLaunchAddRmsNorm(OlQueue q, int elemType, const void *x, size_t ldx, const void *residual, size_t ldr,
+                          const void *weight, int weightType, float eps, void *summed, size_t lds, void *out,
+                          int outType, size_t ldo, float *scale, float *rstd, size_t rows, size_t cols) noexcept {
+  const Call c{q, "hcamdLaunchAddRmsNorm"};
+  if (!q)
+    return 1;
+  if (elemType != HCAMD_F32 && !half16(elemType))
+    return c.fail("element type %d (fp32, fp16, bf16)", elemType);
+  if (outType != elemType && outType != HCAMD_I8)
+    return c.fail("output type %d (the element type, or int8)", outType);
+  if (weight && weightType != HCAMD_F32 && weightType != elemType)
+    return c.fail("weight type %d (fp32, or the element type)", weightType);
+  if (!(eps >= 0.0f))
+    return c.fail("eps must not be negative");
+  if (!dimsOk(c, rows, cols, 0))
+    return 1;
+  if (rows == 0)
+    return 0;
+  if (cols == 0)
+    return c.fail("rows without elements");
+  const size_t e = elemBytes(elemType);
+  if (c.checkAll({{"x", x, ldx, rows, cols, e}, {"out", out, ldo, rows, cols, elemBytes(outType)}}) ||
+      (residual && c.check({"residual", residual, ldr, rows, cols, e})) ||
+      (weight && c.check({"weight", weight, cols, 1, cols, elemBytes(weightType)})) ||
+      (summed && c.check({"summed", summed, lds, rows, cols, e})) ||
+      (rstd && c.check({"rstd", rstd, rows, 1, rows, 4})))
+    return 1;
+  if (outType == HCAMD_I8 ? c.check({"scale", scale, rows, 1, rows, 4}) : scale != nullptr)
+    return outType == HCAMD_I8 ? 1 : c.fail("a scale needs an int8 output");
+  NormArgs a{};
+  a.x = x, a.residual = residual, a.weight = weight, a.summed = summed, a.out = out, a.scale = scale, a.rstd = rstd;
+  a.ldx = ldx, a.ldr = ldr, a.lds = lds, a.ldo = ldo;
+  a.rows = (uint32_t)rows, a.cols = (uint32_t)cols, a.eps = eps;
+  a.weight_f32 = !weight || weightType == HCAMD_F32;
+  char name[64];
+  std::snprintf(name, sizeof(name), "hcamd_rmsnorm_%s%s_general", typeName(elemType), outType == HCAMD_I8 ? "_i8" : "");
+  return c.launch("rmsnorm", name, a, std::min<size_t>(rows, 0x7fffff));
+}
+
+namespace {
+void normBands(size_t rows, size_t &bands, size_t &band) {
+  bands = std::min<size_t>(256, ceilDiv(rows, 16));
+  band = ceilDiv(rows, std::max<size_t>(bands, 1));
+  bands = ceilDiv(rows, std::max<size_t>(band, 1));
+}
+} // namespace
+
+size_t hcamdAddRmsNormBackwardWorkspace(size_t rows, size_t cols) noexcept {
+  if (rows == 0 || rows > kMaxDim || cols > kMaxDim)
+    return 0;
+  size_t bands, band;
+  normBands(rows, bands, band);
+  return bands * cols * 4;
+}
+
+int hcamdLaunchAddRmsNormBackward(OlQueue q, int elemType, const void *gradOut, size_t ldg, const void *summed,
+                                  size_t lds, const void *weight, int weightType, const float *rstd,
+                                  const void *gradSummed, size_t ldgs, void *gradIn, size_t ldgi, void *gradWeight,
+                                  size_t rows, size_t cols, void *work, size_t workBytes) noexcept {
+  const Call c{q, "hcamdLaunchAddRmsNormBackward"};
+  if (!q)
+    return 1;
+  if (elemType != HCAMD_F32 && !half16(elemType))
+    return c.fail("element type %d (fp32, fp16, bf16)", elemType);
+  if (weightType != HCAMD_F32 && weightType != elemType)
+    return c.fail("weight type %d (fp32, or the element type)", weightType);
+  if (!dimsOk(c, rows, cols, 0))
+    return 1;
+  if (cols == 0)
+    return rows == 0 ? 0 : c.fail("rows without elements");
+  const size_t e = elemBytes(elemType), we = elemBytes(weightType);
+  if (gradWeight && c.check({"grad_weight", gradWeight, cols, 1, cols, we}))
+    return 1;
+  if (rows && (c.checkAll({{"grad_out", gradOut, ldg, rows, cols, e},
+                           {"summed", summed, lds, rows, cols, e},
+                           {"rstd", rstd, rows, 1, rows, 4},
+                           {"grad_in", gradIn, ldgi, rows, cols, e}}) ||
+               (gradSummed && c.check({"grad_summed", gradSummed, ldgs, rows, cols, e})) ||
+               (weight && c.check({"weight", weight, cols, 1, cols, we}))))
+    return 1;
+  NormBackArgs a{};
+  a.grad_out = gradOut, a.summed = summed, a.weight = weight, a.grad_summed = gradSummed, a.rstd = rstd;
+  a.grad_in = gradIn, a.grad_weight = gradWeight, a.partial = static_cast<float *>(work);
+  a.ldg = ldg, a.ldh = lds, a.ldgs = ldgs, a.ldgi = ldgi;
+  a.rows = (uint32_t)rows, a.cols = (uint32_t)cols, a.weight_f32 = weightType == HCAMD_F32;
+  size_t bands = 0, band = 0;
+  normBands(rows, bands, band);
+  a.band = (uint32_t)band, a.bands = (uint32_t)bands;
+  char name[64];
+  // the weight's gradient first: grad_in may be grad_out
+  if (gradWeight) {
+    if (c.work(work, workBytes, hcamdAddRmsNormBackwardWorkspace(rows, cols)))
+      return 1;
+    if (rows) {
+      std::snprintf(name, sizeof(name), "hcamd_rmsnorm_back_weight_%s_general", typeName(elemType));
+      if (c.launch("rmsnorm", name, a, ceilDiv(cols, 256), bands))
+        return 1;
+    }
+    std::snprintf(name, sizeof(name), "hcamd_rmsnorm_fold_%s", typeName(weightType));
+    if (c.launch("rmsnorm", name, a, ceilDiv(cols, 256)))
+      return 1;
+  }
+  if (rows == 0)
+    return 0;
+  std::snprintf(name, sizeof(name), "hcamd_rmsnorm_back_%s_general", typeName(elemType));
+  return c.launch("rmsnorm", name, a, std::min<size_t>(rows, 0x7fffff));
+}
+
+// ===========================================================================
+// gated feed-forward block
+// ===========================================================================
+int hcamdLaunchGatedFfn(OlQueue q, int elemType, const void *x, size_t ldx, const float *xScale, const void *wGate,
+                        size_t ldwg, const float *gateScale, const void *wUp, size_t ldwu, const float *upScale,
+                        int activation, void *out, int outType, size_t ldo, void *gate, size_t ldgate, void *up,
+                        size_t ldup, size_t tokens, size_t d, size_t f) noexcept {
+  const Call c{q, "hcamdLaunchGatedFfn"};
+  if (!q)
+    return 1;
+  const bool i8 = elemType == HCAMD_I8;
+  if (!i8 && !half16(elemType))
+    return c.fail("element type %d (fp16, bf16, int8)", elemType);
+  if (i8 ? !half16(outType) : outType != elemType)
+    return c.fail("output type %d (the element type; fp16 or bf16 for int8)", outType);
+  if (activation != HCAMD_SILU && activation != HCAMD_GELU)
+    return c.fail("activation %d", activation);
+  if (!dimsOk(c, tokens, d, f))
+    return 1;
+  if (tokens == 0 || f == 0)
+    return 0;
+  if (d == 0)
+    return c.fail("the inner dimension must be at least 1");
+  if (i8 && d > 131072)
+    return c.fail("an inner dimension of %zu (int8 sums are exact up to 131072)", d);
+  const size_t e = elemBytes(elemType), oe = elemBytes(outType);
+  if (c.checkAll({{"x", x, ldx, tokens, d, e}, {"w_gate", wGate, ldwg, f, d, e}, {"w_up", wUp, ldwu, f, d, e},
+                  {"out", out, ldo, tokens, f, oe}}))
+    return 1;
+  if (i8) {
+    if (gate || up)
+      return c.fail("the pre-activations of an int8 product are not kept");
+    if (c.checkAll({{"x_scale", xScale, tokens, 1, tokens, 4}, {"gate_scale", gateScale, f, 1, f, 4},
+                    {"up_scale", upScale, f, 1, f, 4}}))
+      return 1;
+  } else {
+    if (xScale || gateScale || upScale)
+      return c.fail("scales belong to int8 operands");
+    if ((gate && c.check({"gate", gate, ldgate, tokens, f, oe})) || (up && c.check({"up", up, ldup, tokens, f, oe})))
+      return 1;
+  }
+  GatedArgs a{};
+  a.mma.a[0] = x, a.mma.lda[0] = ldx;
+  a.mma.b[0] = wGate, a.mma.ldb[0] = ldwg, a.mma.b[1] = wUp, a.mma.ldb[1] = ldwu;
+  a.mma.M = (int)tokens, a.mma.N = (int)f, a.mma.K = (int)d, a.mma.segments = 1, a.mma.splits = 1;
+  a.x_scale = xScale, a.gate_scale = gateScale, a.up_scale = upScale;
+  a.out = out, a.gate = gate, a.up = up, a.ldo = ldo, a.ldgate = ldgate, a.ldup = ldup;
+  a.activation = activation, a.out_f16 = outType == HCAMD_F16;
+  char name[64];
+  std::snprintf(name, sizeof(name), "hcamd_gated_%s_general", typeName(elemType));
+  return c.launch("ffn", name, a, ceilDiv(tokens, 128) * ceilDiv(f, 64));
+}
+
+namespace {
+// the workspace of the backward pass: dg, du, then the partial sums of dx, then of
+// the two weight gradients
+struct FfnBack {
+  size_t ldd, dg, dx, dw, bytes;
+  Product px, pw;
+};
+FfnBack ffnBack(size_t tokens, size_t d, size_t f) {
+  FfnBack b;
+  b.ldd = padCols(f);
+  b.dg = alignUp(tokens * b.ldd * 2, 256);
+  b.px = productOf(tokens, d, f, 2);
+  b.pw = productOf(f, d, tokens, 1);
+  b.dx = partialBytes(b.px, tokens, d);
+  b.dw = partialBytes(b.pw, f, d);
+  b.bytes = 2 * b.dg + b.dx + 2 * b.dw;
+  return b;
+}
+} // namespace
+
+size_t hcamdGatedFfnBackwardWorkspace(size_t tokens, size_t d, size_t f) noexcept {
+  if (tokens == 0 || d == 0 || f == 0 || tokens > kMaxDim || d > kMaxDim || f > kMaxDim)
+    return 0;
+  return ffnBack(tokens, d, f).bytes;
+}
+
+int hcamdLaunchGatedFfnBackward(OlQueue q, int elemType, const void *gradOut, size_t ldg, const void *x, size_t ldx,
+                                const void *wGate, size_t ldwg, const void *wUp, size_t ldwu, const void *gate,
+                                size_t ldgate, const void *up, size_t ldup, int activation, void *gradX, size_t ldgx,
+                                void *gradWGate, size_t ldgwg, void *gradWUp, size_t ldgwu, size_t tokens, size_t d,
+                                size_t f, void *work, size_t workBytes) noexcept {
+  const Call c{q, "hcamdLaunchGatedFfnBackward"};
+  if (!q)
+    return 1;
+  if (!half16(elemType))
+    return c.fail("element type %d (fp16, bf16)", elemType);
+  if (activation != HCAMD_SILU && activation != HCAMD_GELU)
+    return c.fail("activation %d", activation);
+  if (!dimsOk(c, tokens, d, f))
+    return 1;
+  if (d == 0 || f == 0)
+    return c.fail("an empty dimension (%zu, %zu)", d, f);
+  if (tokens == 0)
+    gradX = nullptr; // no rows; the weights' gradients are zeros
+  if (tokens && c.checkAll({{"grad_out", gradOut, ldg, tokens, f, 2}, {"gate", gate, ldgate, tokens, f, 2},
+                            {"up", up, ldup, tokens, f, 2}}))
+    return 1;
+  if (gradX && c.checkAll({{"w_gate", wGate, ldwg, f, d, 2}, {"w_up", wUp, ldwu, f, d, 2},
+                           {"grad_x", gradX, ldgx, tokens, d, 2}}))
+    return 1;
+  if (tokens && (gradWGate || gradWUp) && c.check({"x", x, ldx, tokens, d, 2}))
+    return 1;
+  if ((gradWGate && c.check({"grad_w_gate", gradWGate, ldgwg, f, d, 2})) ||
+      (gradWUp && c.check({"grad_w_up", gradWUp, ldgwu, f, d, 2})))
+    return 1;
+  const FfnBack b = ffnBack(tokens, d, f);
+  if (tokens && c.work(work, workBytes, b.bytes))
+    return 1;
+  if (!gradX && !gradWGate && !gradWUp)
+    return 0;
+  char *w = static_cast<char *>(work);
+  char name[64];
+  GatedBackArgs e{};
+  e.grad_out = gradOut, e.gate = gate, e.up = up, e.dgate = w, e.dup = w + b.dg;
+  e.ldg = ldg, e.ldgate = ldgate, e.ldup = ldup, e.ldd = b.ldd;
+  e.rows = (uint32_t)tokens, e.cols = (uint32_t)f, e.activation = activation;
+  std::snprintf(name, sizeof(name), "hcamd_gated_back_%s", typeName(elemType));
+  if (tokens && c.launch("ffn", name, e, std::min<size_t>(ceilDiv(tokens * ceilDiv(f, 8), 256), 8192)))
+    return 1;
+  if (gradX) {
+    StoreArgs s{};
+    s.mma.a[0] = e.dgate, s.mma.a[1] = e.dup, s.mma.lda[0] = s.mma.lda[1] = b.ldd;
+    s.mma.b[0] = wGate, s.mma.b[1] = wUp, s.mma.ldb[0] = ldwg, s.mma.ldb[1] = ldwu;
+    s.mma.M = (int)tokens, s.mma.N = (int)d, s.mma.K = (int)f, s.mma.segments = 2, s.mma.splits = b.px.splits;
+    s.out = gradX, s.ldo = ldgx, s.ldp = padCols(d);
+    s.partial = b.dx ? reinterpret_cast<float *>(w + 2 * b.dg) : nullptr;
+    std::snprintf(name, sizeof(name), "hcamd_product_nn_%s_general", typeName(elemType));
+    if (c.launch("ffn", name, s, b.px.tilesM * b.px.tilesN, b.px.splits))
+      return 1;
+    if (s.partial && launchFold(c, elemType, {s.partial, gradX, s.ldp, ldgx, (uint32_t)tokens, (uint32_t)d,
+                                              (uint32_t)b.px.splits, nullptr}))
+      return 1;
+  }
+  if (gradWGate || gradWUp) {
+    PairStoreArgs s{};
+    size_t n = 0;
+    for (int k = 0; k < 2; ++k) {
+      void *to = k ? gradWUp : gradWGate;
+      if (!to)
+        continue;
+      StoreArgs &t = s.p[n];
+      t.mma.a[0] = k ? e.dup : e.dgate, t.mma.lda[0] = b.ldd;
+      t.mma.b[0] = x, t.mma.ldb[0] = ldx;
+      t.mma.M = (int)f, t.mma.N = (int)d, t.mma.K = (int)tokens, t.mma.segments = 1, t.mma.splits = b.pw.splits;
+      t.out = to, t.ldo = k ? ldgwu : ldgwg, t.ldp = padCols(d);
+      t.partial = b.dw ? reinterpret_cast<float *>(w + 2 * b.dg + b.dx + n * b.dw) : nullptr;
+      ++n;
+    }
+    std::snprintf(name, sizeof(name), "hcamd_product_tn_%s_general", typeName(elemType));
+    if (c.launch("ffn", name, s, b.pw.tilesM * b.pw.tilesN, b.pw.splits, n))
+      return 1;
+    for (size_t k = 0; b.dw && k < n; ++k)
+      if (launchFold(c, elemType, {s.p[k].partial, s.p[k].out, s.p[k].ldp, s.p[k].ldo, (uint32_t)f, (uint32_t)d,
+                                   (uint32_t)b.pw.splits, nullptr}))
+        return 1;
+  }
+  return 0;
+}
+
+// ===========================================================================
+// linear cross entropy
+// ===========================================================================
+namespace {
+constexpr int kStatsCols = 128; // columns of a statistics tile
+int xentCommon(const Call &c, int elemType, const void *x, size_t ldx, const void *weight, size_t ldw,
+               const void *targets, int targetType, size_t tokens, size_t d, size_t vocab) {
+  if (!half16(elemType))
+    return c.fail("element type %d (fp16, bf16)", elemType);
+  if (targetType != HCAMD_I32 && targetType != HCAMD_I64)
+    return c.fail("target type %d (int32, int64)", targetType);
+  if (!dimsOk(c, tokens, d, vocab))
+    return 1;
+  if (d == 0 || vocab == 0)
+    return c.fail("an empty dimension (%zu, vocabulary of %zu)", d, vocab);
+  return tokens && c.checkAll({{"x", x, ldx, tokens, d, 2}, {"weight", weight, ldw, vocab, d, 2},
+                               {"targets", targets, tokens, 1, tokens, targetType == HCAMD_I64 ? 8u : 4u}});
+}
+} // namespace
+
+size_t hcamdLinearCrossEntropyWorkspace(size_t tokens, size_t vocab) noexcept {
+  if (tokens > kMaxDim || vocab > kMaxDim)
+    return 0;
+  return tokens * ceilDiv(vocab, kStatsCols) * 8 + tokens * 4;
+}
+
+int hcamdLaunchLinearCrossEntropy(OlQueue q, int elemType, const void *x, size_t ldx, const void *weight, size_t ldw,
+                                  const void *targets, int targetType, float *loss, float *lse, size_t tokens,
+                                  size_t d, size_t vocab, void *work, size_t workBytes) noexcept {
+  const Call c{q, "hcamdLaunchLinearCrossEntropy"};
+  if (!q || xentCommon(c, elemType, x, ldx, weight, ldw, targets, targetType, tokens, d, vocab))
+    return 1;
+  if (tokens == 0)
+    return 0;
+  if (c.checkAll({{"loss", loss, tokens, 1, tokens, 4}, {"lse", lse, tokens, 1, tokens, 4}}) ||
+      c.work(work, workBytes, hcamdLinearCrossEntropyWorkspace(tokens, vocab)))
+    return 1;
+  XentArgs a{};
+  a.mma.a[0] = x, a.mma.lda[0] = ldx, a.mma.b[0] = weight, a.mma.ldb[0] = ldw;
+  a.mma.M = (int)tokens, a.mma.N = (int)vocab, a.mma.K = (int)d, a.mma.segments = a.mma.splits = 1;
+  a.targets = targets, a.target_i64 = targetType == HCAMD_I64, a.vocab = (int)vocab;
+  a.tiles = (int)ceilDiv(vocab, kStatsCols);
+  a.stats = static_cast<float *>(work);
+  a.zt = a.stats + tokens * a.tiles * 2;
+  char name[64];
+  std::snprintf(name, sizeof(name), "hcamd_xent_stats_%s_general", typeName(elemType));
+  if (c.launch("xent", name, a, ceilDiv(tokens, 128) * a.tiles))
+    return 1;
+  XentRowsArgs r{a.stats, a.zt, targets, a.target_i64, loss, lse, (uint32_t)tokens, (uint32_t)vocab,
+                 (uint32_t)a.tiles};
+  return c.launch("xent", "hcamd_xent_rows", r, ceilDiv(tokens, 4));
+}
+
+namespace {
+// the workspace of the backward pass: the factor, p of a piece, the partial sums of dx,
+// the partial sums of a piece's dW
+struct XentBack {
+  size_t piece, ldp, p, dx, dw, bytes;
+  Product px, pw;
+};
+XentBack xentBack(size_t tokens, size_t d, size_t vocab, size_t piece) {
+  XentBack b;
+  // by default a piece holds 64 Mi elements of p (128 MiB): what the two products of
+  // the piece read again then mostly stays in the 256 MiB memory-side cache, and a
+  // piece is work enough to fill the card
+  if (piece == 0)
+    piece = std::max<size_t>(alignUp(((size_t)64 << 20) / std::max<size_t>(tokens, 1), 256), 1024);
+  b.piece = std::min(alignUp(piece, 8), vocab);
+  b.ldp = padCols(b.piece);
+  b.p = alignUp(tokens * b.ldp * 2, 256);
+  b.px = productOf(tokens, d, b.piece, 1);
+  b.pw = productOf(b.piece, d, tokens, 1);
+  b.dx = alignUp((size_t)b.px.splits * tokens * padCols(d) * 4, 256);
+  b.dw = partialBytes(b.pw, b.piece, d);
+  b.bytes = 256 + b.p + b.dx + b.dw;
+  return b;
+}
+} // namespace
+
+size_t hcamdLinearCrossEntropyBackwardWorkspace(size_t tokens, size_t d, size_t vocab, size_t piece) noexcept {
+  if (tokens == 0 || d == 0 || vocab == 0 || tokens > kMaxDim || d > kMaxDim || vocab > kMaxDim || piece > kMaxDim)
+    return 0;
+  return xentBack(tokens, d, vocab, piece).bytes;
+}
+
+int hcamdLaunchLinearCrossEntropyBackward(OlQueue q, int elemType, const void *x, size_t ldx, const void *weight,
+                                          size_t ldw, const void *targets, int targetType, const float *lse,
+                                          const float *gradLoss, void *gradX, size_t ldgx, void *gradWeight,
+                                          size_t ldgw, size_t tokens, size_t d, size_t vocab, size_t piece,
+                                          void *work, size_t workBytes) noexcept {
+  const Call c{q, "hcamdLaunchLinearCrossEntropyBackward"};
+  if (!q || xentCommon(c, elemType, x, ldx, weight, ldw, targets, targetType, tokens, d, vocab))
+    return 1;
+  if (piece > kMaxDim)
+    return c.fail("a piece of %zu rows", piece);
+  if (tokens == 0)
+    gradX = nullptr; // no rows; the weight's gradient is zero
+  if ((tokens && c.checkAll({{"lse", lse, tokens, 1, tokens, 4}, {"grad_loss", gradLoss, tokens, 1, tokens, 4}})) ||
+      (gradX && c.check({"grad_x", gradX, ldgx, tokens, d, 2})) ||
+      (gradWeight && c.check({"grad_weight", gradWeight, ldgw, vocab, d, 2})))
+    return 1;
+  const XentBack b = xentBack(tokens, d, vocab, piece);
+  if (tokens && c.work(work, workBytes, b.bytes))
+    return 1;
+  if (!gradX && !gradWeight)
+    return 0;
+  char *w = static_cast<char *>(work);
+  char name[64];
+  float *factor = reinterpret_cast<float *>(w);
+  if (tokens) {
+    uint32_t rows = (uint32_t)tokens;
+    float top = elemType == HCAMD_F16 ? 0x1p15f : 1.0f;
+    void *args[] = {&gradLoss, &rows, &top, &factor};
+    if (hcamdInternalLaunch(q, "xent", "hcamd_xent_factor", 1, 1, 1, 1024, args))
+      return 1;
+  }
+  const float *undo = tokens ? factor + 1 : nullptr;
+  float *dx = reinterpret_cast<float *>(w + 256 + b.p);
+  for (size_t v0 = 0; v0 < vocab; v0 += b.piece) {
+    const size_t n = std::min(b.piece, vocab - v0);
+    const char *rows = static_cast<const char *>(weight) + v0 * ldw * 2;
+    XentArgs a{};
+    a.mma.a[0] = x, a.mma.lda[0] = ldx, a.mma.b[0] = rows, a.mma.ldb[0] = ldw;
+    a.mma.M = (int)tokens, a.mma.N = (int)n, a.mma.K = (int)d, a.mma.segments = a.mma.splits = 1;
+    a.targets = targets, a.target_i64 = targetType == HCAMD_I64, a.v0 = (int)v0, a.vocab = (int)vocab;
+    a.lse = lse, a.grad_loss = gradLoss, a.factor = factor, a.p = w + 256, a.ldp = b.ldp;
+    std::snprintf(name, sizeof(name), "hcamd_xent_p_%s_general", typeName(elemType));
+    if (tokens && c.launch("xent", name, a, ceilDiv(tokens, 128) * ceilDiv(n, 128)))
+      return 1;
+    if (gradX) {
+      StoreArgs s{};
+      s.mma.a[0] = a.p, s.mma.lda[0] = b.ldp, s.mma.b[0] = rows, s.mma.ldb[0] = ldw;
+      s.mma.M = (int)tokens, s.mma.N = (int)d, s.mma.K = (int)n, s.mma.segments = 1, s.mma.splits = b.px.splits;
+      s.partial = dx, s.ldp = padCols(d), s.accumulate = v0 != 0;
+      std::snprintf(name, sizeof(name), "hcamd_product_nn_%s_general", typeName(elemType));
+      if (c.launch("ffn", name, s, b.px.tilesM * b.px.tilesN, b.px.splits))
+        return 1;
+    }
+    if (gradWeight) {
+      PairStoreArgs s{};
+      StoreArgs &t = s.p[0];
+      t.mma.a[0] = a.p, t.mma.lda[0] = b.ldp, t.mma.b[0] = x, t.mma.ldb[0] = ldx;
+      t.mma.M = (int)n, t.mma.N = (int)d, t.mma.K = (int)tokens, t.mma.segments = 1, t.mma.splits = b.pw.splits;
+      t.out = static_cast<char *>(gradWeight) + v0 * ldgw * 2, t.ldo = ldgw, t.undo = undo;
+      t.partial = b.dw ? reinterpret_cast<float *>(w + 256 + b.p + b.dx) : nullptr, t.ldp = padCols(d);
+      std::snprintf(name, sizeof(name), "hcamd_product_tn_%s_general", typeName(elemType));
+      if (c.launch("ffn", name, s, ceilDiv(n, 128) * b.pw.tilesN, b.pw.splits))
+        return 1;
+      if (b.dw && launchFold(c, elemType, {t.partial, t.out, t.ldp, ldgw, (uint32_t)n, (uint32_t)d,
+                                           (uint32_t)b.pw.splits, undo}))
+        return 1;
+    }
+  }
+  if (gradX)
+    return launchFold(c, elemType, {dx, gradX, padCols(d), ldgx, (uint32_t)tokens, (uint32_t)d,
+                                    (uint32_t)b.px.splits, undo});
+  return 0;
+}
+
+// ===========================================================================
+// clipping by the global norm
+// ===========================================================================
+namespace {
+constexpr size_t kClipChunk = 16384, kClipCells = 1024;
+// workgroups of the launch that takes `chunks` of `all` chunks
+size_t clipGroups(size_t chunks, size_t all) {
+  return std::max<size_t>(1, std::min(chunks, all <= kClipCells ? chunks : chunks * kClipCells / all));
+}
+} // namespace
+
+size_t hcamdClipGradNormWorkspace(size_t tensors) noexcept { return (kClipCells + ceilDiv(tensors, kClipTensors)) * 8; }
+
+int hcamdLaunchClipGradNorm(OlQueue q, const HcamdClipTensor *tensors, size_t count, float maxNorm, float *norm,
+                            void *work, size_t workBytes) noexcept {
+  const Call c{q, "hcamdLaunchClipGradNorm"};
+  if (!q)
+    return 1;
+  if (!(maxNorm >= 0.0f))
+    return c.fail("the largest norm must not be negative");
+  if ((count && !tensors) || count > 0x7fffffff)
+    return c.fail("tensors is null, or too many");
+  if (c.check({"norm", norm, 1, 1, 1, 4}) || c.work(work, workBytes, hcamdClipGradNormWorkspace(count)))
+    return 1;
+  size_t all = 0;
+  for (size_t i = 0; i < count; ++i) {
+    const HcamdClipTensor &t = tensors[i];
+    if (t.type != HCAMD_F32 && !half16(t.type))
+      return c.fail("tensor %zu: type %d (fp32, fp16, bf16)", i, t.type);
+    if (t.count > ((size_t)1 << 40))
+      return c.fail("tensor %zu: too many elements", i);
+    if (t.count && (c.check({"a tensor", t.in, t.count, 1, t.count, elemBytes(t.type)}) ||
+                    c.check({"a clipped tensor", t.out, t.count, 1, t.count, elemBytes(t.type)})))
+      return 1;
+    all += ceilDiv(t.count, kClipChunk);
+  }
+  if (all > 0x7fffffff)
+    return c.fail("too many elements");
+  const size_t launches = std::max<size_t>(1, ceilDiv(count, (size_t)kClipTensors));
+  size_t cells = 0;
+  for (int pass = 0; pass < 2; ++pass) {
+    size_t cell = 0;
+    for (size_t l = 0; l < launches; ++l) {
+      ClipArgs a{};
+      const size_t first = l * kClipTensors, n = std::min<size_t>(kClipTensors, count - std::min(count, first));
+      size_t chunks = 0;
+      for (size_t i = 0; i < n; ++i) {
+        const HcamdClipTensor &t = tensors[first + i];
+        a.in[i] = t.in, a.out[i] = t.out, a.count[i] = t.count, a.type[i] = (uint8_t)t.type;
+        a.first_chunk[i] = (uint32_t)chunks;
+        chunks += ceilDiv(t.count, kClipChunk);
+      }
+      a.first_chunk[n] = (uint32_t)chunks;
+      a.tensors = (uint32_t)n;
+      a.partial = static_cast<double *>(work), a.first_cell = (uint32_t)cell;
+      a.max_norm = maxNorm, a.norm = norm, a.cells = (uint32_t)cells;
+      const size_t groups = clipGroups(chunks, all);
+      if (pass == 0 ? c.launch("clip", "hcamd_clip_sums", a, groups)
+                    : c.launch("clip", "hcamd_clip_scale", a, std::max<size_t>(1, std::min<size_t>(chunks, 4096))))
+        return 1;
+      cell += groups;
+    }
+    cells = cell;
+  }
+  return 0;
+}
+
+} // extern "C"

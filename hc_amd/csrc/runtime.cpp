@@ -153,6 +153,10 @@ HCAMD_BLOB(gather)
 HCAMD_BLOB(softmax)
 HCAMD_BLOB(quantize)
 HCAMD_BLOB(gemm)
+HCAMD_BLOB(rmsnorm)
+HCAMD_BLOB(ffn)
+HCAMD_BLOB(xent)
+HCAMD_BLOB(clip)
 #undef HCAMD_BLOB
 
 struct Blob {
@@ -164,7 +168,8 @@ struct Blob {
 const Blob kBlobs[] = {HCAMD_BLOB(copy), HCAMD_BLOB(elementwise),
                        HCAMD_BLOB(map), HCAMD_BLOB(imap), HCAMD_BLOB(fmap), HCAMD_BLOB(distance),
                        HCAMD_BLOB(gather), HCAMD_BLOB(softmax),
-                       HCAMD_BLOB(quantize), HCAMD_BLOB(gemm)};
+                       HCAMD_BLOB(quantize), HCAMD_BLOB(gemm), HCAMD_BLOB(rmsnorm),
+                       HCAMD_BLOB(ffn), HCAMD_BLOB(xent), HCAMD_BLOB(clip)};
 #undef HCAMD_BLOB
 constexpr size_t kNumBlobs = sizeof(kBlobs) / sizeof(kBlobs[0]);
 
@@ -273,7 +278,8 @@ std::unordered_map<std::string, int> &variants() {
   static std::unordered_map<std::string, int> v{
       {"add", 0},     {"fma", 0},  {"softmax", 0},
       {"quantize", 0}, {"gemm", 0}, {"copy", 0}, {"map", 0},
-      {"gather", 0}, {"gather_fuse", 0}, {"rows", 0}, {"stream", 0}, {"cols", 0}, {"norm", 0}};
+      {"gather", 0}, {"gather_fuse", 0}, {"rows", 0}, {"stream", 0}, {"cols", 0}, {"norm", 0},
+      {"rmsnorm", 0}, {"mma", 0}};
   return v;
 }
 std::mutex g_variantLock; // guards variants()
@@ -612,6 +618,41 @@ void hcamdInternalReport(OlQueue q, const char *fmt, ...) noexcept {
 
 int hcamdInternalColsKernelsReady(OlQueue q) noexcept {
   return q && static_cast<Queue *>(q)->device->colsKernelsReady ? 1 : 0;
+}
+
+int hcamdInternalLaunch(OlQueue q, const char *module, const char *kernel, size_t gridX, size_t gridY, size_t gridZ,
+                        size_t threads, void **args) noexcept {
+  auto *queue = static_cast<Queue *>(q);
+  if (!queue)
+    return 1;
+  Device *dev = queue->device;
+  int current = dev->index;
+  (void)hipGetDevice(&current);
+  int rc = 1;
+  try {
+    if (current == dev->index || !dev->makeCurrent()) {
+      Kernel *k = builtinKernel(dev, module, kernel);
+      const size_t grid[3] = {gridX, gridY, gridZ}, block[3] = {threads, 1, 1};
+      rc = k ? launch(queue, k, grid, block, args, 0) : 1;
+    }
+  } catch (...) {
+    dev->report("%s: out of host memory", kernel);
+  }
+  if (current != dev->index)
+    (void)hipSetDevice(current);
+  return rc;
+}
+
+int hcamdInternalComputeUnits(OlQueue q) noexcept {
+  return q ? computeUnitsOf(static_cast<Queue *>(q)->device) : 256;
+}
+
+int hcamdInternalVariant(const char *family) noexcept {
+  try {
+    return variantOf(family);
+  } catch (...) {
+    return 0;
+  }
 }
 
 OlDevice hcamdQueueDevice(OlQueue q) noexcept {

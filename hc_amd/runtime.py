@@ -173,6 +173,36 @@ hcamdGatherMapCreate = _sig(_rt, "hcamdGatherMapCreate", _vp, _vp, C.POINTER(Gat
 hcamdGatherMapLaunch = _sig(_rt, "hcamdGatherMapLaunch", _int, _vp, _vp, _vp, _sz, C.POINTER(_vp),
                             C.POINTER(_int), _vp, _int, _int, _sz)
 hcamdGatherMapRelease = _sig(_rt, "hcamdGatherMapRelease", None, _vp)
+
+# Operators of language models
+hcamdLaunchAddRmsNorm = _sig(_rt, "hcamdLaunchAddRmsNorm", _int, _vp, _int, _vp, _sz, _vp, _sz, _vp, _int,
+                             C.c_float, _vp, _sz, _vp, _int, _sz, _vp, _vp, _sz, _sz)
+hcamdAddRmsNormBackwardWorkspace = _sig(_rt, "hcamdAddRmsNormBackwardWorkspace", _sz, _sz, _sz)
+hcamdLaunchAddRmsNormBackward = _sig(_rt, "hcamdLaunchAddRmsNormBackward", _int, _vp, _int, _vp, _sz, _vp, _sz,
+                                     _vp, _int, _vp, _vp, _sz, _vp, _sz, _vp, _sz, _sz, _vp, _sz)
+hcamdLaunchGatedFfn = _sig(_rt, "hcamdLaunchGatedFfn", _int, _vp, _int, _vp, _sz, _vp, _vp, _sz, _vp, _vp, _sz, _vp,
+                           _int, _vp, _int, _sz, _vp, _sz, _vp, _sz, _sz, _sz, _sz)
+hcamdGatedFfnBackwardWorkspace = _sig(_rt, "hcamdGatedFfnBackwardWorkspace", _sz, _sz, _sz, _sz)
+hcamdLaunchGatedFfnBackward = _sig(_rt, "hcamdLaunchGatedFfnBackward", _int, _vp, _int, *[_vp, _sz] * 6, _int,
+                                   *[_vp, _sz] * 3, _sz, _sz, _sz, _vp, _sz)
+hcamdLinearCrossEntropyWorkspace = _sig(_rt, "hcamdLinearCrossEntropyWorkspace", _sz, _sz, _sz)
+hcamdLaunchLinearCrossEntropy = _sig(_rt, "hcamdLaunchLinearCrossEntropy", _int, _vp, _int, _vp, _sz, _vp, _sz, _vp,
+                                     _int, _vp, _vp, _sz, _sz, _sz, _vp, _sz)
+hcamdLinearCrossEntropyBackwardWorkspace = _sig(_rt, "hcamdLinearCrossEntropyBackwardWorkspace", _sz, _sz, _sz, _sz,
+                                                _sz)
+hcamdLaunchLinearCrossEntropyBackward = _sig(_rt, "hcamdLaunchLinearCrossEntropyBackward", _int, _vp, _int, _vp, _sz,
+                                             _vp, _sz, _vp, _int, _vp, _vp, _vp, _sz, _vp, _sz, _sz, _sz, _sz, _sz,
+                                             _vp, _sz)
+
+
+class ClipTensor(C.Structure):
+    """HcamdClipTensor of include/hc_amd_runtime.h."""
+    _fields_ = [("in_", _vp), ("out", _vp), ("count", _sz), ("type", _int)]
+
+
+hcamdClipGradNormWorkspace = _sig(_rt, "hcamdClipGradNormWorkspace", _sz, _sz)
+hcamdLaunchClipGradNorm = _sig(_rt, "hcamdLaunchClipGradNorm", _int, _vp, C.POINTER(ClipTensor), _sz, C.c_float, _vp,
+                               _vp, _sz)
 hcamdConvertPyArray = _sig(_py, "hcamdConvertPyArray", _int, C.py_object, _int, _vp,
                            _sz_p, C.c_char_p, _sz)
 hcamdConvertPyInt64 = _sig(_py, "hcamdConvertPyInt64", _int, C.py_object,
@@ -1048,6 +1078,234 @@ def plan_gemm_f16(a, bt, c) -> Plan:
                 "hcamdLaunchGemmF16", (a, bt, c))
 
 
+# ---------------------------------------------------------------------------
+# Operators of language models (see the same section of hc_amd_runtime.h)
+# ---------------------------------------------------------------------------
+I8 = 6
+ACTIVATIONS = {"silu": 0, "gelu": 1}
+_ELEM_TYPES = {"float32": F32, "float16": F16, "bfloat16": BF16, "int8": I8, "int32": I32, "int64": I64}
+
+
+def _elem_type(x, name: str) -> int:
+    """The element type of an array by its dtype (bf16 data of a DeviceArray by its flag)."""
+    if getattr(x, "bf16", False):
+        return BF16
+    dtype = getattr(x, "dtype", None)
+    code = _ELEM_TYPES.get(str(getattr(dtype, "name", dtype)).replace("torch.", ""))
+    if code is None:
+        raise HcRuntimeError(f"{name}: element type {dtype}")
+    return code
+
+
+class _Operand:
+    """A matrix operand of an operator: address, rows, cols, leading dimension, element type; absent
+    ones are a null pointer."""
+    __slots__ = ("ptr", "rows", "cols", "ld", "type")
+
+    def __init__(self, x, name: str, types=None, shape=None):
+        if x is None:
+            self.ptr, self.rows, self.cols, self.ld, self.type = None, 0, 0, 0, None
+            return
+        m = as_memref(x, 2)
+        self.rows, self.cols = m.shape
+        if self.cols > 1 and m.strides[1] != 1:
+            raise HcRuntimeError(f"{name}: rows must be contiguous (last stride 1)")
+        if self.rows > 1 and m.strides[0] < 0:
+            raise HcRuntimeError(f"{name}: negative stride")
+        self.ptr, self.ld, self.type = m.ptr, (m.strides[0] if self.rows > 1 else self.cols), _elem_type(x, name)
+        if types is not None and self.type not in types:
+            raise HcRuntimeError(f"{name}: element type {getattr(x, 'dtype', None)}")
+        if shape is not None and tuple(m.shape) != tuple(shape):
+            raise HcRuntimeError(f"{name}: shape {tuple(m.shape)}, expected {tuple(shape)}")
+
+
+class _Vector:
+    """A contiguous vector operand (a scale, targets, a loss)."""
+    __slots__ = ("ptr", "type")
+
+    def __init__(self, x, name: str, n: int, types):
+        if x is None:
+            self.ptr, self.type = None, types[0]
+            return
+        m = as_memref(x, 1)
+        if m.shape[0] != n or (n > 1 and m.strides[0] != 1):
+            raise HcRuntimeError(f"{name}: {n} contiguous values expected, shape {m.shape} strides {m.strides}")
+        self.ptr, self.type = m.ptr, _elem_type(x, name)
+        if self.type not in types:
+            raise HcRuntimeError(f"{name}: element type {getattr(x, 'dtype', None)}")
+
+
+def _workspace(nbytes: int, ctx: Context):
+    return DeviceArray((nbytes,), np.uint8, ctx) if nbytes else None
+
+
+def plan_add_rms_norm(x, residual, weight, out, eps: float = 1e-6, summed=None, scale=None, rstd=None) -> Plan:
+    """summed = x + residual and out = summed / rms(summed) * weight along the rows
+    (see hcamdLaunchAddRmsNorm).  residual, weight, summed and rstd may be None; an
+    int8 `out` takes a `scale` (one fp32 value per row)."""
+    ctx = _ctx_of(x, residual, out)
+    mx = _Operand(x, "x", (F32, F16, BF16))
+    shape, one = (mx.rows, mx.cols), (mx.type,)
+    mr, ms = _Operand(residual, "residual", one, shape), _Operand(summed, "summed", one, shape)
+    mo = _Operand(out, "out", (mx.type, I8), shape)
+    w = _Vector(weight, "weight", mx.cols, (F32, mx.type))
+    sc, rs = _Vector(scale, "scale", mx.rows, (F32,)), _Vector(rstd, "rstd", mx.rows, (F32,))
+    return Plan(ctx, hcamdLaunchAddRmsNorm,
+                (ctx.queue, mx.type, mx.ptr, mx.ld, mr.ptr, mr.ld, w.ptr, w.type, float(eps), ms.ptr, ms.ld, mo.ptr,
+                 mo.type, mo.ld, sc.ptr, rs.ptr, mx.rows, mx.cols), "hcamdLaunchAddRmsNorm",
+                (x, residual, weight, out, summed, scale, rstd))
+
+
+def plan_add_rms_norm_backward(grad_out, summed, weight, rstd, grad_in, grad_weight=None, grad_summed=None) -> Plan:
+    """The backward pass of add_rms_norm from its `summed` and `rstd` (see
+    hcamdLaunchAddRmsNormBackward).  grad_in is the gradient of x and residual alike;
+    grad_summed, when given, is what reaches `summed` by other ways.  The workspace
+    is allocated here, once, with the plan."""
+    ctx = _ctx_of(grad_out, summed, grad_in)
+    mg = _Operand(grad_out, "grad_out", (F32, F16, BF16))
+    shape, one = (mg.rows, mg.cols), (mg.type,)
+    mh, mi = _Operand(summed, "summed", one, shape), _Operand(grad_in, "grad_in", one, shape)
+    mgs = _Operand(grad_summed, "grad_summed", one, shape)
+    w = _Vector(weight, "weight", mg.cols, (F32, mg.type))
+    gw = _Vector(grad_weight, "grad_weight", mg.cols, (F32, mg.type))
+    if weight is not None and grad_weight is not None and w.type != gw.type:
+        raise HcRuntimeError("grad_weight: the weight's element type expected")
+    rs = _Vector(rstd, "rstd", mg.rows, (F32,))
+    need = hcamdAddRmsNormBackwardWorkspace(mg.rows, mg.cols) if grad_weight is not None else 0
+    work = _workspace(need, ctx)
+    return Plan(ctx, hcamdLaunchAddRmsNormBackward,
+                (ctx.queue, mg.type, mg.ptr, mg.ld, mh.ptr, mh.ld, w.ptr, gw.type if weight is None else w.type,
+                 rs.ptr, mgs.ptr, mgs.ld, mi.ptr, mi.ld, gw.ptr, mg.rows, mg.cols, work.ptr if work else None, need),
+                "hcamdLaunchAddRmsNormBackward",
+                (grad_out, summed, weight, rstd, grad_in, grad_weight, grad_summed, work))
+
+
+def _activation(name: str) -> int:
+    if name not in ACTIVATIONS:
+        raise HcRuntimeError(f"activation {name!r} (known: {', '.join(ACTIVATIONS)})")
+    return ACTIVATIONS[name]
+
+
+def plan_gated_ffn(x, w_gate, w_up, out, activation: str = "silu", gate=None, up=None, scales=None) -> Plan:
+    """out = act(x @ w_gate.T) * (x @ w_up.T) (see hcamdLaunchGatedFfn): x [T, d], weights [f, d], out
+    [T, f], fp16 or bf16; `gate` and `up` [T, f] receive the two products for the backward pass.
+    int8 operands take scales = (x_scale [T], gate_scale [f], up_scale [f]) and an fp16 or bf16 out."""
+    ctx = _ctx_of(x, w_gate, w_up, out)
+    mx = _Operand(x, "x", (F16, BF16, I8))
+    mg = _Operand(w_gate, "w_gate", (mx.type,))
+    if mg.cols != mx.cols:
+        raise HcRuntimeError(f"w_gate: rows of {mg.cols}, expected {mx.cols}")
+    t, d, f = mx.rows, mx.cols, mg.rows
+    mu = _Operand(w_up, "w_up", (mx.type,), (f, d))
+    mo = _Operand(out, "out", (F16, BF16) if mx.type == I8 else (mx.type,), (t, f))
+    sg, su = _Operand(gate, "gate", (mo.type,), (t, f)), _Operand(up, "up", (mo.type,), (t, f))
+    if (mx.type == I8) != (scales is not None) or (scales is not None and len(scales) != 3):
+        raise HcRuntimeError("gated_ffn: int8 operands take three scales, others none")
+    xs, gs, us = scales if scales is not None else (None, None, None)
+    vx, vg, vu = (_Vector(xs, "x_scale", t, (F32,)), _Vector(gs, "gate_scale", f, (F32,)),
+                  _Vector(us, "up_scale", f, (F32,)))
+    return Plan(ctx, hcamdLaunchGatedFfn,
+                (ctx.queue, mx.type, mx.ptr, mx.ld, vx.ptr, mg.ptr, mg.ld, vg.ptr, mu.ptr, mu.ld, vu.ptr,
+                 _activation(activation), mo.ptr, mo.type, mo.ld, sg.ptr, sg.ld, su.ptr, su.ld, t, d, f),
+                "hcamdLaunchGatedFfn", (x, w_gate, w_up, out, gate, up, scales))
+
+
+def plan_gated_ffn_backward(grad_out, x, w_gate, w_up, gate, up, grad_x=None, grad_w_gate=None, grad_w_up=None,
+                            activation: str = "silu") -> Plan:
+    """The backward pass of gated_ffn from its stored `gate` and `up` (see
+    hcamdLaunchGatedFfnBackward); gradients that are None are not computed.  The
+    workspace is allocated here, once, with the plan."""
+    ctx = _ctx_of(grad_out, x, gate, up)
+    mo = _Operand(grad_out, "grad_out", (F16, BF16))
+    one, (t, f) = (mo.type,), (mo.rows, mo.cols)
+    mx = _Operand(x, "x", one)
+    if mx.rows != t:
+        raise HcRuntimeError(f"x: {mx.rows} rows, expected {t}")
+    d = mx.cols
+    wg, wu = _Operand(w_gate, "w_gate", one, (f, d)), _Operand(w_up, "w_up", one, (f, d))
+    sg, su = _Operand(gate, "gate", one, (t, f)), _Operand(up, "up", one, (t, f))
+    gx = _Operand(grad_x, "grad_x", one, (t, d))
+    gg, gu = _Operand(grad_w_gate, "grad_w_gate", one, (f, d)), _Operand(grad_w_up, "grad_w_up", one, (f, d))
+    need = hcamdGatedFfnBackwardWorkspace(t, d, f)
+    work = _workspace(need, ctx)
+    return Plan(ctx, hcamdLaunchGatedFfnBackward,
+                (ctx.queue, mo.type, mo.ptr, mo.ld, mx.ptr, mx.ld, wg.ptr, wg.ld, wu.ptr, wu.ld, sg.ptr, sg.ld,
+                 su.ptr, su.ld, _activation(activation), gx.ptr, gx.ld, gg.ptr, gg.ld, gu.ptr, gu.ld, t, d, f,
+                 work.ptr if work else None, need), "hcamdLaunchGatedFfnBackward",
+                (grad_out, x, w_gate, w_up, gate, up, grad_x, grad_w_gate, grad_w_up, work))
+
+
+def plan_linear_cross_entropy(x, weight, targets, loss, lse) -> Plan:
+    """Per-row softmax cross entropy of x @ weight.T against `targets`, and the rows'
+    log-sum-exp, without the logits (see hcamdLaunchLinearCrossEntropy): x [T, d] and
+    weight [V, d] fp16 or bf16, targets int32 / int64 (negative: the row takes no
+    part), loss and lse fp32.  The workspace is allocated here, once, with the plan."""
+    ctx = _ctx_of(x, weight, loss)
+    mx = _Operand(x, "x", (F16, BF16))
+    mw = _Operand(weight, "weight", (mx.type,))
+    if mw.cols != mx.cols:
+        raise HcRuntimeError(f"weight: rows of {mw.cols}, expected {mx.cols}")
+    tg = _Vector(targets, "targets", mx.rows, (I32, I64))
+    lo, ls = _Vector(loss, "loss", mx.rows, (F32,)), _Vector(lse, "lse", mx.rows, (F32,))
+    need = hcamdLinearCrossEntropyWorkspace(mx.rows, mw.rows)
+    work = _workspace(need, ctx)
+    return Plan(ctx, hcamdLaunchLinearCrossEntropy,
+                (ctx.queue, mx.type, mx.ptr, mx.ld, mw.ptr, mw.ld, tg.ptr, tg.type, lo.ptr, ls.ptr, mx.rows, mx.cols,
+                 mw.rows, work.ptr if work else None, need), "hcamdLaunchLinearCrossEntropy",
+                (x, weight, targets, loss, lse, work))
+
+
+def plan_linear_cross_entropy_backward(x, weight, targets, lse, grad_loss, grad_x=None, grad_weight=None,
+                                       piece: int = 0) -> Plan:
+    """The backward pass of linear_cross_entropy from its `lse`, for the gradient
+    `grad_loss` of each row's loss (see hcamdLaunchLinearCrossEntropyBackward).  The
+    vocabulary is worked through in pieces of `piece` rows (0: chosen by size); the
+    workspace, which holds one piece, is allocated here, once, with the plan."""
+    ctx = _ctx_of(x, weight, grad_loss)
+    mx = _Operand(x, "x", (F16, BF16))
+    mw = _Operand(weight, "weight", (mx.type,))
+    if mw.cols != mx.cols:
+        raise HcRuntimeError(f"weight: rows of {mw.cols}, expected {mx.cols}")
+    if piece < 0:
+        raise HcRuntimeError("linear_cross_entropy_backward: negative piece")
+    t, d, v = mx.rows, mx.cols, mw.rows
+    tg = _Vector(targets, "targets", t, (I32, I64))
+    ls, gl = _Vector(lse, "lse", t, (F32,)), _Vector(grad_loss, "grad_loss", t, (F32,))
+    gx, gw = _Operand(grad_x, "grad_x", (mx.type,), (t, d)), _Operand(grad_weight, "grad_weight", (mx.type,), (v, d))
+    need = hcamdLinearCrossEntropyBackwardWorkspace(t, d, v, piece)
+    work = _workspace(need, ctx)
+    return Plan(ctx, hcamdLaunchLinearCrossEntropyBackward,
+                (ctx.queue, mx.type, mx.ptr, mx.ld, mw.ptr, mw.ld, tg.ptr, tg.type, ls.ptr, gl.ptr, gx.ptr, gx.ld,
+                 gw.ptr, gw.ld, t, d, v, piece, work.ptr if work else None, need),
+                "hcamdLaunchLinearCrossEntropyBackward",
+                (x, weight, targets, lse, grad_loss, grad_x, grad_weight, work))
+
+
+def plan_clip_grad_norm(grads, outs, norm, max_norm: float) -> Plan:
+    """norm[0] = the joint 2-norm of `grads`, outs[i] = grads[i] * min(1, max_norm / (norm + 1e-6))
+    (see hcamdLaunchClipGradNorm): contiguous fp32 / fp16 / bf16 arrays of any shape, each
+    output of its input's type and size (it may be the input).  The workspace is
+    allocated here, once, with the plan."""
+    grads, outs = list(grads), list(outs)
+    if len(grads) != len(outs):
+        raise HcRuntimeError("clip_grad_norm: one output per gradient")
+    ctx = _ctx_of(*grads, *outs, norm)
+    table = (ClipTensor * max(len(grads), 1))()
+    for i, (g, o) in enumerate(zip(grads, outs)):
+        mg, mo, tg = as_memref(g), as_memref(o), _elem_type(g, f"grads[{i}]")
+        if tg not in (F32, F16, BF16) or _elem_type(o, f"outs[{i}]") != tg or mg.size != mo.size:
+            raise HcRuntimeError(f"clip_grad_norm: tensor {i}: fp32, fp16 or bf16, output of the same type and size")
+        if not mg.is_contiguous() or not mo.is_contiguous():
+            raise HcRuntimeError(f"clip_grad_norm: tensor {i} must be contiguous")
+        table[i].in_, table[i].out, table[i].count, table[i].type = mg.ptr, mo.ptr, mg.size, tg
+    nv = _Vector(norm, "norm", 1, (F32,))
+    need = hcamdClipGradNormWorkspace(len(grads))
+    work = _workspace(need, ctx)
+    return Plan(ctx, hcamdLaunchClipGradNorm,
+                (ctx.queue, table, len(grads), float(max_norm), nv.ptr, work.ptr, need), "hcamdLaunchClipGradNorm",
+                (grads, outs, norm, table, work))
+
+
 # Call-and-wait forms: a kernel call is synchronous on return by default, as in
 # the reference (python/cpp/py-runtime/src/GpuRuntime.cpp:60-69).
 def copy2d(src, dst, sync: bool = True) -> None:
@@ -1076,6 +1334,41 @@ def quantize_f16_i8(x, q, scale, sync: bool = True) -> None:
 
 def gemm_bf16(a, bt, c, sync: bool = True) -> None:
     plan_gemm_bf16(a, bt, c).launch(sync)
+
+
+def add_rms_norm(x, residual, weight, out, eps: float = 1e-6, summed=None, scale=None, rstd=None,
+                 sync: bool = True) -> None:
+    plan_add_rms_norm(x, residual, weight, out, eps, summed, scale, rstd).launch(sync)
+
+
+def add_rms_norm_backward(grad_out, summed, weight, rstd, grad_in, grad_weight=None, grad_summed=None) -> None:
+    # (calls that bring a workspace of their own always wait: it goes with the plan)
+    plan_add_rms_norm_backward(grad_out, summed, weight, rstd, grad_in, grad_weight, grad_summed).launch(sync=True)
+
+
+def gated_ffn(x, w_gate, w_up, out, activation: str = "silu", gate=None, up=None, scales=None,
+              sync: bool = True) -> None:
+    plan_gated_ffn(x, w_gate, w_up, out, activation, gate, up, scales).launch(sync)
+
+
+def gated_ffn_backward(grad_out, x, w_gate, w_up, gate, up, grad_x=None, grad_w_gate=None, grad_w_up=None,
+                       activation: str = "silu") -> None:
+    plan_gated_ffn_backward(grad_out, x, w_gate, w_up, gate, up, grad_x, grad_w_gate, grad_w_up,
+                            activation).launch(sync=True)
+
+
+def linear_cross_entropy(x, weight, targets, loss, lse) -> None:
+    plan_linear_cross_entropy(x, weight, targets, loss, lse).launch(sync=True)
+
+
+def linear_cross_entropy_backward(x, weight, targets, lse, grad_loss, grad_x=None, grad_weight=None,
+                                  piece: int = 0) -> None:
+    plan_linear_cross_entropy_backward(x, weight, targets, lse, grad_loss, grad_x, grad_weight,
+                                       piece).launch(sync=True)
+
+
+def clip_grad_norm(grads, outs, norm, max_norm: float) -> None:
+    plan_clip_grad_norm(grads, outs, norm, max_norm).launch(sync=True)
 
 
 def probes_built() -> bool:

@@ -288,7 +288,7 @@ int hcamdLaunchFmaF16(OlQueue q, const void *a, size_t lda, const void *b,
  * interprets sixteen elements of a lane per dispatch; the results are the same
  * bit for bit (variant 4 of the "map" family: every such program, 5: none). */
 enum HcamdElemType { HCAMD_F32 = 0, HCAMD_F16 = 1, HCAMD_BF16 = 2, HCAMD_I32 = 3, HCAMD_I64 = 4,
-                     HCAMD_U8 = 5 };
+                     HCAMD_U8 = 5, HCAMD_I8 = 6 };
 enum HcamdMapOp {
   HCAMD_MAP_END = 0,
   HCAMD_MAP_IN = 1,    /* push operand `arg` */
@@ -815,6 +815,101 @@ int hcamdSetThreadVariant(const char *family, int variant) HCAMD_NOEXCEPT;
 /* Name and launch geometry of the kernel the most recent typed launcher
  * enqueued on this thread (for reports and profiles). */
 const char *hcamdLastKernelName(void) HCAMD_NOEXCEPT;
+
+/* ---- Operators of language models -----------------------------------------
+ * Like the typed launchers above: asynchronous on the queue's stream, nothing
+ * allocated (also under stream capture), shapes and alignment checked on the
+ * host.  Matrices are row-major with unit inner stride; leading dimensions in
+ * elements; pointers need the alignment of their elements only (16 bytes and
+ * leading dimensions to match take the fast kernels).  Element types are
+ * HCAMD_F32 / F16 / BF16 / I8 where an operator says so.  A workspace is the
+ * caller's, 256-byte aligned, at least the size its function names, its contents
+ * meaningless before and after; calls that may overlap in time (two queues, two
+ * captured graphs) need one each.  Outputs must not overlap inputs or each other
+ * unless stated.  Every result is the same in every run: no atomics.
+ */
+
+/* h = x + residual, rounded to elemType; y = h / sqrt(mean(h^2) + eps) * weight
+ * along the rows, in fp32.  elemType: F32, F16, BF16.  residual (null: 0) and
+ * weight (null: 1; F32 or elemType, cols values) may be absent; summed (may be
+ * null) receives h, rstd (may be null) 1 / sqrt(mean(h^2) + eps) per row.
+ * outType elemType: out = y.  outType HCAMD_I8: out = q = rint(127 v / most), half
+ * to even, v = h * weight, most = max |v| over the row, and scale[row] =
+ * rstd * most / 127, so that q * scale stands for y; a row of zeros has q = 0 and
+ * scale 0, a row with a value that is not finite q = 0 and scale NaN.
+ * summed and out may be x or residual (same leading dimension). */
+int hcamdLaunchAddRmsNorm(OlQueue q, int elemType, const void *x, size_t ldx, const void *residual, size_t ldr,
+                          const void *weight, int weightType, float eps, void *summed, size_t lds, void *out,
+                          int outType, size_t ldo, float *scale, float *rstd, size_t rows,
+                          size_t cols) HCAMD_NOEXCEPT;
+/* Its backward pass, from the stored h and rstd: with a = gradOut * weight and
+ * n = h * rstd, gradIn = gradSummed + rstd * (a - n * mean(a * n)), the gradient of x
+ * and of the residual alike, and gradWeight = sum over the rows of gradOut * n
+ * (weightType; null: not wanted, then no workspace either).  gradSummed (may be
+ * null) is what reaches h by other ways.  gradIn may be gradOut or gradSummed. */
+size_t hcamdAddRmsNormBackwardWorkspace(size_t rows, size_t cols) HCAMD_NOEXCEPT;
+int hcamdLaunchAddRmsNormBackward(OlQueue q, int elemType, const void *gradOut, size_t ldg, const void *summed,
+                                  size_t lds, const void *weight, int weightType, const float *rstd,
+                                  const void *gradSummed, size_t ldgs, void *gradIn, size_t ldgi, void *gradWeight,
+                                  size_t rows, size_t cols, void *work, size_t workBytes) HCAMD_NOEXCEPT;
+
+/* The gated half of a feed-forward block: out = act(x Wg') * (x Wu').  x is
+ * tokens x d, wGate and wUp are f x d, out is tokens x f.  elemType F16 / BF16:
+ * fp32 sums, out in elemType; gate and up (may be null) receive x Wg' and x Wu' for
+ * the backward pass.  elemType I8: whole sums (d at most 131072), the operands
+ * stand for x[t] * xScale[t], wGate[j] * gateScale[j], wUp[j] * upScale[j] (what
+ * hcamdLaunchQuantizeF16I8 and the 8-bit output above make), outType F16 or BF16;
+ * gate and up must be null.  GELU is the tanh form. */
+enum HcamdActivation { HCAMD_SILU = 0, HCAMD_GELU = 1 };
+int hcamdLaunchGatedFfn(OlQueue q, int elemType, const void *x, size_t ldx, const float *xScale, const void *wGate,
+                        size_t ldwg, const float *gateScale, const void *wUp, size_t ldwu, const float *upScale,
+                        int activation, void *out, int outType, size_t ldo, void *gate, size_t ldgate, void *up,
+                        size_t ldup, size_t tokens, size_t d, size_t f) HCAMD_NOEXCEPT;
+/* Its backward pass from the stored gate and up (F16 / BF16): dg = gradOut * up *
+ * act'(gate) and du = gradOut * act(gate), each rounded to elemType, then gradX = dg Wg +
+ * du Wu, gradWGate = dg' x, gradWUp = du' x, summed in fp32.  Gradients that are
+ * null are not computed (x, wGate and wUp may be null where only others need them).
+ * Without tokens the weights' gradients are zeros. */
+size_t hcamdGatedFfnBackwardWorkspace(size_t tokens, size_t d, size_t f) HCAMD_NOEXCEPT;
+int hcamdLaunchGatedFfnBackward(OlQueue q, int elemType, const void *gradOut, size_t ldg, const void *x, size_t ldx,
+                                const void *wGate, size_t ldwg, const void *wUp, size_t ldwu, const void *gate,
+                                size_t ldgate, const void *up, size_t ldup, int activation, void *gradX, size_t ldgx,
+                                void *gradWGate, size_t ldgwg, void *gradWUp, size_t ldgwu, size_t tokens, size_t d,
+                                size_t f, void *work, size_t workBytes) HCAMD_NOEXCEPT;
+
+/* Softmax cross entropy of z = x W' (x tokens x d, weight vocab x d, F16 / BF16, z in
+ * fp32 and never stored): lse = log(sum(exp(z))) and loss = lse - z[target] per row.
+ * targets: I32 or I64; a negative one takes its row out (loss 0), one of vocab or
+ * more is an error that shows as a loss of NaN. */
+size_t hcamdLinearCrossEntropyWorkspace(size_t tokens, size_t vocab) HCAMD_NOEXCEPT;
+int hcamdLaunchLinearCrossEntropy(OlQueue q, int elemType, const void *x, size_t ldx, const void *weight, size_t ldw,
+                                  const void *targets, int targetType, float *loss, float *lse, size_t tokens,
+                                  size_t d, size_t vocab, void *work, size_t workBytes) HCAMD_NOEXCEPT;
+/* Its backward pass from the stored lse: p = (exp(z - lse) - onehot(target)) *
+ * gradLoss[row], gradX = p W, gradWeight = p' x (either may be null).  The vocabulary
+ * goes through the workspace in pieces of `piece` rows (0: chosen by size); p is
+ * rounded to elemType there, scaled so that the largest |gradLoss| is 1 (fp16: 2^15),
+ * which the results undo.  Rows whose target is negative or not
+ * below vocab have no gradient, whatever their logits. */
+size_t hcamdLinearCrossEntropyBackwardWorkspace(size_t tokens, size_t d, size_t vocab, size_t piece) HCAMD_NOEXCEPT;
+int hcamdLaunchLinearCrossEntropyBackward(OlQueue q, int elemType, const void *x, size_t ldx, const void *weight,
+                                          size_t ldw, const void *targets, int targetType, const float *lse,
+                                          const float *gradLoss, void *gradX, size_t ldgx, void *gradWeight,
+                                          size_t ldgw, size_t tokens, size_t d, size_t vocab, size_t piece,
+                                          void *work, size_t workBytes) HCAMD_NOEXCEPT;
+
+/* norm[0] = sqrt of the sum of squares over all tensors (summed in fp64), out = in *
+ * min(1, maxNorm / (norm + 1e-6)) for each, in fp32 and rounded to the tensor's type
+ * (F32, F16, BF16, types may mix; contiguous; count 0 allowed).  out may be in. */
+typedef struct HcamdClipTensor {
+  const void *in;
+  void *out;
+  size_t count;
+  int type;
+} HcamdClipTensor;
+size_t hcamdClipGradNormWorkspace(size_t tensors) HCAMD_NOEXCEPT;
+int hcamdLaunchClipGradNorm(OlQueue q, const HcamdClipTensor *tensors, size_t count, float maxNorm, float *norm,
+                            void *work, size_t workBytes) HCAMD_NOEXCEPT;
 
 #ifdef __cplusplus
 } /* extern "C" */
