@@ -33,8 +33,10 @@ NATIVE = PKG / "_native"
 BUILD = NATIVE / "build"
 INCLUDE = PKG.parent / "include"
 
-KERNEL_MODULES = ("copy", "elementwise", "map", "imap", "fmap", "distance", "gather", "softmax", "quantize", "gemm",
-                  "rmsnorm", "ffn", "xent", "clip")
+KERNEL_MODULES = ("copy", "elementwise", "map", "imap", "fmap", "distance", "gather", "softmax", "quantize", "gemm")
+# the operators of language models
+OPERATOR_MODULES = ("rmsnorm", "ffn", "xent", "clip")
+ALL_MODULES = KERNEL_MODULES + OPERATOR_MODULES
 ARCH = "gfx950"
 
 # Packed fp32 VALU forms are kept out of every kernel.
@@ -130,11 +132,11 @@ def build_pyabi() -> Path:
     return out
 
 
-def build_all(modules: tuple[str, ...] = KERNEL_MODULES, keep_asm: bool = False) -> None:
+def build_all(modules: tuple[str, ...] = ALL_MODULES, keep_asm: bool = False) -> None:
     BUILD.mkdir(parents=True, exist_ok=True)
     with ThreadPoolExecutor(max_workers=min(8, len(modules) or 1)) as pool:
         list(pool.map(lambda m: build_kernel_module(m, keep_asm), modules))
-    missing = [m for m in KERNEL_MODULES if not (BUILD / f"{m}.hsaco").exists()]
+    missing = [m for m in ALL_MODULES if not (BUILD / f"{m}.hsaco").exists()]
     if missing:
         raise RuntimeError(f"code objects missing, build them first: {missing}")
     build_runtime()
@@ -145,10 +147,10 @@ def main(argv: list[str]) -> int:
     global PROBES
     keep = "--asm" in argv
     PROBES = "--probes" in argv
-    names = tuple(a for a in argv if not a.startswith("--")) or KERNEL_MODULES
-    unknown = [n for n in names if n not in KERNEL_MODULES]
+    names = tuple(a for a in argv if not a.startswith("--")) or ALL_MODULES
+    unknown = [n for n in names if n not in ALL_MODULES]
     if unknown:
-        print(f"unknown kernel module(s): {unknown}; known: {KERNEL_MODULES}",
+        print(f"unknown kernel module(s): {unknown}; known: {ALL_MODULES}",
               file=sys.stderr)
         return 2
     build_all(names, keep)

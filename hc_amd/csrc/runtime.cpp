@@ -168,8 +168,11 @@ struct Blob {
 const Blob kBlobs[] = {HCAMD_BLOB(copy), HCAMD_BLOB(elementwise),
                        HCAMD_BLOB(map), HCAMD_BLOB(imap), HCAMD_BLOB(fmap), HCAMD_BLOB(distance),
                        HCAMD_BLOB(gather), HCAMD_BLOB(softmax),
-                       HCAMD_BLOB(quantize), HCAMD_BLOB(gemm), HCAMD_BLOB(rmsnorm),
-                       HCAMD_BLOB(ffn), HCAMD_BLOB(xent), HCAMD_BLOB(clip)};
+                       HCAMD_BLOB(quantize), HCAMD_BLOB(gemm)};
+// The operators of language models: found by name like the others, not among
+// the modules that hcamdGetBuiltinModule counts out (those are the kernels that
+// a traced body binds to).
+const Blob kOperatorBlobs[] = {HCAMD_BLOB(rmsnorm), HCAMD_BLOB(ffn), HCAMD_BLOB(xent), HCAMD_BLOB(clip)};
 #undef HCAMD_BLOB
 constexpr size_t kNumBlobs = sizeof(kBlobs) / sizeof(kBlobs[0]);
 
@@ -189,6 +192,9 @@ Kernel *builtinKernel(Device *dev, const char *moduleName,
   } else {
     const Blob *blob = nullptr;
     for (const Blob &b : kBlobs)
+      if (std::strcmp(b.name, moduleName) == 0)
+        blob = &b;
+    for (const Blob &b : kOperatorBlobs)
       if (std::strcmp(b.name, moduleName) == 0)
         blob = &b;
     if (!blob) {

@@ -160,7 +160,9 @@ OlDevice hcamdQueueDevice(OlQueue q) HCAMD_NOEXCEPT;
 /* Built-in gfx950 code objects, embedded in the library the way JIT'd host
  * code embeds its blob (GpuToGpuRuntime.cpp:161-169).  Index 0..count-1;
  * returns 0 and fills name/data/len, or 1 when the index is out of range.
- * The blobs can be handed to olCreateModule / hcgpuGetKernel. */
+ * The blobs can be handed to olCreateModule / hcgpuGetKernel.  The modules of the
+ * language-model operators (rmsnorm, ffn, xent, clip) are not counted here; their
+ * kernels are found by name like the others. */
 size_t hcamdBuiltinModuleCount(void) HCAMD_NOEXCEPT;
 int hcamdGetBuiltinModule(size_t index, const char **name, const void **data,
                           size_t *len) HCAMD_NOEXCEPT;
