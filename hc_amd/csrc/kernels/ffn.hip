@@ -19,8 +19,8 @@ namespace {
 enum { kSilu = 0, kGelu = 1 };
 
 // 1 / (1 + exp(-x)): exp overflows to infinity for large negative x, the
-// quotient is then 0
-__device__ __forceinline__ float sigmoid(float x) { return 1.0f / (1.0f + __expf(-x)); }
+// reciprocal is then 0 (the hardware's exponential and reciprocal, 1 ulp each)
+__device__ __forceinline__ float sigmoid(float x) { return __builtin_amdgcn_rcpf(1.0f + __expf(-x)); }
 
 constexpr float kGeluA = 0.7978845608028654f; // sqrt(2 / pi)
 constexpr float kGeluB = 0.044715f;
@@ -45,56 +45,79 @@ __device__ __forceinline__ void activate_both(int kind, float x, float &f, float
   df = p == 0.0f ? s : s + x * dt * p;
 }
 
-template <class E, class O, int MI, int NI>
-__device__ __forceinline__ void gated_store(const GatedArgs &a, typename MmaType<E>::acc (&acc)[MI][NI], int m0,
-                                            int f0, int lane) {
+// the outputs of a wave: blocks j and j + NI / 2 are the two projections of the same
+// columns.  LDS: through the wave's region `mine`, else straight from registers
+template <class E, class O, int MI, int NI, bool LDS>
+__device__ __forceinline__ void gated_store(const GatedArgs &a, typename MmaType<E>::acc (&acc)[MI][NI],
+                                            const Tile &t, int m0, int f0, int lane, unsigned char *mine) {
   constexpr int H = NI / 2;
   const int M = a.mma.M, F = a.mma.N;
-  const bool vo = can_store4<O>(a.out, a.ldo);
-  const bool vg = a.gate && can_store4<O>(a.gate, a.ldgate), vu = a.up && can_store4<O>(a.up, a.ldup);
+  const Window w = {t.m_lo, M, t.n_lo, F};
+  auto both = [&](int i, int j, f32x4 &g, f32x4 &u) {
+    const float xs = sizeof(E) == 1 ? a.x_scale[min(m0 + i * 16 + lane % 16, M - 1)] : 1.0f;
 #pragma unroll
-  for (int i = 0; i < MI; ++i) {
-    const int m = m0 + i * 16 + lane % 16;
-    if (m >= M)
-      continue;
-    const float xs = sizeof(E) == 1 ? a.x_scale[m] : 1.0f;
-#pragma unroll
-    for (int j = 0; j < H; ++j) {
-      const int f = f0 + j * 16 + lane / 16 * 4;
-      f32x4 g, u, o;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        g[e] = (float)acc[i][j][e];
-        u[e] = (float)acc[i][j + H][e];
-        if constexpr (sizeof(E) == 1) {
-          const int c = min(f + e, F - 1);
-          g[e] = g[e] * xs * a.gate_scale[c];
-          u[e] = u[e] * xs * a.up_scale[c];
-        }
-        o[e] = activate(a.activation, g[e]) * u[e];
+    for (int e = 0; e < 4; ++e) {
+      g[e] = (float)acc[i][j][e];
+      u[e] = (float)acc[i][j + H][e];
+      if constexpr (sizeof(E) == 1) {
+        const int c = min(f0 + j * 16 + lane / 16 * 4 + e, F - 1);
+        g[e] = g[e] * xs * a.gate_scale[c];
+        u[e] = u[e] * xs * a.up_scale[c];
       }
-      store4<O>(static_cast<O *>(a.out) + (size_t)m * a.ldo, f, F, vo, o);
-      if (a.gate)
-        store4<O>(static_cast<O *>(a.gate) + (size_t)m * a.ldgate, f, F, vg, g);
-      if (a.up)
-        store4<O>(static_cast<O *>(a.up) + (size_t)m * a.ldup, f, F, vu, u);
     }
+  };
+  auto value = [&](int i, int j) {
+    f32x4 g, u, o;
+    both(i, j, g, u);
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      o[e] = activate(a.activation, g[e]) * u[e];
+    return o;
+  };
+  auto pre_gate = [&](int i, int j) { return __builtin_convertvector(acc[i][j], f32x4); };
+  auto pre_up = [&](int i, int j) { return __builtin_convertvector(acc[i][j + H], f32x4); };
+  auto store = [&](void *to, size_t ld, auto &&what) {
+    if constexpr (LDS)
+      store_block<O, MI, H>(mine, static_cast<O *>(to), ld, m0, f0, w, lane, what);
+    else
+      store_direct<O, MI, H>(static_cast<O *>(to), ld, m0, f0, w, lane, what);
+  };
+  store(a.out, a.ldo, value);
+  if constexpr (sizeof(E) == 2) {
+    if (a.gate)
+      store(a.gate, a.ldgate, pre_gate);
+    if (a.up)
+      store(a.up, a.ldup, pre_up);
+  }
+}
+
+template <class E, int MI, int NI, bool LDS>
+__device__ __forceinline__ void gated_epilogue(const GatedArgs &a, typename MmaType<E>::acc (&acc)[MI][NI],
+                                               const Tile &t, int m0, int f0, int lane, unsigned char *mine) {
+  if constexpr (sizeof(E) == 1) {
+    if (a.out_f16)
+      gated_store<E, _Float16, MI, NI, LDS>(a, acc, t, m0, f0, lane, mine);
+    else
+      gated_store<E, __bf16, MI, NI, LDS>(a, acc, t, m0, f0, lane, mine);
+  } else {
+    gated_store<E, E, MI, NI, LDS>(a, acc, t, m0, f0, lane, mine);
   }
 }
 
 template <class E> __device__ __forceinline__ void gated_general(const GatedArgs &a) {
   __shared__ __attribute__((aligned(1024))) unsigned char lds[4 * 128 * 128];
   mma_general<E, kKFast, kKFast, true>(
-      a.mma, lds, [&](auto &acc, int m0, int wave_m, int tn, int wave_n, int lane, unsigned char *) {
-        const int f0 = tn * 64 + wave_n / 2;
-        if constexpr (sizeof(E) == 1) {
-          if (a.out_f16)
-            gated_store<E, _Float16>(a, acc, m0 + wave_m, f0, lane);
-          else
-            gated_store<E, __bf16>(a, acc, m0 + wave_m, f0, lane);
-        } else {
-          gated_store<E, E>(a, acc, m0 + wave_m, f0, lane);
-        }
+      a.mma, lds, FromZero{}, [&](auto &acc, const Tile &t, int wave_m, int wave_n, int lane, unsigned char *) {
+        gated_epilogue<E, 4, 4, false>(a, acc, t, t.m0 + wave_m, t.n0 + wave_n / 2, lane, nullptr);
+      });
+}
+template <class E, int B, int WM, int WN> __device__ __forceinline__ void gated_tile(const GatedArgs &a) {
+  constexpr int MI = B / WM / 16, NI = B / WN / 16;
+  __shared__ __attribute__((aligned(1024))) unsigned char lds[pipelined_lds<B, B>()];
+  mma_pipelined<E, kKFast, kKFast, true, B, B, WM, WN>(
+      a.mma, lds, FromZero{}, [&](auto &acc, const Tile &t, int wave_m, int wave_n, int lane, unsigned char *l) {
+        gated_epilogue<E, MI, NI, true>(a, acc, t, t.m0 + wave_m, t.n0 + wave_n / 2, lane,
+                                        l + (wave_m / (MI * 16) * WN + wave_n / (NI * 16)) * (MI * NI * 256));
       });
 }
 
@@ -124,21 +147,29 @@ template <class E> __device__ __forceinline__ void gated_back(const GatedBackArg
   }
 }
 
-// dx: A k-fast, B k-slow, sum over both pairs
-template <class E> __device__ __forceinline__ void product_nn(const StoreArgs &s) {
+template <class E, Layout LA, Layout LB> __device__ __forceinline__ void product_general(const StoreArgs &s) {
   __shared__ __attribute__((aligned(1024))) unsigned char lds[4 * 128 * 128];
-  mma_general<E, kKFast, kKSlow, false>(
-      s.mma, lds, [&](auto &acc, int m0, int wave_m, int tn, int wave_n, int lane, unsigned char *) {
-        store_tile<E, 4, 4, 128>(s, acc, m0 + wave_m, tn * 128 + wave_n, lane);
+  mma_general<E, LA, LB, false>(
+      s.mma, lds,
+      [&](auto &acc, const Tile &t, int wave_m, int wave_n, int lane) {
+        begin_tile<4, 4>(s, acc, t.m0 + wave_m, t.n0 + wave_n, lane);
+      },
+      [&](auto &acc, const Tile &t, int wave_m, int wave_n, int lane, unsigned char *) {
+        store_tile<E, 4, 4, false>(s, acc, t, t.m0 + wave_m, t.n0 + wave_n, lane, nullptr);
       });
 }
-// dW: both operands k-slow, grid z selects the product
-template <class E> __device__ __forceinline__ void product_tn(const PairStoreArgs &a) {
-  const StoreArgs &s = a.p[blockIdx.z];
-  __shared__ __attribute__((aligned(1024))) unsigned char lds[4 * 128 * 128];
-  mma_general<E, kKSlow, kKSlow, false>(
-      s.mma, lds, [&](auto &acc, int m0, int wave_m, int tn, int wave_n, int lane, unsigned char *) {
-        store_tile<E, 4, 4, 128>(s, acc, m0 + wave_m, tn * 128 + wave_n, lane);
+template <class E, Layout LA, Layout LB, int B, int WM, int WN>
+__device__ __forceinline__ void product_tile(const StoreArgs &s) {
+  constexpr int MI = B / WM / 16, NI = B / WN / 16;
+  __shared__ __attribute__((aligned(1024))) unsigned char lds[pipelined_lds<B, B>()];
+  mma_pipelined<E, LA, LB, false, B, B, WM, WN>(
+      s.mma, lds,
+      [&](auto &acc, const Tile &t, int wave_m, int wave_n, int lane) {
+        begin_tile<MI, NI>(s, acc, t.m0 + wave_m, t.n0 + wave_n, lane);
+      },
+      [&](auto &acc, const Tile &t, int wave_m, int wave_n, int lane, unsigned char *l) {
+        store_tile<E, MI, NI, true>(s, acc, t, t.m0 + wave_m, t.n0 + wave_n, lane,
+                                    l + (wave_m / (MI * 16) * WN + wave_n / (NI * 16)) * (MI * NI * 512));
       });
 }
 
@@ -161,6 +192,12 @@ template <class E> __device__ __forceinline__ void fold(const FoldArgs &a) {
 #define HCAMD_FFN(SUFFIX, E)                                                                              \
   extern "C" __global__ __launch_bounds__(256) void hcamd_gated_##SUFFIX##_general(GatedArgs a) {         \
     gated_general<E>(a);                                                                                  \
+  }                                                                                                       \
+  extern "C" __global__ __launch_bounds__(512) void hcamd_gated_##SUFFIX##_t256(GatedArgs a) {            \
+    gated_tile<E, 256, 2, 4>(a);                                                                          \
+  }                                                                                                       \
+  extern "C" __global__ __launch_bounds__(256) void hcamd_gated_##SUFFIX##_t128(GatedArgs a) {            \
+    gated_tile<E, 128, 2, 2>(a);                                                                          \
   }
 HCAMD_FFN(bf16, __bf16)
 HCAMD_FFN(f16, _Float16)
@@ -170,10 +207,22 @@ HCAMD_FFN(i8, int8_t)
     gated_back<E>(a);                                                                                     \
   }                                                                                                       \
   extern "C" __global__ __launch_bounds__(256) void hcamd_product_nn_##SUFFIX##_general(StoreArgs a) {    \
-    product_nn<E>(a);                                                                                     \
+    product_general<E, kKFast, kKSlow>(a);                                                                                   \
   }                                                                                                       \
   extern "C" __global__ __launch_bounds__(256) void hcamd_product_tn_##SUFFIX##_general(PairStoreArgs a) { \
-    product_tn<E>(a);                                                                                     \
+    product_general<E, kKSlow, kKSlow>(a.p[blockIdx.z]);                                                                                     \
+  }                                                                                                       \
+  extern "C" __global__ __launch_bounds__(512) void hcamd_product_nn_##SUFFIX##_t256(StoreArgs a) {       \
+    product_tile<E, kKFast, kKSlow, 256, 2, 4>(a);                                                        \
+  }                                                                                                       \
+  extern "C" __global__ __launch_bounds__(256) void hcamd_product_nn_##SUFFIX##_t128(StoreArgs a) {       \
+    product_tile<E, kKFast, kKSlow, 128, 2, 2>(a);                                                        \
+  }                                                                                                       \
+  extern "C" __global__ __launch_bounds__(512) void hcamd_product_tn_##SUFFIX##_t256(PairStoreArgs a) {   \
+    product_tile<E, kKSlow, kKSlow, 256, 2, 4>(a.p[blockIdx.z]);                                          \
+  }                                                                                                       \
+  extern "C" __global__ __launch_bounds__(256) void hcamd_product_tn_##SUFFIX##_t128(PairStoreArgs a) {   \
+    product_tile<E, kKSlow, kKSlow, 128, 2, 2>(a.p[blockIdx.z]);                                          \
   }                                                                                                       \
   extern "C" __global__ __launch_bounds__(256) void hcamd_fold_##SUFFIX(FoldArgs a) { fold<E>(a); }
 HCAMD_FFN_BACK(bf16, __bf16)

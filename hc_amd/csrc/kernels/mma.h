@@ -66,8 +66,16 @@ __device__ __forceinline__ void tile_of(int wg, int tiles_m, int tiles_n, int &t
   const int first = (wg / band) * kBand;
   const int rows = min(tiles_m - first, kBand);
   const int in = wg % band;
-  tm = first + in % rows;
-  tn = in / rows;
+  // (quotients come out of the vector unit; the tile is the same for every lane)
+  tm = __builtin_amdgcn_readfirstlane(first + in % rows);
+  tn = __builtin_amdgcn_readfirstlane(in / rows);
+}
+
+// the k tiles [kt0, kt1) of this workgroup's split
+__device__ __forceinline__ void split_of(int all, int splits, int &kt0, int &kt1) {
+  const int split = blockIdx.y, each = all / splits, more = all % splits;
+  kt0 = __builtin_amdgcn_readfirstlane(split * each + min(split, more));
+  kt1 = __builtin_amdgcn_readfirstlane(kt0 + each + (split < more ? 1 : 0));
 }
 
 // 16 bytes of which the first `valid` elements exist; the rest reads as zero.
@@ -115,6 +123,13 @@ __device__ __forceinline__ u32x4 read_operand(const unsigned char *panel, int ro
   }
 }
 
+// Where a workgroup's tile lies: it covers rows m0 .. and columns n0 .., and owns those
+// from m_lo and n_lo on (an edge tile of the pipelined kernel begins inside its
+// neighbour, whose part it computes again and does not store).
+struct Tile {
+  int m0, n0, m_lo, n_lo, tn;
+};
+
 // ---------------------------------------------------------------------------
 // General kernel body: any sizes, leading dimensions and alignment.  128 x 128
 // tile, four waves of 64 x 64, panels through registers (unaligned 16-byte
@@ -123,8 +138,8 @@ __device__ __forceinline__ u32x4 read_operand(const unsigned char *panel, int ro
 // of b[1], alternating, so that a wave's blocks j and j + 2 are the two
 // projections of the same outputs.
 // ---------------------------------------------------------------------------
-template <class E, Layout LA, Layout LB, bool GATED, class Epilogue>
-__device__ __forceinline__ void mma_general(const MmaArgs &g, unsigned char *lds, Epilogue &&epilogue) {
+template <class E, Layout LA, Layout LB, bool GATED, class Init, class Epilogue>
+__device__ __forceinline__ void mma_general(const MmaArgs &g, unsigned char *lds, Init &&init, Epilogue &&epilogue) {
   using T = MmaType<E>;
   constexpr int BM = 128, BN = 128, BNO = GATED ? BN / 2 : BN;
   constexpr int kPanel = 128 * 128, kStage = 2 * kPanel;
@@ -134,8 +149,8 @@ __device__ __forceinline__ void mma_general(const MmaArgs &g, unsigned char *lds
   const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
   const int wave_m = wave / 2 * 64, wave_n = wave % 2 * 64;
   const int tiles_k = (g.K + T::kBK - 1) / T::kBK, all = tiles_k * g.segments;
-  const int split = blockIdx.y;
-  const int kt0 = (int)((int64_t)all * split / g.splits), kt1 = (int)((int64_t)all * (split + 1) / g.splits);
+  int kt0, kt1;
+  split_of(all, g.splits, kt0, kt1);
 
   u32x4 ra[4], rb[4];
   auto load = [&](int kt) {
@@ -180,7 +195,9 @@ __device__ __forceinline__ void mma_general(const MmaArgs &g, unsigned char *lds
     }
   };
 
+  const Tile tile = {tm * BM, tn * BNO, tm * BM, tn * BNO, tn};
   typename T::acc acc[4][4] = {};
+  init(acc, tile, wave_m, wave_n, lane);
   if (kt0 < kt1) {
     load(kt0);
     store(0);
@@ -209,70 +226,429 @@ __device__ __forceinline__ void mma_general(const MmaArgs &g, unsigned char *lds
       __syncthreads();
     }
   }
-  epilogue(acc, tm * BM, wave_m, tn, wave_n, lane, lds);
+  epilogue(acc, tile, wave_m, wave_n, lane, lds);
+}
+
+// ---------------------------------------------------------------------------
+// Pipelined kernel body for operands that can be fetched in aligned 16-byte pieces.
+//   * Panels go from global memory straight into LDS (16 bytes per lane; a wave-level
+//     load fills 1 KiB of consecutive LDS, the layouts' swizzles are applied on the
+//     global side).  Two stages; the loads of tile t + 2 are issued while tile t is
+//     consumed.
+//   * A tile is two halves of k.  While the MFMAs of one half run, the operands of
+//     the next are read from LDS into a second register set, one fenced slot per
+//     MFMA in hand order: reads over the first RS MFMAs, loads every LS-th.
+//   * One barrier per tile, in front of its second half: there this wave's loads
+//     of the next tile have landed and its reads of this tile are done.
+//   * Edges: the last tile of a row or column of tiles begins BM rows (BN columns)
+//     before the end; M >= BM and N >= BN.  In the last tile of a k segment the
+//     pieces past K are fetched from valid addresses and overwritten with zeros in
+//     LDS by the lane that fetched them.  A k-fast operand whose K is not a multiple
+//     of 8 must hold zeros up to there, a k-slow one whose rows are not must have
+//     readable elements up to there (the library's own buffers).
+// A load's address is a lane part, held in a register for the whole loop, plus a
+// scalar part; from tile to tile only the base of the buffer descriptor moves.
+// ---------------------------------------------------------------------------
+constexpr int waitcnt_imm(int vmcnt, int lgkmcnt) {
+  return (vmcnt & 0xf) | ((vmcnt >> 4) << 14) | (7 << 4) | ((lgkmcnt & 0xf) << 8);
+}
+constexpr int kNoVm = 63, kNoLgkm = 15;
+typedef __attribute__((address_space(3))) void *lds_void_ptr;
+
+template <int BM, int BN> constexpr int pipelined_lds() { return 2 * (BM + BN) * 128; }
+
+template <class E, Layout LA, Layout LB, bool GATED, int BM, int BN, int WM, int WN, class Init, class Epilogue>
+__device__ __forceinline__ void mma_pipelined(const MmaArgs &g, unsigned char *lds, Init &&init,
+                                              Epilogue &&epilogue) {
+  using T = MmaType<E>;
+  constexpr int kWaves = WM * WN, kWaveM = BM / WM, kWaveN = BN / WN;
+  constexpr int kMI = kWaveM / 16, kNI = kWaveN / 16, kMfma = kMI * kNI;
+  constexpr int kALoads = BM / (8 * kWaves), kBLoads = BN / (8 * kWaves), kLoads = kALoads + kBLoads;
+  constexpr int kReads = kMI + kNI;
+  // The MFMA in front of which an operand read or a load goes.  k-fast operands: reads
+  // over the first half of the MFMAs, loads evenly over all.  The compiler lets a
+  // transposed read wait for every load into LDS that is under way, whatever stage it
+  // fills, so k-slow operands are read before a half's loads are issued (second
+  // half of a tile), and as late as there is time for them (first half), when the
+  // loads of the half before have had most of a tile to land.
+  constexpr int kSlow = (LA == kKSlow ? kMI : 0) + (LB == kKSlow ? kNI : 0), kQuick = kReads - kSlow;
+  constexpr int kSlowSpan = kSlow == 0 ? 0 : kSlow * kMfma / 32 > kMfma / 4 ? kMfma / 4 : kMfma / 8;
+  constexpr int LF = kSlow == 0 ? 1 : kSlowSpan;
+  constexpr int LS = kSlow == 0 ? kMfma / kLoads : kMfma / 2 / kLoads > 0 ? kMfma / 2 / kLoads : 1;
+  static_assert(LF + (kLoads - 1) * LS < kMfma, "every load has its MFMA");
+  // read r of a half, in the order B blocks, A blocks (as the MFMAs take them); first:
+  // the half that reads the same tile's second half
+  auto slot_of = [](int r, bool first) constexpr {
+    const bool slow = r < kNI ? LB == kKSlow : LA == kKSlow;
+    const int nth = slow ? (LB == kKSlow ? r : r - kNI) : (LB == kKSlow ? r - kNI : r);
+    if (kSlow == 0)
+      return nth * (kMfma / 2) / kReads;
+    if (slow)
+      return first ? kMfma * 9 / 16 + nth * (kMfma * 5 / 16) / kSlow : nth * kSlowSpan / kSlow;
+    return (first ? 0 : kSlowSpan) + nth * (kMfma / 2) / (kQuick ? kQuick : 1);
+  };
+  constexpr int kPanelA = BM * 128, kStage = (BM + BN) * 128;
+  constexpr int BNO = GATED ? BN / 2 : BN;
+  static_assert(sizeof(E) == 2 || (LA == kKFast && LB == kKFast), "transposed reads are for 16-bit elements");
+
+  int tm, tn;
+  tile_of(blockIdx.x, (g.M + BM - 1) / BM, (g.N + BNO - 1) / BNO, tm, tn);
+  // (k-slow rows come in aligned pieces of 8: their origin stays a multiple of 8)
+  const int end_m = LA == kKSlow ? (g.M + 7) & ~7 : g.M, end_n = LB == kKSlow ? (g.N + 7) & ~7 : g.N;
+  const Tile tile = {min(tm * BM, end_m - BM), min(tn * BNO, end_n - BNO), tm * BM, tn * BNO, tn};
+  const int lane = threadIdx.x % kWave;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int wave_m = wave / WN * kWaveM, wave_n = wave % WN * kWaveN;
+  const int tiles_k = (g.K + T::kBK - 1) / T::kBK, all = tiles_k * g.segments;
+  int kt0, kt1;
+  split_of(all, g.splits, kt0, kt1);
+  const int steps = kt1 - kt0;
+  // valid k of the last tile of a segment: elements (k-slow), 16-byte chunks (k-fast)
+  const int tail_k = g.K - (tiles_k - 1) * T::kBK;
+  const int tail_chunks = (tail_k + T::kChunk - 1) / T::kChunk;
+  const bool has_tail = tail_k < T::kBK;
+  auto is_tail = [&](int kt) { return has_tail && (kt == tiles_k - 1 || kt == all - 1); };
+
+  // ---- global -> LDS -----------------------------------------------------------
+  // The wave-level load v of a panel fills its rows (k-fast) (v * kWaves + wave) * 8 .. + 7,
+  // or its k (k-slow) (v * kWaves + wave) * kPer .. + kPer - 1, kPer = 512 / R.
+  const int fast_chunk = (lane % 8) ^ (lane / 8);
+  // the lane parts: k-fast row * ld + chunk; k-slow k * ld + column, and the same with
+  // the k of a group that K cuts clamped to its last valid one
+  struct Lane {
+    int off, cut;
+  };
+  auto lane_part = [&](Layout l, int R, int ld, bool tail) {
+    Lane p;
+    if (l == kKFast) {
+      p.off = lane / 8 * ld + (tail && fast_chunk >= tail_chunks ? 0 : fast_chunk) * 16;
+      p.cut = 0;
+    } else {
+      const int per = 512 / R, sub = lane / (R / 8), pos = lane % (R / 8);
+      // (the k of a load differ from these by multiples of 16 or of 4 * kWaves: the swizzle is the lane's)
+      const int col = ((pos / 2) ^ slow_swizzle(wave * per + sub)) * 16 + pos % 2 * 8;
+      const int left = tail_k % per;
+      p.off = sub * ld + col * 2;
+      p.cut = (tail && left ? min(sub, left - 1) : sub) * ld + col * 2;
+    }
+    return p;
+  };
+  static_assert(LA == kKFast || (kWaves * 512 / BM) % 16 == 0, "the swizzle repeats from load to load");
+  static_assert(LB == kKFast || (kWaves * 512 / BN) % 16 == 0, "the swizzle repeats from load to load");
+  // GATED: rows of the N panel alternate in 32s between the two matrices; eight waves
+  // meet one of them in all their loads, four waves the other one in every other
+  constexpr int kBOps = GATED && kWaves == 4 ? 2 : 1;
+  const int my_b = GATED && kWaves == 8 ? wave / 4 : 0;
+  Lane lane_a, lane_b[kBOps];
+  int ld_a, ld_b[kBOps];
+  __amdgpu_buffer_rsrc_t rsrc_a, rsrc_b[kBOps];
+  auto rsrc_of = [&](const void *p, size_t bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(static_cast<const char *>(p)) + bytes, 0, 0x7fffffff,
+                                             0x00020000);
+  };
+  auto origin = [&](Layout l, size_t row, size_t ld, size_t kt) {
+    return l == kKFast ? row * ld * sizeof(E) + kt * 128 : (kt * 64 * ld + row) * 2;
+  };
+  int state = -1; // segment and tail that the lane parts are set for
+  auto prepare = [&](int kt) {
+    const int seg = kt >= tiles_k ? 1 : 0, k = kt - seg * tiles_k;
+    rsrc_a = rsrc_of(g.a[seg], origin(LA, tile.m0, g.lda[seg], k));
+#pragma unroll
+    for (int o = 0; o < kBOps; ++o) {
+      const int w = GATED ? (kBOps == 2 ? o : my_b) : seg;
+      rsrc_b[o] = rsrc_of(w ? g.b[1] : g.b[0], origin(LB, tile.n0, w ? g.ldb[1] : g.ldb[0], k));
+    }
+    const int want = seg * 2 + (is_tail(kt) ? 1 : 0);
+    if (want != state) {
+      ld_a = (int)g.lda[seg] * (int)sizeof(E);
+      lane_a = lane_part(LA, BM, ld_a, want & 1);
+#pragma unroll
+      for (int o = 0; o < kBOps; ++o) {
+        const int w = GATED ? (kBOps == 2 ? o : my_b) : seg;
+        ld_b[o] = (int)(w ? g.ldb[1] : g.ldb[0]) * (int)sizeof(E);
+        lane_b[o] = lane_part(LB, BN, ld_b[o], want & 1);
+      }
+      state = want;
+    }
+  };
+  auto fetch = [&](Layout l, int R, const __amdgpu_buffer_rsrc_t &rsrc, const Lane &p, int ld, int first, void *to) {
+    // first: the load's first row or k
+    if (l == kKFast) {
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_void_ptr)to, 16, p.off, first * ld, 0, 0);
+    } else {
+      const int limit = (state & 1) ? tail_k : 64;
+      const int off = first + 512 / R <= limit ? p.off : p.cut;
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_void_ptr)to, 16, off, first < limit ? first * ld : 0, 0, 0);
+    }
+  };
+  auto load_one = [&](int buf, int v) {
+    unsigned char *base = lds + buf * kStage + wave * 1024;
+    if (v < kALoads) {
+      const int first = (v * kWaves + wave) * (LA == kKFast ? 8 : 512 / BM);
+      fetch(LA, BM, rsrc_a, lane_a, ld_a, first, base + v * kWaves * 1024);
+    } else {
+      const int b = v - kALoads;
+      int first = (b * kWaves + wave) * (LB == kKFast ? 8 : 512 / BN);
+      if constexpr (GATED)
+        first = first / 64 * 32 + first % 32;
+      const int o = kBOps == 2 ? b % 2 : 0;
+      fetch(LB, BN, rsrc_b[o], lane_b[o], ld_b[o], first, base + kPanelA + b * kWaves * 1024);
+    }
+  };
+  auto zero_tail = [&](int buf) {
+    unsigned char *base = lds + buf * kStage + wave * 1024 + lane * 16;
+    const u32x4 zero = {0u, 0u, 0u, 0u};
+#pragma unroll
+    for (int v = 0; v < kALoads; ++v)
+      if (LA == kKFast ? fast_chunk >= tail_chunks : (v * kWaves + wave) * (512 / BM) + lane / (BM / 8) >= tail_k)
+        *reinterpret_cast<u32x4 *>(base + v * kWaves * 1024) = zero;
+#pragma unroll
+    for (int v = 0; v < kBLoads; ++v)
+      if (LB == kKFast ? fast_chunk >= tail_chunks : (v * kWaves + wave) * (512 / BN) + lane / (BN / 8) >= tail_k)
+        *reinterpret_cast<u32x4 *>(base + kPanelA + v * kWaves * 1024) = zero;
+  };
+
+  // ---- LDS -> operand registers --------------------------------------------------
+  // byte offsets of this lane in a panel, per block (k-slow) or common (k-fast, a block
+  // is 2 KiB further)
+  const int lk = 8 * (lane / 16) + lane % 16 / 4; // k-slow: k of the first read
+  const int fast_lane = lane % 16 * 128;
+  const int coff[2] = {((lane / 16) ^ (lane & 7)) * 16, ((4 + lane / 16) ^ (lane & 7)) * 16};
+  // a k-slow block i is at block 0's address with bits 5 .. 7 xored by i (the origin of
+  // a wave is a multiple of its blocks, and every other part of the address lies
+  // outside those bits)
+  const int slow_a = lk * (BM * 2) + (((wave_m / 16) ^ slow_swizzle(lk)) * 32) + lane % 4 * 8;
+  const int slow_b = lk * (BN * 2) + (((wave_n / 16) ^ slow_swizzle(lk)) * 32) + lane % 4 * 8;
+  static_assert(LA == kKFast || kMI <= 8, "blocks of a wave lie in one 256-byte group");
+  auto read_slow = [&](const unsigned char *p, int four_k) {
+    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_ptr)p);
+    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_ptr)(p + four_k));
+    const u32x2 a = __builtin_bit_cast(u32x2, lo), b = __builtin_bit_cast(u32x2, hi);
+    return u32x4{a[0], a[1], b[0], b[1]};
+  };
+  u32x4 fa[2][kMI], fb[2][kNI];
+  // fragment r of half h in stage buf: the B blocks first, then the A blocks, as the MFMAs take them
+  auto read_one = [&](int buf, int h, auto slot, int r) {
+    constexpr int S = decltype(slot)::value;
+    const unsigned char *stage = lds + buf * kStage;
+    if (r < kNI) {
+      if constexpr (LB == kKFast)
+        fb[S][r] = *reinterpret_cast<const u32x4 *>(stage + kPanelA + fast_lane + coff[h] + (wave_n + r * 16) * 128);
+      else
+        fb[S][r] = read_slow(stage + kPanelA + ((slow_b ^ (r * 32)) + h * 32 * (BN * 2)), 4 * BN * 2);
+    } else {
+      const int i = r - kNI;
+      if constexpr (LA == kKFast)
+        fa[S][i] = *reinterpret_cast<const u32x4 *>(stage + fast_lane + coff[h] + (wave_m + i * 16) * 128);
+      else
+        fa[S][i] = read_slow(stage + ((slow_a ^ (i * 32)) + h * 32 * (BM * 2)), 4 * BM * 2);
+    }
+  };
+
+  typename T::acc acc[kMI][kNI] = {};
+  init(acc, tile, wave_m, wave_n, lane);
+  using Slot0 = std::integral_constant<int, 0>;
+  using Slot1 = std::integral_constant<int, 1>;
+  // MFMAs in a serpentine over the blocks: consecutive ones share an operand
+  auto half_step = [&](auto use, auto fill, int buf, int h, bool do_read, bool do_load, int load_buf) {
+    constexpr int Uu = decltype(use)::value;
+#pragma unroll
+    for (int slot = 0; slot < kMfma; ++slot) {
+      const int i = slot / kNI, j = i % 2 ? kNI - 1 - slot % kNI : slot % kNI;
+      if (do_read) {
+#pragma unroll
+        for (int r = 0; r < kReads; ++r)
+          if (slot_of(r, h == 1) == slot)
+            read_one(buf, h, fill, r);
+      }
+      if (do_load && slot >= LF && (slot - LF) % LS == 0 && (slot - LF) / LS < kLoads)
+        load_one(load_buf, (slot - LF) / LS);
+      acc[i][j] = mma16<E>(fb[Uu][j], fa[Uu][i], acc[i][j]);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  auto tile_step = [&](int t, auto load_next2, auto read_next) {
+    constexpr bool LOAD = decltype(load_next2)::value, READ = decltype(read_next)::value;
+    const int buf = t & 1;
+    __builtin_amdgcn_s_waitcnt(waitcnt_imm(kNoVm, 0));
+    __builtin_amdgcn_sched_barrier(0);
+    half_step(Slot0{}, Slot1{}, buf, 1, true, false, 0);
+    if constexpr (LOAD)
+      prepare(kt0 + t + 2);
+    __builtin_amdgcn_s_waitcnt(waitcnt_imm(0, 0));
+    if constexpr (READ) {
+      if (is_tail(kt0 + t + 1)) {
+        zero_tail(buf ^ 1);
+        __builtin_amdgcn_s_waitcnt(waitcnt_imm(kNoVm, 0));
+      }
+    }
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_sched_barrier(0);
+    half_step(Slot1{}, Slot0{}, buf ^ 1, 0, READ, LOAD, buf);
+  };
+
+  if (steps > 0) {
+    prepare(kt0);
+#pragma unroll
+    for (int v = 0; v < kLoads; ++v)
+      load_one(0, v);
+    if (steps > 1) {
+      prepare(kt0 + 1);
+#pragma unroll
+      for (int v = 0; v < kLoads; ++v)
+        load_one(1, v);
+      __builtin_amdgcn_s_waitcnt(waitcnt_imm(kLoads, kNoLgkm));
+    } else {
+      __builtin_amdgcn_s_waitcnt(waitcnt_imm(0, kNoLgkm));
+    }
+    if (is_tail(kt0)) {
+      zero_tail(0);
+      __builtin_amdgcn_s_waitcnt(waitcnt_imm(kNoVm, 0));
+    }
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int r = 0; r < kReads; ++r)
+      read_one(0, 0, Slot0{}, r);
+    int t = 0;
+    for (; t < steps - 2; ++t)
+      tile_step(t, std::true_type{}, std::true_type{});
+    if (steps > 1)
+      tile_step(t++, std::false_type{}, std::true_type{});
+    tile_step(t, std::false_type{}, std::false_type{});
+  }
+  // the epilogue may use the stages: every wave has read its last operands
+  __builtin_amdgcn_s_waitcnt(waitcnt_imm(kNoVm, 0));
+  __builtin_amdgcn_s_barrier();
+  epilogue(acc, tile, wave_m, wave_n, lane, lds);
 }
 
 // ---- stores ------------------------------------------------------------------
-// four consecutive columns n .. n + 3 of one row, as far as they exist
-template <class E>
-__device__ __forceinline__ void store4(E *row, int n, int N, bool vec, f32x4 v) {
-  typedef E ex4 __attribute__((ext_vector_type(4)));
-  if (vec && n + 3 < N) {
-    ex4 o;
+// The part of the result a workgroup stores: rows [m_lo, m_hi), columns [n_lo, n_hi).
+struct Window {
+  int m_lo, m_hi, n_lo, n_hi;
+};
+
+// four consecutive columns n .. n + 3 of one row, as far as they are in [lo, hi)
+template <class O> __device__ __forceinline__ void store4(O *row, int n, int lo, int hi, f32x4 v) {
+  typedef O ox4 __attribute__((ext_vector_type(4)));
+  typedef ox4 ox4_u __attribute__((aligned(1)));
+  ox4 o;
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
-      o[e] = (E)v[e];
-    *reinterpret_cast<ex4 *>(row + n) = o;
+  for (int e = 0; e < 4; ++e)
+    o[e] = (O)v[e];
+  if (n >= lo && n + 4 <= hi) {
+    *reinterpret_cast<ox4_u *>(row + n) = o;
   } else {
 #pragma unroll
     for (int e = 0; e < 4; ++e)
-      if (n + e < N)
-        row[n + e] = (E)v[e];
+      if (n + e >= lo && n + e < hi)
+        row[n + e] = o[e];
   }
-}
-template <class E> __device__ __forceinline__ bool can_store4(const void *p, size_t ld) {
-  return ld % 4 == 0 && reinterpret_cast<uintptr_t>(p) % (4 * sizeof(E)) == 0;
 }
 
-// C to `out` (element type) or `partial` (fp32)
-template <class E, int MI, int NI, int BN>
-__device__ __forceinline__ void store_tile(const StoreArgs &s, f32x4 (&acc)[MI][NI], int m0, int n0, int lane) {
-  const int M = s.mma.M, N = s.mma.N;
-  if (s.partial) {
-    const bool vec = can_store4<float>(s.partial, s.ldp);
-    float *base = s.partial + (size_t)blockIdx.y * M * s.ldp;
+// A wave's block of MI * 16 x NJ * 16 16-bit values through LDS (a region of the
+// wave's own, MI * NJ * 512 bytes), so that whole row segments are written with
+// 16-byte stores.  Chunk c of row r lies at c ^ (r & mask).  value(i, j): the lane's
+// four consecutive columns of block (i, j).
+template <class O, int MI, int NJ, class F>
+__device__ __forceinline__ void store_block(unsigned char *mine, O *out, size_t ld, int m0, int n0, const Window &w,
+                                            int lane, F &&value) {
+  typedef O ox4 __attribute__((ext_vector_type(4)));
+  constexpr int kRow = NJ * 32, kChunks = NJ * 2, kRows = kWave / kChunks;
 #pragma unroll
-    for (int i = 0; i < MI; ++i) {
-      const int m = m0 + i * 16 + lane % 16;
-      if (m >= M)
-        continue;
+  for (int i = 0; i < MI; ++i)
 #pragma unroll
-      for (int j = 0; j < NI; ++j) {
-        const int n = n0 + j * 16 + lane / 16 * 4;
-        float *row = base + (size_t)m * s.ldp;
-        f32x4 v = acc[i][j];
-        if (s.accumulate) {
+    for (int j = 0; j < NJ; ++j) {
+      const f32x4 v = value(i, j);
+      ox4 o;
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (n + e < N)
-              v[e] += row[n + e];
-        }
-        store4<float>(row, n, N, vec, v);
-      }
+      for (int e = 0; e < 4; ++e)
+        o[e] = (O)v[e];
+      const int r = i * 16 + lane % 16, c = 2 * j + lane / 32;
+      *reinterpret_cast<ox4 *>(mine + r * kRow + ((c ^ (r & (kChunks - 1))) * 16) + lane / 16 % 2 * 8) = o;
     }
-    return;
+  __builtin_amdgcn_s_waitcnt(waitcnt_imm(kNoVm, 0));
+#pragma unroll 4
+  for (int r0 = 0; r0 < MI * 16; r0 += kRows) {
+    const int r = r0 + lane / kChunks, c = lane % kChunks;
+    const u32x4 v = *reinterpret_cast<const u32x4 *>(mine + r * kRow + ((c ^ (r & (kChunks - 1))) * 16));
+    const int m = m0 + r, n = n0 + c * 8;
+    if (m < w.m_lo || m >= w.m_hi)
+      continue;
+    O *dst = out + (size_t)m * ld + n;
+    if (n >= w.n_lo && n + 8 <= w.n_hi) {
+      *reinterpret_cast<u32x4_u *>(dst) = v;
+    } else {
+      typedef O ox8 __attribute__((ext_vector_type(8)));
+      const ox8 o = __builtin_bit_cast(ox8, v);
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (n + e >= w.n_lo && n + e < w.n_hi)
+          dst[e] = o[e];
+    }
   }
-  const float by = s.undo ? *s.undo : 1.0f;
-  const bool vec = can_store4<E>(s.out, s.ldo);
+  __builtin_amdgcn_s_waitcnt(waitcnt_imm(kNoVm, 0)); // the region may be used again
+}
+
+// a wave's block straight from registers
+template <class O, int MI, int NJ, class F>
+__device__ __forceinline__ void store_direct(O *out, size_t ld, int m0, int n0, const Window &w, int lane, F &&value) {
 #pragma unroll
   for (int i = 0; i < MI; ++i) {
     const int m = m0 + i * 16 + lane % 16;
-    if (m >= M)
+    if (m < w.m_lo || m >= w.m_hi)
       continue;
 #pragma unroll
-    for (int j = 0; j < NI; ++j)
-      store4<E>(static_cast<E *>(s.out) + (size_t)m * s.ldo, n0 + j * 16 + lane / 16 * 4, N, vec, acc[i][j] * by);
+    for (int j = 0; j < NJ; ++j)
+      store4<O>(out + (size_t)m * ld, n0 + j * 16 + lane / 16 * 4, w.n_lo, w.n_hi, value(i, j));
   }
 }
+
+// C to `out` (element type) or `partial` (fp32; its rows are padded to a multiple of 8
+// and tiles begin at multiples of 8, so four columns are stored or not as a whole)
+template <class E, int MI, int NI, bool LDS>
+__device__ __forceinline__ void store_tile(const StoreArgs &s, f32x4 (&acc)[MI][NI], const Tile &t, int m0, int n0,
+                                           int lane, unsigned char *mine) {
+  if (s.partial) {
+    float *base = s.partial + (size_t)blockIdx.y * s.mma.M * s.ldp + n0 + lane / 16 * 4;
+    const int left = s.mma.N - n0 - lane / 16 * 4, skip = t.n_lo - n0 - lane / 16 * 4;
+#pragma unroll
+    for (int i = 0; i < MI; ++i) {
+      const int m = m0 + i * 16 + lane % 16;
+      if (m < t.m_lo || m >= s.mma.M)
+        continue;
+#pragma unroll
+      for (int j = 0; j < NI; ++j)
+        if (j * 16 < left && j * 16 >= skip)
+          *reinterpret_cast<f32x4 *>(base + (size_t)m * s.ldp + j * 16) = acc[i][j];
+    }
+    return;
+  }
+  const Window w = {t.m_lo, s.mma.M, t.n_lo, s.mma.N};
+  const float by = s.undo ? *s.undo : 1.0f;
+  auto value = [&](int i, int j) { return acc[i][j] * by; };
+  if constexpr (LDS)
+    store_block<E, MI, NI>(mine, static_cast<E *>(s.out), s.ldo, m0, n0, w, lane, value);
+  else
+    store_direct<E, MI, NI>(static_cast<E *>(s.out), s.ldo, m0, n0, w, lane, value);
+}
+// what the sums begin with: zero, or the partial sums of the calls before
+template <int MI, int NI>
+__device__ __forceinline__ void begin_tile(const StoreArgs &s, f32x4 (&acc)[MI][NI], int m0, int n0, int lane) {
+  if (!s.accumulate)
+    return;
+  const float *base = s.partial + (size_t)blockIdx.y * s.mma.M * s.ldp;
+#pragma unroll
+  for (int i = 0; i < MI; ++i) {
+    const float *row = base + (size_t)min(m0 + i * 16 + lane % 16, s.mma.M - 1) * s.ldp;
+#pragma unroll
+    for (int j = 0; j < NI; ++j) // (columns past the padded row are not stored)
+      acc[i][j] = *reinterpret_cast<const f32x4 *>(row + min(n0 + j * 16 + lane / 16 * 4, (int)s.ldp - 4));
+  }
+}
+struct FromZero {
+  template <class A> __device__ __forceinline__ void operator()(A &, const Tile &, int, int, int) const {}
+};
 
 } // namespace hcamd

@@ -24,22 +24,41 @@ __device__ __forceinline__ int64_t target_of(const void *targets, int is64, size
 // per-row statistics of a tile: lanes l, l + 16, l + 32, l + 48 hold one row's
 // columns; WN waves share the row and meet in LDS
 template <int MI, int NI, int WN, int BM, int BN>
-__device__ __forceinline__ void tile_stats(const XentArgs &a, f32x4 (&acc)[MI][NI], int tile_m0, int wave_m, int tn,
+__device__ __forceinline__ void tile_stats(const XentArgs &a, f32x4 (&acc)[MI][NI], const Tile &t, int wave_m,
                                            int wave_n, int lane, float *lds) {
   const int M = a.mma.M, N = a.mma.N;
   const int wn = wave_n / (NI * 16);
   float *slot_m = lds, *slot_s = lds + WN * BM; // [WN][BM] each
-  const int n0 = tn * BN + wave_n + lane / 16 * 4;
+  const int n0 = t.n0 + wave_n + lane / 16 * 4;
+  const bool whole = t.n0 >= t.n_lo && t.n0 + BN <= N;
 #pragma unroll
   for (int i = 0; i < MI; ++i) {
-    const int in_tile = wave_m + i * 16 + lane % 16, m = tile_m0 + in_tile;
+    const int in_tile = wave_m + i * 16 + lane % 16, m = t.m0 + in_tile;
+    if (m >= t.m_lo && m < M) {
+      const int64_t at = target_of(a.targets, a.target_i64, m) - n0;
+      if (at >= 0 && at < NI * 16) {
+#pragma unroll
+        for (int j = 0; j < NI; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (at == j * 16 + e && n0 + j * 16 + e >= t.n_lo && n0 + j * 16 + e < N)
+              a.zt[m] = acc[i][j][e];
+      }
+    }
+    if (!whole) { // columns past the last, or a neighbour's, take no part
+#pragma unroll
+      for (int j = 0; j < NI; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (n0 + j * 16 + e < t.n_lo || n0 + j * 16 + e >= N)
+            acc[i][j][e] = -INFINITY;
+    }
     float most = -INFINITY;
 #pragma unroll
     for (int j = 0; j < NI; ++j)
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        if (n0 + j * 16 + e < N)
-          most = fmaxf(most, acc[i][j][e]);
+        most = fmaxf(most, acc[i][j][e]);
     most = fmaxf(most, __shfl_xor(most, 16));
     most = fmaxf(most, __shfl_xor(most, 32));
     // a row of -infinities: subtract 0, every term is then 0
@@ -49,19 +68,9 @@ __device__ __forceinline__ void tile_stats(const XentArgs &a, f32x4 (&acc)[MI][N
     for (int j = 0; j < NI; ++j)
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        if (n0 + j * 16 + e < N)
-          sum += __expf(acc[i][j][e] - from);
+        sum += __expf(acc[i][j][e] - from);
     sum += __shfl_xor(sum, 16);
     sum += __shfl_xor(sum, 32);
-    if (m < M) {
-      const int64_t at = target_of(a.targets, a.target_i64, m) - n0;
-#pragma unroll
-      for (int j = 0; j < NI; ++j)
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (at == j * 16 + e && n0 + j * 16 + e < N)
-            a.zt[m] = acc[i][j][e];
-    }
     if (lane < 16) {
       slot_m[wn * BM + in_tile] = most;
       slot_s[wn * BM + in_tile] = sum;
@@ -69,8 +78,8 @@ __device__ __forceinline__ void tile_stats(const XentArgs &a, f32x4 (&acc)[MI][N
   }
   __syncthreads();
   for (int r = threadIdx.x; r < BM; r += blockDim.x) {
-    const int m = tile_m0 + r;
-    if (m >= M)
+    const int m = t.m0 + r;
+    if (m < t.m_lo || m >= M)
       continue;
     float most = slot_m[r];
 #pragma unroll
@@ -81,7 +90,7 @@ __device__ __forceinline__ void tile_stats(const XentArgs &a, f32x4 (&acc)[MI][N
 #pragma unroll
     for (int w = 0; w < WN; ++w)
       sum += slot_s[w * BM + r] * __expf(slot_m[w * BM + r] - from);
-    float *cell = a.stats + ((size_t)m * a.tiles + tn) * 2;
+    float *cell = a.stats + ((size_t)m * a.tiles + t.tn) * 2;
     cell[0] = most;
     cell[1] = sum;
   }
@@ -90,46 +99,77 @@ __device__ __forceinline__ void tile_stats(const XentArgs &a, f32x4 (&acc)[MI][N
 template <class E> __device__ __forceinline__ void stats_general(const XentArgs &a) {
   __shared__ __attribute__((aligned(1024))) unsigned char lds[4 * 128 * 128];
   mma_general<E, kKFast, kKFast, false>(
-      a.mma, lds, [&](auto &acc, int m0, int wave_m, int tn, int wave_n, int lane, unsigned char *l) {
+      a.mma, lds, FromZero{}, [&](auto &acc, const Tile &t, int wave_m, int wave_n, int lane, unsigned char *l) {
         // (the main loop ends with a barrier: its stages are free)
-        tile_stats<4, 4, 2, 128, 128>(a, acc, m0, wave_m, tn, wave_n, lane, reinterpret_cast<float *>(l));
+        tile_stats<4, 4, 2, 128, 128>(a, acc, t, wave_m, wave_n, lane, reinterpret_cast<float *>(l));
       });
 }
 
-// p of a tile, from registers
-template <class E, int MI, int NI>
-__device__ __forceinline__ void tile_p(const XentArgs &a, f32x4 (&acc)[MI][NI], int m0, int n0, int lane) {
-  const int M = a.mma.M, N = a.mma.N;
+template <class E, int B, int WM, int WN> __device__ __forceinline__ void stats_tile(const XentArgs &a) {
+  constexpr int MI = B / WM / 16, NI = B / WN / 16;
+  __shared__ __attribute__((aligned(1024))) unsigned char lds[pipelined_lds<B, B>()];
+  mma_pipelined<E, kKFast, kKFast, false, B, B, WM, WN>(
+      a.mma, lds, FromZero{}, [&](auto &acc, const Tile &t, int wave_m, int wave_n, int lane, unsigned char *l) {
+        tile_stats<MI, NI, WN, B, B>(a, acc, t, wave_m, wave_n, lane, reinterpret_cast<float *>(l));
+      });
+}
+
+// p of a tile; the columns up to the next multiple of 8 become zeros (the products
+// that read p take it in pieces of 8)
+template <class E, int MI, int NI, bool LDS>
+__device__ __forceinline__ void tile_p(const XentArgs &a, f32x4 (&acc)[MI][NI], const Tile &tile, int m0, int n0,
+                                       int lane, unsigned char *mine) {
+  const int M = a.mma.M, N = a.mma.N, padded = (N + 7) & ~7;
   const float factor = *a.factor;
-  const bool vec = can_store4<E>(a.p, a.ldp);
 #pragma unroll
   for (int i = 0; i < MI; ++i) {
-    const int m = m0 + i * 16 + lane % 16;
-    if (m >= M)
-      continue;
+    const int m = min(m0 + i * 16 + lane % 16, M - 1);
     const int64_t t = target_of(a.targets, a.target_i64, m);
     const bool live = t >= 0 && t < a.vocab;
     const float g = live ? a.grad_loss[m] * factor : 0.0f, lse = a.lse[m];
 #pragma unroll
     for (int j = 0; j < NI; ++j) {
       const int n = n0 + j * 16 + lane / 16 * 4;
-      f32x4 p;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const float hot = t - a.v0 == n + e ? 1.0f : 0.0f;
         // a row without a target: 0, whatever its logits are
-        p[e] = live ? (__expf(acc[i][j][e] - lse) - hot) * g : 0.0f;
+        acc[i][j][e] = live && n + e < N ? (__expf(acc[i][j][e] - lse) - hot) * g : 0.0f;
       }
-      store4<E>(static_cast<E *>(a.p) + (size_t)m * a.ldp, n, N, vec, p);
     }
   }
+  const Window w = {tile.m_lo, M, tile.n_lo, N};
+  // the padding is written by the lanes of the tile that holds the last column
+  if (n0 < N && n0 + NI * 16 >= N && N < padded) {
+#pragma unroll
+    for (int i = 0; i < MI; ++i) {
+      const int m = m0 + i * 16 + lane % 16;
+      if (m >= tile.m_lo && m < M)
+        for (int n = N + lane / 16; n < padded; n += 4)
+          static_cast<E *>(a.p)[(size_t)m * a.ldp + n] = (E)0.0f;
+    }
+  }
+  auto value = [&](int i, int j) { return acc[i][j]; };
+  if constexpr (LDS)
+    store_block<E, MI, NI>(mine, static_cast<E *>(a.p), a.ldp, m0, n0, w, lane, value);
+  else
+    store_direct<E, MI, NI>(static_cast<E *>(a.p), a.ldp, m0, n0, w, lane, value);
 }
 
 template <class E> __device__ __forceinline__ void p_general(const XentArgs &a) {
   __shared__ __attribute__((aligned(1024))) unsigned char lds[4 * 128 * 128];
   mma_general<E, kKFast, kKFast, false>(
-      a.mma, lds, [&](auto &acc, int m0, int wave_m, int tn, int wave_n, int lane, unsigned char *) {
-        tile_p<E, 4, 4>(a, acc, m0 + wave_m, tn * 128 + wave_n, lane);
+      a.mma, lds, FromZero{}, [&](auto &acc, const Tile &t, int wave_m, int wave_n, int lane, unsigned char *) {
+        tile_p<E, 4, 4, false>(a, acc, t, t.m0 + wave_m, t.n0 + wave_n, lane, nullptr);
+      });
+}
+template <class E, int B, int WM, int WN> __device__ __forceinline__ void p_tile(const XentArgs &a) {
+  constexpr int MI = B / WM / 16, NI = B / WN / 16;
+  __shared__ __attribute__((aligned(1024))) unsigned char lds[pipelined_lds<B, B>()];
+  mma_pipelined<E, kKFast, kKFast, false, B, B, WM, WN>(
+      a.mma, lds, FromZero{}, [&](auto &acc, const Tile &t, int wave_m, int wave_n, int lane, unsigned char *l) {
+        tile_p<E, MI, NI, true>(a, acc, t, t.m0 + wave_m, t.n0 + wave_n, lane,
+                                l + (wave_m / (MI * 16) * WN + wave_n / (NI * 16)) * (MI * NI * 512));
       });
 }
 
@@ -184,6 +224,18 @@ __device__ __forceinline__ void p_factor(const float *grad_loss, uint32_t rows, 
   }                                                                                                       \
   extern "C" __global__ __launch_bounds__(256) void hcamd_xent_p_##SUFFIX##_general(XentArgs a) {         \
     p_general<E>(a);                                                                                      \
+  }                                                                                                       \
+  extern "C" __global__ __launch_bounds__(512) void hcamd_xent_stats_##SUFFIX##_t256(XentArgs a) {        \
+    stats_tile<E, 256, 2, 4>(a);                                                                          \
+  }                                                                                                       \
+  extern "C" __global__ __launch_bounds__(256) void hcamd_xent_stats_##SUFFIX##_t128(XentArgs a) {        \
+    stats_tile<E, 128, 2, 2>(a);                                                                          \
+  }                                                                                                       \
+  extern "C" __global__ __launch_bounds__(512) void hcamd_xent_p_##SUFFIX##_t256(XentArgs a) {            \
+    p_tile<E, 256, 2, 4>(a);                                                                              \
+  }                                                                                                       \
+  extern "C" __global__ __launch_bounds__(256) void hcamd_xent_p_##SUFFIX##_t128(XentArgs a) {            \
+    p_tile<E, 128, 2, 2>(a);                                                                              \
   }
 HCAMD_XENT(bf16, __bf16)
 HCAMD_XENT(f16, _Float16)

@@ -81,26 +81,56 @@ struct Call {
 };
 
 // ---- tiled products -----------------------------------------------------------
-// How many workgroups share the k tiles of an output tile: as many as bring the
-// launch to about one workgroup per compute unit, each with at least 8 k tiles, and
-// no more than 64 MiB of fp32 partial sums.
+// Tile and splits of a product, from its shape alone (a workspace is sized before any
+// pointer is seen).  256 x 256 tiles run one workgroup on a compute unit, 128 x 128
+// tiles two.  When the tiles do not fill the card, several workgroups share the k
+// tiles of each, each with at least 8 of them, and no more than 64 MiB of fp32 partial
+// sums in all.
 struct Product {
-  size_t tilesM, tilesN;
+  int tile; // 256 or 128
   int splits;
 };
 size_t padCols(size_t n) { return alignUp(n, 8); }
+int tileOf(size_t m, size_t n) {
+  const int v = hcamdInternalVariant("mma");
+  if (v == 2 || v == 3)
+    return v == 3 && m >= 256 && n >= 256 ? 256 : 128;
+  return m >= 256 && n >= 256 && ceilDiv(m, 256) * ceilDiv(n, 256) >= 192 ? 256 : 128;
+}
 Product productOf(size_t m, size_t n, size_t k, int segments) {
   Product p;
-  p.tilesM = ceilDiv(m, (size_t)128);
-  p.tilesN = ceilDiv(n, (size_t)128);
-  const size_t tiles = p.tilesM * p.tilesN, kTiles = ceilDiv(k, (size_t)64) * segments;
-  size_t s = std::min<size_t>(256 / std::max<size_t>(tiles, 1), kTiles / 8);
+  p.tile = tileOf(m, n);
+  const size_t tiles = ceilDiv(m, p.tile) * ceilDiv(n, p.tile), kTiles = ceilDiv(k, (size_t)64) * segments;
+  size_t s = std::min<size_t>((p.tile == 256 ? 256 : 512) / std::max<size_t>(tiles, 1), kTiles / 8);
   s = std::min(s, ((size_t)64 << 20) / std::max<size_t>(m * padCols(n) * 4, 1));
   p.splits = (int)std::max<size_t>(s, 1);
   return p;
 }
 size_t partialBytes(const Product &p, size_t m, size_t n) {
   return p.splits > 1 ? alignUp((size_t)p.splits * m * padCols(n) * 4, 256) : 0;
+}
+
+// Whether the pipelined kernels can fetch an operand: 16-byte pieces, offsets inside a
+// tile below 2^31.  `along` is its extent in the direction that runs through memory
+// (k for a k-fast operand, its rows for a k-slow one); the library's own buffers are
+// padded there.
+bool fetchable(const void *p, size_t ld, size_t along, size_t bytes, bool padded) {
+  const size_t piece = 16 / bytes;
+  return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % piece == 0 && (padded || along % piece == 0) &&
+         ld * bytes < ((size_t)1 << 23);
+}
+// The kernel of a product: "general", "t128" or "t256"; `threads` and the tile it uses.
+struct Kernel {
+  const char *suffix;
+  size_t threads;
+  int tile;
+};
+Kernel kernelOf(int tile, size_t m, size_t n, bool fetch) {
+  if (!fetch || hcamdInternalVariant("mma") == 1 || m < 128 || n < 128)
+    return {"general", 256, 128};
+  if (tile == 256)
+    return {"t256", 512, 256};
+  return {"t128", 256, 128};
 }
 
 int launchFold(const Call &c, int type, const FoldArgs &f) {
@@ -281,9 +311,13 @@ int hcamdLaunchGatedFfn(OlQueue q, int elemType, const void *x, size_t ldx, cons
   a.x_scale = xScale, a.gate_scale = gateScale, a.up_scale = upScale;
   a.out = out, a.gate = gate, a.up = up, a.ldo = ldo, a.ldgate = ldgate, a.ldup = ldup;
   a.activation = activation, a.out_f16 = outType == HCAMD_F16;
+  // (a tile of outputs takes twice its columns of the two weight matrices)
+  const Kernel k = kernelOf(tileOf(tokens, 2 * f), tokens, 2 * f,
+                            fetchable(x, ldx, d, e, false) && fetchable(wGate, ldwg, d, e, false) &&
+                                fetchable(wUp, ldwu, d, e, false));
   char name[64];
-  std::snprintf(name, sizeof(name), "hcamd_gated_%s_general", typeName(elemType));
-  return c.launch("ffn", name, a, ceilDiv(tokens, 128) * ceilDiv(f, 64));
+  std::snprintf(name, sizeof(name), "hcamd_gated_%s_%s", typeName(elemType), k.suffix);
+  return c.launch("ffn", name, a, ceilDiv(tokens, k.tile) * ceilDiv(f, k.tile / 2), 1, 1, k.threads);
 }
 
 namespace {
@@ -362,8 +396,10 @@ int hcamdLaunchGatedFfnBackward(OlQueue q, int elemType, const void *gradOut, si
     s.mma.M = (int)tokens, s.mma.N = (int)d, s.mma.K = (int)f, s.mma.segments = 2, s.mma.splits = b.px.splits;
     s.out = gradX, s.ldo = ldgx, s.ldp = padCols(d);
     s.partial = b.dx ? reinterpret_cast<float *>(w + 2 * b.dg) : nullptr;
-    std::snprintf(name, sizeof(name), "hcamd_product_nn_%s_general", typeName(elemType));
-    if (c.launch("ffn", name, s, b.px.tilesM * b.px.tilesN, b.px.splits))
+    const Kernel k = kernelOf(b.px.tile, tokens, d, fetchable(wGate, ldwg, d, 2, false) &&
+                                                        fetchable(wUp, ldwu, d, 2, false));
+    std::snprintf(name, sizeof(name), "hcamd_product_nn_%s_%s", typeName(elemType), k.suffix);
+    if (c.launch("ffn", name, s, ceilDiv(tokens, k.tile) * ceilDiv(d, k.tile), b.px.splits, 1, k.threads))
       return 1;
     if (s.partial && launchFold(c, elemType, {s.partial, gradX, s.ldp, ldgx, (uint32_t)tokens, (uint32_t)d,
                                               (uint32_t)b.px.splits, nullptr}))
@@ -384,8 +420,9 @@ int hcamdLaunchGatedFfnBackward(OlQueue q, int elemType, const void *gradOut, si
       t.partial = b.dw ? reinterpret_cast<float *>(w + 2 * b.dg + b.dx + n * b.dw) : nullptr;
       ++n;
     }
-    std::snprintf(name, sizeof(name), "hcamd_product_tn_%s_general", typeName(elemType));
-    if (c.launch("ffn", name, s, b.pw.tilesM * b.pw.tilesN, b.pw.splits, n))
+    const Kernel k = kernelOf(b.pw.tile, f, d, fetchable(x, ldx, d, 2, false));
+    std::snprintf(name, sizeof(name), "hcamd_product_tn_%s_%s", typeName(elemType), k.suffix);
+    if (c.launch("ffn", name, s, ceilDiv(f, k.tile) * ceilDiv(d, k.tile), b.pw.splits, n, k.threads))
       return 1;
     for (size_t k = 0; b.dw && k < n; ++k)
       if (launchFold(c, elemType, {s.p[k].partial, s.p[k].out, s.p[k].ldp, s.p[k].ldo, (uint32_t)f, (uint32_t)d,
@@ -436,12 +473,14 @@ int hcamdLaunchLinearCrossEntropy(OlQueue q, int elemType, const void *x, size_t
   a.mma.a[0] = x, a.mma.lda[0] = ldx, a.mma.b[0] = weight, a.mma.ldb[0] = ldw;
   a.mma.M = (int)tokens, a.mma.N = (int)vocab, a.mma.K = (int)d, a.mma.segments = a.mma.splits = 1;
   a.targets = targets, a.target_i64 = targetType == HCAMD_I64, a.vocab = (int)vocab;
-  a.tiles = (int)ceilDiv(vocab, kStatsCols);
+  const Kernel k = kernelOf(tileOf(tokens, vocab), tokens, vocab,
+                            fetchable(x, ldx, d, 2, false) && fetchable(weight, ldw, d, 2, false));
+  a.tiles = (int)ceilDiv(vocab, k.tile);
   a.stats = static_cast<float *>(work);
   a.zt = a.stats + tokens * a.tiles * 2;
   char name[64];
-  std::snprintf(name, sizeof(name), "hcamd_xent_stats_%s_general", typeName(elemType));
-  if (c.launch("xent", name, a, ceilDiv(tokens, 128) * a.tiles))
+  std::snprintf(name, sizeof(name), "hcamd_xent_stats_%s_%s", typeName(elemType), k.suffix);
+  if (c.launch("xent", name, a, ceilDiv(tokens, k.tile) * a.tiles, 1, 1, k.threads))
     return 1;
   XentRowsArgs r{a.stats, a.zt, targets, a.target_i64, loss, lse, (uint32_t)tokens, (uint32_t)vocab,
                  (uint32_t)a.tiles};
@@ -521,16 +560,18 @@ int hcamdLaunchLinearCrossEntropyBackward(OlQueue q, int elemType, const void *x
     a.mma.M = (int)tokens, a.mma.N = (int)n, a.mma.K = (int)d, a.mma.segments = a.mma.splits = 1;
     a.targets = targets, a.target_i64 = targetType == HCAMD_I64, a.v0 = (int)v0, a.vocab = (int)vocab;
     a.lse = lse, a.grad_loss = gradLoss, a.factor = factor, a.p = w + 256, a.ldp = b.ldp;
-    std::snprintf(name, sizeof(name), "hcamd_xent_p_%s_general", typeName(elemType));
-    if (tokens && c.launch("xent", name, a, ceilDiv(tokens, 128) * ceilDiv(n, 128)))
+    Kernel k = kernelOf(tileOf(tokens, n), tokens, n, fetchable(x, ldx, d, 2, false) && fetchable(rows, ldw, d, 2, false));
+    std::snprintf(name, sizeof(name), "hcamd_xent_p_%s_%s", typeName(elemType), k.suffix);
+    if (tokens && c.launch("xent", name, a, ceilDiv(tokens, k.tile) * ceilDiv(n, k.tile), 1, 1, k.threads))
       return 1;
     if (gradX) {
       StoreArgs s{};
       s.mma.a[0] = a.p, s.mma.lda[0] = b.ldp, s.mma.b[0] = rows, s.mma.ldb[0] = ldw;
       s.mma.M = (int)tokens, s.mma.N = (int)d, s.mma.K = (int)n, s.mma.segments = 1, s.mma.splits = b.px.splits;
       s.partial = dx, s.ldp = padCols(d), s.accumulate = v0 != 0;
-      std::snprintf(name, sizeof(name), "hcamd_product_nn_%s_general", typeName(elemType));
-      if (c.launch("ffn", name, s, b.px.tilesM * b.px.tilesN, b.px.splits))
+      k = kernelOf(b.px.tile, tokens, d, fetchable(rows, ldw, d, 2, false));
+      std::snprintf(name, sizeof(name), "hcamd_product_nn_%s_%s", typeName(elemType), k.suffix);
+      if (c.launch("ffn", name, s, ceilDiv(tokens, k.tile) * ceilDiv(d, k.tile), b.px.splits, 1, k.threads))
         return 1;
     }
     if (gradWeight) {
@@ -540,8 +581,9 @@ int hcamdLaunchLinearCrossEntropyBackward(OlQueue q, int elemType, const void *x
       t.mma.M = (int)n, t.mma.N = (int)d, t.mma.K = (int)tokens, t.mma.segments = 1, t.mma.splits = b.pw.splits;
       t.out = static_cast<char *>(gradWeight) + v0 * ldgw * 2, t.ldo = ldgw, t.undo = undo;
       t.partial = b.dw ? reinterpret_cast<float *>(w + 256 + b.p + b.dx) : nullptr, t.ldp = padCols(d);
-      std::snprintf(name, sizeof(name), "hcamd_product_tn_%s_general", typeName(elemType));
-      if (c.launch("ffn", name, s, ceilDiv(n, 128) * b.pw.tilesN, b.pw.splits))
+      k = kernelOf(n >= 256 ? b.pw.tile : 128, n, d, fetchable(x, ldx, d, 2, false));
+      std::snprintf(name, sizeof(name), "hcamd_product_tn_%s_%s", typeName(elemType), k.suffix);
+      if (c.launch("ffn", name, s, ceilDiv(n, k.tile) * ceilDiv(d, k.tile), b.pw.splits, 1, k.threads))
         return 1;
       if (b.dw && launchFold(c, elemType, {t.partial, t.out, t.ldp, ldgw, (uint32_t)n, (uint32_t)d,
                                            (uint32_t)b.pw.splits, undo}))

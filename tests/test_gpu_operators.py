@@ -766,3 +766,72 @@ def test_refusals_on_the_device():
         p.launch(sync=True)
     torch.cuda.synchronize()
     assert bool((out == 77).all())
+
+
+# ---------------------------------------------------------------------------
+# every kernel of the products on the same shapes
+# ---------------------------------------------------------------------------
+@pytest.fixture(params=[1, 2, 3], ids=["general", "t128", "t256"])
+def product_kernel(request):
+    rt.set_variant("mma", request.param)
+    yield request.param
+    rt.set_variant("mma", 0)
+
+
+# whole tiles; edges in every direction; k tiles of one, two, three and with every kind of tail (k is d forward, f
+# and t backward)
+TILED = [(256, 64, 256), (512, 128, 512), (257, 200, 264), (300, 328, 391), (1000, 136, 520), (384, 1032, 777), (263, 256, 1001)]
+
+
+@pytest.mark.parametrize("layout", ["dense", "strided"])
+@pytest.mark.parametrize("shape", TILED, ids=str)
+@pytest.mark.parametrize("ty", ["f16", "bf16"])
+def test_block_on_every_kernel(product_kernel, ty, shape, layout):
+    test_gated_ffn(ty, shape, layout)
+    test_gated_ffn_backward(ty, shape, layout)
+
+
+@pytest.mark.parametrize("shape", TILED, ids=str)
+def test_block_int8_on_every_kernel(product_kernel, shape):
+    t, d, f = shape
+    test_gated_ffn_int8("bf16", (t, d // 16 * 16, f), "dense")
+    test_gated_ffn_int8("f16", (t, d // 16 * 16, f), "strided")
+
+
+@pytest.mark.parametrize("layout", ["dense", "strided", "odd"])
+@pytest.mark.parametrize("shape", TILED, ids=str)
+@pytest.mark.parametrize("ty", ["f16", "bf16"])
+def test_cross_entropy_on_every_kernel(product_kernel, ty, shape, layout):
+    test_linear_cross_entropy(ty, shape, layout)
+    test_linear_cross_entropy_backward(ty, shape, layout)
+
+
+def test_poisoned_surroundings(product_kernel):
+    """NaN around every operand and output: nothing outside the windows is read into a result or written."""
+    t, d, f, k = 300, 264, 520, torch.bfloat16
+
+    def framed(x, pad=24):
+        wide = torch.full((x.shape[0] + 2, x.shape[1] + pad), float("nan"), device="cuda", dtype=x.dtype)
+        view = wide[1:-1, 8:8 + x.shape[1]]
+        view.copy_(x)
+        return view
+    x, wg, wu = ffn_inputs(t, d, f, k)
+    dh = dev(normal(8, t, f), k)
+    plain, framed_out = [], []
+    for wrap, results in ((lambda v: v, plain), (framed, framed_out)):
+        out, gate, up = (wrap(empty(t, f, ty=k)) for _ in range(3))
+        gx, gg, gu = wrap(empty(t, d, ty=k)), wrap(empty(f, d, ty=k)), wrap(empty(f, d, ty=k))
+        xs, a, b, g = wrap(x), wrap(wg), wrap(wu), wrap(dh)
+        rt.gated_ffn(xs, a, b, out, gate=gate, up=up)
+        rt.gated_ffn_backward(g, xs, a, b, gate, up, gx, gg, gu)
+        targets = (torch.arange(t) % f).cuda()
+        loss, lse = empty(t, ty=torch.float32), empty(t, ty=torch.float32)
+        cx, cw = wrap(empty(t, d, ty=k)), wrap(empty(f, d, ty=k))
+        rt.linear_cross_entropy(xs, a, targets, loss, lse)
+        rt.linear_cross_entropy_backward(xs, a, targets, lse, torch.ones(t, device="cuda"), cx, cw, piece=264)
+        results += [out, gate, up, gx, gg, gu, loss, lse, cx, cw]
+    for a, b in zip(plain, framed_out):
+        assert torch.equal(a, b)
+        if b._base is not None:
+            inside = int(torch.isnan(b._base).sum())
+            assert inside == b._base.numel() - b.numel()
