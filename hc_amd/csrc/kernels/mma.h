@@ -19,6 +19,7 @@
 #pragma once
 #include "common.h"
 #include "op_args.h"
+#include "pieces.h"
 
 #include <type_traits>
 
@@ -29,7 +30,6 @@ enum Layout { kKFast = 0, kKSlow = 1 };
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
-typedef u32x4 u32x4_u __attribute__((aligned(1)));
 typedef __attribute__((address_space(3))) s16x4 *lds_s16x4_ptr;
 
 template <class E> struct MmaType {
@@ -76,30 +76,6 @@ __device__ __forceinline__ void split_of(int all, int splits, int &kt0, int &kt1
   const int split = blockIdx.y, each = all / splits, more = all % splits;
   kt0 = __builtin_amdgcn_readfirstlane(split * each + min(split, more));
   kt1 = __builtin_amdgcn_readfirstlane(kt0 + each + (split < more ? 1 : 0));
-}
-
-// 16 bytes of which the first `valid` elements exist; the rest reads as zero.
-template <class E> __device__ __forceinline__ u32x4 load_chunk(const E *p, int valid) {
-  constexpr int n = 16 / (int)sizeof(E);
-  if (valid >= n)
-    return *reinterpret_cast<const u32x4_u *>(p);
-  u32x4 v = {0u, 0u, 0u, 0u};
-  if (valid <= 0)
-    return v;
-  if constexpr (sizeof(E) == 2) {
-    const uint16_t *s = reinterpret_cast<const uint16_t *>(p);
-#pragma unroll
-    for (int e = 0; e < n; ++e)
-      if (e < valid)
-        v[e / 2] |= (uint32_t)s[e] << (16 * (e % 2));
-  } else {
-    const uint8_t *s = reinterpret_cast<const uint8_t *>(p);
-#pragma unroll
-    for (int e = 0; e < n; ++e)
-      if (e < valid)
-        v[e / 4] |= (uint32_t)s[e] << (8 * (e % 4));
-  }
-  return v;
 }
 
 __device__ __forceinline__ int slow_swizzle(int k) { return (k & 3) | ((k >> 3 & 1) << 2); }

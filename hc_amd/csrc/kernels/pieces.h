@@ -1,0 +1,56 @@
+// Rows in 16-byte pieces at any alignment.  gfx950 serves 16-byte accesses at every
+// address; a piece that crosses the end of its row goes element by element.
+#pragma once
+#include "common.h"
+
+namespace hcamd {
+
+typedef u32x4 u32x4_u __attribute__((aligned(1)));
+typedef u32x2 u32x2_u __attribute__((aligned(1)));
+
+// 16 bytes of which the first `valid` elements exist; the rest reads as zero.
+template <class E> __device__ __forceinline__ u32x4 load_chunk(const E *p, int valid) {
+  constexpr int n = 16 / (int)sizeof(E);
+  if (valid >= n)
+    return *reinterpret_cast<const u32x4_u *>(p);
+  u32x4 v = {0u, 0u, 0u, 0u};
+  if (valid <= 0)
+    return v;
+  if constexpr (sizeof(E) == 2) {
+    const uint16_t *s = reinterpret_cast<const uint16_t *>(p);
+#pragma unroll
+    for (int e = 0; e < n; ++e)
+      if (e < valid)
+        v[e / 2] |= (uint32_t)s[e] << (16 * (e % 2));
+  } else if constexpr (sizeof(E) == 4) {
+    const uint32_t *s = reinterpret_cast<const uint32_t *>(p);
+#pragma unroll
+    for (int e = 0; e < n; ++e)
+      if (e < valid)
+        v[e] = s[e];
+  } else {
+    const uint8_t *s = reinterpret_cast<const uint8_t *>(p);
+#pragma unroll
+    for (int e = 0; e < n; ++e)
+      if (e < valid)
+        v[e / 4] |= (uint32_t)s[e] << (8 * (e % 4));
+  }
+  return v;
+}
+
+// the first `valid` of the elements of 16 bytes
+template <class E> __device__ __forceinline__ void store_chunk(E *p, u32x4 v, int valid) {
+  constexpr int n = 16 / (int)sizeof(E);
+  typedef E exn __attribute__((ext_vector_type(n)));
+  if (valid >= n) {
+    *reinterpret_cast<u32x4_u *>(p) = v;
+    return;
+  }
+  const exn e = __builtin_bit_cast(exn, v);
+#pragma unroll
+  for (int i = 0; i < n; ++i)
+    if (i < valid)
+      p[i] = e[i];
+}
+
+} // namespace hcamd

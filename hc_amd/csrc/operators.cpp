@@ -150,6 +150,37 @@ bool dimsOk(const Call &c, size_t a, size_t b, size_t d) {
 
 } // namespace
 
+namespace {
+// The kernel of a row length: the fewest 16-byte pieces a lane, and lanes a row, that
+// hold it.  A wave to a row needs no barrier; longer rows take 256 lanes or more, where a
+// row's latency is shared.  Rows beyond 512 lanes x 4 pieces (fp32: 1024 x 4) are read
+// twice by the general kernel.
+struct RowKernel {
+  const char *suffix;
+  size_t lanes, threads;
+  bool general;
+};
+RowKernel rowKernel(int type, size_t cols) {
+  static const RowKernel kernels[] = {{"r64v1", 64, 256, false},   {"r64v2", 64, 256, false},
+                                      {"r256v1", 256, 256, false}, {"r256v2", 256, 256, false},
+                                      {"r256v4", 256, 256, false}, {"r512v4", 512, 512, false},
+                                      {"r1024v4", 1024, 1024, false}};
+  static const size_t pieces[] = {64, 128, 256, 512, 1024, 2048, 4096};
+  const size_t need = ceilDiv(cols, 16 / elemBytes(type));
+  if (hcamdInternalVariant("rmsnorm") != 1)
+    for (int i = 0; i < (type == HCAMD_F32 ? 7 : 6); ++i)
+      if (need <= pieces[i])
+        return kernels[i];
+  return {"general", 256, 256, true};
+}
+// workgroups walk the rows: as many as fill the card
+size_t rowGroups(OlQueue q, const RowKernel &k, size_t rows) {
+  if (k.general)
+    return std::min<size_t>(rows, 0x7fffff);
+  return std::min(ceilDiv(rows, k.threads / k.lanes), (size_t)hcamdInternalComputeUnits(q) * 2048 / k.threads);
+}
+} // namespace
+
 extern "C" {
 
 // ===========================================================================
@@ -189,25 +220,22 @@ int hcamdLaunchAddRmsNorm(OlQueue q, int elemType, const void *x, size_t ldx, co
   a.ldx = ldx, a.ldr = ldr, a.lds = lds, a.ldo = ldo;
   a.rows = (uint32_t)rows, a.cols = (uint32_t)cols, a.eps = eps;
   a.weight_f32 = !weight || weightType == HCAMD_F32;
+  const RowKernel k = rowKernel(elemType, cols);
   char name[64];
-  std::snprintf(name, sizeof(name), "hcamd_rmsnorm_%s%s_general", typeName(elemType), outType == HCAMD_I8 ? "_i8" : "");
-  return c.launch("rmsnorm", name, a, std::min<size_t>(rows, 0x7fffff));
+  std::snprintf(name, sizeof(name), "hcamd_rmsnorm_%s%s_%s", typeName(elemType), outType == HCAMD_I8 ? "_i8" : "",
+                k.suffix);
+  return c.launch("rmsnorm", name, a, rowGroups(q, k, rows), 1, 1, k.threads);
 }
 
 namespace {
-void normBands(size_t rows, size_t &bands, size_t &band) {
-  bands = std::min<size_t>(256, ceilDiv(rows, 16));
-  band = ceilDiv(rows, std::max<size_t>(bands, 1));
-  bands = ceilDiv(rows, std::max<size_t>(band, 1));
-}
+// lines of partial sums of the weight's gradient: enough workgroups to fill the card
+size_t normBands(size_t rows) { return std::min<size_t>(rows, 512); }
 } // namespace
 
 size_t hcamdAddRmsNormBackwardWorkspace(size_t rows, size_t cols) noexcept {
   if (rows == 0 || rows > kMaxDim || cols > kMaxDim)
     return 0;
-  size_t bands, band;
-  normBands(rows, bands, band);
-  return bands * cols * 4;
+  return normBands(rows) * cols * 4;
 }
 
 int hcamdLaunchAddRmsNormBackward(OlQueue q, int elemType, const void *gradOut, size_t ldg, const void *summed,
@@ -240,27 +268,31 @@ int hcamdLaunchAddRmsNormBackward(OlQueue q, int elemType, const void *gradOut, 
   a.grad_in = gradIn, a.grad_weight = gradWeight, a.partial = static_cast<float *>(work);
   a.ldg = ldg, a.ldh = lds, a.ldgs = ldgs, a.ldgi = ldgi;
   a.rows = (uint32_t)rows, a.cols = (uint32_t)cols, a.weight_f32 = weightType == HCAMD_F32;
-  size_t bands = 0, band = 0;
-  normBands(rows, bands, band);
-  a.band = (uint32_t)band, a.bands = (uint32_t)bands;
+  const RowKernel k = rowKernel(elemType, cols);
+  const size_t lines = normBands(rows);
   char name[64];
-  // the weight's gradient first: grad_in may be grad_out
-  if (gradWeight) {
-    if (c.work(work, workBytes, hcamdAddRmsNormBackwardWorkspace(rows, cols)))
+  if (gradWeight && c.work(work, workBytes, hcamdAddRmsNormBackwardWorkspace(rows, cols)))
+    return 1;
+  if (k.general) {
+    // the weight's gradient first: grad_in may be grad_out
+    a.band = (uint32_t)ceilDiv(rows, std::max<size_t>(lines, 1));
+    a.bands = rows ? (uint32_t)ceilDiv(rows, a.band) : 0;
+    std::snprintf(name, sizeof(name), "hcamd_rmsnorm_back_weight_%s_general", typeName(elemType));
+    if (gradWeight && rows && c.launch("rmsnorm", name, a, ceilDiv(cols, 256), a.bands))
       return 1;
-    if (rows) {
-      std::snprintf(name, sizeof(name), "hcamd_rmsnorm_back_weight_%s_general", typeName(elemType));
-      if (c.launch("rmsnorm", name, a, ceilDiv(cols, 256), bands))
-        return 1;
-    }
-    std::snprintf(name, sizeof(name), "hcamd_rmsnorm_fold_%s", typeName(weightType));
-    if (c.launch("rmsnorm", name, a, ceilDiv(cols, 256)))
+    std::snprintf(name, sizeof(name), "hcamd_rmsnorm_back_%s_general", typeName(elemType));
+    if (rows && c.launch("rmsnorm", name, a, std::min<size_t>(rows, 0x7fffff)))
+      return 1;
+  } else if (rows) {
+    a.bands = (uint32_t)std::min(ceilDiv(rows, k.threads / k.lanes), lines);
+    std::snprintf(name, sizeof(name), "hcamd_rmsnorm_back_%s_%s", typeName(elemType), k.suffix);
+    if (c.launch("rmsnorm", name, a, a.bands, 1, 1, k.threads))
       return 1;
   }
-  if (rows == 0)
+  if (!gradWeight)
     return 0;
-  std::snprintf(name, sizeof(name), "hcamd_rmsnorm_back_%s_general", typeName(elemType));
-  return c.launch("rmsnorm", name, a, std::min<size_t>(rows, 0x7fffff));
+  std::snprintf(name, sizeof(name), "hcamd_rmsnorm_fold_%s", typeName(weightType));
+  return c.launch("rmsnorm", name, a, ceilDiv(cols, 64), 1, 1, 1024);
 }
 
 // ===========================================================================

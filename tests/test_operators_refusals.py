@@ -140,7 +140,7 @@ ENTRIES = [
     ("rows without elements", norm, dict(cols=0)), ("a dimension exceeds", norm, dict(rows=1 << 31)),
     ("summed is not aligned", norm, dict(summed=P + 1)),
     ("element type 6", norm_back, dict(ty=I8)), ("weight type 2", norm_back, dict(wt=BF16)),
-    ("grad_out is null", norm_back, dict(g=None)), ("workspace of 0 bytes, 32 needed", norm_back, dict(gw=P)),
+    ("grad_out is null", norm_back, dict(g=None)), ("workspace of 0 bytes, 64 needed", norm_back, dict(gw=P)),
     ("aligned to 256", norm_back, dict(gw=P, work=P + 16, have=1024)), ("rstd is null", norm_back, dict(rstd=None)),
     ("element type 0", ffn, dict(ty=F32)), ("output type 2", ffn, dict(ot=BF16)), ("activation 2", ffn, dict(act=2)),
     ("inner dimension must", ffn, dict(d=0)), ("x_scale is null", ffn, dict(ty=I8)), ("scales belong", ffn, dict(xs=P)),
