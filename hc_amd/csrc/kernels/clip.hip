@@ -6,26 +6,16 @@
 // the result does not depend on how the tensors are cut.
 #include "common.h"
 #include "op_args.h"
+#include "pieces.h"
 
 using namespace hcamd;
 
 namespace {
 
-constexpr uint32_t kChunkElems = 16384; // elements a workgroup takes at a time
+constexpr int kAhead = 4; // 16-byte pieces a lane requests at a time
 
-__device__ __forceinline__ float load1(const void *p, int type, uint64_t i) {
-  return type == 0 ? static_cast<const float *>(p)[i]
-         : type == 1 ? (float)static_cast<const _Float16 *>(p)[i]
-                     : (float)static_cast<const __bf16 *>(p)[i];
-}
-__device__ __forceinline__ void store1(void *p, int type, uint64_t i, float v) {
-  if (type == 0)
-    static_cast<float *>(p)[i] = v;
-  else if (type == 1)
-    static_cast<_Float16 *>(p)[i] = (_Float16)v;
-  else
-    static_cast<__bf16 *>(p)[i] = (__bf16)v;
-}
+template <class T> constexpr int kPiece = 16 / (int)sizeof(T);
+template <class T> using Piece __attribute__((ext_vector_type(kPiece<T>))) = T;
 
 __device__ __forceinline__ double group_sum64(double v, double *slots) {
 #pragma unroll
@@ -50,17 +40,59 @@ __device__ __forceinline__ uint32_t tensor_of(const ClipArgs &a, uint32_t chunk)
   return lo;
 }
 
+// f(piece, first element, valid elements) for this lane's pieces of n elements (a chunk:
+// positions are plain ints, and what lies past the end is a count of 0 or less)
+template <class T, class F> __device__ __forceinline__ void each_piece(const T *in, int n, F &&f) {
+  constexpr int N = kPiece<T>;
+  for (int at = threadIdx.x * N; at < n; at += 256 * N * kAhead) {
+    u32x4 v[kAhead];
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k)
+      v[k] = load_chunk(in + at + k * 256 * N, n - (at + k * 256 * N));
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k)
+      f(__builtin_bit_cast(Piece<T>, v[k]), at + k * 256 * N, n - (at + k * 256 * N));
+  }
+}
+
+template <class T> __device__ __forceinline__ double chunk_squares(const void *in, uint64_t first, int n) {
+  double sum = 0.0;
+  each_piece(static_cast<const T *>(in) + first, n, [&](Piece<T> v, int, int) {
+#pragma unroll
+    for (int e = 0; e < kPiece<T>; ++e) { // (elements that do not exist are zeros)
+      const double x = (double)(float)v[e];
+      sum = __builtin_fma(x, x, sum);
+    }
+  });
+  return sum;
+}
+template <class T>
+__device__ __forceinline__ void chunk_scale(const void *in, void *out, uint64_t first, int n, float by) {
+  T *to = static_cast<T *>(out) + first;
+  each_piece(static_cast<const T *>(in) + first, n, [&](Piece<T> v, int at, int valid) {
+#pragma unroll
+    for (int e = 0; e < kPiece<T>; ++e)
+      v[e] = (T)((float)v[e] * by);
+    store_chunk(to + at, __builtin_bit_cast(u32x4, v), valid);
+  });
+}
+// a chunk of a tensor: its first element, and how many it has
+__device__ __forceinline__ int chunk_of(const ClipArgs &a, uint32_t chunk, uint32_t t, uint64_t &first) {
+  first = (uint64_t)(chunk - a.first_chunk[t]) * a.chunk;
+  const uint64_t left = a.count[t] - first;
+  return left < a.chunk ? (int)left : (int)a.chunk;
+}
+
 __device__ __forceinline__ void square_sums(const ClipArgs &a) {
   __shared__ double slots[4];
   double sum = 0.0;
   for (uint32_t chunk = blockIdx.x; chunk < a.first_chunk[a.tensors]; chunk += gridDim.x) {
     const uint32_t t = tensor_of(a, chunk);
-    const uint64_t first = (uint64_t)(chunk - a.first_chunk[t]) * kChunkElems;
-    const uint64_t last = min(a.count[t], first + kChunkElems);
-    for (uint64_t i = first + threadIdx.x; i < last; i += 256) {
-      const double v = (double)load1(a.in[t], a.type[t], i);
-      sum = __builtin_fma(v, v, sum);
-    }
+    uint64_t first;
+    const int n = chunk_of(a, chunk, t, first);
+    sum += a.type[t] == 0   ? chunk_squares<float>(a.in[t], first, n)
+           : a.type[t] == 1 ? chunk_squares<_Float16>(a.in[t], first, n)
+                            : chunk_squares<__bf16>(a.in[t], first, n);
   }
   sum = group_sum64(sum, slots);
   if (threadIdx.x == 0)
@@ -78,12 +110,19 @@ __device__ __forceinline__ void scale(const ClipArgs &a) {
   factor = factor > 1.0f ? 1.0f : factor;
   if (blockIdx.x == 0 && threadIdx.x == 0)
     *a.norm = norm;
-  for (uint32_t chunk = blockIdx.x; chunk < a.first_chunk[a.tensors]; chunk += gridDim.x) {
-    const uint32_t t = tensor_of(a, chunk);
-    const uint64_t first = (uint64_t)(chunk - a.first_chunk[t]) * kChunkElems;
-    const uint64_t last = min(a.count[t], first + kChunkElems);
-    for (uint64_t i = first + threadIdx.x; i < last; i += 256)
-      store1(a.out[t], a.type[t], i, load1(a.in[t], a.type[t], i) * factor);
+  // from the last chunk to the first: what the sums read last is still in the
+  // memory-side cache
+  const uint32_t chunks = a.first_chunk[a.tensors];
+  for (uint32_t k = blockIdx.x; k < chunks; k += gridDim.x) {
+    const uint32_t chunk = chunks - 1 - k, t = tensor_of(a, chunk);
+    uint64_t first;
+    const int n = chunk_of(a, chunk, t, first);
+    if (a.type[t] == 0)
+      chunk_scale<float>(a.in[t], a.out[t], first, n, factor);
+    else if (a.type[t] == 1)
+      chunk_scale<_Float16>(a.in[t], a.out[t], first, n, factor);
+    else
+      chunk_scale<__bf16>(a.in[t], a.out[t], first, n, factor);
   }
 }
 

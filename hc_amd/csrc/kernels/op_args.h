@@ -106,7 +106,7 @@ struct ClipArgs {
   uint64_t count[kClipTensors];
   uint32_t first_chunk[kClipTensors + 1]; // chunks before this tensor
   uint8_t type[kClipTensors];
-  uint32_t tensors;
+  uint32_t tensors, chunk;                // elements to a chunk
   double *partial;       // one cell per workgroup of every launch of the call
   uint32_t first_cell, cells;
   float max_norm;

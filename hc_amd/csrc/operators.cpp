@@ -632,7 +632,9 @@ int hcamdLaunchLinearCrossEntropyBackward(OlQueue q, int elemType, const void *x
 // clipping by the global norm
 // ===========================================================================
 namespace {
-constexpr size_t kClipChunk = 16384, kClipCells = 1024;
+constexpr size_t kClipCells = 1024;
+// elements to a chunk: small totals are cut finer, so that more workgroups share them
+size_t clipChunk(size_t elems) { return elems >= ((size_t)16 << 20) ? 16384 : 4096; }
 // workgroups of the launch that takes `chunks` of `all` chunks
 size_t clipGroups(size_t chunks, size_t all) {
   return std::max<size_t>(1, std::min(chunks, all <= kClipCells ? chunks : chunks * kClipCells / all));
@@ -652,7 +654,7 @@ int hcamdLaunchClipGradNorm(OlQueue q, const HcamdClipTensor *tensors, size_t co
     return c.fail("tensors is null, or too many");
   if (c.check({"norm", norm, 1, 1, 1, 4}) || c.work(work, workBytes, hcamdClipGradNormWorkspace(count)))
     return 1;
-  size_t all = 0;
+  size_t all = 0, elems = 0;
   for (size_t i = 0; i < count; ++i) {
     const HcamdClipTensor &t = tensors[i];
     if (t.type != HCAMD_F32 && !half16(t.type))
@@ -662,8 +664,11 @@ int hcamdLaunchClipGradNorm(OlQueue q, const HcamdClipTensor *tensors, size_t co
     if (t.count && (c.check({"a tensor", t.in, t.count, 1, t.count, elemBytes(t.type)}) ||
                     c.check({"a clipped tensor", t.out, t.count, 1, t.count, elemBytes(t.type)})))
       return 1;
-    all += ceilDiv(t.count, kClipChunk);
+    elems += t.count;
   }
+  const size_t chunk = clipChunk(elems);
+  for (size_t i = 0; i < count; ++i)
+    all += ceilDiv(tensors[i].count, chunk);
   if (all > 0x7fffffff)
     return c.fail("too many elements");
   const size_t launches = std::max<size_t>(1, ceilDiv(count, (size_t)kClipTensors));
@@ -678,10 +683,10 @@ int hcamdLaunchClipGradNorm(OlQueue q, const HcamdClipTensor *tensors, size_t co
         const HcamdClipTensor &t = tensors[first + i];
         a.in[i] = t.in, a.out[i] = t.out, a.count[i] = t.count, a.type[i] = (uint8_t)t.type;
         a.first_chunk[i] = (uint32_t)chunks;
-        chunks += ceilDiv(t.count, kClipChunk);
+        chunks += ceilDiv(t.count, chunk);
       }
       a.first_chunk[n] = (uint32_t)chunks;
-      a.tensors = (uint32_t)n;
+      a.tensors = (uint32_t)n, a.chunk = (uint32_t)chunk;
       a.partial = static_cast<double *>(work), a.first_cell = (uint32_t)cell;
       a.max_norm = maxNorm, a.norm = norm, a.cells = (uint32_t)cells;
       const size_t groups = clipGroups(chunks, all);

@@ -567,9 +567,13 @@ def test_linear_cross_entropy_without_tokens():
 @pytest.mark.parametrize("sizes", [[1], [5], [16384], [16385, 1, 3], [0, 7, 0], [100003, 40000, 2], [9] * 130, [1_000_000, 3] * 3], ids=str)
 @pytest.mark.parametrize("most", [0.0, 1.0, 1e9])
 def test_clip_grad_norm(sizes, most):
-    grads = [dev(normal(i, n) * 0.3, list(TYPES.values())[i % 3]) for i, n in enumerate(sizes)]
-    outs, norm = [torch.full_like(g, 77) for g in grads], empty(1, ty=torch.float32)
+    grads = [dev(normal(i, n) * 0.3, list(TYPES.values())[(i + len(sizes)) % 3]) for i, n in enumerate(sizes)]
+    # every output lies between 9000 elements that stay as they are
+    wide = [torch.full((g.numel() + 18000,), 55.0, device="cuda").to(g.dtype) for g in grads]
+    outs, norm = [w[9000:9000 + g.numel()] for w, g in zip(wide, grads)], empty(1, ty=torch.float32)
     rt.clip_grad_norm(grads, outs, norm, most)
+    for w, g in zip(wide, grads):
+        assert bool((w[:9000] == 55).all()) and bool((w[9000 + g.numel():] == 55).all())
     want = sum(f64(g).square().sum() for g in grads).sqrt()
     near(norm, want.reshape(1), want * 4 * U)
     factor = min(1.0, most / (float(want) + 1e-6))
