@@ -121,6 +121,44 @@ template <class E, int B, int WM, int WN> __device__ __forceinline__ void gated_
       });
 }
 
+// Few tokens: one pass over the weights; a workgroup holds sixteen outputs' rows of
+// both.
+template <class E, class O, int MB> __device__ __forceinline__ void gated_skinny(const GatedArgs &a, unsigned char *lds) {
+  const int f0 = blockIdx.x * 16, left = a.mma.N - f0;
+  mma_skinny<E, MB>(a.mma, static_cast<const E *>(a.mma.b[0]) + (size_t)f0 * a.mma.ldb[0], a.mma.ldb[0], left,
+                    static_cast<const E *>(a.mma.b[1]) + (size_t)f0 * a.mma.ldb[1], a.mma.ldb[1], left, lds);
+  typedef typename MmaType<E>::acc acc_t;
+  using V = decltype(acc_t{}[0] + acc_t{}[0]);
+  const V *cells = reinterpret_cast<const V *>(lds);
+  for (int c = threadIdx.x; c < MB * 256; c += 512) {
+    const int n = c % 16, m = c / 16; // sixteen lanes write one token's outputs
+    if (m >= a.mma.M || n >= left)
+      continue;
+    const int at = m / 16 * 256 + ((n / 4) * 16 + m % 16) * 4 + n % 4;
+    float g = (float)cells[at], u = (float)cells[MB * 256 + at];
+    if constexpr (sizeof(E) == 1) {
+      g = g * a.x_scale[m] * a.gate_scale[f0 + n];
+      u = u * a.x_scale[m] * a.up_scale[f0 + n];
+    }
+    static_cast<O *>(a.out)[(size_t)m * a.ldo + f0 + n] = (O)(activate(a.activation, g) * u);
+    if (sizeof(E) == 2 && a.gate)
+      static_cast<O *>(a.gate)[(size_t)m * a.ldgate + f0 + n] = (O)g;
+    if (sizeof(E) == 2 && a.up)
+      static_cast<O *>(a.up)[(size_t)m * a.ldup + f0 + n] = (O)u;
+  }
+}
+template <class E, int MB> __device__ __forceinline__ void gated_few(const GatedArgs &a) {
+  __shared__ __attribute__((aligned(16))) unsigned char lds[skinny_lds<MB>()];
+  if constexpr (sizeof(E) == 1) {
+    if (a.out_f16)
+      gated_skinny<E, _Float16, MB>(a, lds);
+    else
+      gated_skinny<E, __bf16, MB>(a, lds);
+  } else {
+    gated_skinny<E, E, MB>(a, lds);
+  }
+}
+
 // pre-activation gradients: a workgroup walks rows, eight elements a lane.  The
 // destination is the library's own, its rows padded to a multiple of 8.
 template <class E> __device__ __forceinline__ void gated_back(const GatedBackArgs &a) {
@@ -202,6 +240,19 @@ template <class E> __device__ __forceinline__ void fold(const FoldArgs &a) {
 HCAMD_FFN(bf16, __bf16)
 HCAMD_FFN(f16, _Float16)
 HCAMD_FFN(i8, int8_t)
+#define HCAMD_FFN_FEW(SUFFIX, E)                                                                          \
+  extern "C" __global__ __launch_bounds__(512) void hcamd_gated_##SUFFIX##_s16(GatedArgs a) {             \
+    gated_few<E, 1>(a);                                                                                   \
+  }                                                                                                       \
+  extern "C" __global__ __launch_bounds__(512) void hcamd_gated_##SUFFIX##_s32(GatedArgs a) {             \
+    gated_few<E, 2>(a);                                                                                   \
+  }                                                                                                       \
+  extern "C" __global__ __launch_bounds__(512) void hcamd_gated_##SUFFIX##_s64(GatedArgs a) {             \
+    gated_few<E, 4>(a);                                                                                   \
+  }
+HCAMD_FFN_FEW(bf16, __bf16)
+HCAMD_FFN_FEW(f16, _Float16)
+HCAMD_FFN_FEW(i8, int8_t)
 #define HCAMD_FFN_BACK(SUFFIX, E)                                                                         \
   extern "C" __global__ __launch_bounds__(256) void hcamd_gated_back_##SUFFIX(GatedBackArgs a) {          \
     gated_back<E>(a);                                                                                     \

@@ -217,7 +217,8 @@ __device__ __forceinline__ void mma_general(const MmaArgs &g, unsigned char *lds
 //   * One barrier per tile, in front of its second half: there this wave's loads
 //     of the next tile have landed and its reads of this tile are done.
 //   * Edges: the last tile of a row or column of tiles begins BM rows (BN columns)
-//     before the end; M >= BM and N >= BN.  In the last tile of a k segment the
+//     before the end; N >= BN, and M >= BM except with 128-row tiles and a k-fast A,
+//     whose rows past M are fetched from row 0's group.  In the last tile of a k segment the
 //     pieces past K are fetched from valid addresses and overwritten with zeros in
 //     LDS by the lane that fetched them.  A k-fast operand whose K is not a multiple
 //     of 8 must hold zeros up to there, a k-slow one whose rows are not must have
@@ -271,7 +272,9 @@ __device__ __forceinline__ void mma_pipelined(const MmaArgs &g, unsigned char *l
   tile_of(blockIdx.x, (g.M + BM - 1) / BM, (g.N + BNO - 1) / BNO, tm, tn);
   // (k-slow rows come in aligned pieces of 8: their origin stays a multiple of 8)
   const int end_m = LA == kKSlow ? (g.M + 7) & ~7 : g.M, end_n = LB == kKSlow ? (g.N + 7) & ~7 : g.N;
-  const Tile tile = {min(tm * BM, end_m - BM), min(tn * BNO, end_n - BNO), tm * BM, tn * BNO, tn};
+  constexpr bool kFewRows = BM == 128 && LA == kKFast; // M may be less than a tile
+  const Tile tile = {kFewRows ? max(min(tm * BM, end_m - BM), 0) : min(tm * BM, end_m - BM),
+                     min(tn * BNO, end_n - BNO), tm * BM, tn * BNO, tn};
   const int lane = threadIdx.x % kWave;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int wave_m = wave / WN * kWaveM, wave_n = wave % WN * kWaveN;
@@ -297,8 +300,9 @@ __device__ __forceinline__ void mma_pipelined(const MmaArgs &g, unsigned char *l
   auto lane_part = [&](Layout l, int R, int ld, bool tail) {
     Lane p;
     if (l == kKFast) {
-      p.off = lane / 8 * ld + (tail && fast_chunk >= tail_chunks ? 0 : fast_chunk) * 16;
-      p.cut = 0;
+      const int chunk = (tail && fast_chunk >= tail_chunks ? 0 : fast_chunk) * 16, left = g.M % 8;
+      p.off = lane / 8 * ld + chunk;
+      p.cut = (left ? min(lane / 8, left - 1) : lane / 8) * ld + chunk; // (A with few rows only)
     } else {
       const int per = 512 / R, sub = lane / (R / 8), pos = lane % (R / 8);
       // (the k of a load differ from these by multiples of 16 or of 4 * kWaves: the swizzle is the lane's)
@@ -347,9 +351,13 @@ __device__ __forceinline__ void mma_pipelined(const MmaArgs &g, unsigned char *l
       state = want;
     }
   };
-  auto fetch = [&](Layout l, int R, const __amdgpu_buffer_rsrc_t &rsrc, const Lane &p, int ld, int first, void *to) {
+  auto fetch = [&](Layout l, int R, const __amdgpu_buffer_rsrc_t &rsrc, const Lane &p, int ld, int first, void *to,
+                   bool few) {
     // first: the load's first row or k
-    if (l == kKFast) {
+    if (few) {
+      const int off = first + 8 <= g.M ? p.off : p.cut;
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_void_ptr)to, 16, off, first < g.M ? first * ld : 0, 0, 0);
+    } else if (l == kKFast) {
       __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_void_ptr)to, 16, p.off, first * ld, 0, 0);
     } else {
       const int limit = (state & 1) ? tail_k : 64;
@@ -361,14 +369,14 @@ __device__ __forceinline__ void mma_pipelined(const MmaArgs &g, unsigned char *l
     unsigned char *base = lds + buf * kStage + wave * 1024;
     if (v < kALoads) {
       const int first = (v * kWaves + wave) * (LA == kKFast ? 8 : 512 / BM);
-      fetch(LA, BM, rsrc_a, lane_a, ld_a, first, base + v * kWaves * 1024);
+      fetch(LA, BM, rsrc_a, lane_a, ld_a, first, base + v * kWaves * 1024, kFewRows);
     } else {
       const int b = v - kALoads;
       int first = (b * kWaves + wave) * (LB == kKFast ? 8 : 512 / BN);
       if constexpr (GATED)
         first = first / 64 * 32 + first % 32;
       const int o = kBOps == 2 ? b % 2 : 0;
-      fetch(LB, BN, rsrc_b[o], lane_b[o], ld_b[o], first, base + kPanelA + b * kWaves * 1024);
+      fetch(LB, BN, rsrc_b[o], lane_b[o], ld_b[o], first, base + kPanelA + b * kWaves * 1024, false);
     }
   };
   auto zero_tail = [&](int buf) {
@@ -497,6 +505,106 @@ __device__ __forceinline__ void mma_pipelined(const MmaArgs &g, unsigned char *l
   __builtin_amdgcn_s_waitcnt(waitcnt_imm(kNoVm, 0));
   __builtin_amdgcn_s_barrier();
   epilogue(acc, tile, wave_m, wave_n, lane, lds);
+}
+
+// ---------------------------------------------------------------------------
+// Few tokens: M <= 16 * MB rows of A against 32 rows of B, for products that are one
+// pass over B.  Eight waves share the k of the tile; each reads B and A straight into
+// MFMA operand registers (sixteen rows, 64 consecutive bytes of a row per four lanes;
+// which k a lane holds does not matter as long as both operands agree), the next block
+// of k is requested before the present one is multiplied, and the eight partial sums
+// meet in LDS.  Any size and alignment: rows past the end are read from the last one and
+// not stored, pieces that cross K go element by element.
+//   b0, b1: first rows of the two blocks of sixteen; last0, last1: rows left from there
+// The result lies in LDS as float or int [2][MB][256], element (m, n) of a block at
+// ((n / 4) * 16 + m) * 4 + n % 4.
+// ---------------------------------------------------------------------------
+template <int MB> constexpr int skinny_lds() { return 8 * 2 * MB * 1024; }
+
+template <class E, int MB>
+__device__ __forceinline__ void mma_skinny(const MmaArgs &g, const E *b0, size_t ld0, int rows0, const E *b1,
+                                           size_t ld1, int rows1, unsigned char *lds) {
+  using T = MmaType<E>;
+  constexpr int U = 4, kStep = 4 * T::kChunk, kBlock = U * kStep;
+  const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int row = lane % 16, k_lane = lane / 16 * T::kChunk;
+  const E *pb[2] = {b0 + (size_t)min(row, rows0 - 1) * ld0 + k_lane, b1 + (size_t)min(row, rows1 - 1) * ld1 + k_lane};
+  const E *pa[MB];
+#pragma unroll
+  for (int i = 0; i < MB; ++i)
+    pa[i] = static_cast<const E *>(g.a[0]) + (size_t)min(i * 16 + row, g.M - 1) * g.lda[0] + k_lane;
+  typename T::acc acc[2][MB] = {};
+  u32x4 fb[2][U], fa[MB][U];
+  auto request = [&](int block) {
+    const int k = block * kBlock;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+        fb[j][u] = *reinterpret_cast<const u32x4_u *>(pb[j] + k + u * kStep);
+#pragma unroll
+      for (int i = 0; i < MB; ++i)
+        fa[i][u] = *reinterpret_cast<const u32x4_u *>(pa[i] + k + u * kStep);
+    }
+  };
+  auto multiply = [&](const u32x4 (&b)[2][U], const u32x4 (&a)[MB][U]) {
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int i = 0; i < MB; ++i)
+          acc[j][i] = mma16<E>(b[j][u], a[i][u], acc[j][i]);
+  };
+  const int blocks = g.K / kBlock;
+  if (wave < blocks)
+    request(wave);
+  for (int block = wave; block < blocks; block += 8) {
+    u32x4 b[2][U], a[MB][U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+        b[j][u] = fb[j][u];
+#pragma unroll
+      for (int i = 0; i < MB; ++i)
+        a[i][u] = fa[i][u];
+    }
+    if (block + 8 < blocks)
+      request(block + 8);
+    multiply(b, a);
+  }
+  if (wave == blocks % 8 && g.K % kBlock) { // what is left of k
+    const int k = blocks * kBlock;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int valid = g.K - (k + u * kStep + k_lane);
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+        fb[j][u] = load_chunk(pb[j] + k + u * kStep, valid);
+#pragma unroll
+      for (int i = 0; i < MB; ++i)
+        fa[i][u] = load_chunk(pa[i] + k + u * kStep, valid);
+    }
+    multiply(fb, fa);
+  }
+  using V = typename T::acc;
+  V *cells = reinterpret_cast<V *>(lds); // [8][2][MB][64]
+#pragma unroll
+  for (int j = 0; j < 2; ++j)
+#pragma unroll
+    for (int i = 0; i < MB; ++i)
+      cells[((wave * 2 + j) * MB + i) * kWave + lane] = acc[j][i];
+  __syncthreads();
+  // the eight waves' sums, added in their order, four elements a thread
+  for (int c = threadIdx.x; c < 2 * MB * kWave; c += 512) {
+    V sum = cells[c];
+#pragma unroll
+    for (int w = 1; w < 8; ++w)
+      sum += cells[w * (2 * MB * kWave) + c];
+    cells[c] = sum; // (only this thread reads or writes this cell here)
+  }
+  __syncthreads();
 }
 
 // ---- stores ------------------------------------------------------------------

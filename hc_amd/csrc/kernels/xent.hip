@@ -114,6 +114,43 @@ template <class E, int B, int WM, int WN> __device__ __forceinline__ void stats_
       });
 }
 
+// Few tokens: one pass over the weight, 32 of its rows a workgroup.
+template <class E, int MB> __device__ __forceinline__ void stats_few(const XentArgs &a) {
+  __shared__ __attribute__((aligned(16))) unsigned char lds[skinny_lds<MB>()];
+  const int n0 = blockIdx.x * 32, left = a.mma.N - n0;
+  const size_t ld = a.mma.ldb[0];
+  const E *b = static_cast<const E *>(a.mma.b[0]) + (size_t)n0 * ld;
+  // (a second block past the end reads the first one's rows and is left out below)
+  mma_skinny<E, MB>(a.mma, b, ld, left, left > 16 ? b + 16 * ld : b, ld, left > 16 ? left - 16 : left, lds);
+  const float *cells = reinterpret_cast<const float *>(lds);
+  for (int c = threadIdx.x; c < MB * 256; c += 512) {
+    const int n = c % 16, m = c / 16; // sixteen lanes share a row
+    const int at = m / 16 * 256 + ((n / 4) * 16 + m % 16) * 4 + n % 4;
+    const float z0 = n < left ? cells[at] : -INFINITY, z1 = n + 16 < left ? cells[MB * 256 + at] : -INFINITY;
+    float most = fmaxf(z0, z1);
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1)
+      most = fmaxf(most, __shfl_xor(most, o));
+    const float from = most == -INFINITY ? 0.0f : most;
+    float sum = __expf(z0 - from) + __expf(z1 - from);
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1)
+      sum += __shfl_xor(sum, o);
+    if (m >= a.mma.M)
+      continue;
+    const int64_t t = target_of(a.targets, a.target_i64, m) - n0;
+    if (t == n && n < left)
+      a.zt[m] = z0;
+    if (t == n + 16 && n + 16 < left)
+      a.zt[m] = z1;
+    if (n == 0) {
+      float *cell = a.stats + ((size_t)m * a.tiles + blockIdx.x) * 2;
+      cell[0] = most;
+      cell[1] = sum;
+    }
+  }
+}
+
 // p of a tile; the columns up to the next multiple of 8 become zeros (the products
 // that read p take it in pieces of 8)
 template <class E, int MI, int NI, bool LDS>
@@ -239,6 +276,18 @@ __device__ __forceinline__ void p_factor(const float *grad_loss, uint32_t rows, 
   }
 HCAMD_XENT(bf16, __bf16)
 HCAMD_XENT(f16, _Float16)
+#define HCAMD_XENT_FEW(SUFFIX, E)                                                                         \
+  extern "C" __global__ __launch_bounds__(512) void hcamd_xent_stats_##SUFFIX##_s16(XentArgs a) {         \
+    stats_few<E, 1>(a);                                                                                   \
+  }                                                                                                       \
+  extern "C" __global__ __launch_bounds__(512) void hcamd_xent_stats_##SUFFIX##_s32(XentArgs a) {         \
+    stats_few<E, 2>(a);                                                                                   \
+  }                                                                                                       \
+  extern "C" __global__ __launch_bounds__(512) void hcamd_xent_stats_##SUFFIX##_s64(XentArgs a) {         \
+    stats_few<E, 4>(a);                                                                                   \
+  }
+HCAMD_XENT_FEW(bf16, __bf16)
+HCAMD_XENT_FEW(f16, _Float16)
 extern "C" __global__ __launch_bounds__(256) void hcamd_xent_rows(XentRowsArgs a) { rows_join(a); }
 extern "C" __global__ __launch_bounds__(1024) void hcamd_xent_factor(const float *grad_loss, uint32_t rows,
                                                                       float top, float *factor) {

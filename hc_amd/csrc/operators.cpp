@@ -125,12 +125,23 @@ struct Kernel {
   size_t threads;
   int tile;
 };
-Kernel kernelOf(int tile, size_t m, size_t n, bool fetch) {
-  if (!fetch || hcamdInternalVariant("mma") == 1 || m < 128 || n < 128)
+// (fewM: a k-fast A may have fewer rows than the tile)
+Kernel kernelOf(int tile, size_t m, size_t n, bool fetch, bool fewM) {
+  if (!fetch || hcamdInternalVariant("mma") == 1 || (m < 128 && !fewM) || n < 128)
     return {"general", 256, 128};
   if (tile == 256)
     return {"t256", 512, 256};
   return {"t128", 256, 128};
+}
+// Up to 64 tokens the forward products are one pass over the weights, which the tiled
+// kernels feed from too few workgroups: one token, 2 x 11264 x 4096 bf16: 94 us tiled.
+// Returns the kernel's suffix, or null.
+constexpr size_t kFewTokens = 64;
+const char *fewSuffix(size_t tokens) {
+  const int v = hcamdInternalVariant("mma");
+  if (tokens > kFewTokens || (v >= 1 && v <= 3))
+    return nullptr;
+  return tokens <= 16 ? "s16" : tokens <= 32 ? "s32" : "s64";
 }
 
 int launchFold(const Call &c, int type, const FoldArgs &f) {
@@ -343,11 +354,16 @@ int hcamdLaunchGatedFfn(OlQueue q, int elemType, const void *x, size_t ldx, cons
   a.x_scale = xScale, a.gate_scale = gateScale, a.up_scale = upScale;
   a.out = out, a.gate = gate, a.up = up, a.ldo = ldo, a.ldgate = ldgate, a.ldup = ldup;
   a.activation = activation, a.out_f16 = outType == HCAMD_F16;
+  char name[64];
+  if (const char *few = fewSuffix(tokens)) {
+    std::snprintf(name, sizeof(name), "hcamd_gated_%s_%s", typeName(elemType), few);
+    return c.launch("ffn", name, a, ceilDiv(f, 16), 1, 1, 512);
+  }
   // (a tile of outputs takes twice its columns of the two weight matrices)
   const Kernel k = kernelOf(tileOf(tokens, 2 * f), tokens, 2 * f,
                             fetchable(x, ldx, d, e, false) && fetchable(wGate, ldwg, d, e, false) &&
-                                fetchable(wUp, ldwu, d, e, false));
-  char name[64];
+                                fetchable(wUp, ldwu, d, e, false),
+                            true);
   std::snprintf(name, sizeof(name), "hcamd_gated_%s_%s", typeName(elemType), k.suffix);
   return c.launch("ffn", name, a, ceilDiv(tokens, k.tile) * ceilDiv(f, k.tile / 2), 1, 1, k.threads);
 }
@@ -429,7 +445,7 @@ int hcamdLaunchGatedFfnBackward(OlQueue q, int elemType, const void *gradOut, si
     s.out = gradX, s.ldo = ldgx, s.ldp = padCols(d);
     s.partial = b.dx ? reinterpret_cast<float *>(w + 2 * b.dg) : nullptr;
     const Kernel k = kernelOf(b.px.tile, tokens, d, fetchable(wGate, ldwg, d, 2, false) &&
-                                                        fetchable(wUp, ldwu, d, 2, false));
+                                                        fetchable(wUp, ldwu, d, 2, false), true);
     std::snprintf(name, sizeof(name), "hcamd_product_nn_%s_%s", typeName(elemType), k.suffix);
     if (c.launch("ffn", name, s, ceilDiv(tokens, k.tile) * ceilDiv(d, k.tile), b.px.splits, 1, k.threads))
       return 1;
@@ -452,7 +468,7 @@ int hcamdLaunchGatedFfnBackward(OlQueue q, int elemType, const void *gradOut, si
       t.partial = b.dw ? reinterpret_cast<float *>(w + 2 * b.dg + b.dx + n * b.dw) : nullptr;
       ++n;
     }
-    const Kernel k = kernelOf(b.pw.tile, f, d, fetchable(x, ldx, d, 2, false));
+    const Kernel k = kernelOf(b.pw.tile, f, d, fetchable(x, ldx, d, 2, false), false);
     std::snprintf(name, sizeof(name), "hcamd_product_tn_%s_%s", typeName(elemType), k.suffix);
     if (c.launch("ffn", name, s, ceilDiv(f, k.tile) * ceilDiv(d, k.tile), b.pw.splits, n, k.threads))
       return 1;
@@ -468,7 +484,8 @@ int hcamdLaunchGatedFfnBackward(OlQueue q, int elemType, const void *gradOut, si
 // linear cross entropy
 // ===========================================================================
 namespace {
-constexpr int kStatsCols = 128; // columns of a statistics tile
+// columns of the narrowest statistics tile
+size_t statsCols(size_t tokens) { return tokens <= kFewTokens ? 32 : 128; }
 int xentCommon(const Call &c, int elemType, const void *x, size_t ldx, const void *weight, size_t ldw,
                const void *targets, int targetType, size_t tokens, size_t d, size_t vocab) {
   if (!half16(elemType))
@@ -487,7 +504,7 @@ int xentCommon(const Call &c, int elemType, const void *x, size_t ldx, const voi
 size_t hcamdLinearCrossEntropyWorkspace(size_t tokens, size_t vocab) noexcept {
   if (tokens > kMaxDim || vocab > kMaxDim)
     return 0;
-  return tokens * ceilDiv(vocab, kStatsCols) * 8 + tokens * 4;
+  return tokens * ceilDiv(vocab, statsCols(tokens)) * 8 + tokens * 4;
 }
 
 int hcamdLaunchLinearCrossEntropy(OlQueue q, int elemType, const void *x, size_t ldx, const void *weight, size_t ldw,
@@ -505,14 +522,15 @@ int hcamdLaunchLinearCrossEntropy(OlQueue q, int elemType, const void *x, size_t
   a.mma.a[0] = x, a.mma.lda[0] = ldx, a.mma.b[0] = weight, a.mma.ldb[0] = ldw;
   a.mma.M = (int)tokens, a.mma.N = (int)vocab, a.mma.K = (int)d, a.mma.segments = a.mma.splits = 1;
   a.targets = targets, a.target_i64 = targetType == HCAMD_I64, a.vocab = (int)vocab;
+  const char *few = fewSuffix(tokens);
   const Kernel k = kernelOf(tileOf(tokens, vocab), tokens, vocab,
-                            fetchable(x, ldx, d, 2, false) && fetchable(weight, ldw, d, 2, false));
-  a.tiles = (int)ceilDiv(vocab, k.tile);
+                            fetchable(x, ldx, d, 2, false) && fetchable(weight, ldw, d, 2, false), true);
+  a.tiles = (int)ceilDiv(vocab, few ? 32 : k.tile);
   a.stats = static_cast<float *>(work);
   a.zt = a.stats + tokens * a.tiles * 2;
   char name[64];
-  std::snprintf(name, sizeof(name), "hcamd_xent_stats_%s_%s", typeName(elemType), k.suffix);
-  if (c.launch("xent", name, a, ceilDiv(tokens, k.tile) * a.tiles, 1, 1, k.threads))
+  std::snprintf(name, sizeof(name), "hcamd_xent_stats_%s_%s", typeName(elemType), few ? few : k.suffix);
+  if (c.launch("xent", name, a, few ? a.tiles : ceilDiv(tokens, k.tile) * a.tiles, 1, 1, few ? 512 : k.threads))
     return 1;
   XentRowsArgs r{a.stats, a.zt, targets, a.target_i64, loss, lse, (uint32_t)tokens, (uint32_t)vocab,
                  (uint32_t)a.tiles};
@@ -592,7 +610,7 @@ int hcamdLaunchLinearCrossEntropyBackward(OlQueue q, int elemType, const void *x
     a.mma.M = (int)tokens, a.mma.N = (int)n, a.mma.K = (int)d, a.mma.segments = a.mma.splits = 1;
     a.targets = targets, a.target_i64 = targetType == HCAMD_I64, a.v0 = (int)v0, a.vocab = (int)vocab;
     a.lse = lse, a.grad_loss = gradLoss, a.factor = factor, a.p = w + 256, a.ldp = b.ldp;
-    Kernel k = kernelOf(tileOf(tokens, n), tokens, n, fetchable(x, ldx, d, 2, false) && fetchable(rows, ldw, d, 2, false));
+    Kernel k = kernelOf(tileOf(tokens, n), tokens, n, fetchable(x, ldx, d, 2, false) && fetchable(rows, ldw, d, 2, false), true);
     std::snprintf(name, sizeof(name), "hcamd_xent_p_%s_%s", typeName(elemType), k.suffix);
     if (tokens && c.launch("xent", name, a, ceilDiv(tokens, k.tile) * ceilDiv(n, k.tile), 1, 1, k.threads))
       return 1;
@@ -601,7 +619,7 @@ int hcamdLaunchLinearCrossEntropyBackward(OlQueue q, int elemType, const void *x
       s.mma.a[0] = a.p, s.mma.lda[0] = b.ldp, s.mma.b[0] = rows, s.mma.ldb[0] = ldw;
       s.mma.M = (int)tokens, s.mma.N = (int)d, s.mma.K = (int)n, s.mma.segments = 1, s.mma.splits = b.px.splits;
       s.partial = dx, s.ldp = padCols(d), s.accumulate = v0 != 0;
-      k = kernelOf(b.px.tile, tokens, d, fetchable(rows, ldw, d, 2, false));
+      k = kernelOf(b.px.tile, tokens, d, fetchable(rows, ldw, d, 2, false), true);
       std::snprintf(name, sizeof(name), "hcamd_product_nn_%s_%s", typeName(elemType), k.suffix);
       if (c.launch("ffn", name, s, ceilDiv(tokens, k.tile) * ceilDiv(d, k.tile), b.px.splits, 1, k.threads))
         return 1;
@@ -613,7 +631,7 @@ int hcamdLaunchLinearCrossEntropyBackward(OlQueue q, int elemType, const void *x
       t.mma.M = (int)n, t.mma.N = (int)d, t.mma.K = (int)tokens, t.mma.segments = 1, t.mma.splits = b.pw.splits;
       t.out = static_cast<char *>(gradWeight) + v0 * ldgw * 2, t.ldo = ldgw, t.undo = undo;
       t.partial = b.dw ? reinterpret_cast<float *>(w + 256 + b.p + b.dx) : nullptr, t.ldp = padCols(d);
-      k = kernelOf(n >= 256 ? b.pw.tile : 128, n, d, fetchable(x, ldx, d, 2, false));
+      k = kernelOf(n >= 256 ? b.pw.tile : 128, n, d, fetchable(x, ldx, d, 2, false), false);
       std::snprintf(name, sizeof(name), "hcamd_product_tn_%s_%s", typeName(elemType), k.suffix);
       if (c.launch("ffn", name, s, ceilDiv(n, k.tile) * ceilDiv(d, k.tile), b.pw.splits, 1, k.threads))
         return 1;

@@ -784,7 +784,7 @@ def product_kernel(request):
 
 # whole tiles; edges in every direction; k tiles of one, two, three and with every kind of tail (k is d forward, f
 # and t backward)
-TILED = [(256, 64, 256), (512, 128, 512), (257, 200, 264), (300, 328, 391), (1000, 136, 520), (384, 1032, 777), (263, 256, 1001)]
+TILED = [(1, 200, 264), (12, 328, 520), (100, 136, 136), (256, 64, 256), (512, 128, 512), (257, 200, 264), (300, 328, 391), (1000, 136, 520), (384, 1032, 777), (263, 256, 1001)]
 
 
 @pytest.mark.parametrize("layout", ["dense", "strided"])
