@@ -11,6 +11,12 @@
 //   dx = dg Wg + du Wu                        one product, k runs through both pairs
 //   dWg = dg' x, dWu = du' x                  one launch, both operands k-slow
 #include "mma.h"
+#ifndef S16NB
+#define S16NB 2
+#define S16U 4
+#define S32NB 4
+#define S32U 2
+#endif
 
 using namespace hcamd;
 
@@ -107,35 +113,44 @@ __device__ __forceinline__ void gated_epilogue(const GatedArgs &a, typename MmaT
 template <class E> __device__ __forceinline__ void gated_general(const GatedArgs &a) {
   __shared__ __attribute__((aligned(1024))) unsigned char lds[4 * 128 * 128];
   mma_general<E, kKFast, kKFast, true>(
-      a.mma, lds, FromZero{}, [&](auto &acc, const Tile &t, int wave_m, int wave_n, int lane, unsigned char *) {
+      a.mma, blockIdx.x, lds, FromZero{},
+      [&](auto &acc, const Tile &t, int wave_m, int wave_n, int lane, unsigned char *) {
         gated_epilogue<E, 4, 4, false>(a, acc, t, t.m0 + wave_m, t.n0 + wave_n / 2, lane, nullptr);
       });
 }
-template <class E, int B, int WM, int WN> __device__ __forceinline__ void gated_tile(const GatedArgs &a) {
-  constexpr int MI = B / WM / 16, NI = B / WN / 16;
-  __shared__ __attribute__((aligned(1024))) unsigned char lds[pipelined_lds<B, B>()];
-  mma_pipelined<E, kKFast, kKFast, true, B, B, WM, WN>(
-      a.mma, lds, FromZero{}, [&](auto &acc, const Tile &t, int wave_m, int wave_n, int lane, unsigned char *l) {
+template <class E, int B> __device__ __forceinline__ void gated_tile(const GatedArgs &a) {
+  __shared__ __attribute__((aligned(1024))) unsigned char lds[pipelined_lds<B>()];
+  mma_tiles<E, kKFast, kKFast, true, B>(
+      a.mma, blockIdx.x, a.mma.half_from, lds, FromZero{},
+      [&](auto &acc, const Tile &t, int wave_m, int wave_n, int lane, unsigned char *l) {
+        constexpr int MI = sizeof(acc) / sizeof(acc[0]), NI = sizeof(acc[0]) / sizeof(acc[0][0]);
         gated_epilogue<E, MI, NI, true>(a, acc, t, t.m0 + wave_m, t.n0 + wave_n / 2, lane,
-                                        l + (wave_m / (MI * 16) * WN + wave_n / (NI * 16)) * (MI * NI * 256));
+                                        l + threadIdx.x / kWave * (MI * NI * 256));
       });
 }
 
-// Few tokens: one pass over the weights; a workgroup holds sixteen outputs' rows of
-// both.
-template <class E, class O, int MB> __device__ __forceinline__ void gated_skinny(const GatedArgs &a, unsigned char *lds) {
-  const int f0 = blockIdx.x * 16, left = a.mma.N - f0;
-  mma_skinny<E, MB>(a.mma, static_cast<const E *>(a.mma.b[0]) + (size_t)f0 * a.mma.ldb[0], a.mma.ldb[0], left,
-                    static_cast<const E *>(a.mma.b[1]) + (size_t)f0 * a.mma.ldb[1], a.mma.ldb[1], left, lds);
+// Few tokens: one pass over the weights; a workgroup holds NB * 8 outputs' rows of both
+// (blocks j and j + NB / 2 belong together).
+template <class E, class O, int MB, int NB, int U>
+__device__ __forceinline__ void gated_skinny(const GatedArgs &a, unsigned char *lds) {
+  constexpr int H = NB / 2;
+  const int f0 = blockIdx.x * (H * 16), left = a.mma.N - f0;
+  mma_skinny<E, MB, NB, U>(
+      a.mma,
+      [&](int j) {
+        const int f = min(f0 + j % H * 16 + (int)threadIdx.x % 16, a.mma.N - 1), w = j / H;
+        return static_cast<const E *>(a.mma.b[w]) + (size_t)f * a.mma.ldb[w];
+      },
+      lds);
   typedef typename MmaType<E>::acc acc_t;
   using V = decltype(acc_t{}[0] + acc_t{}[0]);
   const V *cells = reinterpret_cast<const V *>(lds);
-  for (int c = threadIdx.x; c < MB * 256; c += 512) {
-    const int n = c % 16, m = c / 16; // sixteen lanes write one token's outputs
+  for (int c = threadIdx.x; c < H * MB * 256; c += 512) {
+    const int n = c % (H * 16), m = c / (H * 16); // neighbouring lanes write one token's outputs
     if (m >= a.mma.M || n >= left)
       continue;
-    const int at = m / 16 * 256 + ((n / 4) * 16 + m % 16) * 4 + n % 4;
-    float g = (float)cells[at], u = (float)cells[MB * 256 + at];
+    const int at = (n / 16 * MB + m / 16) * 256 + ((n % 16 / 4) * 16 + m % 16) * 4 + n % 4;
+    float g = (float)cells[at], u = (float)cells[H * MB * 256 + at];
     if constexpr (sizeof(E) == 1) {
       g = g * a.x_scale[m] * a.gate_scale[f0 + n];
       u = u * a.x_scale[m] * a.up_scale[f0 + n];
@@ -147,15 +162,15 @@ template <class E, class O, int MB> __device__ __forceinline__ void gated_skinny
       static_cast<O *>(a.up)[(size_t)m * a.ldup + f0 + n] = (O)u;
   }
 }
-template <class E, int MB> __device__ __forceinline__ void gated_few(const GatedArgs &a) {
-  __shared__ __attribute__((aligned(16))) unsigned char lds[skinny_lds<MB>()];
+template <class E, int MB, int NB, int U> __device__ __forceinline__ void gated_few(const GatedArgs &a) {
+  __shared__ __attribute__((aligned(16))) unsigned char lds[skinny_lds<MB, NB>()];
   if constexpr (sizeof(E) == 1) {
     if (a.out_f16)
-      gated_skinny<E, _Float16, MB>(a, lds);
+      gated_skinny<E, _Float16, MB, NB, U>(a, lds);
     else
-      gated_skinny<E, __bf16, MB>(a, lds);
+      gated_skinny<E, __bf16, MB, NB, U>(a, lds);
   } else {
-    gated_skinny<E, E, MB>(a, lds);
+    gated_skinny<E, E, MB, NB, U>(a, lds);
   }
 }
 
@@ -185,10 +200,11 @@ template <class E> __device__ __forceinline__ void gated_back(const GatedBackArg
   }
 }
 
-template <class E, Layout LA, Layout LB> __device__ __forceinline__ void product_general(const StoreArgs &s) {
+// a product that is stored; `tile` counts its workgroups
+template <class E, Layout LA, Layout LB> __device__ __forceinline__ void product_general(const StoreArgs &s, int tile) {
   __shared__ __attribute__((aligned(1024))) unsigned char lds[4 * 128 * 128];
   mma_general<E, LA, LB, false>(
-      s.mma, lds,
+      s.mma, tile, lds,
       [&](auto &acc, const Tile &t, int wave_m, int wave_n, int lane) {
         begin_tile<4, 4>(s, acc, t.m0 + wave_m, t.n0 + wave_n, lane);
       },
@@ -196,32 +212,51 @@ template <class E, Layout LA, Layout LB> __device__ __forceinline__ void product
         store_tile<E, 4, 4, false>(s, acc, t, t.m0 + wave_m, t.n0 + wave_n, lane, nullptr);
       });
 }
-template <class E, Layout LA, Layout LB, int B, int WM, int WN>
-__device__ __forceinline__ void product_tile(const StoreArgs &s) {
-  constexpr int MI = B / WM / 16, NI = B / WN / 16;
-  __shared__ __attribute__((aligned(1024))) unsigned char lds[pipelined_lds<B, B>()];
-  mma_pipelined<E, LA, LB, false, B, B, WM, WN>(
-      s.mma, lds,
+template <class E, Layout LA, Layout LB, int B>
+__device__ __forceinline__ void product_tile(const StoreArgs &s, int tile, int half_from) {
+  __shared__ __attribute__((aligned(1024))) unsigned char lds[pipelined_lds<B>()];
+  mma_tiles<E, LA, LB, false, B>(
+      s.mma, tile, half_from, lds,
       [&](auto &acc, const Tile &t, int wave_m, int wave_n, int lane) {
+        constexpr int MI = sizeof(acc) / sizeof(acc[0]), NI = sizeof(acc[0]) / sizeof(acc[0][0]);
         begin_tile<MI, NI>(s, acc, t.m0 + wave_m, t.n0 + wave_n, lane);
       },
       [&](auto &acc, const Tile &t, int wave_m, int wave_n, int lane, unsigned char *l) {
+        constexpr int MI = sizeof(acc) / sizeof(acc[0]), NI = sizeof(acc[0]) / sizeof(acc[0][0]);
         store_tile<E, MI, NI, true>(s, acc, t, t.m0 + wave_m, t.n0 + wave_n, lane,
-                                    l + (wave_m / (MI * 16) * WN + wave_n / (NI * 16)) * (MI * NI * 512));
+                                    l + threadIdx.x / kWave * (MI * NI * 512));
       });
 }
+// Up to two products: workgroups below `tiles` belong to the first; half tiles, which
+// come last, to the one their tile belongs to.
+struct OfPair {
+  int which, tile, half_from;
+};
+__device__ __forceinline__ OfPair of_pair(const PairStoreArgs &a) {
+  const int wg = blockIdx.x, from = a.p[0].mma.half_from;
+  const int tile = wg < from ? wg : from + (wg - from) / 2; // among the tiles of both
+  const int which = tile >= a.tiles ? 1 : 0, first = which * a.tiles;
+  // the product's own count, with its half tiles from half_from on
+  const int half_from = max(0, min(from - first, a.tiles));
+  const int own = tile - first;
+  return {which, own < half_from ? own : half_from + 2 * (own - half_from) + (wg - from) % 2, half_from};
+}
 
-// the partial sums of the splits, added in the order of the splits
+// the partial sums of the splits, added in the order of the splits, four columns a lane
+// (rows of partial sums are padded to a multiple of 8)
 template <class E> __device__ __forceinline__ void fold(const FoldArgs &a) {
-  const uint64_t total = (uint64_t)a.rows * a.cols;
+  const uint32_t quads = (a.cols + 3) / 4;
+  const uint64_t total = (uint64_t)a.rows * quads;
   const float by = a.undo ? *a.undo : 1.0f;
   for (uint64_t id = (uint64_t)blockIdx.x * blockDim.x + threadIdx.x; id < total;
        id += (uint64_t)gridDim.x * blockDim.x) {
-    const uint32_t r = (uint32_t)(id / a.cols), c = (uint32_t)(id % a.cols);
-    float v = 0.0f;
-    for (uint32_t s = 0; s < a.splits; ++s)
-      v += a.partial[((size_t)s * a.rows + r) * a.ldp + c];
-    static_cast<E *>(a.out)[(size_t)r * a.ldo + c] = (E)(v * by);
+    const uint32_t r = (uint32_t)(id / quads), c = (uint32_t)(id % quads) * 4;
+    const float *from = a.partial + (size_t)r * a.ldp + c;
+    f32x4 v = *reinterpret_cast<const f32x4 *>(from);
+#pragma unroll 4
+    for (uint32_t s = 1; s < a.splits; ++s)
+      v += *reinterpret_cast<const f32x4 *>(from + (size_t)s * a.rows * a.ldp);
+    store4<E>(static_cast<E *>(a.out) + (size_t)r * a.ldo, (int)c, 0, (int)a.cols, v * by);
   }
 }
 
@@ -232,23 +267,20 @@ template <class E> __device__ __forceinline__ void fold(const FoldArgs &a) {
     gated_general<E>(a);                                                                                  \
   }                                                                                                       \
   extern "C" __global__ __launch_bounds__(512) void hcamd_gated_##SUFFIX##_t256(GatedArgs a) {            \
-    gated_tile<E, 256, 2, 4>(a);                                                                          \
+    gated_tile<E, 256>(a);                                                                          \
   }                                                                                                       \
   extern "C" __global__ __launch_bounds__(256) void hcamd_gated_##SUFFIX##_t128(GatedArgs a) {            \
-    gated_tile<E, 128, 2, 2>(a);                                                                          \
+    gated_tile<E, 128>(a);                                                                          \
   }
 HCAMD_FFN(bf16, __bf16)
 HCAMD_FFN(f16, _Float16)
 HCAMD_FFN(i8, int8_t)
 #define HCAMD_FFN_FEW(SUFFIX, E)                                                                          \
   extern "C" __global__ __launch_bounds__(512) void hcamd_gated_##SUFFIX##_s16(GatedArgs a) {             \
-    gated_few<E, 1>(a);                                                                                   \
+    gated_few<E, 1, S16NB, S16U>(a);                                                                      \
   }                                                                                                       \
   extern "C" __global__ __launch_bounds__(512) void hcamd_gated_##SUFFIX##_s32(GatedArgs a) {             \
-    gated_few<E, 2>(a);                                                                                   \
-  }                                                                                                       \
-  extern "C" __global__ __launch_bounds__(512) void hcamd_gated_##SUFFIX##_s64(GatedArgs a) {             \
-    gated_few<E, 4>(a);                                                                                   \
+    gated_few<E, 2, S32NB, S32U>(a);                                                                      \
   }
 HCAMD_FFN_FEW(bf16, __bf16)
 HCAMD_FFN_FEW(f16, _Float16)
@@ -258,22 +290,25 @@ HCAMD_FFN_FEW(i8, int8_t)
     gated_back<E>(a);                                                                                     \
   }                                                                                                       \
   extern "C" __global__ __launch_bounds__(256) void hcamd_product_nn_##SUFFIX##_general(StoreArgs a) {    \
-    product_general<E, kKFast, kKSlow>(a);                                                                                   \
+    product_general<E, kKFast, kKSlow>(a, blockIdx.x);                                                                                   \
   }                                                                                                       \
   extern "C" __global__ __launch_bounds__(256) void hcamd_product_tn_##SUFFIX##_general(PairStoreArgs a) { \
-    product_general<E, kKSlow, kKSlow>(a.p[blockIdx.z]);                                                                                     \
+    const OfPair o = of_pair(a);                                                                          \
+    product_general<E, kKSlow, kKSlow>(a.p[o.which], o.tile);                                                                                     \
   }                                                                                                       \
   extern "C" __global__ __launch_bounds__(512) void hcamd_product_nn_##SUFFIX##_t256(StoreArgs a) {       \
-    product_tile<E, kKFast, kKSlow, 256, 2, 4>(a);                                                        \
+    product_tile<E, kKFast, kKSlow, 256>(a, blockIdx.x, a.mma.half_from);                                                        \
   }                                                                                                       \
   extern "C" __global__ __launch_bounds__(256) void hcamd_product_nn_##SUFFIX##_t128(StoreArgs a) {       \
-    product_tile<E, kKFast, kKSlow, 128, 2, 2>(a);                                                        \
+    product_tile<E, kKFast, kKSlow, 128>(a, blockIdx.x, 0);                                                        \
   }                                                                                                       \
   extern "C" __global__ __launch_bounds__(512) void hcamd_product_tn_##SUFFIX##_t256(PairStoreArgs a) {   \
-    product_tile<E, kKSlow, kKSlow, 256, 2, 4>(a.p[blockIdx.z]);                                          \
+    const OfPair o = of_pair(a);                                                                          \
+    product_tile<E, kKSlow, kKSlow, 256>(a.p[o.which], o.tile, o.half_from);                                          \
   }                                                                                                       \
   extern "C" __global__ __launch_bounds__(256) void hcamd_product_tn_##SUFFIX##_t128(PairStoreArgs a) {   \
-    product_tile<E, kKSlow, kKSlow, 128, 2, 2>(a.p[blockIdx.z]);                                          \
+    const OfPair o = of_pair(a);                                                                          \
+    product_tile<E, kKSlow, kKSlow, 128>(a.p[o.which], o.tile, o.half_from);                                          \
   }                                                                                                       \
   extern "C" __global__ __launch_bounds__(256) void hcamd_fold_##SUFFIX(FoldArgs a) { fold<E>(a); }
 HCAMD_FFN_BACK(bf16, __bf16)

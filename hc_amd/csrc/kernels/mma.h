@@ -23,6 +23,12 @@
 
 #include <type_traits>
 
+#ifndef SPT
+#define SPT 8
+#define SPN 4
+#define EVS 18
+#define EVN 10
+#endif
 namespace hcamd {
 
 enum Layout { kKFast = 0, kKSlow = 1 };
@@ -115,13 +121,14 @@ struct Tile {
 // projections of the same outputs.
 // ---------------------------------------------------------------------------
 template <class E, Layout LA, Layout LB, bool GATED, class Init, class Epilogue>
-__device__ __forceinline__ void mma_general(const MmaArgs &g, unsigned char *lds, Init &&init, Epilogue &&epilogue) {
+__device__ __forceinline__ void mma_general(const MmaArgs &g, int wg, unsigned char *lds, Init &&init,
+                                            Epilogue &&epilogue) {
   using T = MmaType<E>;
   constexpr int BM = 128, BN = 128, BNO = GATED ? BN / 2 : BN;
   constexpr int kPanel = 128 * 128, kStage = 2 * kPanel;
   static_assert(sizeof(E) == 2 || (LA == kKFast && LB == kKFast), "transposed reads are for 16-bit elements");
   int tm, tn;
-  tile_of(blockIdx.x, (g.M + BM - 1) / BM, (g.N + BNO - 1) / BNO, tm, tn);
+  tile_of(wg, (g.M + BM - 1) / BM, (g.N + BNO - 1) / BNO, tm, tn);
   const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
   const int wave_m = wave / 2 * 64, wave_n = wave % 2 * 64;
   const int tiles_k = (g.K + T::kBK - 1) / T::kBK, all = tiles_k * g.segments;
@@ -232,10 +239,10 @@ constexpr int waitcnt_imm(int vmcnt, int lgkmcnt) {
 constexpr int kNoVm = 63, kNoLgkm = 15;
 typedef __attribute__((address_space(3))) void *lds_void_ptr;
 
-template <int BM, int BN> constexpr int pipelined_lds() { return 2 * (BM + BN) * 128; }
+template <int B> constexpr int pipelined_lds() { return 4 * B * 128; }
 
 template <class E, Layout LA, Layout LB, bool GATED, int BM, int BN, int WM, int WN, class Init, class Epilogue>
-__device__ __forceinline__ void mma_pipelined(const MmaArgs &g, unsigned char *lds, Init &&init,
+__device__ __forceinline__ void mma_pipelined(const MmaArgs &g, int m_lo, int tn, unsigned char *lds, Init &&init,
                                               Epilogue &&epilogue) {
   using T = MmaType<E>;
   constexpr int kWaves = WM * WN, kWaveM = BM / WM, kWaveN = BN / WN;
@@ -249,9 +256,9 @@ __device__ __forceinline__ void mma_pipelined(const MmaArgs &g, unsigned char *l
   // half of a tile), and as late as there is time for them (first half), when the
   // loads of the half before have had most of a tile to land.
   constexpr int kSlow = (LA == kKSlow ? kMI : 0) + (LB == kKSlow ? kNI : 0), kQuick = kReads - kSlow;
-  constexpr int kSlowSpan = kSlow == 0 ? 0 : kSlow * kMfma / 32 > kMfma / 4 ? kMfma / 4 : kMfma / 8;
+  constexpr int kSlowSpan = kSlow == 0 ? 0 : kSlow * kMfma / 32 > kMfma / 4 ? kMfma * SPT / 32 : kMfma * SPN / 32;
   constexpr int LF = kSlow == 0 ? 1 : kSlowSpan;
-  constexpr int LS = kSlow == 0 ? kMfma / kLoads : kMfma / 2 / kLoads > 0 ? kMfma / 2 / kLoads : 1;
+  constexpr int LS = kSlow == 0 ? kMfma / kLoads : (kMfma * 3 / 4 - LF) / kLoads;
   static_assert(LF + (kLoads - 1) * LS < kMfma, "every load has its MFMA");
   // read r of a half, in the order B blocks, A blocks (as the MFMAs take them); first:
   // the half that reads the same tile's second half
@@ -261,20 +268,18 @@ __device__ __forceinline__ void mma_pipelined(const MmaArgs &g, unsigned char *l
     if (kSlow == 0)
       return nth * (kMfma / 2) / kReads;
     if (slow)
-      return first ? kMfma * 9 / 16 + nth * (kMfma * 5 / 16) / kSlow : nth * kSlowSpan / kSlow;
+      return first ? kMfma * EVS / 32 + nth * (kMfma * EVN / 32) / kSlow : nth * kSlowSpan / kSlow;
     return (first ? 0 : kSlowSpan) + nth * (kMfma / 2) / (kQuick ? kQuick : 1);
   };
   constexpr int kPanelA = BM * 128, kStage = (BM + BN) * 128;
   constexpr int BNO = GATED ? BN / 2 : BN;
   static_assert(sizeof(E) == 2 || (LA == kKFast && LB == kKFast), "transposed reads are for 16-bit elements");
 
-  int tm, tn;
-  tile_of(blockIdx.x, (g.M + BM - 1) / BM, (g.N + BNO - 1) / BNO, tm, tn);
   // (k-slow rows come in aligned pieces of 8: their origin stays a multiple of 8)
   const int end_m = LA == kKSlow ? (g.M + 7) & ~7 : g.M, end_n = LB == kKSlow ? (g.N + 7) & ~7 : g.N;
   constexpr bool kFewRows = BM == 128 && LA == kKFast; // M may be less than a tile
-  const Tile tile = {kFewRows ? max(min(tm * BM, end_m - BM), 0) : min(tm * BM, end_m - BM),
-                     min(tn * BNO, end_n - BNO), tm * BM, tn * BNO, tn};
+  const Tile tile = {kFewRows ? max(min(m_lo, end_m - BM), 0) : min(m_lo, end_m - BM), min(tn * BNO, end_n - BNO), m_lo,
+                     tn * BNO, tn};
   const int lane = threadIdx.x % kWave;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int wave_m = wave / WN * kWaveM, wave_n = wave % WN * kWaveN;
@@ -297,7 +302,11 @@ __device__ __forceinline__ void mma_pipelined(const MmaArgs &g, unsigned char *l
   struct Lane {
     int off, cut;
   };
-  auto lane_part = [&](Layout l, int R, int ld, bool tail) {
+  // (k-slow: the k of consecutive loads of a wave differ by kWaves * 512 / R, 16 or 8; with
+  // 8 the swizzle of every other load differs, in its third bit)
+  constexpr int kParA = LA == kKSlow && kWaves * 512 / BM % 16 ? 2 : 1;
+  constexpr int kParB = LB == kKSlow && kWaves * 512 / BN % 16 ? 2 : 1;
+  auto lane_part = [&](Layout l, int R, int ld, bool tail, int odd) {
     Lane p;
     if (l == kKFast) {
       const int chunk = (tail && fast_chunk >= tail_chunks ? 0 : fast_chunk) * 16, left = g.M % 8;
@@ -305,21 +314,21 @@ __device__ __forceinline__ void mma_pipelined(const MmaArgs &g, unsigned char *l
       p.cut = (left ? min(lane / 8, left - 1) : lane / 8) * ld + chunk; // (A with few rows only)
     } else {
       const int per = 512 / R, sub = lane / (R / 8), pos = lane % (R / 8);
-      // (the k of a load differ from these by multiples of 16 or of 4 * kWaves: the swizzle is the lane's)
-      const int col = ((pos / 2) ^ slow_swizzle(wave * per + sub)) * 16 + pos % 2 * 8;
+      const int col = ((pos / 2) ^ slow_swizzle(wave * per + sub) ^ (odd * 4)) * 16 + pos % 2 * 8;
       const int left = tail_k % per;
       p.off = sub * ld + col * 2;
       p.cut = (tail && left ? min(sub, left - 1) : sub) * ld + col * 2;
     }
     return p;
   };
-  static_assert(LA == kKFast || (kWaves * 512 / BM) % 16 == 0, "the swizzle repeats from load to load");
-  static_assert(LB == kKFast || (kWaves * 512 / BN) % 16 == 0, "the swizzle repeats from load to load");
+  static_assert(LA == kKFast || kWaves * 512 / BM % 8 == 0, "the swizzle repeats from load to load");
+  static_assert(LB == kKFast || kWaves * 512 / BN % 8 == 0, "the swizzle repeats from load to load");
   // GATED: rows of the N panel alternate in 32s between the two matrices; eight waves
   // meet one of them in all their loads, four waves the other one in every other
   constexpr int kBOps = GATED && kWaves == 4 ? 2 : 1;
+  static_assert(!GATED || kParB == 1, "");
   const int my_b = GATED && kWaves == 8 ? wave / 4 : 0;
-  Lane lane_a, lane_b[kBOps];
+  Lane lane_a[kParA], lane_b[kBOps * kParB];
   int ld_a, ld_b[kBOps];
   __amdgpu_buffer_rsrc_t rsrc_a, rsrc_b[kBOps];
   auto rsrc_of = [&](const void *p, size_t bytes) {
@@ -341,12 +350,16 @@ __device__ __forceinline__ void mma_pipelined(const MmaArgs &g, unsigned char *l
     const int want = seg * 2 + (is_tail(kt) ? 1 : 0);
     if (want != state) {
       ld_a = (int)g.lda[seg] * (int)sizeof(E);
-      lane_a = lane_part(LA, BM, ld_a, want & 1);
+#pragma unroll
+      for (int o = 0; o < kParA; ++o)
+        lane_a[o] = lane_part(LA, BM, ld_a, want & 1, o);
 #pragma unroll
       for (int o = 0; o < kBOps; ++o) {
         const int w = GATED ? (kBOps == 2 ? o : my_b) : seg;
         ld_b[o] = (int)(w ? g.ldb[1] : g.ldb[0]) * (int)sizeof(E);
-        lane_b[o] = lane_part(LB, BN, ld_b[o], want & 1);
+#pragma unroll
+        for (int q = 0; q < kParB; ++q)
+          lane_b[o * kParB + q] = lane_part(LB, BN, ld_b[o], want & 1, q);
       }
       state = want;
     }
@@ -369,14 +382,14 @@ __device__ __forceinline__ void mma_pipelined(const MmaArgs &g, unsigned char *l
     unsigned char *base = lds + buf * kStage + wave * 1024;
     if (v < kALoads) {
       const int first = (v * kWaves + wave) * (LA == kKFast ? 8 : 512 / BM);
-      fetch(LA, BM, rsrc_a, lane_a, ld_a, first, base + v * kWaves * 1024, kFewRows);
+      fetch(LA, BM, rsrc_a, lane_a[v % kParA], ld_a, first, base + v * kWaves * 1024, kFewRows);
     } else {
       const int b = v - kALoads;
       int first = (b * kWaves + wave) * (LB == kKFast ? 8 : 512 / BN);
       if constexpr (GATED)
         first = first / 64 * 32 + first % 32;
       const int o = kBOps == 2 ? b % 2 : 0;
-      fetch(LB, BN, rsrc_b[o], lane_b[o], ld_b[o], first, base + kPanelA + b * kWaves * 1024, false);
+      fetch(LB, BN, rsrc_b[o], lane_b[o * kParB + b % kParB], ld_b[o], first, base + kPanelA + b * kWaves * 1024, false);
     }
   };
   auto zero_tail = [&](int buf) {
@@ -433,12 +446,13 @@ __device__ __forceinline__ void mma_pipelined(const MmaArgs &g, unsigned char *l
   init(acc, tile, wave_m, wave_n, lane);
   using Slot0 = std::integral_constant<int, 0>;
   using Slot1 = std::integral_constant<int, 1>;
-  // MFMAs in a serpentine over the blocks: consecutive ones share an operand
+  // MFMAs in a serpentine over the blocks: consecutive ones share an operand (four
+  // waves: row by row, the serpentine costs them)
   auto half_step = [&](auto use, auto fill, int buf, int h, bool do_read, bool do_load, int load_buf) {
     constexpr int Uu = decltype(use)::value;
 #pragma unroll
     for (int slot = 0; slot < kMfma; ++slot) {
-      const int i = slot / kNI, j = i % 2 ? kNI - 1 - slot % kNI : slot % kNI;
+      const int i = slot / kNI, j = kWaves == 8 && i % 2 ? kNI - 1 - slot % kNI : slot % kNI;
       if (do_read) {
 #pragma unroll
         for (int r = 0; r < kReads; ++r)
@@ -507,51 +521,78 @@ __device__ __forceinline__ void mma_pipelined(const MmaArgs &g, unsigned char *l
   epilogue(acc, tile, wave_m, wave_n, lane, lds);
 }
 
+// The tiles of a launch: 128 x 128, or 256 x 256 of which those from half_from on are
+// worked as two halves of 128 rows.  A last round of tiles that fills at most half the
+// card then takes half as long (4096 x 11264 outputs of the gated block: 5.5 rounds
+// instead of 6).  `tile` counts the launch's workgroups from this product's first.
+template <class E, Layout LA, Layout LB, bool GATED, int B, class Init, class Epilogue>
+__device__ __forceinline__ void mma_tiles(const MmaArgs &g, int tile, int half_from, unsigned char *lds, Init &&init,
+                                          Epilogue &&epilogue) {
+  constexpr int BNO = GATED ? B / 2 : B;
+  const int tiles_m = (g.M + B - 1) / B, tiles_n = (g.N + BNO - 1) / BNO;
+  int tm, tn;
+  if constexpr (B == 128) {
+    tile_of(tile, tiles_m, tiles_n, tm, tn);
+    mma_pipelined<E, LA, LB, GATED, 128, 128, 2, 2>(g, tm * 128, tn, lds, init, epilogue);
+  } else {
+    if (tile < half_from) {
+      tile_of(tile, tiles_m, tiles_n, tm, tn);
+      mma_pipelined<E, LA, LB, GATED, 256, 256, 2, 4>(g, tm * 256, tn, lds, init, epilogue);
+    } else {
+      tile_of(half_from + (tile - half_from) / 2, tiles_m, tiles_n, tm, tn);
+      const int m_lo = tm * 256 + (tile - half_from) % 2 * 128;
+      if (m_lo < g.M)
+        mma_pipelined<E, LA, LB, GATED, 128, 256, 2, 4>(g, m_lo, tn, lds, init, epilogue);
+    }
+  }
+}
+
 // ---------------------------------------------------------------------------
-// Few tokens: M <= 16 * MB rows of A against 32 rows of B, for products that are one
-// pass over B.  Eight waves share the k of the tile; each reads B and A straight into
+// Few tokens: M <= 16 * MB rows of A against NB blocks of sixteen rows of B, for
+// products that are one pass over B.  Eight waves share the k of the tile; each reads B and A straight into
 // MFMA operand registers (sixteen rows, 64 consecutive bytes of a row per four lanes;
 // which k a lane holds does not matter as long as both operands agree), the next block
 // of k is requested before the present one is multiplied, and the eight partial sums
 // meet in LDS.  Any size and alignment: rows past the end are read from the last one and
 // not stored, pieces that cross K go element by element.
-//   b0, b1: first rows of the two blocks of sixteen; last0, last1: rows left from there
-// The result lies in LDS as float or int [2][MB][256], element (m, n) of a block at
+//   row_of(j): this lane's row lane % 16 of block j
+// The result lies in LDS as float or int [NB][MB][256], element (m, n) of a block at
 // ((n / 4) * 16 + m) * 4 + n % 4.
 // ---------------------------------------------------------------------------
-template <int MB> constexpr int skinny_lds() { return 8 * 2 * MB * 1024; }
+template <int MB, int NB> constexpr int skinny_lds() { return 8 * NB * MB * 1024; }
 
-template <class E, int MB>
-__device__ __forceinline__ void mma_skinny(const MmaArgs &g, const E *b0, size_t ld0, int rows0, const E *b1,
-                                           size_t ld1, int rows1, unsigned char *lds) {
+template <class E, int MB, int NB, int U, class R>
+__device__ __forceinline__ void mma_skinny(const MmaArgs &g, R &&row_of, unsigned char *lds) {
   using T = MmaType<E>;
-  constexpr int U = 4, kStep = 4 * T::kChunk, kBlock = U * kStep;
+  constexpr int kStep = 4 * T::kChunk, kBlock = U * kStep;
   const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int row = lane % 16, k_lane = lane / 16 * T::kChunk;
-  const E *pb[2] = {b0 + (size_t)min(row, rows0 - 1) * ld0 + k_lane, b1 + (size_t)min(row, rows1 - 1) * ld1 + k_lane};
-  const E *pa[MB];
+  const E *pb[NB], *pa[MB];
+#pragma unroll
+  for (int j = 0; j < NB; ++j)
+    pb[j] = row_of(j) + k_lane;
 #pragma unroll
   for (int i = 0; i < MB; ++i)
     pa[i] = static_cast<const E *>(g.a[0]) + (size_t)min(i * 16 + row, g.M - 1) * g.lda[0] + k_lane;
-  typename T::acc acc[2][MB] = {};
-  u32x4 fb[2][U], fa[MB][U];
+  typename T::acc acc[NB][MB] = {};
+  u32x4 fb[NB][U], fa[MB][U];
   auto request = [&](int block) {
     const int k = block * kBlock;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
 #pragma unroll
-      for (int j = 0; j < 2; ++j)
+      for (int j = 0; j < NB; ++j)
         fb[j][u] = *reinterpret_cast<const u32x4_u *>(pb[j] + k + u * kStep);
 #pragma unroll
       for (int i = 0; i < MB; ++i)
         fa[i][u] = *reinterpret_cast<const u32x4_u *>(pa[i] + k + u * kStep);
     }
   };
-  auto multiply = [&](const u32x4 (&b)[2][U], const u32x4 (&a)[MB][U]) {
+  auto multiply = [&](const u32x4 (&b)[NB][U], const u32x4 (&a)[MB][U]) {
 #pragma unroll
     for (int u = 0; u < U; ++u)
 #pragma unroll
-      for (int j = 0; j < 2; ++j)
+      for (int j = 0; j < NB; ++j)
 #pragma unroll
         for (int i = 0; i < MB; ++i)
           acc[j][i] = mma16<E>(b[j][u], a[i][u], acc[j][i]);
@@ -560,11 +601,11 @@ __device__ __forceinline__ void mma_skinny(const MmaArgs &g, const E *b0, size_t
   if (wave < blocks)
     request(wave);
   for (int block = wave; block < blocks; block += 8) {
-    u32x4 b[2][U], a[MB][U];
+    u32x4 b[NB][U], a[MB][U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
 #pragma unroll
-      for (int j = 0; j < 2; ++j)
+      for (int j = 0; j < NB; ++j)
         b[j][u] = fb[j][u];
 #pragma unroll
       for (int i = 0; i < MB; ++i)
@@ -580,7 +621,7 @@ __device__ __forceinline__ void mma_skinny(const MmaArgs &g, const E *b0, size_t
     for (int u = 0; u < U; ++u) {
       const int valid = g.K - (k + u * kStep + k_lane);
 #pragma unroll
-      for (int j = 0; j < 2; ++j)
+      for (int j = 0; j < NB; ++j)
         fb[j][u] = load_chunk(pb[j] + k + u * kStep, valid);
 #pragma unroll
       for (int i = 0; i < MB; ++i)
@@ -589,19 +630,19 @@ __device__ __forceinline__ void mma_skinny(const MmaArgs &g, const E *b0, size_t
     multiply(fb, fa);
   }
   using V = typename T::acc;
-  V *cells = reinterpret_cast<V *>(lds); // [8][2][MB][64]
+  V *cells = reinterpret_cast<V *>(lds); // [8][NB][MB][64]
 #pragma unroll
-  for (int j = 0; j < 2; ++j)
+  for (int j = 0; j < NB; ++j)
 #pragma unroll
     for (int i = 0; i < MB; ++i)
-      cells[((wave * 2 + j) * MB + i) * kWave + lane] = acc[j][i];
+      cells[((wave * NB + j) * MB + i) * kWave + lane] = acc[j][i];
   __syncthreads();
   // the eight waves' sums, added in their order, four elements a thread
-  for (int c = threadIdx.x; c < 2 * MB * kWave; c += 512) {
+  for (int c = threadIdx.x; c < NB * MB * kWave; c += 512) {
     V sum = cells[c];
 #pragma unroll
     for (int w = 1; w < 8; ++w)
-      sum += cells[w * (2 * MB * kWave) + c];
+      sum += cells[w * (NB * MB * kWave) + c];
     cells[c] = sum; // (only this thread reads or writes this cell here)
   }
   __syncthreads();

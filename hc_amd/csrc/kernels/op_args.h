@@ -36,6 +36,7 @@ struct MmaArgs {
   int M, N, K;
   int segments;   // 1, or 2: k runs through (a[0], b[0]), then (a[1], b[1])
   int splits;     // k tiles are dealt to this many workgroups (grid y)
+  int half_from;  // 256 x 256 tiles from here on are worked as two halves
 };
 
 struct GatedArgs {
@@ -64,8 +65,9 @@ struct StoreArgs {
   const float *undo; // when not null: *undo multiplies what goes to `out`
   int accumulate;      // add to `partial` instead of replacing it
 };
-struct PairStoreArgs { // two products of one shape, selected by grid z
+struct PairStoreArgs { // two products of one shape, one after the other in grid x
   StoreArgs p[2];
+  int tiles; // of one of them
 };
 struct FoldArgs { // out = sum over splits of partial (* *undo)
   const float *partial;

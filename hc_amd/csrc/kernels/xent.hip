@@ -12,6 +12,12 @@
 // A target below 0 takes its row out: loss 0, no gradient.  A target of V or more
 // is an error of the caller's: loss NaN, no gradient.
 #include "mma.h"
+#ifndef S16NB
+#define S16NB 2
+#define S16U 4
+#define S32NB 4
+#define S32U 2
+#endif
 
 using namespace hcamd;
 
@@ -99,50 +105,63 @@ __device__ __forceinline__ void tile_stats(const XentArgs &a, f32x4 (&acc)[MI][N
 template <class E> __device__ __forceinline__ void stats_general(const XentArgs &a) {
   __shared__ __attribute__((aligned(1024))) unsigned char lds[4 * 128 * 128];
   mma_general<E, kKFast, kKFast, false>(
-      a.mma, lds, FromZero{}, [&](auto &acc, const Tile &t, int wave_m, int wave_n, int lane, unsigned char *l) {
+      a.mma, blockIdx.x, lds, FromZero{},
+      [&](auto &acc, const Tile &t, int wave_m, int wave_n, int lane, unsigned char *l) {
         // (the main loop ends with a barrier: its stages are free)
         tile_stats<4, 4, 2, 128, 128>(a, acc, t, wave_m, wave_n, lane, reinterpret_cast<float *>(l));
       });
 }
 
-template <class E, int B, int WM, int WN> __device__ __forceinline__ void stats_tile(const XentArgs &a) {
-  constexpr int MI = B / WM / 16, NI = B / WN / 16;
-  __shared__ __attribute__((aligned(1024))) unsigned char lds[pipelined_lds<B, B>()];
-  mma_pipelined<E, kKFast, kKFast, false, B, B, WM, WN>(
-      a.mma, lds, FromZero{}, [&](auto &acc, const Tile &t, int wave_m, int wave_n, int lane, unsigned char *l) {
-        tile_stats<MI, NI, WN, B, B>(a, acc, t, wave_m, wave_n, lane, reinterpret_cast<float *>(l));
+template <class E, int B> __device__ __forceinline__ void stats_tile(const XentArgs &a) {
+  __shared__ __attribute__((aligned(1024))) unsigned char lds[pipelined_lds<B>()];
+  mma_tiles<E, kKFast, kKFast, false, B>(
+      a.mma, blockIdx.x, a.mma.half_from, lds, FromZero{},
+      [&](auto &acc, const Tile &t, int wave_m, int wave_n, int lane, unsigned char *l) {
+        constexpr int MI = sizeof(acc) / sizeof(acc[0]), NI = sizeof(acc[0]) / sizeof(acc[0][0]);
+        constexpr int WN = B / (NI * 16), BM = MI * 16 * 2;
+        tile_stats<MI, NI, WN, BM, B>(a, acc, t, wave_m, wave_n, lane, reinterpret_cast<float *>(l));
       });
 }
 
-// Few tokens: one pass over the weight, 32 of its rows a workgroup.
-template <class E, int MB> __device__ __forceinline__ void stats_few(const XentArgs &a) {
-  __shared__ __attribute__((aligned(16))) unsigned char lds[skinny_lds<MB>()];
-  const int n0 = blockIdx.x * 32, left = a.mma.N - n0;
-  const size_t ld = a.mma.ldb[0];
-  const E *b = static_cast<const E *>(a.mma.b[0]) + (size_t)n0 * ld;
-  // (a second block past the end reads the first one's rows and is left out below)
-  mma_skinny<E, MB>(a.mma, b, ld, left, left > 16 ? b + 16 * ld : b, ld, left > 16 ? left - 16 : left, lds);
+// Few tokens: one pass over the weight, NB * 16 of its rows a workgroup.
+template <class E, int MB, int NB, int U> __device__ __forceinline__ void stats_few(const XentArgs &a) {
+  __shared__ __attribute__((aligned(16))) unsigned char lds[skinny_lds<MB, NB>()];
+  const int n0 = blockIdx.x * (NB * 16), left = a.mma.N - n0;
+  mma_skinny<E, MB, NB, U>(
+      a.mma,
+      [&](int j) {
+        const int n = min(n0 + j * 16 + (int)threadIdx.x % 16, a.mma.N - 1);
+        return static_cast<const E *>(a.mma.b[0]) + (size_t)n * a.mma.ldb[0];
+      },
+      lds);
   const float *cells = reinterpret_cast<const float *>(lds);
   for (int c = threadIdx.x; c < MB * 256; c += 512) {
-    const int n = c % 16, m = c / 16; // sixteen lanes share a row
+    const int n = c % 16, m = c / 16; // sixteen lanes share a row, a column of each block
     const int at = m / 16 * 256 + ((n / 4) * 16 + m % 16) * 4 + n % 4;
-    const float z0 = n < left ? cells[at] : -INFINITY, z1 = n + 16 < left ? cells[MB * 256 + at] : -INFINITY;
-    float most = fmaxf(z0, z1);
+    float z[NB], most = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < NB; ++j) {
+      z[j] = n + j * 16 < left ? cells[j * MB * 256 + at] : -INFINITY;
+      most = fmaxf(most, z[j]);
+    }
 #pragma unroll
     for (int o = 8; o > 0; o >>= 1)
       most = fmaxf(most, __shfl_xor(most, o));
     const float from = most == -INFINITY ? 0.0f : most;
-    float sum = __expf(z0 - from) + __expf(z1 - from);
+    float sum = 0.0f;
+#pragma unroll
+    for (int j = 0; j < NB; ++j)
+      sum += __expf(z[j] - from);
 #pragma unroll
     for (int o = 8; o > 0; o >>= 1)
       sum += __shfl_xor(sum, o);
     if (m >= a.mma.M)
       continue;
     const int64_t t = target_of(a.targets, a.target_i64, m) - n0;
-    if (t == n && n < left)
-      a.zt[m] = z0;
-    if (t == n + 16 && n + 16 < left)
-      a.zt[m] = z1;
+#pragma unroll
+    for (int j = 0; j < NB; ++j)
+      if (t == n + j * 16 && n + j * 16 < left)
+        a.zt[m] = z[j];
     if (n == 0) {
       float *cell = a.stats + ((size_t)m * a.tiles + blockIdx.x) * 2;
       cell[0] = most;
@@ -196,17 +215,19 @@ __device__ __forceinline__ void tile_p(const XentArgs &a, f32x4 (&acc)[MI][NI], 
 template <class E> __device__ __forceinline__ void p_general(const XentArgs &a) {
   __shared__ __attribute__((aligned(1024))) unsigned char lds[4 * 128 * 128];
   mma_general<E, kKFast, kKFast, false>(
-      a.mma, lds, FromZero{}, [&](auto &acc, const Tile &t, int wave_m, int wave_n, int lane, unsigned char *) {
+      a.mma, blockIdx.x, lds, FromZero{},
+      [&](auto &acc, const Tile &t, int wave_m, int wave_n, int lane, unsigned char *) {
         tile_p<E, 4, 4, false>(a, acc, t, t.m0 + wave_m, t.n0 + wave_n, lane, nullptr);
       });
 }
-template <class E, int B, int WM, int WN> __device__ __forceinline__ void p_tile(const XentArgs &a) {
-  constexpr int MI = B / WM / 16, NI = B / WN / 16;
-  __shared__ __attribute__((aligned(1024))) unsigned char lds[pipelined_lds<B, B>()];
-  mma_pipelined<E, kKFast, kKFast, false, B, B, WM, WN>(
-      a.mma, lds, FromZero{}, [&](auto &acc, const Tile &t, int wave_m, int wave_n, int lane, unsigned char *l) {
+template <class E, int B> __device__ __forceinline__ void p_tile(const XentArgs &a) {
+  __shared__ __attribute__((aligned(1024))) unsigned char lds[pipelined_lds<B>()];
+  mma_tiles<E, kKFast, kKFast, false, B>(
+      a.mma, blockIdx.x, a.mma.half_from, lds, FromZero{},
+      [&](auto &acc, const Tile &t, int wave_m, int wave_n, int lane, unsigned char *l) {
+        constexpr int MI = sizeof(acc) / sizeof(acc[0]), NI = sizeof(acc[0]) / sizeof(acc[0][0]);
         tile_p<E, MI, NI, true>(a, acc, t, t.m0 + wave_m, t.n0 + wave_n, lane,
-                                l + (wave_m / (MI * 16) * WN + wave_n / (NI * 16)) * (MI * NI * 512));
+                                l + threadIdx.x / kWave * (MI * NI * 512));
       });
 }
 
@@ -263,28 +284,25 @@ __device__ __forceinline__ void p_factor(const float *grad_loss, uint32_t rows, 
     p_general<E>(a);                                                                                      \
   }                                                                                                       \
   extern "C" __global__ __launch_bounds__(512) void hcamd_xent_stats_##SUFFIX##_t256(XentArgs a) {        \
-    stats_tile<E, 256, 2, 4>(a);                                                                          \
+    stats_tile<E, 256>(a);                                                                          \
   }                                                                                                       \
   extern "C" __global__ __launch_bounds__(256) void hcamd_xent_stats_##SUFFIX##_t128(XentArgs a) {        \
-    stats_tile<E, 128, 2, 2>(a);                                                                          \
+    stats_tile<E, 128>(a);                                                                          \
   }                                                                                                       \
   extern "C" __global__ __launch_bounds__(512) void hcamd_xent_p_##SUFFIX##_t256(XentArgs a) {            \
-    p_tile<E, 256, 2, 4>(a);                                                                              \
+    p_tile<E, 256>(a);                                                                              \
   }                                                                                                       \
   extern "C" __global__ __launch_bounds__(256) void hcamd_xent_p_##SUFFIX##_t128(XentArgs a) {            \
-    p_tile<E, 128, 2, 2>(a);                                                                              \
+    p_tile<E, 128>(a);                                                                              \
   }
 HCAMD_XENT(bf16, __bf16)
 HCAMD_XENT(f16, _Float16)
 #define HCAMD_XENT_FEW(SUFFIX, E)                                                                         \
   extern "C" __global__ __launch_bounds__(512) void hcamd_xent_stats_##SUFFIX##_s16(XentArgs a) {         \
-    stats_few<E, 1>(a);                                                                                   \
+    stats_few<E, 1, S16NB, S16U>(a);                                                                      \
   }                                                                                                       \
   extern "C" __global__ __launch_bounds__(512) void hcamd_xent_stats_##SUFFIX##_s32(XentArgs a) {         \
-    stats_few<E, 2>(a);                                                                                   \
-  }                                                                                                       \
-  extern "C" __global__ __launch_bounds__(512) void hcamd_xent_stats_##SUFFIX##_s64(XentArgs a) {         \
-    stats_few<E, 4>(a);                                                                                   \
+    stats_few<E, 2, S32NB, S32U>(a);                                                                      \
   }
 HCAMD_XENT_FEW(bf16, __bf16)
 HCAMD_XENT_FEW(f16, _Float16)

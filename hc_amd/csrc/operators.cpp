@@ -82,30 +82,50 @@ struct Call {
 
 // ---- tiled products -----------------------------------------------------------
 // Tile and splits of a product, from its shape alone (a workspace is sized before any
-// pointer is seen).  256 x 256 tiles run one workgroup on a compute unit, 128 x 128
-// tiles two.  When the tiles do not fill the card, several workgroups share the k
-// tiles of each, each with at least 8 of them, and no more than 64 MiB of fp32 partial
-// sums in all.
+// pointer is seen): the cheapest by a model of the card's 256 compute units.  Its unit is
+// what a 256 x 256 tile takes for one k tile, 1.65 us at the 1.3 PFLOP/s those kernels
+// reach; measured beside it: two 128 x 128 tiles on a unit 0.64, one alone 0.4, half a
+// 256 x 256 tile 0.55; a tile's beginning and end cost about three k tiles; fp32 partial
+// sums move at 4 TB/s and their folding is one more launch (5 us).
+constexpr size_t kUnits = 256;
 struct Product {
   int tile; // 256 or 128
   int splits;
 };
 size_t padCols(size_t n) { return alignUp(n, 8); }
-int tileOf(size_t m, size_t n) {
+// units of time of `groups` workgroups that each hold one tile's share of k
+double roundsOf(int tile, size_t groups) {
+  if (tile == 128) {
+    const size_t rem = groups % (2 * kUnits);
+    return 0.64 * (groups / (2 * kUnits)) + (rem == 0 ? 0.0 : rem <= kUnits ? 0.4 : 0.64);
+  }
+  const size_t rem = groups % kUnits;
+  return (double)(groups / kUnits) + (rem == 0 ? 0.0 : rem <= kUnits / 2 ? 0.55 : 1.0);
+}
+// `products` of one shape in one launch; maxSplits 1: the k of a tile stays with one workgroup
+Product productOf(size_t m, size_t n, size_t k, int segments, size_t products, size_t maxSplits) {
   const int v = hcamdInternalVariant("mma");
-  if (v == 2 || v == 3)
-    return v == 3 && m >= 256 && n >= 256 ? 256 : 128;
-  return m >= 256 && n >= 256 && ceilDiv(m, 256) * ceilDiv(n, 256) >= 192 ? 256 : 128;
+  const size_t kTiles = ceilDiv(k, (size_t)64) * segments;
+  Product best{128, 1};
+  double least = 1e300;
+  for (int tile : {128, 256}) {
+    if ((tile == 256 && (m < 256 || n < 256 || v == 2)) || (tile == 128 && v == 3 && m >= 256 && n >= 256))
+      continue;
+    const size_t tiles = ceilDiv(m, tile) * ceilDiv(n, tile) * products;
+    for (size_t s = 1; s <= maxSplits && (s == 1 || kTiles / s >= 4); s *= 2) {
+      const double bytes = s > 1 ? (double)s * m * padCols(n) * 4 * products : 0.0;
+      if (bytes > (double)((size_t)128 << 20) * products)
+        break;
+      // (split tiles are not halved)
+      const double rounds = s > 1 && tile == 256 ? (double)ceilDiv(tiles * s, kUnits) : roundsOf(tile, tiles * s);
+      const double cost = rounds * ((double)ceilDiv(kTiles, s) + 3.0) + (s > 1 ? (2 * bytes / 8e12 * 1e6 + 5.0) / 1.65 : 0.0);
+      if (cost < least)
+        least = cost, best = {tile, (int)s};
+    }
+  }
+  return best;
 }
-Product productOf(size_t m, size_t n, size_t k, int segments) {
-  Product p;
-  p.tile = tileOf(m, n);
-  const size_t tiles = ceilDiv(m, p.tile) * ceilDiv(n, p.tile), kTiles = ceilDiv(k, (size_t)64) * segments;
-  size_t s = std::min<size_t>((p.tile == 256 ? 256 : 512) / std::max<size_t>(tiles, 1), kTiles / 8);
-  s = std::min(s, ((size_t)64 << 20) / std::max<size_t>(m * padCols(n) * 4, 1));
-  p.splits = (int)std::max<size_t>(s, 1);
-  return p;
-}
+constexpr size_t kMaxSplits = 64;
 size_t partialBytes(const Product &p, size_t m, size_t n) {
   return p.splits > 1 ? alignUp((size_t)p.splits * m * padCols(n) * 4, 256) : 0;
 }
@@ -119,7 +139,7 @@ bool fetchable(const void *p, size_t ld, size_t along, size_t bytes, bool padded
   return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % piece == 0 && (padded || along % piece == 0) &&
          ld * bytes < ((size_t)1 << 23);
 }
-// The kernel of a product: "general", "t128" or "t256"; `threads` and the tile it uses.
+// The kernel of a product: "general", "t128" or "t256", and its workgroups.
 struct Kernel {
   const char *suffix;
   size_t threads;
@@ -129,26 +149,42 @@ struct Kernel {
 Kernel kernelOf(int tile, size_t m, size_t n, bool fetch, bool fewM) {
   if (!fetch || hcamdInternalVariant("mma") == 1 || (m < 128 && !fewM) || n < 128)
     return {"general", 256, 128};
-  if (tile == 256)
+  if (tile == 256 && m >= 256 && n >= 256)
     return {"t256", 512, 256};
   return {"t128", 256, 128};
 }
-// Up to 64 tokens the forward products are one pass over the weights, which the tiled
-// kernels feed from too few workgroups: one token, 2 x 11264 x 4096 bf16: 94 us tiled.
-// Returns the kernel's suffix, or null.
-constexpr size_t kFewTokens = 64;
-const char *fewSuffix(size_t tokens) {
+// The workgroups of `tiles` tiles: a last round of 256 x 256 tiles that fills at most half
+// the card is worked in halves, from `halfFrom` on.
+size_t groupsOf(const Kernel &k, size_t tiles, int splits, int &halfFrom) {
+  const size_t rem = tiles % kUnits;
+  const bool halves = k.tile == 256 && splits == 1 && rem != 0 && rem <= kUnits / 2;
+  halfFrom = halves ? (int)(tiles - rem) : 0x7fffffff;
+  return halves ? tiles + rem : tiles;
+}
+
+// Up to 32 tokens the forward products are one pass over the weights, which the tiled
+// kernels feed from too few workgroups.
+struct Few {
+  const char *suffix; // null: not for this many tokens
+  int rows;           // weight rows of a workgroup
+};
+#ifndef S16NB
+#define S16NB 2
+#define S32NB 4
+#endif
+constexpr size_t kFewTokens = 32;
+Few fewOf(size_t tokens) {
   const int v = hcamdInternalVariant("mma");
   if (tokens > kFewTokens || (v >= 1 && v <= 3))
-    return nullptr;
-  return tokens <= 16 ? "s16" : tokens <= 32 ? "s32" : "s64";
+    return {nullptr, 128};
+  return tokens <= 16 ? Few{"s16", S16NB * 16} : Few{"s32", S32NB * 16};
 }
 
 int launchFold(const Call &c, int type, const FoldArgs &f) {
   FoldArgs a = f;
   char name[64];
   std::snprintf(name, sizeof(name), "hcamd_fold_%s", typeName(type));
-  return c.launch("ffn", name, a, std::min<size_t>(ceilDiv((size_t)a.rows * a.cols, (size_t)256), 4096));
+  return c.launch("ffn", name, a, std::min<size_t>(ceilDiv((size_t)a.rows * ceilDiv(a.cols, 4), (size_t)256), 4096));
 }
 
 bool dimsOk(const Call &c, size_t a, size_t b, size_t d) {
@@ -355,17 +391,19 @@ int hcamdLaunchGatedFfn(OlQueue q, int elemType, const void *x, size_t ldx, cons
   a.out = out, a.gate = gate, a.up = up, a.ldo = ldo, a.ldgate = ldgate, a.ldup = ldup;
   a.activation = activation, a.out_f16 = outType == HCAMD_F16;
   char name[64];
-  if (const char *few = fewSuffix(tokens)) {
-    std::snprintf(name, sizeof(name), "hcamd_gated_%s_%s", typeName(elemType), few);
-    return c.launch("ffn", name, a, ceilDiv(f, 16), 1, 1, 512);
+  const Few few = fewOf(tokens);
+  if (few.suffix) {
+    std::snprintf(name, sizeof(name), "hcamd_gated_%s_%s", typeName(elemType), few.suffix);
+    return c.launch("ffn", name, a, ceilDiv(f, few.rows / 2), 1, 1, 512);
   }
   // (a tile of outputs takes twice its columns of the two weight matrices)
-  const Kernel k = kernelOf(tileOf(tokens, 2 * f), tokens, 2 * f,
+  const Kernel k = kernelOf(productOf(tokens, 2 * f, i8 ? d / 2 : d, 1, 1, 1).tile, tokens, 2 * f,
                             fetchable(x, ldx, d, e, false) && fetchable(wGate, ldwg, d, e, false) &&
                                 fetchable(wUp, ldwu, d, e, false),
                             true);
   std::snprintf(name, sizeof(name), "hcamd_gated_%s_%s", typeName(elemType), k.suffix);
-  return c.launch("ffn", name, a, ceilDiv(tokens, k.tile) * ceilDiv(f, k.tile / 2), 1, 1, k.threads);
+  const size_t groups = groupsOf(k, ceilDiv(tokens, k.tile) * ceilDiv(f, k.tile / 2), 1, a.mma.half_from);
+  return c.launch("ffn", name, a, groups, 1, 1, k.threads);
 }
 
 namespace {
@@ -379,8 +417,8 @@ FfnBack ffnBack(size_t tokens, size_t d, size_t f) {
   FfnBack b;
   b.ldd = padCols(f);
   b.dg = alignUp(tokens * b.ldd * 2, 256);
-  b.px = productOf(tokens, d, f, 2);
-  b.pw = productOf(f, d, tokens, 1);
+  b.px = productOf(tokens, d, f, 2, 1, kMaxSplits);
+  b.pw = productOf(f, d, tokens, 1, 2, kMaxSplits);
   b.dx = partialBytes(b.px, tokens, d);
   b.dw = partialBytes(b.pw, f, d);
   b.bytes = 2 * b.dg + b.dx + 2 * b.dw;
@@ -447,7 +485,8 @@ int hcamdLaunchGatedFfnBackward(OlQueue q, int elemType, const void *gradOut, si
     const Kernel k = kernelOf(b.px.tile, tokens, d, fetchable(wGate, ldwg, d, 2, false) &&
                                                         fetchable(wUp, ldwu, d, 2, false), true);
     std::snprintf(name, sizeof(name), "hcamd_product_nn_%s_%s", typeName(elemType), k.suffix);
-    if (c.launch("ffn", name, s, ceilDiv(tokens, k.tile) * ceilDiv(d, k.tile), b.px.splits, 1, k.threads))
+    const size_t groups = groupsOf(k, ceilDiv(tokens, k.tile) * ceilDiv(d, k.tile), b.px.splits, s.mma.half_from);
+    if (c.launch("ffn", name, s, groups, b.px.splits, 1, k.threads))
       return 1;
     if (s.partial && launchFold(c, elemType, {s.partial, gradX, s.ldp, ldgx, (uint32_t)tokens, (uint32_t)d,
                                               (uint32_t)b.px.splits, nullptr}))
@@ -470,7 +509,9 @@ int hcamdLaunchGatedFfnBackward(OlQueue q, int elemType, const void *gradOut, si
     }
     const Kernel k = kernelOf(b.pw.tile, f, d, fetchable(x, ldx, d, 2, false), false);
     std::snprintf(name, sizeof(name), "hcamd_product_tn_%s_%s", typeName(elemType), k.suffix);
-    if (c.launch("ffn", name, s, ceilDiv(f, k.tile) * ceilDiv(d, k.tile), b.pw.splits, n, k.threads))
+    s.tiles = (int)(ceilDiv(f, k.tile) * ceilDiv(d, k.tile));
+    const size_t groups = groupsOf(k, s.tiles * n, b.pw.splits, s.p[0].mma.half_from);
+    if (c.launch("ffn", name, s, groups, b.pw.splits, 1, k.threads))
       return 1;
     for (size_t k = 0; b.dw && k < n; ++k)
       if (launchFold(c, elemType, {s.p[k].partial, s.p[k].out, s.p[k].ldp, s.p[k].ldo, (uint32_t)f, (uint32_t)d,
@@ -522,15 +563,16 @@ int hcamdLaunchLinearCrossEntropy(OlQueue q, int elemType, const void *x, size_t
   a.mma.a[0] = x, a.mma.lda[0] = ldx, a.mma.b[0] = weight, a.mma.ldb[0] = ldw;
   a.mma.M = (int)tokens, a.mma.N = (int)vocab, a.mma.K = (int)d, a.mma.segments = a.mma.splits = 1;
   a.targets = targets, a.target_i64 = targetType == HCAMD_I64, a.vocab = (int)vocab;
-  const char *few = fewSuffix(tokens);
-  const Kernel k = kernelOf(tileOf(tokens, vocab), tokens, vocab,
+  const Few few = fewOf(tokens);
+  const Kernel k = kernelOf(productOf(tokens, vocab, d, 1, 1, 1).tile, tokens, vocab,
                             fetchable(x, ldx, d, 2, false) && fetchable(weight, ldw, d, 2, false), true);
-  a.tiles = (int)ceilDiv(vocab, few ? 32 : k.tile);
+  a.tiles = (int)ceilDiv(vocab, few.suffix ? few.rows : k.tile);
   a.stats = static_cast<float *>(work);
   a.zt = a.stats + tokens * a.tiles * 2;
   char name[64];
-  std::snprintf(name, sizeof(name), "hcamd_xent_stats_%s_%s", typeName(elemType), few ? few : k.suffix);
-  if (c.launch("xent", name, a, few ? a.tiles : ceilDiv(tokens, k.tile) * a.tiles, 1, 1, few ? 512 : k.threads))
+  std::snprintf(name, sizeof(name), "hcamd_xent_stats_%s_%s", typeName(elemType), few.suffix ? few.suffix : k.suffix);
+  const size_t groups = few.suffix ? a.tiles : groupsOf(k, ceilDiv(tokens, k.tile) * a.tiles, 1, a.mma.half_from);
+  if (c.launch("xent", name, a, groups, 1, 1, few.suffix ? 512 : k.threads))
     return 1;
   XentRowsArgs r{a.stats, a.zt, targets, a.target_i64, loss, lse, (uint32_t)tokens, (uint32_t)vocab,
                  (uint32_t)a.tiles};
@@ -554,8 +596,8 @@ XentBack xentBack(size_t tokens, size_t d, size_t vocab, size_t piece) {
   b.piece = std::min(alignUp(piece, 8), vocab);
   b.ldp = padCols(b.piece);
   b.p = alignUp(tokens * b.ldp * 2, 256);
-  b.px = productOf(tokens, d, b.piece, 1);
-  b.pw = productOf(b.piece, d, tokens, 1);
+  b.px = productOf(tokens, d, b.piece, 1, 1, kMaxSplits);
+  b.pw = productOf(b.piece, d, tokens, 1, 1, kMaxSplits);
   b.dx = alignUp((size_t)b.px.splits * tokens * padCols(d) * 4, 256);
   b.dw = partialBytes(b.pw, b.piece, d);
   b.bytes = 256 + b.p + b.dx + b.dw;
@@ -610,9 +652,10 @@ int hcamdLaunchLinearCrossEntropyBackward(OlQueue q, int elemType, const void *x
     a.mma.M = (int)tokens, a.mma.N = (int)n, a.mma.K = (int)d, a.mma.segments = a.mma.splits = 1;
     a.targets = targets, a.target_i64 = targetType == HCAMD_I64, a.v0 = (int)v0, a.vocab = (int)vocab;
     a.lse = lse, a.grad_loss = gradLoss, a.factor = factor, a.p = w + 256, a.ldp = b.ldp;
-    Kernel k = kernelOf(tileOf(tokens, n), tokens, n, fetchable(x, ldx, d, 2, false) && fetchable(rows, ldw, d, 2, false), true);
+    Kernel k = kernelOf(productOf(tokens, n, d, 1, 1, 1).tile, tokens, n, fetchable(x, ldx, d, 2, false) && fetchable(rows, ldw, d, 2, false), true);
     std::snprintf(name, sizeof(name), "hcamd_xent_p_%s_%s", typeName(elemType), k.suffix);
-    if (tokens && c.launch("xent", name, a, ceilDiv(tokens, k.tile) * ceilDiv(n, k.tile), 1, 1, k.threads))
+    size_t groups = groupsOf(k, ceilDiv(tokens, k.tile) * ceilDiv(n, k.tile), 1, a.mma.half_from);
+    if (tokens && c.launch("xent", name, a, groups, 1, 1, k.threads))
       return 1;
     if (gradX) {
       StoreArgs s{};
@@ -621,7 +664,8 @@ int hcamdLaunchLinearCrossEntropyBackward(OlQueue q, int elemType, const void *x
       s.partial = dx, s.ldp = padCols(d), s.accumulate = v0 != 0;
       k = kernelOf(b.px.tile, tokens, d, fetchable(rows, ldw, d, 2, false), true);
       std::snprintf(name, sizeof(name), "hcamd_product_nn_%s_%s", typeName(elemType), k.suffix);
-      if (c.launch("ffn", name, s, ceilDiv(tokens, k.tile) * ceilDiv(d, k.tile), b.px.splits, 1, k.threads))
+      groups = groupsOf(k, ceilDiv(tokens, k.tile) * ceilDiv(d, k.tile), b.px.splits, s.mma.half_from);
+      if (c.launch("ffn", name, s, groups, b.px.splits, 1, k.threads))
         return 1;
     }
     if (gradWeight) {
@@ -631,9 +675,11 @@ int hcamdLaunchLinearCrossEntropyBackward(OlQueue q, int elemType, const void *x
       t.mma.M = (int)n, t.mma.N = (int)d, t.mma.K = (int)tokens, t.mma.segments = 1, t.mma.splits = b.pw.splits;
       t.out = static_cast<char *>(gradWeight) + v0 * ldgw * 2, t.ldo = ldgw, t.undo = undo;
       t.partial = b.dw ? reinterpret_cast<float *>(w + 256 + b.p + b.dx) : nullptr, t.ldp = padCols(d);
-      k = kernelOf(n >= 256 ? b.pw.tile : 128, n, d, fetchable(x, ldx, d, 2, false), false);
+      k = kernelOf(b.pw.tile, n, d, fetchable(x, ldx, d, 2, false), false);
       std::snprintf(name, sizeof(name), "hcamd_product_tn_%s_%s", typeName(elemType), k.suffix);
-      if (c.launch("ffn", name, s, ceilDiv(n, k.tile) * ceilDiv(d, k.tile), b.pw.splits, 1, k.threads))
+      s.tiles = (int)(ceilDiv(n, k.tile) * ceilDiv(d, k.tile));
+      groups = groupsOf(k, s.tiles, b.pw.splits, t.mma.half_from);
+      if (c.launch("ffn", name, s, groups, b.pw.splits, 1, k.threads))
         return 1;
       if (b.dw && launchFold(c, elemType, {t.partial, t.out, t.ldp, ldgw, (uint32_t)n, (uint32_t)d,
                                            (uint32_t)b.pw.splits, undo}))
