@@ -116,7 +116,8 @@ struct Tile {
 // General kernel body: any sizes, leading dimensions and alignment.  128 x 128
 // tile, four waves of 64 x 64, panels through registers (unaligned 16-byte
 // loads, element loads where a chunk crosses an edge), two LDS stages, one
-// barrier per K tile.  GATED: the N panel holds 32 rows of b[0], then the same 32
+// barrier per k tile.  (Loads two k tiles ahead cost more registers than they hide:
+// 1038 -> 1483 us for the gated block of 4096 x 4096 x 11264.)  GATED: the N panel holds 32 rows of b[0], then the same 32
 // of b[1], alternating, so that a wave's blocks j and j + 2 are the two
 // projections of the same outputs.
 // ---------------------------------------------------------------------------
@@ -135,33 +136,54 @@ __device__ __forceinline__ void mma_general(const MmaArgs &g, int wg, unsigned c
   int kt0, kt1;
   split_of(all, g.splits, kt0, kt1);
 
+  // This thread's four pieces of each panel: their address at k tile 0 of a segment
+  // (rows past the end read the last one, their results are not stored).  Tiles whose
+  // pieces all exist in full are fetched without a question; in the last k tile, and in
+  // edge tiles of k-slow operands, every piece asks how much of it exists.
   u32x4 ra[4], rb[4];
-  auto load = [&](int kt) {
-    const int seg = kt >= tiles_k ? 1 : 0;
-    const int k0 = (kt - seg * tiles_k) * T::kBK;
+  const E *pa[4], *pb[4];
+  int segment = -1;
+  // (a k-slow operand's last tile begins 128 rows before its end, where it has as many)
+  const Tile tile = {LA == kKSlow && g.M >= BM ? min(tm * BM, g.M - BM) : tm * BM,
+                     LB == kKSlow && g.N >= BN ? min(tn * BNO, g.N - BN) : tn * BNO, tm * BM, tn * BNO, tn};
+  const bool edge = (LA == kKSlow && g.M < BM) || (LB == kKSlow && g.N < BN);
+  auto aim = [&](int seg) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int id = tid + i * 256;
-      if constexpr (LA == kKFast) {
-        const int m = tm * BM + id / 8, k = k0 + id % 8 * T::kChunk;
-        const E *p = static_cast<const E *>(g.a[seg]) + (size_t)m * g.lda[seg] + k;
-        ra[i] = load_chunk(p, m < g.M ? g.K - k : 0);
-      } else {
-        const int k = k0 + id / 16, m = tm * BM + id % 16 * 8;
-        const E *p = static_cast<const E *>(g.a[seg]) + (size_t)k * g.lda[seg] + m;
-        ra[i] = load_chunk(p, k < g.K ? g.M - m : 0);
-      }
+      if constexpr (LA == kKFast)
+        pa[i] = static_cast<const E *>(g.a[seg]) + (size_t)min(tm * BM + id / 8, g.M - 1) * g.lda[seg] + id % 8 * T::kChunk;
+      else
+        pa[i] = static_cast<const E *>(g.a[seg]) + (size_t)(id / 16) * g.lda[seg] + tile.m0 + id % 16 * 8;
       if constexpr (LB == kKFast) {
-        const int r = id / 8, k = k0 + id % 8 * T::kChunk;
-        const int which = GATED ? r / 32 % 2 : seg;
-        const int n = GATED ? tn * BNO + r / 64 * 32 + r % 32 : tn * BN + r;
-        const E *p = static_cast<const E *>(g.b[which]) + (size_t)n * g.ldb[which] + k;
-        rb[i] = load_chunk(p, n < g.N ? g.K - k : 0);
+        const int r = id / 8, which = GATED ? r / 32 % 2 : seg;
+        const int n = min(GATED ? tn * BNO + r / 64 * 32 + r % 32 : tn * BN + r, g.N - 1);
+        pb[i] = static_cast<const E *>(g.b[which]) + (size_t)n * g.ldb[which] + id % 8 * T::kChunk;
       } else {
-        const int k = k0 + id / 16, n = tn * BN + id % 16 * 8;
-        const E *p = static_cast<const E *>(g.b[seg]) + (size_t)k * g.ldb[seg] + n;
-        rb[i] = load_chunk(p, k < g.K ? g.N - n : 0);
+        pb[i] = static_cast<const E *>(g.b[seg]) + (size_t)(id / 16) * g.ldb[seg] + tile.n0 + id % 16 * 8;
       }
+    }
+    segment = seg;
+  };
+  auto load = [&](int kt) {
+    const int seg = kt >= tiles_k ? 1 : 0;
+    const int k0 = (kt - seg * tiles_k) * T::kBK;
+    if (seg != segment)
+      aim(seg);
+    const size_t step_a = LA == kKFast ? (size_t)k0 : k0 * g.lda[seg], step_b = LB == kKFast ? (size_t)k0 : k0 * g.ldb[seg];
+    if (k0 + T::kBK <= g.K && !edge) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        ra[i] = *reinterpret_cast<const u32x4_u *>(pa[i] + step_a);
+        rb[i] = *reinterpret_cast<const u32x4_u *>(pb[i] + step_b);
+      }
+      return;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int id = tid + i * 256, fast = g.K - k0 - id % 8 * T::kChunk, slow = k0 + id / 16;
+      ra[i] = load_chunk(pa[i] + step_a, LA == kKFast ? fast : slow < g.K ? g.M - (tile.m0 + id % 16 * 8) : 0);
+      rb[i] = load_chunk(pb[i] + step_b, LB == kKFast ? fast : slow < g.K ? g.N - (tile.n0 + id % 16 * 8) : 0);
     }
   };
   auto offset = [&](Layout l, int id) {
@@ -178,7 +200,6 @@ __device__ __forceinline__ void mma_general(const MmaArgs &g, int wg, unsigned c
     }
   };
 
-  const Tile tile = {tm * BM, tn * BNO, tm * BM, tn * BNO, tn};
   typename T::acc acc[4][4] = {};
   init(acc, tile, wave_m, wave_n, lane);
   if (kt0 < kt1) {
@@ -731,10 +752,16 @@ __device__ __forceinline__ void store_direct(O *out, size_t ld, int m0, int n0, 
 }
 
 // C to `out` (element type) or `partial` (fp32; its rows are padded to a multiple of 8
-// and tiles begin at multiples of 8, so four columns are stored or not as a whole)
+// and the pipelined kernels' tiles begin at multiples of 8, so four columns are stored
+// or not as a whole)
 template <class E, int MI, int NI, bool LDS>
 __device__ __forceinline__ void store_tile(const StoreArgs &s, f32x4 (&acc)[MI][NI], const Tile &t, int m0, int n0,
                                            int lane, unsigned char *mine) {
+  if (s.partial && !LDS) {
+    store_direct<float, MI, NI>(s.partial + (size_t)blockIdx.y * s.mma.M * s.ldp, s.ldp, m0, n0,
+                                Window{t.m_lo, s.mma.M, t.n_lo, s.mma.N}, lane, [&](int i, int j) { return acc[i][j]; });
+    return;
+  }
   if (s.partial) {
     float *base = s.partial + (size_t)blockIdx.y * s.mma.M * s.ldp + n0 + lane / 16 * 4;
     const int left = s.mma.N - n0 - lane / 16 * 4, skip = t.n_lo - n0 - lane / 16 * 4;
@@ -763,13 +790,14 @@ template <int MI, int NI>
 __device__ __forceinline__ void begin_tile(const StoreArgs &s, f32x4 (&acc)[MI][NI], int m0, int n0, int lane) {
   if (!s.accumulate)
     return;
+  typedef f32x4 f32x4_u __attribute__((aligned(4)));
   const float *base = s.partial + (size_t)blockIdx.y * s.mma.M * s.ldp;
 #pragma unroll
   for (int i = 0; i < MI; ++i) {
     const float *row = base + (size_t)min(m0 + i * 16 + lane % 16, s.mma.M - 1) * s.ldp;
 #pragma unroll
     for (int j = 0; j < NI; ++j) // (columns past the padded row are not stored)
-      acc[i][j] = *reinterpret_cast<const f32x4 *>(row + min(n0 + j * 16 + lane / 16 * 4, (int)s.ldp - 4));
+      acc[i][j] = *reinterpret_cast<const f32x4_u *>(row + min(n0 + j * 16 + lane / 16 * 4, (int)s.ldp - 4));
   }
 }
 struct FromZero {

@@ -163,22 +163,17 @@ size_t groupsOf(const Kernel &k, size_t tiles, int splits, int &halfFrom) {
 }
 
 // Up to 32 tokens the forward products are one pass over the weights, which the tiled
-// kernels feed from too few workgroups.
-struct Few {
-  const char *suffix; // null: not for this many tokens
-  int rows;           // weight rows of a workgroup
-};
-#ifndef S16NB
-#define S16NB 2
-#define S32NB 4
-#endif
+// kernels feed from too few workgroups (one token, 2 x 11264 x 4096 bf16: 36 us against
+// 65 us; 48 tokens: 67 us against 65 us).  Null: not for this many tokens.
 constexpr size_t kFewTokens = 32;
-Few fewOf(size_t tokens) {
+const char *fewOf(size_t tokens) {
   const int v = hcamdInternalVariant("mma");
   if (tokens > kFewTokens || (v >= 1 && v <= 3))
-    return {nullptr, 128};
-  return tokens <= 16 ? Few{"s16", S16NB * 16} : Few{"s32", S32NB * 16};
+    return nullptr;
+  return tokens <= 16 ? "s16" : "s32";
 }
+constexpr size_t kFewOutputs = 16; // of the gated block to a workgroup
+constexpr size_t kFewColumns = 64; // of the loss to a workgroup
 
 int launchFold(const Call &c, int type, const FoldArgs &f) {
   FoldArgs a = f;
@@ -391,10 +386,9 @@ int hcamdLaunchGatedFfn(OlQueue q, int elemType, const void *x, size_t ldx, cons
   a.out = out, a.gate = gate, a.up = up, a.ldo = ldo, a.ldgate = ldgate, a.ldup = ldup;
   a.activation = activation, a.out_f16 = outType == HCAMD_F16;
   char name[64];
-  const Few few = fewOf(tokens);
-  if (few.suffix) {
-    std::snprintf(name, sizeof(name), "hcamd_gated_%s_%s", typeName(elemType), few.suffix);
-    return c.launch("ffn", name, a, ceilDiv(f, few.rows / 2), 1, 1, 512);
+  if (const char *few = fewOf(tokens)) {
+    std::snprintf(name, sizeof(name), "hcamd_gated_%s_%s", typeName(elemType), few);
+    return c.launch("ffn", name, a, ceilDiv(f, kFewOutputs), 1, 1, 512);
   }
   // (a tile of outputs takes twice its columns of the two weight matrices)
   const Kernel k = kernelOf(productOf(tokens, 2 * f, i8 ? d / 2 : d, 1, 1, 1).tile, tokens, 2 * f,
@@ -526,7 +520,7 @@ int hcamdLaunchGatedFfnBackward(OlQueue q, int elemType, const void *gradOut, si
 // ===========================================================================
 namespace {
 // columns of the narrowest statistics tile
-size_t statsCols(size_t tokens) { return tokens <= kFewTokens ? 32 : 128; }
+size_t statsCols(size_t tokens) { return tokens <= kFewTokens ? kFewColumns : 128; }
 int xentCommon(const Call &c, int elemType, const void *x, size_t ldx, const void *weight, size_t ldw,
                const void *targets, int targetType, size_t tokens, size_t d, size_t vocab) {
   if (!half16(elemType))
@@ -563,16 +557,16 @@ int hcamdLaunchLinearCrossEntropy(OlQueue q, int elemType, const void *x, size_t
   a.mma.a[0] = x, a.mma.lda[0] = ldx, a.mma.b[0] = weight, a.mma.ldb[0] = ldw;
   a.mma.M = (int)tokens, a.mma.N = (int)vocab, a.mma.K = (int)d, a.mma.segments = a.mma.splits = 1;
   a.targets = targets, a.target_i64 = targetType == HCAMD_I64, a.vocab = (int)vocab;
-  const Few few = fewOf(tokens);
+  const char *few = fewOf(tokens);
   const Kernel k = kernelOf(productOf(tokens, vocab, d, 1, 1, 1).tile, tokens, vocab,
                             fetchable(x, ldx, d, 2, false) && fetchable(weight, ldw, d, 2, false), true);
-  a.tiles = (int)ceilDiv(vocab, few.suffix ? few.rows : k.tile);
+  a.tiles = (int)ceilDiv(vocab, few ? kFewColumns : k.tile);
   a.stats = static_cast<float *>(work);
   a.zt = a.stats + tokens * a.tiles * 2;
   char name[64];
-  std::snprintf(name, sizeof(name), "hcamd_xent_stats_%s_%s", typeName(elemType), few.suffix ? few.suffix : k.suffix);
-  const size_t groups = few.suffix ? a.tiles : groupsOf(k, ceilDiv(tokens, k.tile) * a.tiles, 1, a.mma.half_from);
-  if (c.launch("xent", name, a, groups, 1, 1, few.suffix ? 512 : k.threads))
+  std::snprintf(name, sizeof(name), "hcamd_xent_stats_%s_%s", typeName(elemType), few ? few : k.suffix);
+  const size_t groups = few ? a.tiles : groupsOf(k, ceilDiv(tokens, k.tile) * a.tiles, 1, a.mma.half_from);
+  if (c.launch("xent", name, a, groups, 1, 1, few ? 512 : k.threads))
     return 1;
   XentRowsArgs r{a.stats, a.zt, targets, a.target_i64, loss, lse, (uint32_t)tokens, (uint32_t)vocab,
                  (uint32_t)a.tiles};
