@@ -127,11 +127,11 @@ template <class E, int B> __device__ __forceinline__ void gated_tile(const Gated
 // (blocks j and j + NB / 2 belong together).  NB 2, U 4: 36 us for one token and 50 us for
 // 32 over 2 x 11264 x 4096 bf16 (5.1 and 3.7 TB/s); NB 4, U 2: 47 and 54 us, half as
 // many workgroups.
-template <class E, class O, int MB, int NB, int U>
+template <class E, class O, int MB, int NB, int U, bool ODD>
 __device__ __forceinline__ void gated_skinny(const GatedArgs &a, unsigned char *lds) {
   constexpr int H = NB / 2;
   const int f0 = blockIdx.x * (H * 16), left = a.mma.N - f0;
-  mma_skinny<E, MB, NB, U>(
+  mma_skinny<E, MB, NB, U, ODD>(
       a.mma,
       [&](int j) {
         const int f = min(f0 + j % H * 16 + (int)threadIdx.x % 16, a.mma.N - 1), w = j / H;
@@ -158,15 +158,15 @@ __device__ __forceinline__ void gated_skinny(const GatedArgs &a, unsigned char *
       static_cast<O *>(a.up)[(size_t)m * a.ldup + f0 + n] = (O)u;
   }
 }
-template <class E, int MB, int NB, int U> __device__ __forceinline__ void gated_few(const GatedArgs &a) {
+template <class E, int MB, int NB, int U, bool ODD> __device__ __forceinline__ void gated_few(const GatedArgs &a) {
   __shared__ __attribute__((aligned(16))) unsigned char lds[skinny_lds<MB, NB>()];
   if constexpr (sizeof(E) == 1) {
     if (a.out_f16)
-      gated_skinny<E, _Float16, MB, NB, U>(a, lds);
+      gated_skinny<E, _Float16, MB, NB, U, ODD>(a, lds);
     else
-      gated_skinny<E, __bf16, MB, NB, U>(a, lds);
+      gated_skinny<E, __bf16, MB, NB, U, ODD>(a, lds);
   } else {
-    gated_skinny<E, E, MB, NB, U>(a, lds);
+    gated_skinny<E, E, MB, NB, U, ODD>(a, lds);
   }
 }
 
@@ -273,10 +273,16 @@ HCAMD_FFN(f16, _Float16)
 HCAMD_FFN(i8, int8_t)
 #define HCAMD_FFN_FEW(SUFFIX, E)                                                                          \
   extern "C" __global__ __launch_bounds__(512) void hcamd_gated_##SUFFIX##_s16(GatedArgs a) {             \
-    gated_few<E, 1, 2, 4>(a);                                                                             \
+    gated_few<E, 1, 2, 4, false>(a);                                                                      \
   }                                                                                                       \
   extern "C" __global__ __launch_bounds__(512) void hcamd_gated_##SUFFIX##_s32(GatedArgs a) {             \
-    gated_few<E, 2, 2, 4>(a);                                                                             \
+    gated_few<E, 2, 2, 4, false>(a);                                                                      \
+  }                                                                                                       \
+  extern "C" __global__ __launch_bounds__(512) void hcamd_gated_##SUFFIX##_s16odd(GatedArgs a) {          \
+    gated_few<E, 1, 2, 4, true>(a);                                                                       \
+  }                                                                                                       \
+  extern "C" __global__ __launch_bounds__(512) void hcamd_gated_##SUFFIX##_s32odd(GatedArgs a) {          \
+    gated_few<E, 2, 2, 4, true>(a);                                                                       \
   }
 HCAMD_FFN_FEW(bf16, __bf16)
 HCAMD_FFN_FEW(f16, _Float16)

@@ -577,12 +577,16 @@ __device__ __forceinline__ void mma_tiles(const MmaArgs &g, int tile, int half_f
 // meet in LDS.  Any size and alignment: rows past the end are read from the last one and
 // not stored, pieces that cross K go element by element.
 //   row_of(j): this lane's row lane % 16 of block j
+// ODD: rows that do not all begin at a multiple of 4 bytes.  Loads of 16 bytes run at full
+// speed from such addresses only (odd rows of bf16, 60000 x 2231: 2.4 TB/s as they lie), so
+// a piece is fetched from the 4-byte word its first element lies in, with the word that
+// holds its last bytes, and shifted into place.  Both words hold an element of the piece.
 // The result lies in LDS as float or int [NB][MB][256], element (m, n) of a block at
 // ((n / 4) * 16 + m) * 4 + n % 4.
 // ---------------------------------------------------------------------------
 template <int MB, int NB> constexpr int skinny_lds() { return 8 * NB * MB * 1024; }
 
-template <class E, int MB, int NB, int U, class R>
+template <class E, int MB, int NB, int U, bool ODD, class R>
 __device__ __forceinline__ void mma_skinny(const MmaArgs &g, R &&row_of, unsigned char *lds) {
   using T = MmaType<E>;
   constexpr int kStep = 4 * T::kChunk, kBlock = U * kStep;
@@ -596,17 +600,45 @@ __device__ __forceinline__ void mma_skinny(const MmaArgs &g, R &&row_of, unsigne
   for (int i = 0; i < MB; ++i)
     pa[i] = static_cast<const E *>(g.a[0]) + (size_t)min(i * 16 + row, g.M - 1) * g.lda[0] + k_lane;
   typename T::acc acc[NB][MB] = {};
+  uint32_t sb[NB], sa[MB]; // bits to shift by
+  if constexpr (ODD) {
+#pragma unroll
+    for (int j = 0; j < NB; ++j)
+      sb[j] = (uint32_t)(reinterpret_cast<uintptr_t>(pb[j]) & 3) * 8;
+#pragma unroll
+    for (int i = 0; i < MB; ++i)
+      sa[i] = (uint32_t)(reinterpret_cast<uintptr_t>(pa[i]) & 3) * 8;
+  }
   u32x4 fb[NB][U], fa[MB][U];
+  uint32_t eb[NB][U], ea[MB][U]; // ODD: the words behind
+  auto fetch = [&](const E *p, uint32_t bits, u32x4 &v, uint32_t &extra) {
+    if constexpr (ODD) {
+      typedef u32x4 u32x4_w __attribute__((aligned(4)));
+      const uint32_t *w = reinterpret_cast<const uint32_t *>(reinterpret_cast<uintptr_t>(p) & ~(uintptr_t)3);
+      v = *reinterpret_cast<const u32x4_w *>(w);
+      extra = 0;
+      if (bits)
+        extra = w[4];
+    } else {
+      v = *reinterpret_cast<const u32x4_u *>(p);
+    }
+  };
+  auto place = [](const u32x4 &v, uint32_t extra, uint32_t bits) {
+    if constexpr (!ODD)
+      return v;
+    return u32x4{__builtin_amdgcn_alignbit(v[1], v[0], bits), __builtin_amdgcn_alignbit(v[2], v[1], bits),
+                 __builtin_amdgcn_alignbit(v[3], v[2], bits), __builtin_amdgcn_alignbit(extra, v[3], bits)};
+  };
   auto request = [&](int block) {
     const int k = block * kBlock;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
 #pragma unroll
       for (int j = 0; j < NB; ++j)
-        fb[j][u] = *reinterpret_cast<const u32x4_u *>(pb[j] + k + u * kStep);
+        fetch(pb[j] + k + u * kStep, sb[j], fb[j][u], eb[j][u]);
 #pragma unroll
       for (int i = 0; i < MB; ++i)
-        fa[i][u] = *reinterpret_cast<const u32x4_u *>(pa[i] + k + u * kStep);
+        fetch(pa[i] + k + u * kStep, sa[i], fa[i][u], ea[i][u]);
     }
   };
   auto multiply = [&](const u32x4 (&b)[NB][U], const u32x4 (&a)[MB][U]) {
@@ -627,10 +659,10 @@ __device__ __forceinline__ void mma_skinny(const MmaArgs &g, R &&row_of, unsigne
     for (int u = 0; u < U; ++u) {
 #pragma unroll
       for (int j = 0; j < NB; ++j)
-        b[j][u] = fb[j][u];
+        b[j][u] = place(fb[j][u], eb[j][u], sb[j]);
 #pragma unroll
       for (int i = 0; i < MB; ++i)
-        a[i][u] = fa[i][u];
+        a[i][u] = place(fa[i][u], ea[i][u], sa[i]);
     }
     if (block + 8 < blocks)
       request(block + 8);

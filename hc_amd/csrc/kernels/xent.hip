@@ -120,10 +120,10 @@ template <class E, int B> __device__ __forceinline__ void stats_tile(const XentA
 // Few tokens: one pass over the weight, NB * 16 of its rows a workgroup.  NB 4, U 2: 57 us
 // for one token and 61 us for 32 over 32000 x 4096 bf16 with the joining (4.6 and 4.3
 // TB/s); NB 2, U 4: 65 and 85 us (x is read once per workgroup).
-template <class E, int MB, int NB, int U> __device__ __forceinline__ void stats_few(const XentArgs &a) {
+template <class E, int MB, int NB, int U, bool ODD> __device__ __forceinline__ void stats_few(const XentArgs &a) {
   __shared__ __attribute__((aligned(16))) unsigned char lds[skinny_lds<MB, NB>()];
   const int n0 = blockIdx.x * (NB * 16), left = a.mma.N - n0;
-  mma_skinny<E, MB, NB, U>(
+  mma_skinny<E, MB, NB, U, ODD>(
       a.mma,
       [&](int j) {
         const int n = min(n0 + j * 16 + (int)threadIdx.x % 16, a.mma.N - 1);
@@ -296,10 +296,16 @@ HCAMD_XENT(bf16, __bf16)
 HCAMD_XENT(f16, _Float16)
 #define HCAMD_XENT_FEW(SUFFIX, E)                                                                         \
   extern "C" __global__ __launch_bounds__(512) void hcamd_xent_stats_##SUFFIX##_s16(XentArgs a) {         \
-    stats_few<E, 1, 4, 2>(a);                                                                             \
+    stats_few<E, 1, 4, 2, false>(a);                                                                      \
   }                                                                                                       \
   extern "C" __global__ __launch_bounds__(512) void hcamd_xent_stats_##SUFFIX##_s32(XentArgs a) {         \
-    stats_few<E, 2, 4, 2>(a);                                                                             \
+    stats_few<E, 2, 4, 2, false>(a);                                                                      \
+  }                                                                                                       \
+  extern "C" __global__ __launch_bounds__(512) void hcamd_xent_stats_##SUFFIX##_s16odd(XentArgs a) {      \
+    stats_few<E, 1, 4, 2, true>(a);                                                                       \
+  }                                                                                                       \
+  extern "C" __global__ __launch_bounds__(512) void hcamd_xent_stats_##SUFFIX##_s32odd(XentArgs a) {      \
+    stats_few<E, 2, 4, 2, true>(a);                                                                       \
   }
 HCAMD_XENT_FEW(bf16, __bf16)
 HCAMD_XENT_FEW(f16, _Float16)

@@ -24,6 +24,11 @@ inline const char *typeName(int type) {
 }
 inline bool half16(int type) { return type == HCAMD_F16 || type == HCAMD_BF16; }
 
+// rows that do not all begin at a multiple of 4 bytes
+bool oddRows(const void *p, size_t ld, size_t bytes) {
+  return reinterpret_cast<uintptr_t>(p) % 4 != 0 || ld * bytes % 4 != 0;
+}
+
 // One operand of a call: what the checks look at.
 struct Arg {
   const char *name;
@@ -166,11 +171,11 @@ size_t groupsOf(const Kernel &k, size_t tiles, int splits, int &halfFrom) {
 // kernels feed from too few workgroups (one token, 2 x 11264 x 4096 bf16: 36 us against
 // 65 us; 48 tokens: 67 us against 65 us).  Null: not for this many tokens.
 constexpr size_t kFewTokens = 32;
-const char *fewOf(size_t tokens) {
+const char *fewOf(size_t tokens, bool odd) {
   const int v = hcamdInternalVariant("mma");
   if (tokens > kFewTokens || (v >= 1 && v <= 3))
     return nullptr;
-  return tokens <= 16 ? "s16" : "s32";
+  return odd ? (tokens <= 16 ? "s16odd" : "s32odd") : tokens <= 16 ? "s16" : "s32";
 }
 constexpr size_t kFewOutputs = 16; // of the gated block to a workgroup
 constexpr size_t kFewColumns = 64; // of the loss to a workgroup
@@ -386,7 +391,7 @@ int hcamdLaunchGatedFfn(OlQueue q, int elemType, const void *x, size_t ldx, cons
   a.out = out, a.gate = gate, a.up = up, a.ldo = ldo, a.ldgate = ldgate, a.ldup = ldup;
   a.activation = activation, a.out_f16 = outType == HCAMD_F16;
   char name[64];
-  if (const char *few = fewOf(tokens)) {
+  if (const char *few = fewOf(tokens, oddRows(x, ldx, e) || oddRows(wGate, ldwg, e) || oddRows(wUp, ldwu, e))) {
     std::snprintf(name, sizeof(name), "hcamd_gated_%s_%s", typeName(elemType), few);
     return c.launch("ffn", name, a, ceilDiv(f, kFewOutputs), 1, 1, 512);
   }
@@ -557,7 +562,7 @@ int hcamdLaunchLinearCrossEntropy(OlQueue q, int elemType, const void *x, size_t
   a.mma.a[0] = x, a.mma.lda[0] = ldx, a.mma.b[0] = weight, a.mma.ldb[0] = ldw;
   a.mma.M = (int)tokens, a.mma.N = (int)vocab, a.mma.K = (int)d, a.mma.segments = a.mma.splits = 1;
   a.targets = targets, a.target_i64 = targetType == HCAMD_I64, a.vocab = (int)vocab;
-  const char *few = fewOf(tokens);
+  const char *few = fewOf(tokens, oddRows(x, ldx, 2) || oddRows(weight, ldw, 2));
   const Kernel k = kernelOf(productOf(tokens, vocab, d, 1, 1, 1).tile, tokens, vocab,
                             fetchable(x, ldx, d, 2, false) && fetchable(weight, ldw, d, 2, false), true);
   a.tiles = (int)ceilDiv(vocab, few ? kFewColumns : k.tile);
