@@ -23,12 +23,6 @@
 
 #include <type_traits>
 
-#ifndef SPT
-#define SPT 8
-#define SPN 4
-#define EVS 18
-#define EVN 10
-#endif
 namespace hcamd {
 
 enum Layout { kKFast = 0, kKSlow = 1 };
@@ -277,7 +271,7 @@ __device__ __forceinline__ void mma_pipelined(const MmaArgs &g, int m_lo, int tn
   // half of a tile), and as late as there is time for them (first half), when the
   // loads of the half before have had most of a tile to land.
   constexpr int kSlow = (LA == kKSlow ? kMI : 0) + (LB == kKSlow ? kNI : 0), kQuick = kReads - kSlow;
-  constexpr int kSlowSpan = kSlow == 0 ? 0 : kSlow * kMfma / 32 > kMfma / 4 ? kMfma * SPT / 32 : kMfma * SPN / 32;
+  constexpr int kSlowSpan = kSlow == 0 ? 0 : kSlow * kMfma / 32 > kMfma / 4 ? kMfma / 4 : kMfma / 8;
   constexpr int LF = kSlow == 0 ? 1 : kSlowSpan;
   constexpr int LS = kSlow == 0 ? kMfma / kLoads : (kMfma * 3 / 4 - LF) / kLoads;
   static_assert(LF + (kLoads - 1) * LS < kMfma, "every load has its MFMA");
@@ -289,7 +283,7 @@ __device__ __forceinline__ void mma_pipelined(const MmaArgs &g, int m_lo, int tn
     if (kSlow == 0)
       return nth * (kMfma / 2) / kReads;
     if (slow)
-      return first ? kMfma * EVS / 32 + nth * (kMfma * EVN / 32) / kSlow : nth * kSlowSpan / kSlow;
+      return first ? kMfma * 9 / 16 + nth * (kMfma * 5 / 16) / kSlow : nth * kSlowSpan / kSlow;
     return (first ? 0 : kSlowSpan) + nth * (kMfma / 2) / (kQuick ? kQuick : 1);
   };
   constexpr int kPanelA = BM * 128, kStage = (BM + BN) * 128;

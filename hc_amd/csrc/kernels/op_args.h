@@ -92,6 +92,16 @@ struct XentArgs {
   void *p;           // [T][ldp] (softmax - onehot) * grad_loss * *factor
   size_t ldp;
 };
+struct XentPrepareArgs { // before the backward pass
+  const void *x, *targets;
+  const float *grad_loss;
+  int target_i64;
+  float top;        // what the largest |grad_loss| becomes
+  float *factor;    // [2]
+  void *live_x;     // x with zeros in the rows that take no part, padded to pieces of 8 (null: not wanted)
+  size_t ldx, ldl;
+  uint32_t rows, cols, vocab;
+};
 struct XentRowsArgs {
   const float *stats, *zt;
   const void *targets;

@@ -21,6 +21,11 @@ __device__ __forceinline__ int64_t target_of(const void *targets, int is64, size
   return is64 ? static_cast<const int64_t *>(targets)[row] : (int64_t)static_cast<const int32_t *>(targets)[row];
 }
 
+__device__ __forceinline__ bool takes_part(const void *targets, int is64, size_t row, uint32_t vocab) {
+  const int64_t t = target_of(targets, is64, row);
+  return t >= 0 && t < (int64_t)vocab;
+}
+
 // per-row statistics of a tile: lanes l, l + 16, l + 32, l + 48 hold one row's
 // columns; WN waves share the row and meet in LDS
 template <int MI, int NI, int WN, int BM, int BN>
@@ -258,16 +263,33 @@ __device__ __forceinline__ void rows_join(const XentRowsArgs &a) {
 // represented exactly, where -grad_loss itself would carry one and the same rounding
 // error into every row's largest entry; and fp16 keeps the small p of a large
 // vocabulary above its subnormals.  One workgroup.
-__device__ __forceinline__ void p_factor(const float *grad_loss, uint32_t rows, float top, float *factor) {
+__device__ __forceinline__ void p_factor(const XentPrepareArgs &a) {
   __shared__ float slots[16];
   float most = 0.0f;
-  for (uint32_t r = threadIdx.x; r < rows; r += blockDim.x)
-    most = fmaxf(most, fabsf(grad_loss[r]));
+  for (uint32_t r = threadIdx.x; r < a.rows; r += blockDim.x)
+    if (takes_part(a.targets, a.target_i64, r, a.vocab))
+      most = fmaxf(most, fabsf(a.grad_loss[r]));
   most = group_reduce<MaxOp, 16>(most, slots);
   if (threadIdx.x == 0) {
     const bool usable = most > 0x1p-100f && most < 0x1p100f;
-    factor[0] = usable ? top / most : 1.0f;
-    factor[1] = usable ? most / top : 1.0f;
+    a.factor[0] = usable ? a.top / most : 1.0f;
+    a.factor[1] = usable ? most / a.top : 1.0f;
+  }
+}
+
+// x as the weight's gradient takes it: rows that take no part are zeros, so that
+// whatever stands in them (padding, NaN) meets no zero of p in a product; rows are
+// padded to pieces of 8.
+template <class E> __device__ __forceinline__ void live_rows(const XentPrepareArgs &a) {
+  const uint32_t pieces = (a.cols + 7) / 8;
+  const uint64_t total = (uint64_t)a.rows * pieces;
+  for (uint64_t id = (uint64_t)blockIdx.x * blockDim.x + threadIdx.x; id < total;
+       id += (uint64_t)gridDim.x * blockDim.x) {
+    const uint32_t r = (uint32_t)(id / pieces), c = (uint32_t)(id % pieces) * 8;
+    u32x4 v = {0u, 0u, 0u, 0u};
+    if (takes_part(a.targets, a.target_i64, r, a.vocab))
+      v = load_chunk(static_cast<const E *>(a.x) + (size_t)r * a.ldx + c, (int)a.cols - (int)c);
+    *reinterpret_cast<u32x4 *>(static_cast<E *>(a.live_x) + (size_t)r * a.ldl + c) = v;
   }
 }
 
@@ -310,7 +332,6 @@ HCAMD_XENT(f16, _Float16)
 HCAMD_XENT_FEW(bf16, __bf16)
 HCAMD_XENT_FEW(f16, _Float16)
 extern "C" __global__ __launch_bounds__(256) void hcamd_xent_rows(XentRowsArgs a) { rows_join(a); }
-extern "C" __global__ __launch_bounds__(1024) void hcamd_xent_factor(const float *grad_loss, uint32_t rows,
-                                                                      float top, float *factor) {
-  p_factor(grad_loss, rows, top, factor);
-}
+extern "C" __global__ __launch_bounds__(1024) void hcamd_xent_factor(XentPrepareArgs a) { p_factor(a); }
+// (a copy of 16-bit values: one kernel for both types)
+extern "C" __global__ __launch_bounds__(256) void hcamd_xent_live(XentPrepareArgs a) { live_rows<uint16_t>(a); }

@@ -580,9 +580,9 @@ int hcamdLaunchLinearCrossEntropy(OlQueue q, int elemType, const void *x, size_t
 
 namespace {
 // the workspace of the backward pass: the factor, p of a piece, the partial sums of dx,
-// the partial sums of a piece's dW
+// the partial sums of a piece's dW, the rows of x that take part
 struct XentBack {
-  size_t piece, ldp, p, dx, dw, bytes;
+  size_t piece, ldp, p, dx, dw, live, bytes;
   Product px, pw;
 };
 XentBack xentBack(size_t tokens, size_t d, size_t vocab, size_t piece) {
@@ -599,7 +599,8 @@ XentBack xentBack(size_t tokens, size_t d, size_t vocab, size_t piece) {
   b.pw = productOf(b.piece, d, tokens, 1, 1, kMaxSplits);
   b.dx = alignUp((size_t)b.px.splits * tokens * padCols(d) * 4, 256);
   b.dw = partialBytes(b.pw, b.piece, d);
-  b.bytes = 256 + b.p + b.dx + b.dw;
+  b.live = alignUp(tokens * padCols(d) * 2, 256);
+  b.bytes = 256 + b.p + b.dx + b.dw + b.live;
   return b;
 }
 } // namespace
@@ -634,11 +635,17 @@ int hcamdLaunchLinearCrossEntropyBackward(OlQueue q, int elemType, const void *x
   char *w = static_cast<char *>(work);
   char name[64];
   float *factor = reinterpret_cast<float *>(w);
+  const void *live = w + 256 + b.p + b.dx + b.dw;
   if (tokens) {
-    uint32_t rows = (uint32_t)tokens;
-    float top = elemType == HCAMD_F16 ? 0x1p15f : 1.0f;
-    void *args[] = {&gradLoss, &rows, &top, &factor};
-    if (hcamdInternalLaunch(q, "xent", "hcamd_xent_factor", 1, 1, 1, 1024, args))
+    XentPrepareArgs a{};
+    a.x = x, a.targets = targets, a.grad_loss = gradLoss, a.target_i64 = targetType == HCAMD_I64;
+    a.top = elemType == HCAMD_F16 ? 0x1p15f : 1.0f, a.factor = factor;
+    a.live_x = const_cast<void *>(live), a.ldx = ldx, a.ldl = padCols(d);
+    a.rows = (uint32_t)tokens, a.cols = (uint32_t)d, a.vocab = (uint32_t)vocab;
+    if (c.launch("xent", "hcamd_xent_factor", a, 1, 1, 1, 1024))
+      return 1;
+    if (gradWeight && c.launch("xent", "hcamd_xent_live", a,
+                               std::min<size_t>(ceilDiv(tokens * ceilDiv(d, 8), 256), 4096)))
       return 1;
   }
   const float *undo = tokens ? factor + 1 : nullptr;
@@ -670,11 +677,11 @@ int hcamdLaunchLinearCrossEntropyBackward(OlQueue q, int elemType, const void *x
     if (gradWeight) {
       PairStoreArgs s{};
       StoreArgs &t = s.p[0];
-      t.mma.a[0] = a.p, t.mma.lda[0] = b.ldp, t.mma.b[0] = x, t.mma.ldb[0] = ldx;
+      t.mma.a[0] = a.p, t.mma.lda[0] = b.ldp, t.mma.b[0] = live, t.mma.ldb[0] = padCols(d);
       t.mma.M = (int)n, t.mma.N = (int)d, t.mma.K = (int)tokens, t.mma.segments = 1, t.mma.splits = b.pw.splits;
       t.out = static_cast<char *>(gradWeight) + v0 * ldgw * 2, t.ldo = ldgw, t.undo = undo;
       t.partial = b.dw ? reinterpret_cast<float *>(w + 256 + b.p + b.dx) : nullptr, t.ldp = padCols(d);
-      k = kernelOf(b.pw.tile, n, d, fetchable(x, ldx, d, 2, false), false);
+      k = kernelOf(b.pw.tile, n, d, fetchable(live, padCols(d), d, 2, true), false);
       std::snprintf(name, sizeof(name), "hcamd_product_tn_%s_%s", typeName(elemType), k.suffix);
       s.tiles = (int)(ceilDiv(n, k.tile) * ceilDiv(d, k.tile));
       groups = groupsOf(k, s.tiles, b.pw.splits, t.mma.half_from);

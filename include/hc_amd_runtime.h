@@ -820,8 +820,9 @@ const char *hcamdLastKernelName(void) HCAMD_NOEXCEPT;
 
 /* ---- Operators of language models -----------------------------------------
  * Like the typed launchers above: asynchronous on the queue's stream, nothing
- * allocated (also under stream capture), shapes and alignment checked on the
- * host.  Matrices are row-major with unit inner stride; leading dimensions in
+ * allocated, shapes and alignment checked on the host.  Launches can be captured
+ * into a graph once the same call has run before (the first one on a device loads
+ * the kernel's code object).  Matrices are row-major with unit inner stride; leading dimensions in
  * elements; pointers need the alignment of their elements only (16 bytes and
  * leading dimensions to match take the fast kernels).  Element types are
  * HCAMD_F32 / F16 / BF16 / I8 where an operator says so.  A workspace is the
@@ -892,7 +893,7 @@ int hcamdLaunchLinearCrossEntropy(OlQueue q, int elemType, const void *x, size_t
  * goes through the workspace in pieces of `piece` rows (0: chosen by size); p is
  * rounded to elemType there, scaled so that the largest |gradLoss| is 1 (fp16: 2^15),
  * which the results undo.  Rows whose target is negative or not
- * below vocab have no gradient, whatever their logits. */
+ * below vocab take no part, whatever stands in their x, lse and gradLoss. */
 size_t hcamdLinearCrossEntropyBackwardWorkspace(size_t tokens, size_t d, size_t vocab, size_t piece) HCAMD_NOEXCEPT;
 int hcamdLaunchLinearCrossEntropyBackward(OlQueue q, int elemType, const void *x, size_t ldx, const void *weight,
                                           size_t ldw, const void *targets, int targetType, const float *lse,

@@ -523,8 +523,7 @@ def test_linear_cross_entropy_rows_that_take_no_part(t):
     rt.linear_cross_entropy(x, w, targets, loss, lse)
     assert not bool(loss.any()) and bool(torch.isnan(lse[0])) and bool(torch.isfinite(lse[1:]).all())
     rt.linear_cross_entropy_backward(x, w, targets, lse, torch.ones(t, device="cuda"), gx, gw)
-    assert not bool(gx.any())
-    # (0 times a NaN operand is NaN: a padding row that is not finite reaches the weight's gradient)
+    assert not bool(gx.any()) and not bool(gw.any())
     x[0] = 1
     rt.linear_cross_entropy(x, w, targets, loss, lse)
     rt.linear_cross_entropy_backward(x, w, targets, lse, torch.ones(t, device="cuda"), gx, gw)
@@ -533,6 +532,33 @@ def test_linear_cross_entropy_rows_that_take_no_part(t):
     rt.linear_cross_entropy(x, w, targets, loss, lse)
     rt.linear_cross_entropy_backward(x, w, targets, lse, torch.ones(t, device="cuda"), gx, gw)
     assert bool(torch.isnan(loss[0])) and not bool(loss[1:].any()) and not bool(gx.any()) and not bool(gw.any())
+
+
+@pytest.mark.parametrize("ty", ["f16", "bf16"])
+@pytest.mark.parametrize("shape", [(40, 200, 300), (300, 263, 520)], ids=str)
+def test_linear_cross_entropy_padding_holds_anything(ty, shape):
+    """Padding rows of NaN with a huge or NaN grad_loss: the others' gradients are as without them."""
+    t, d, v = shape
+    k = TYPES[ty]
+    x, w, targets = ce_inputs(t, d, v, k)
+    pad = torch.arange(t, device="cuda") % 3 == 1
+    targets = torch.where(pad, -100, targets.clamp_min(0))
+    g = torch.where(pad, 0.0, dev(normal(4, t).abs() * 1e-3))
+    results = []
+    for dirty in (False, True):
+        xs, gs = x.clone(), g.clone()
+        if dirty:
+            xs[pad], gs[pad] = float("nan"), 1e30
+            gs[1] = float("nan")
+        else:
+            xs[pad] = 0
+        loss, lse = empty(t, ty=torch.float32), empty(t, ty=torch.float32)
+        gx, gw = torch.empty_like(x), torch.empty_like(w)
+        rt.linear_cross_entropy(xs, w, targets, loss, lse)
+        rt.linear_cross_entropy_backward(xs, w, targets, lse, gs, gx, gw)
+        results.append((loss, gx, gw))
+    for a, b in zip(*results):
+        assert torch.equal(a, b) and bool(torch.isfinite(b).all())
 
 
 def test_linear_cross_entropy_large_logits():
@@ -839,3 +865,170 @@ def test_poisoned_surroundings(product_kernel):
         if b._base is not None:
             inside = int(torch.isnan(b._base).sum())
             assert inside == b._base.numel() - b.numel()
+
+
+# ---------------------------------------------------------------------------
+# far offsets, graphs
+# ---------------------------------------------------------------------------
+def test_offsets_past_32_bits():
+    """Rows more than 2^31 elements apart, and a weight matrix of more than 2^31 elements."""
+    k = torch.bfloat16
+    base = torch.zeros(3 * 1_100_000_000, device="cuda", dtype=k)
+    far = base.as_strided((3, 520), (1_100_000_000, 1))
+    x = dev(normal(1, 3, 520), k)
+    far.copy_(x)
+    y, q, scale = torch.empty_like(x), torch.empty(3, 520, device="cuda", dtype=torch.int8), empty(3, ty=torch.float32)
+    rt.add_rms_norm(far, None, None, y)
+    want = torch.empty_like(x)
+    rt.add_rms_norm(x, None, None, want)
+    assert torch.equal(y, want)
+    rt.add_rms_norm(far, None, None, far)                    # results as far apart
+    assert torch.equal(far, want)
+    wg, wu = (dev(normal(s, 200, 520) * 0.04, k) for s in (2, 3))
+    near_out, far_out = torch.empty(3, 200, device="cuda", dtype=k), base.as_strided((3, 200), (1_100_000_000, 1), 600)
+    rt.gated_ffn(far, wg, wu, near_out)
+    rt.gated_ffn(want, wg, wu, far_out)
+    assert torch.equal(near_out, far_out)
+    del base, far, far_out
+    t, d, v = 256, 1024, 2_200_000
+    w = torch.zeros(v, d, device="cuda", dtype=k)
+    special = torch.tensor([0, 5, 1_000_003, 2_097_152, 2_097_153, 2_199_999], device="cuda")
+    w[special] = dev(normal(4, 6, d) * 0.05, k)
+    x = dev(normal(5, t, d), k)
+    targets = special[torch.arange(t, device="cuda") % 6]
+    loss, lse = empty(t, ty=torch.float32), empty(t, ty=torch.float32)
+    rt.linear_cross_entropy(x, w, targets, loss, lse)
+    z = f64(x) @ f64(w[special]).t()
+    total = torch.exp(z).sum(1) + (v - 6)                    # every other logit is 0
+    near(lse, total.log(), 1e-5)
+    near(loss, total.log() - z[torch.arange(t), torch.arange(t) % 6], 2e-5)
+    gx, gw = torch.empty_like(x), torch.empty_like(w)
+    g = torch.full((t,), 1 / t, device="cuda")
+    rt.linear_cross_entropy_backward(x, w, targets, lse, g, gx, gw)
+    p = torch.exp(z) / total[:, None]
+    p[torch.arange(t), torch.arange(t) % 6] -= 1
+    p = p / t
+    # p is rounded once (half a step; here it is up to 1 / t times the scale), the results once more
+    want = p.t() @ f64(x)
+    near(gw[special], want, want.abs() * half(k) + p.abs().t() @ f64(x).abs() * (half(k) + 2e-5))
+    want = p @ f64(w[special])
+    near(gx, want, want.abs() * half(k) + p.abs() @ f64(w[special]).abs() * (half(k) + 2e-5))
+    rest = gw[torch.tensor([1, 1_500_000, 2_199_998], device="cuda")]
+    want = ((1 / total / t)[:, None] * f64(x)).sum(0)
+    near(rest, want.expand(3, d), want.abs() * half(k) + ((1 / total / t)[:, None] * f64(x).abs()).sum(0) * (half(k) + 2e-5))
+
+
+def test_norm_backward_in_place():
+    rows, cols = 600, 1032
+    for t in TYPES.values():
+        h, dy, ds = (dev(normal(k, rows, cols), t) for k in (1, 2, 3))
+        w = dev(1 + 0.2 * normal(4, cols))
+        rstd = (1 / (f64(h).square().mean(1) + 1e-6).sqrt()).float().cuda()
+        want, gw = torch.empty_like(h), empty(cols, ty=torch.float32)
+        rt.add_rms_norm_backward(dy, h, w, rstd, want, gw, grad_summed=ds)
+        for which in (0, 1):
+            a, b, g2 = dy.clone(), ds.clone(), empty(cols, ty=torch.float32)
+            rt.add_rms_norm_backward(a, h, w, rstd, (a, b)[which], g2, grad_summed=b)
+            assert torch.equal((a, b)[which], want) and torch.equal(gw, g2)
+
+
+class Graph:
+    """Launches of one queue recorded into a graph (the queue's second word is its stream)."""
+    hip = None
+
+    def __init__(self, ctx, launch):
+        if Graph.hip is None:
+            Graph.hip = C.CDLL("libamdhip64.so.7")       # the copy that is loaded already
+        self.stream = C.c_void_p(C.cast(ctx.queue, C.POINTER(C.c_uint64))[1])
+        graph, self.exec = C.c_void_p(), C.c_void_p()
+        assert self.hip.hipStreamBeginCapture(self.stream, 1) == 0          # of this thread
+        try:
+            launch()
+        finally:
+            rc = self.hip.hipStreamEndCapture(self.stream, C.byref(graph))
+        assert rc == 0 and self.hip.hipGraphInstantiate(C.byref(self.exec), graph, None, None, C.c_size_t(0)) == 0
+        self.graph = graph
+
+    def replay(self):
+        assert self.hip.hipGraphLaunch(self.exec, self.stream) == 0
+
+    def close(self):
+        assert self.hip.hipGraphExecDestroy(self.exec) == 0 and self.hip.hipGraphDestroy(self.graph) == 0
+
+
+def test_captured_and_replayed():
+    """Every operator recorded into graphs, two graphs of the same operators with plans of their own, replayed in turn
+    with new inputs and eager work in between, against the eager results."""
+    ctx = rt.default_context()
+    k = torch.bfloat16
+
+    def program(t, d, f, v):
+        x, r = dev(normal(1, t, d), k), dev(normal(2, t, d), k)
+        w1 = dev(1 + 0.1 * normal(3, d))
+        wg, wu, head = (dev(normal(s, n, d) * d ** -0.5, k) for s, n in ((4, f), (5, f), (6, v)))
+        targets = (torch.arange(t) % v).cuda()
+        g = torch.full((t,), 1 / t, device="cuda")
+        dh = dev(normal(7, t, f), k)
+        h, n1, gx, gh, cx = (torch.empty_like(x) for _ in range(5))
+        q, scale = torch.empty(t, d, device="cuda", dtype=torch.int8), empty(t, ty=torch.float32)
+        out, gate, up = (torch.empty(t, f, device="cuda", dtype=k) for _ in range(3))
+        gg, gu, gw, cw = torch.empty_like(wg), torch.empty_like(wu), empty(d, ty=torch.float32), torch.empty_like(head)
+        rstd, loss, lse, norm = (empty(n, ty=torch.float32) for n in (t, t, t, 1))
+        clipped = [torch.empty_like(a) for a in (gg, gu, gw, cw)]
+        plans = [rt.plan_add_rms_norm(x, r, w1, n1, summed=h, rstd=rstd),
+                 rt.plan_add_rms_norm(x, r, w1, q, scale=scale),
+                 rt.plan_gated_ffn(n1, wg, wu, out, gate=gate, up=up),
+                 rt.plan_gated_ffn_backward(dh, n1, wg, wu, gate, up, gx, gg, gu),
+                 rt.plan_add_rms_norm_backward(gx, h, w1, rstd, gh, gw),
+                 rt.plan_linear_cross_entropy(n1, head, targets, loss, lse),
+                 rt.plan_linear_cross_entropy_backward(n1, head, targets, lse, g, cx, cw, piece=520),
+                 rt.plan_clip_grad_norm([gg, gu, gw, cw], clipped, norm, 0.5)]
+        return x, plans, [h, n1, q, scale, out, gate, up, gx, gg, gu, gh, gw, loss, lse, cx, cw, norm] + clipped
+
+    programs = [program(20, 136, 200, 777), program(300, 264, 520, 1500)]
+    for _, plans, _ in programs:
+        for p in plans:
+            p.launch()                                       # everything is loaded before the capture
+    torch.cuda.synchronize()
+    graphs = [Graph(ctx, lambda plans=plans: [p.launch() for p in plans]) for _, plans, _ in programs]
+    for turn in range(4):
+        wants = []
+        for x, plans, outs in programs:
+            x.copy_(dev(normal(50 + turn, *x.shape), k))
+            torch.cuda.synchronize()
+            for p in plans:
+                p.launch()
+            torch.cuda.synchronize()
+            wants.append([o.clone() for o in outs])
+            for o in outs:
+                o.fill_(1)
+        torch.cuda.synchronize()
+        for gr in graphs:
+            gr.replay()
+        ctx.synchronize()
+        for (_, _, outs), want in zip(programs, wants):
+            assert all(torch.equal(a, b) for a, b in zip(outs, want)), turn
+    for gr in graphs:
+        gr.close()
+
+
+def test_nothing_is_allocated_by_a_launch():
+    hip = C.CDLL("libamdhip64.so.7")
+
+    def free_bytes():
+        free, total = C.c_size_t(), C.c_size_t()
+        assert hip.hipMemGetInfo(C.byref(free), C.byref(total)) == 0
+        return free.value
+    t, d, v = 200, 136, 1000
+    x, w, targets = ce_inputs(t, d, v, torch.bfloat16)
+    loss, lse, gx, gw = empty(t, ty=torch.float32), empty(t, ty=torch.float32), torch.empty_like(x), torch.empty_like(w)
+    plans = [rt.plan_linear_cross_entropy(x, w, targets, loss, lse),
+             rt.plan_linear_cross_entropy_backward(x, w, targets, lse, torch.ones(t, device="cuda"), gx, gw),
+             rt.plan_add_rms_norm(x, None, None, gx)]
+    for p in plans:
+        p.launch(sync=True)
+    before = free_bytes()
+    for _ in range(5):
+        for p in plans:
+            p.launch(sync=True)
+    assert free_bytes() == before
