@@ -463,18 +463,27 @@ HCAMD_NORM(__bf16, bf16)
   }                                                                                                        \
   extern "C" __global__ __launch_bounds__(THREADS) void hcamd_rmsnorm_##NAME##_i8_r##TPR##v##VPT(NormArgs a) { \
     norm_rows<T, TPR, VPT, THREADS, true>(a);                                                              \
-  }                                                                                                        \
+  }
+#define HCAMD_NORM_BACK(T, NAME, TPR, VPT, THREADS)                                                        \
   extern "C" __global__ __launch_bounds__(THREADS) void hcamd_rmsnorm_back_##NAME##_r##TPR##v##VPT(NormBackArgs a) { \
     back_rows<T, TPR, VPT, THREADS>(a);                                                                    \
   }
+#define HCAMD_NORM_BOTH(T, NAME, TPR, VPT, THREADS)                                                        \
+  HCAMD_NORM_ROWS(T, NAME, TPR, VPT, THREADS)                                                              \
+  HCAMD_NORM_BACK(T, NAME, TPR, VPT, THREADS)
+#define HCAMD_NORM_SHORT(T, NAME)                                                                          \
+  HCAMD_NORM_BOTH(T, NAME, 64, 1, 256)                                                                     \
+  HCAMD_NORM_BOTH(T, NAME, 64, 2, 256)                                                                     \
+  HCAMD_NORM_BOTH(T, NAME, 256, 1, 256)                                                                    \
+  HCAMD_NORM_BOTH(T, NAME, 256, 2, 256)
 #define HCAMD_NORM_16(T, NAME)                                                                             \
-  HCAMD_NORM_ROWS(T, NAME, 64, 1, 256)                                                                     \
-  HCAMD_NORM_ROWS(T, NAME, 64, 2, 256)                                                                     \
-  HCAMD_NORM_ROWS(T, NAME, 256, 1, 256)                                                                    \
-  HCAMD_NORM_ROWS(T, NAME, 256, 2, 256)                                                                    \
-  HCAMD_NORM_ROWS(T, NAME, 256, 4, 256)                                                                    \
-  HCAMD_NORM_ROWS(T, NAME, 512, 4, 512)
+  HCAMD_NORM_SHORT(T, NAME)                                                                                \
+  HCAMD_NORM_ROWS(T, NAME, 1024, 1, 1024)                                                                  \
+  HCAMD_NORM_BACK(T, NAME, 512, 2, 512)                                                                    \
+  HCAMD_NORM_BOTH(T, NAME, 1024, 2, 1024)
 HCAMD_NORM_16(__bf16, bf16)
 HCAMD_NORM_16(_Float16, f16)
-HCAMD_NORM_16(float, f32)
-HCAMD_NORM_ROWS(float, f32, 1024, 4, 1024)
+HCAMD_NORM_SHORT(float, f32)
+HCAMD_NORM_BOTH(float, f32, 256, 4, 256)
+HCAMD_NORM_BOTH(float, f32, 512, 4, 512)
+HCAMD_NORM_BOTH(float, f32, 1024, 4, 1024)

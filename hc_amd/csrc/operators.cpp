@@ -198,26 +198,46 @@ bool dimsOk(const Call &c, size_t a, size_t b, size_t d) {
 } // namespace
 
 namespace {
-// The kernel of a row length: the fewest 16-byte pieces a lane, and lanes a row, that
-// hold it.  A wave to a row needs no barrier; longer rows take 256 lanes or more, where a
-// row's latency is shared.  Rows beyond 512 lanes x 4 pieces (fp32: 1024 x 4) are read
-// twice by the general kernel.
+// The kernel of a row length: as many lanes a row and 16-byte pieces a lane as hold it.  A
+// wave to a row needs no barrier; longer rows take more lanes.  Beyond 512 pieces 16-bit
+// rows, whose values take twice their size in registers, do better with 1024 lanes than
+// with more pieces to a lane (4096 x 8192 bf16: 45 us forward against 51 us, 50 against 58 us
+// in 8 bits; the backward pass 58 us with 512 lanes, 62 us with 1024), fp32 rows do not.
+// Rows beyond 1024 lanes x 2 pieces (fp32: x 4) are read twice by the general kernel.
 struct RowKernel {
   const char *suffix;
   size_t lanes, threads;
   bool general;
 };
-RowKernel rowKernel(int type, size_t cols) {
-  static const RowKernel kernels[] = {{"r64v1", 64, 256, false},   {"r64v2", 64, 256, false},
-                                      {"r256v1", 256, 256, false}, {"r256v2", 256, 256, false},
-                                      {"r256v4", 256, 256, false}, {"r512v4", 512, 512, false},
-                                      {"r1024v4", 1024, 1024, false}};
-  static const size_t pieces[] = {64, 128, 256, 512, 1024, 2048, 4096};
+RowKernel rowKernel(int type, size_t cols, bool back) {
+  struct Entry {
+    size_t pieces;
+    RowKernel kernel;
+  };
+  static const Entry shortRows[] = {{64, {"r64v1", 64, 256, false}},
+                                    {128, {"r64v2", 64, 256, false}},
+                                    {256, {"r256v1", 256, 256, false}},
+                                    {512, {"r256v2", 256, 256, false}}};
+  static const Entry forward16[] = {{1024, {"r1024v1", 1024, 1024, false}}, {2048, {"r1024v2", 1024, 1024, false}}};
+  static const Entry back16[] = {{1024, {"r512v2", 512, 512, false}}, {2048, {"r1024v2", 1024, 1024, false}}};
+  static const Entry rows32[] = {{1024, {"r256v4", 256, 256, false}},
+                                 {2048, {"r512v4", 512, 512, false}},
+                                 {4096, {"r1024v4", 1024, 1024, false}}};
   const size_t need = ceilDiv(cols, 16 / elemBytes(type));
-  if (hcamdInternalVariant("rmsnorm") != 1)
-    for (int i = 0; i < (type == HCAMD_F32 ? 7 : 6); ++i)
-      if (need <= pieces[i])
-        return kernels[i];
+  if (hcamdInternalVariant("rmsnorm") == 1)
+    return {"general", 256, 256, true};
+  for (const Entry &e : shortRows)
+    if (need <= e.pieces)
+      return e.kernel;
+  if (type == HCAMD_F32) {
+    for (const Entry &e : rows32)
+      if (need <= e.pieces)
+        return e.kernel;
+  } else {
+    for (const Entry &e : back ? back16 : forward16)
+      if (need <= e.pieces)
+        return e.kernel;
+  }
   return {"general", 256, 256, true};
 }
 // workgroups walk the rows: as many as fill the card
@@ -267,7 +287,7 @@ int hcamdLaunchAddRmsNorm(OlQueue q, int elemType, const void *x, size_t ldx, co
   a.ldx = ldx, a.ldr = ldr, a.lds = lds, a.ldo = ldo;
   a.rows = (uint32_t)rows, a.cols = (uint32_t)cols, a.eps = eps;
   a.weight_f32 = !weight || weightType == HCAMD_F32;
-  const RowKernel k = rowKernel(elemType, cols);
+  const RowKernel k = rowKernel(elemType, cols, false);
   char name[64];
   std::snprintf(name, sizeof(name), "hcamd_rmsnorm_%s%s_%s", typeName(elemType), outType == HCAMD_I8 ? "_i8" : "",
                 k.suffix);
@@ -315,7 +335,7 @@ int hcamdLaunchAddRmsNormBackward(OlQueue q, int elemType, const void *gradOut, 
   a.grad_in = gradIn, a.grad_weight = gradWeight, a.partial = static_cast<float *>(work);
   a.ldg = ldg, a.ldh = lds, a.ldgs = ldgs, a.ldgi = ldgi;
   a.rows = (uint32_t)rows, a.cols = (uint32_t)cols, a.weight_f32 = weightType == HCAMD_F32;
-  const RowKernel k = rowKernel(elemType, cols);
+  const RowKernel k = rowKernel(elemType, cols, true);
   const size_t lines = normBands(rows);
   char name[64];
   if (gradWeight && c.work(work, workBytes, hcamdAddRmsNormBackwardWorkspace(rows, cols)))

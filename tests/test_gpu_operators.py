@@ -65,7 +65,7 @@ def near(got, want, tol, what=""):
 # ---------------------------------------------------------------------------
 # add + RMS norm
 # ---------------------------------------------------------------------------
-NORM_SHAPES = [(1, 1), (3, 7), (5, 64), (2, 520), (70, 1000), (4, 4096), (3, 5001), (2, 8192), (1, 16384), (2, 33000)]
+NORM_SHAPES = [(1, 1), (3, 7), (5, 64), (2, 520), (70, 1000), (4, 4096), (3, 5001), (2, 8192), (5, 9000), (1, 16384), (2, 33000)]
 
 
 def norm_reference(x, r, w, eps, ty):
