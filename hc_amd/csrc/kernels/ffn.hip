@@ -312,6 +312,6 @@ HCAMD_FFN_FEW(i8, int8_t)
     const OfPair o = of_pair(a);                                                                          \
     product_tile<E, kKSlow, kKSlow, 128>(a.p[o.which], o.tile, o.half_from);                                          \
   }                                                                                                       \
-  extern "C" __global__ __launch_bounds__(256) void hcamd_fold_##SUFFIX(FoldArgs a) { fold<E>(a); }
+  extern "C" __global__ __launch_bounds__(256) void hcamd_fold_##SUFFIX(FoldJobs a) { fold<E>(a.job[blockIdx.y]); }
 HCAMD_FFN_BACK(bf16, __bf16)
 HCAMD_FFN_BACK(f16, _Float16)

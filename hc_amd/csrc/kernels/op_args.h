@@ -77,6 +77,10 @@ struct FoldArgs { // out = sum over splits of partial (* *undo)
   const float *undo;
 };
 
+struct FoldJobs { // grid y selects
+  FoldArgs job[3];
+};
+
 struct XentArgs {
   MmaArgs mma; // a = x [T,D], b = weight rows of this piece; N = rows of the piece
   const void *targets;

@@ -180,12 +180,24 @@ const char *fewOf(size_t tokens, bool odd) {
 constexpr size_t kFewOutputs = 16; // of the gated block to a workgroup
 constexpr size_t kFewColumns = 64; // of the loss to a workgroup
 
-int launchFold(const Call &c, int type, const FoldArgs &f) {
-  FoldArgs a = f;
-  char name[64];
-  std::snprintf(name, sizeof(name), "hcamd_fold_%s", typeName(type));
-  return c.launch("ffn", name, a, std::min<size_t>(ceilDiv((size_t)a.rows * ceilDiv(a.cols, 4), (size_t)256), 4096));
-}
+// The folds of a call, one launch for up to three of them.
+struct Folds {
+  FoldJobs jobs{};
+  size_t count = 0, most = 0;
+  void add(const FoldArgs &f) {
+    jobs.job[count++] = f;
+    most = std::max(most, (size_t)f.rows * ceilDiv(f.cols, 4));
+  }
+  int launch(const Call &c, int type) {
+    if (count == 0)
+      return 0;
+    char name[64];
+    std::snprintf(name, sizeof(name), "hcamd_fold_%s", typeName(type));
+    const size_t n = count, groups = std::min<size_t>(ceilDiv(most, (size_t)256), 4096);
+    count = most = 0;
+    return c.launch("ffn", name, jobs, groups, n);
+  }
+};
 
 bool dimsOk(const Call &c, size_t a, size_t b, size_t d) {
   if (a > kMaxDim || b > kMaxDim || d > kMaxDim) {
@@ -494,6 +506,7 @@ int hcamdLaunchGatedFfnBackward(OlQueue q, int elemType, const void *gradOut, si
   std::snprintf(name, sizeof(name), "hcamd_gated_back_%s", typeName(elemType));
   if (tokens && c.launch("ffn", name, e, std::min<size_t>(ceilDiv(tokens * ceilDiv(f, 8), 256), 8192)))
     return 1;
+  Folds folds;
   if (gradX) {
     StoreArgs s{};
     s.mma.a[0] = e.dgate, s.mma.a[1] = e.dup, s.mma.lda[0] = s.mma.lda[1] = b.ldd;
@@ -507,9 +520,8 @@ int hcamdLaunchGatedFfnBackward(OlQueue q, int elemType, const void *gradOut, si
     const size_t groups = groupsOf(k, ceilDiv(tokens, k.tile) * ceilDiv(d, k.tile), b.px.splits, s.mma.half_from);
     if (c.launch("ffn", name, s, groups, b.px.splits, 1, k.threads))
       return 1;
-    if (s.partial && launchFold(c, elemType, {s.partial, gradX, s.ldp, ldgx, (uint32_t)tokens, (uint32_t)d,
-                                              (uint32_t)b.px.splits, nullptr}))
-      return 1;
+    if (s.partial)
+      folds.add({s.partial, gradX, s.ldp, ldgx, (uint32_t)tokens, (uint32_t)d, (uint32_t)b.px.splits, nullptr});
   }
   if (gradWGate || gradWUp) {
     PairStoreArgs s{};
@@ -533,11 +545,10 @@ int hcamdLaunchGatedFfnBackward(OlQueue q, int elemType, const void *gradOut, si
     if (c.launch("ffn", name, s, groups, b.pw.splits, 1, k.threads))
       return 1;
     for (size_t k = 0; b.dw && k < n; ++k)
-      if (launchFold(c, elemType, {s.p[k].partial, s.p[k].out, s.p[k].ldp, s.p[k].ldo, (uint32_t)f, (uint32_t)d,
-                                   (uint32_t)b.pw.splits, nullptr}))
-        return 1;
+      folds.add({s.p[k].partial, s.p[k].out, s.p[k].ldp, s.p[k].ldo, (uint32_t)f, (uint32_t)d, (uint32_t)b.pw.splits,
+                 nullptr});
   }
-  return 0;
+  return folds.launch(c, elemType);
 }
 
 // ===========================================================================
@@ -670,6 +681,7 @@ int hcamdLaunchLinearCrossEntropyBackward(OlQueue q, int elemType, const void *x
   }
   const float *undo = tokens ? factor + 1 : nullptr;
   float *dx = reinterpret_cast<float *>(w + 256 + b.p);
+  Folds folds;
   for (size_t v0 = 0; v0 < vocab; v0 += b.piece) {
     const size_t n = std::min(b.piece, vocab - v0);
     const char *rows = static_cast<const char *>(weight) + v0 * ldw * 2;
@@ -707,14 +719,14 @@ int hcamdLaunchLinearCrossEntropyBackward(OlQueue q, int elemType, const void *x
       groups = groupsOf(k, s.tiles, b.pw.splits, t.mma.half_from);
       if (c.launch("ffn", name, s, groups, b.pw.splits, 1, k.threads))
         return 1;
-      if (b.dw && launchFold(c, elemType, {t.partial, t.out, t.ldp, ldgw, (uint32_t)n, (uint32_t)d,
-                                           (uint32_t)b.pw.splits, undo}))
-        return 1;
+      if (b.dw)
+        folds.add({t.partial, t.out, t.ldp, ldgw, (uint32_t)n, (uint32_t)d, (uint32_t)b.pw.splits, undo});
     }
+    if (gradX && v0 + n == vocab)
+      folds.add({dx, gradX, padCols(d), ldgx, (uint32_t)tokens, (uint32_t)d, (uint32_t)b.px.splits, undo});
+    if (folds.launch(c, elemType)) // (the next piece writes the partial sums of dW again)
+      return 1;
   }
-  if (gradX)
-    return launchFold(c, elemType, {dx, gradX, padCols(d), ldgx, (uint32_t)tokens, (uint32_t)d,
-                                    (uint32_t)b.px.splits, undo});
   return 0;
 }
 
