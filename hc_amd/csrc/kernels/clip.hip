@@ -48,7 +48,7 @@ template <class T, class F> __device__ __forceinline__ void each_piece(const T *
     u32x4 v[kAhead];
 #pragma unroll
     for (int k = 0; k < kAhead; ++k)
-      v[k] = load_chunk(in + at + k * 256 * N, n - (at + k * 256 * N));
+      v[k] = load_chunk(in + at + k * 256 * N, n - (at + k * 256 * N), at + k * 256 * N);
 #pragma unroll
     for (int k = 0; k < kAhead; ++k)
       f(__builtin_bit_cast(Piece<T>, v[k]), at + k * 256 * N, n - (at + k * 256 * N));

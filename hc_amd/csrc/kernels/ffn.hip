@@ -180,9 +180,9 @@ template <class E> __device__ __forceinline__ void gated_back(const GatedBackArg
     const uint32_t r = (uint32_t)(id / chunks), c = (uint32_t)(id % chunks) * 8;
     const int valid = (int)(a.cols - c);
     typedef E ex8 __attribute__((ext_vector_type(8)));
-    const ex8 dh = __builtin_bit_cast(ex8, load_chunk(static_cast<const E *>(a.grad_out) + (size_t)r * a.ldg + c, valid));
-    const ex8 g = __builtin_bit_cast(ex8, load_chunk(static_cast<const E *>(a.gate) + (size_t)r * a.ldgate + c, valid));
-    const ex8 u = __builtin_bit_cast(ex8, load_chunk(static_cast<const E *>(a.up) + (size_t)r * a.ldup + c, valid));
+    const ex8 dh = __builtin_bit_cast(ex8, load_chunk(static_cast<const E *>(a.grad_out) + (size_t)r * a.ldg + c, valid, (int)c));
+    const ex8 g = __builtin_bit_cast(ex8, load_chunk(static_cast<const E *>(a.gate) + (size_t)r * a.ldgate + c, valid, (int)c));
+    const ex8 u = __builtin_bit_cast(ex8, load_chunk(static_cast<const E *>(a.up) + (size_t)r * a.ldup + c, valid, (int)c));
     ex8 dg, du;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {

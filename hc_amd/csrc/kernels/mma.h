@@ -176,8 +176,9 @@ __device__ __forceinline__ void mma_general(const MmaArgs &g, int wg, unsigned c
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int id = tid + i * 256, fast = g.K - k0 - id % 8 * T::kChunk, slow = k0 + id / 16;
-      ra[i] = load_chunk(pa[i] + step_a, LA == kKFast ? fast : slow < g.K ? g.M - (tile.m0 + id % 16 * 8) : 0);
-      rb[i] = load_chunk(pb[i] + step_b, LB == kKFast ? fast : slow < g.K ? g.N - (tile.n0 + id % 16 * 8) : 0);
+      const int m = tile.m0 + id % 16 * 8, n = tile.n0 + id % 16 * 8;
+      ra[i] = load_chunk(pa[i] + step_a, LA == kKFast ? fast : slow < g.K ? g.M - m : 0, LA == kKFast ? g.K - fast : m);
+      rb[i] = load_chunk(pb[i] + step_b, LB == kKFast ? fast : slow < g.K ? g.N - n : 0, LB == kKFast ? g.K - fast : n);
     }
   };
   auto offset = [&](Layout l, int id) {
@@ -669,10 +670,10 @@ __device__ __forceinline__ void mma_skinny(const MmaArgs &g, R &&row_of, unsigne
       const int valid = g.K - (k + u * kStep + k_lane);
 #pragma unroll
       for (int j = 0; j < NB; ++j)
-        fb[j][u] = load_chunk(pb[j] + k + u * kStep, valid);
+        fb[j][u] = load_chunk(pb[j] + k + u * kStep, valid, g.K - valid);
 #pragma unroll
       for (int i = 0; i < MB; ++i)
-        fa[i][u] = load_chunk(pa[i] + k + u * kStep, valid);
+        fa[i][u] = load_chunk(pa[i] + k + u * kStep, valid, g.K - valid);
     }
     multiply(fb, fa);
   }

@@ -8,14 +8,30 @@ namespace hcamd {
 typedef u32x4 u32x4_u __attribute__((aligned(1)));
 typedef u32x2 u32x2_u __attribute__((aligned(1)));
 
-// 16 bytes of which the first `valid` elements exist; the rest reads as zero.
-template <class E> __device__ __forceinline__ u32x4 load_chunk(const E *p, int valid) {
+// v shifted down by `bytes` (0 .. 15), zeros from above
+__device__ __forceinline__ u32x4 shift_down(u32x4 v, int bytes) {
+  if (bytes & 8)
+    v = u32x4{v[2], v[3], 0u, 0u};
+  if (bytes & 4)
+    v = u32x4{v[1], v[2], v[3], 0u};
+  const uint32_t bits = (bytes & 3) * 8;
+  return u32x4{__builtin_amdgcn_alignbit(v[1], v[0], bits), __builtin_amdgcn_alignbit(v[2], v[1], bits),
+               __builtin_amdgcn_alignbit(v[3], v[2], bits), v[3] >> bits};
+}
+
+// 16 bytes of which the first `valid` elements exist; the rest reads as zero.  With
+// `before` elements of the row in front of p the last piece of a row is the row's last 16
+// bytes, shifted; only rows shorter than a piece go element by element (the
+// gated block of 200 x 300 x 400 in 8 bits: 16.9 us when every last piece did).
+template <class E> __device__ __forceinline__ u32x4 load_chunk(const E *p, int valid, int before) {
   constexpr int n = 16 / (int)sizeof(E);
   if (valid >= n)
     return *reinterpret_cast<const u32x4_u *>(p);
   u32x4 v = {0u, 0u, 0u, 0u};
   if (valid <= 0)
     return v;
+  if (before >= n - valid)
+    return shift_down(*reinterpret_cast<const u32x4_u *>(p - (n - valid)), (n - valid) * (int)sizeof(E));
   if constexpr (sizeof(E) == 2) {
     const uint16_t *s = reinterpret_cast<const uint16_t *>(p);
 #pragma unroll

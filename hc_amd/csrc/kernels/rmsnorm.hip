@@ -145,7 +145,7 @@ __device__ __forceinline__ void load_pieces(u32x4 (&v)[VPT], const T *row, uint3
 #pragma unroll
   for (int j = 0; j < VPT; ++j) {
     const int c = (j * TPR + t) * kPiece<T>;
-    v[j] = load_chunk(row + c, (int)cols - c);
+    v[j] = load_chunk(row + c, (int)cols - c, c);
   }
 }
 // the weight's values for those pieces (1 where there is none; 0 past the row)

@@ -288,7 +288,7 @@ template <class E> __device__ __forceinline__ void live_rows(const XentPrepareAr
     const uint32_t r = (uint32_t)(id / pieces), c = (uint32_t)(id % pieces) * 8;
     u32x4 v = {0u, 0u, 0u, 0u};
     if (takes_part(a.targets, a.target_i64, r, a.vocab))
-      v = load_chunk(static_cast<const E *>(a.x) + (size_t)r * a.ldx + c, (int)a.cols - (int)c);
+      v = load_chunk(static_cast<const E *>(a.x) + (size_t)r * a.ldx + c, (int)a.cols - (int)c, (int)c);
     *reinterpret_cast<u32x4 *>(static_cast<E *>(a.live_x) + (size_t)r * a.ldl + c) = v;
   }
 }
