@@ -54,19 +54,41 @@ template <class E> __device__ __forceinline__ u32x4 load_chunk(const E *p, int v
   return v;
 }
 
-// the first `valid` of the elements of 16 bytes
+// the first `valid` of the elements of 16 bytes: what is not whole goes in pieces of 8, 4,
+// 2 and 1 bytes
 template <class E> __device__ __forceinline__ void store_chunk(E *p, u32x4 v, int valid) {
   constexpr int n = 16 / (int)sizeof(E);
-  typedef E exn __attribute__((ext_vector_type(n)));
   if (valid >= n) {
     *reinterpret_cast<u32x4_u *>(p) = v;
     return;
   }
-  const exn e = __builtin_bit_cast(exn, v);
-#pragma unroll
-  for (int i = 0; i < n; ++i)
-    if (i < valid)
-      p[i] = e[i];
+  if (valid <= 0)
+    return;
+  const int bytes = valid * (int)sizeof(E);
+  char *to = reinterpret_cast<char *>(p);
+  if (bytes & 8) {
+    *reinterpret_cast<u32x2_u *>(to) = u32x2{v[0], v[1]};
+    v = shift_down(v, 8);
+    to += 8;
+  }
+  if (bytes & 4) {
+    typedef uint32_t u32_u __attribute__((aligned(1)));
+    *reinterpret_cast<u32_u *>(to) = v[0];
+    v[0] = v[1];
+    to += 4;
+  }
+  if constexpr (sizeof(E) <= 2) {
+    typedef uint16_t u16_u __attribute__((aligned(1)));
+    if (bytes & 2) {
+      *reinterpret_cast<u16_u *>(to) = (uint16_t)v[0];
+      v[0] >>= 16;
+      to += 2;
+    }
+  }
+  if constexpr (sizeof(E) == 1) {
+    if (bytes & 1)
+      *reinterpret_cast<uint8_t *>(to) = (uint8_t)v[0];
+  }
 }
 
 } // namespace hcamd

@@ -284,10 +284,7 @@ __device__ __forceinline__ void norm_rows(const NormArgs &a) {
           else
             __builtin_memcpy(out, o, 4);
         } else {
-#pragma unroll
-          for (int e = 0; e < N; ++e)
-            if (e < valid)
-              out[e] = (int8_t)(o[e / 4] >> (8 * (e % 4)));
+          store_chunk(out, u32x4{o[0], N == 8 ? o[N / 4 - 1] : 0u, 0u, 0u}, valid);
         }
       } else {
         Piece<T> o;
