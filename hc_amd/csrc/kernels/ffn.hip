@@ -256,6 +256,30 @@ template <class E> __device__ __forceinline__ void fold(const FoldArgs &a) {
   }
 }
 
+// Rows of any length and alignment copied to rows the pipelined kernels can fetch: whole
+// 16-byte pieces, zeros behind the last element.  One wave to a row, kAhead pieces a lane
+// under way.
+template <class E> __device__ __forceinline__ void lay_out(const LayArgs &a) {
+  constexpr int n = 16 / (int)sizeof(E), kAhead = 4;
+  const uint32_t lane = threadIdx.x % kWave, cols = a.cols;
+  for (uint32_t r = blockIdx.x * 4 + threadIdx.x / kWave; r < a.rows; r += gridDim.x * 4) {
+    const E *from = static_cast<const E *>(a.from) + (size_t)r * a.ld_from;
+    E *to = static_cast<E *>(a.to) + (size_t)r * a.ld_to;
+    for (uint32_t c0 = lane * n; c0 < cols; c0 += kAhead * kWave * n) {
+      u32x4 v[kAhead];
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k) {
+        const uint32_t c = c0 + k * kWave * n;
+        v[k] = load_chunk(from + c, (int)(cols - c), (int)c);
+      }
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k)
+        if (c0 + k * kWave * n < cols)
+          *reinterpret_cast<u32x4 *>(to + c0 + k * kWave * n) = v[k];
+    }
+  }
+}
+
 } // namespace
 
 #define HCAMD_FFN(SUFFIX, E)                                                                              \
@@ -315,3 +339,6 @@ HCAMD_FFN_FEW(i8, int8_t)
   extern "C" __global__ __launch_bounds__(256) void hcamd_fold_##SUFFIX(FoldJobs a) { fold<E>(a.job[blockIdx.y]); }
 HCAMD_FFN_BACK(bf16, __bf16)
 HCAMD_FFN_BACK(f16, _Float16)
+// (copies: one kernel for both 16-bit types)
+extern "C" __global__ __launch_bounds__(256) void hcamd_lay_out_2(LayJobs a) { lay_out<uint16_t>(a.job[blockIdx.y]); }
+extern "C" __global__ __launch_bounds__(256) void hcamd_lay_out_1(LayJobs a) { lay_out<uint8_t>(a.job[blockIdx.y]); }

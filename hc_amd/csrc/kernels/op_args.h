@@ -81,11 +81,22 @@ struct FoldJobs { // grid y selects
   FoldArgs job[3];
 };
 
+struct LayArgs { // a matrix copied to rows of ld_to, a multiple of 16 bytes, zeros behind each row's last element
+  const void *from;
+  void *to;
+  size_t ld_from, ld_to;
+  uint32_t rows, cols;
+};
+struct LayJobs { // grid y selects
+  LayArgs job[3];
+};
+
 struct XentArgs {
   MmaArgs mma; // a = x [T,D], b = weight rows of this piece; N = rows of the piece
   const void *targets;
   int target_i64;
   int v0;            // first vocabulary row of the piece
+  int tile0;         // column tiles before the piece
   int vocab;         // rows of the whole weight matrix
   // forward: per row and column tile (max, sum of exp(z - max)), target logit
   float *stats;      // [T][tiles][2]

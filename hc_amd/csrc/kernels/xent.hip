@@ -40,7 +40,7 @@ __device__ __forceinline__ void tile_stats(const XentArgs &a, f32x4 (&acc)[MI][N
   for (int i = 0; i < MI; ++i) {
     const int in_tile = wave_m + i * 16 + lane % 16, m = t.m0 + in_tile;
     if (m >= t.m_lo && m < M) {
-      const int64_t at = target_of(a.targets, a.target_i64, m) - n0;
+      const int64_t at = target_of(a.targets, a.target_i64, m) - a.v0 - n0;
       if (at >= 0 && at < NI * 16) {
 #pragma unroll
         for (int j = 0; j < NI; ++j)
@@ -95,7 +95,7 @@ __device__ __forceinline__ void tile_stats(const XentArgs &a, f32x4 (&acc)[MI][N
 #pragma unroll
     for (int w = 0; w < WN; ++w)
       sum += slot_s[w * BM + r] * __expf(slot_m[w * BM + r] - from);
-    float *cell = a.stats + ((size_t)m * a.tiles + t.tn) * 2;
+    float *cell = a.stats + ((size_t)m * a.tiles + a.tile0 + t.tn) * 2;
     cell[0] = most;
     cell[1] = sum;
   }

@@ -180,6 +180,30 @@ const char *fewOf(size_t tokens, bool odd) {
 constexpr size_t kFewOutputs = 16; // of the gated block to a workgroup
 constexpr size_t kFewColumns = 64; // of the loss to a workgroup
 
+// Products over rows whose length is not a multiple of 16 bytes.  The general kernel reads
+// them as they lie; with enough tokens a copy in rows that the pipelined kernels can fetch
+// costs less than those kernels gain.
+constexpr size_t kLayTokens = 768;
+bool laidOut(size_t tokens, size_t d, size_t bytes) { return tokens >= kLayTokens && d * bytes % 16 != 0; }
+size_t layBytes(size_t rows, size_t d, size_t bytes) { return alignUp(rows * alignUp(d * bytes, 16), 256); }
+// The copies of a call, one launch for up to three of them.
+struct Lays {
+  LayJobs jobs{};
+  size_t count = 0, most = 0;
+  // p and ld become those of the copy at `to`
+  void add(const void *&p, size_t &ld, void *to, size_t rows, size_t d, size_t bytes) {
+    const size_t own = alignUp(d * bytes, 16) / bytes;
+    jobs.job[count++] = {p, to, ld, own, (uint32_t)rows, (uint32_t)d};
+    most = std::max(most, rows);
+    p = to, ld = own;
+  }
+  int launch(const Call &c, size_t bytes) {
+    const size_t n = count, groups = std::min<size_t>(ceilDiv(most, (size_t)4), 4096);
+    count = most = 0;
+    return n == 0 ? 0 : c.launch("ffn", bytes == 1 ? "hcamd_lay_out_1" : "hcamd_lay_out_2", jobs, groups, n);
+  }
+};
+
 // The folds of a call, one launch for up to three of them.
 struct Folds {
   FoldJobs jobs{};
@@ -377,10 +401,17 @@ int hcamdLaunchAddRmsNormBackward(OlQueue q, int elemType, const void *gradOut, 
 // ===========================================================================
 // gated feed-forward block
 // ===========================================================================
+size_t hcamdGatedFfnWorkspace(int elemType, size_t tokens, size_t d, size_t f) noexcept {
+  if (d == 0 || f == 0 || tokens > kMaxDim || d > kMaxDim || f > kMaxDim)
+    return 0;
+  const size_t e = elemBytes(elemType);
+  return laidOut(tokens, d, e) ? layBytes(tokens, d, e) + 2 * layBytes(f, d, e) : 0;
+}
+
 int hcamdLaunchGatedFfn(OlQueue q, int elemType, const void *x, size_t ldx, const float *xScale, const void *wGate,
                         size_t ldwg, const float *gateScale, const void *wUp, size_t ldwu, const float *upScale,
                         int activation, void *out, int outType, size_t ldo, void *gate, size_t ldgate, void *up,
-                        size_t ldup, size_t tokens, size_t d, size_t f) noexcept {
+                        size_t ldup, size_t tokens, size_t d, size_t f, void *work, size_t workBytes) noexcept {
   const Call c{q, "hcamdLaunchGatedFfn"};
   if (!q)
     return 1;
@@ -415,6 +446,18 @@ int hcamdLaunchGatedFfn(OlQueue q, int elemType, const void *x, size_t ldx, cons
     if ((gate && c.check({"gate", gate, ldgate, tokens, f, oe})) || (up && c.check({"up", up, ldup, tokens, f, oe})))
       return 1;
   }
+  if (c.work(work, workBytes, hcamdGatedFfnWorkspace(elemType, tokens, d, f)))
+    return 1;
+  const bool lay = laidOut(tokens, d, e);
+  if (lay) {
+    char *w = static_cast<char *>(work);
+    Lays l;
+    l.add(x, ldx, w, tokens, d, e);
+    l.add(wGate, ldwg, w + layBytes(tokens, d, e), f, d, e);
+    l.add(wUp, ldwu, w + layBytes(tokens, d, e) + layBytes(f, d, e), f, d, e);
+    if (l.launch(c, e))
+      return 1;
+  }
   GatedArgs a{};
   a.mma.a[0] = x, a.mma.lda[0] = ldx;
   a.mma.b[0] = wGate, a.mma.ldb[0] = ldwg, a.mma.b[1] = wUp, a.mma.ldb[1] = ldwu;
@@ -429,8 +472,8 @@ int hcamdLaunchGatedFfn(OlQueue q, int elemType, const void *x, size_t ldx, cons
   }
   // (a tile of outputs takes twice its columns of the two weight matrices)
   const Kernel k = kernelOf(productOf(tokens, 2 * f, i8 ? d / 2 : d, 1, 1, 1).tile, tokens, 2 * f,
-                            fetchable(x, ldx, d, e, false) && fetchable(wGate, ldwg, d, e, false) &&
-                                fetchable(wUp, ldwu, d, e, false),
+                            fetchable(x, ldx, d, e, lay) && fetchable(wGate, ldwg, d, e, lay) &&
+                                fetchable(wUp, ldwu, d, e, lay),
                             true);
   std::snprintf(name, sizeof(name), "hcamd_gated_%s_%s", typeName(elemType), k.suffix);
   const size_t groups = groupsOf(k, ceilDiv(tokens, k.tile) * ceilDiv(f, k.tile / 2), 1, a.mma.half_from);
@@ -439,9 +482,9 @@ int hcamdLaunchGatedFfn(OlQueue q, int elemType, const void *x, size_t ldx, cons
 
 namespace {
 // the workspace of the backward pass: dg, du, then the partial sums of dx, then of
-// the two weight gradients
+// the two weight gradients, then the copies of x, Wg and Wu
 struct FfnBack {
-  size_t ldd, dg, dx, dw, bytes;
+  size_t ldd, dg, dx, dw, lay, bytes;
   Product px, pw;
 };
 FfnBack ffnBack(size_t tokens, size_t d, size_t f) {
@@ -452,7 +495,8 @@ FfnBack ffnBack(size_t tokens, size_t d, size_t f) {
   b.pw = productOf(f, d, tokens, 1, 2, kMaxSplits);
   b.dx = partialBytes(b.px, tokens, d);
   b.dw = partialBytes(b.pw, f, d);
-  b.bytes = 2 * b.dg + b.dx + 2 * b.dw;
+  b.lay = 2 * b.dg + b.dx + 2 * b.dw;
+  b.bytes = b.lay + (laidOut(tokens, d, 2) ? layBytes(tokens, d, 2) + 2 * layBytes(f, d, 2) : 0);
   return b;
 }
 } // namespace
@@ -506,6 +550,19 @@ int hcamdLaunchGatedFfnBackward(OlQueue q, int elemType, const void *gradOut, si
   std::snprintf(name, sizeof(name), "hcamd_gated_back_%s", typeName(elemType));
   if (tokens && c.launch("ffn", name, e, std::min<size_t>(ceilDiv(tokens * ceilDiv(f, 8), 256), 8192)))
     return 1;
+  const bool lay = laidOut(tokens, d, 2);
+  if (lay) {
+    char *to = w + b.lay;
+    Lays l;
+    if (gradWGate || gradWUp)
+      l.add(x, ldx, to, tokens, d, 2);
+    if (gradX) {
+      l.add(wGate, ldwg, to + layBytes(tokens, d, 2), f, d, 2);
+      l.add(wUp, ldwu, to + layBytes(tokens, d, 2) + layBytes(f, d, 2), f, d, 2);
+    }
+    if (l.launch(c, 2))
+      return 1;
+  }
   Folds folds;
   if (gradX) {
     StoreArgs s{};
@@ -514,8 +571,8 @@ int hcamdLaunchGatedFfnBackward(OlQueue q, int elemType, const void *gradOut, si
     s.mma.M = (int)tokens, s.mma.N = (int)d, s.mma.K = (int)f, s.mma.segments = 2, s.mma.splits = b.px.splits;
     s.out = gradX, s.ldo = ldgx, s.ldp = padCols(d);
     s.partial = b.dx ? reinterpret_cast<float *>(w + 2 * b.dg) : nullptr;
-    const Kernel k = kernelOf(b.px.tile, tokens, d, fetchable(wGate, ldwg, d, 2, false) &&
-                                                        fetchable(wUp, ldwu, d, 2, false), true);
+    const Kernel k = kernelOf(b.px.tile, tokens, d, fetchable(wGate, ldwg, d, 2, lay) && fetchable(wUp, ldwu, d, 2, lay),
+                              true);
     std::snprintf(name, sizeof(name), "hcamd_product_nn_%s_%s", typeName(elemType), k.suffix);
     const size_t groups = groupsOf(k, ceilDiv(tokens, k.tile) * ceilDiv(d, k.tile), b.px.splits, s.mma.half_from);
     if (c.launch("ffn", name, s, groups, b.px.splits, 1, k.threads))
@@ -538,7 +595,7 @@ int hcamdLaunchGatedFfnBackward(OlQueue q, int elemType, const void *gradOut, si
       t.partial = b.dw ? reinterpret_cast<float *>(w + 2 * b.dg + b.dx + n * b.dw) : nullptr;
       ++n;
     }
-    const Kernel k = kernelOf(b.pw.tile, f, d, fetchable(x, ldx, d, 2, false), false);
+    const Kernel k = kernelOf(b.pw.tile, f, d, fetchable(x, ldx, d, 2, lay), false);
     std::snprintf(name, sizeof(name), "hcamd_product_tn_%s_%s", typeName(elemType), k.suffix);
     s.tiles = (int)(ceilDiv(f, k.tile) * ceilDiv(d, k.tile));
     const size_t groups = groupsOf(k, s.tiles * n, b.pw.splits, s.p[0].mma.half_from);
@@ -572,10 +629,34 @@ int xentCommon(const Call &c, int elemType, const void *x, size_t ldx, const voi
 }
 } // namespace
 
-size_t hcamdLinearCrossEntropyWorkspace(size_t tokens, size_t vocab) noexcept {
-  if (tokens > kMaxDim || vocab > kMaxDim)
+namespace {
+// The workspace of the forward pass: the tiles' statistics and the targets' logits, then the
+// copies of x and of a piece of the weight.  Without copies the vocabulary is one piece;
+// with them a piece holds 64 Mi elements, so that its copy mostly stays in the 256 MiB
+// memory-side cache, and 4096 rows at least.
+struct XentFront {
+  size_t piece, stats, bytes;
+  bool lay;
+};
+XentFront xentFront(size_t tokens, size_t d, size_t vocab) {
+  XentFront b;
+  b.lay = laidOut(tokens, d, 2);
+  b.stats = tokens * ceilDiv(vocab, statsCols(tokens)) * 8 + tokens * 4;
+  b.piece = vocab;
+  b.bytes = b.stats;
+  if (b.lay) {
+    b.piece = std::min(vocab, std::max<size_t>(((size_t)64 << 20) / d / 256 * 256, 4096));
+    b.stats = alignUp(b.stats, 256);
+    b.bytes = b.stats + layBytes(tokens, d, 2) + layBytes(b.piece, d, 2);
+  }
+  return b;
+}
+} // namespace
+
+size_t hcamdLinearCrossEntropyWorkspace(size_t tokens, size_t d, size_t vocab) noexcept {
+  if (tokens > kMaxDim || d > kMaxDim || vocab > kMaxDim || d == 0)
     return 0;
-  return tokens * ceilDiv(vocab, statsCols(tokens)) * 8 + tokens * 4;
+  return xentFront(tokens, d, vocab).bytes;
 }
 
 int hcamdLaunchLinearCrossEntropy(OlQueue q, int elemType, const void *x, size_t ldx, const void *weight, size_t ldw,
@@ -586,24 +667,47 @@ int hcamdLaunchLinearCrossEntropy(OlQueue q, int elemType, const void *x, size_t
     return 1;
   if (tokens == 0)
     return 0;
+  const XentFront b = xentFront(tokens, d, vocab);
   if (c.checkAll({{"loss", loss, tokens, 1, tokens, 4}, {"lse", lse, tokens, 1, tokens, 4}}) ||
-      c.work(work, workBytes, hcamdLinearCrossEntropyWorkspace(tokens, vocab)))
+      c.work(work, workBytes, b.bytes))
     return 1;
-  XentArgs a{};
-  a.mma.a[0] = x, a.mma.lda[0] = ldx, a.mma.b[0] = weight, a.mma.ldb[0] = ldw;
-  a.mma.M = (int)tokens, a.mma.N = (int)vocab, a.mma.K = (int)d, a.mma.segments = a.mma.splits = 1;
-  a.targets = targets, a.target_i64 = targetType == HCAMD_I64, a.vocab = (int)vocab;
+  char *w = static_cast<char *>(work);
   const char *few = fewOf(tokens, oddRows(x, ldx, 2) || oddRows(weight, ldw, 2));
-  const Kernel k = kernelOf(productOf(tokens, vocab, d, 1, 1, 1).tile, tokens, vocab,
-                            fetchable(x, ldx, d, 2, false) && fetchable(weight, ldw, d, 2, false), true);
-  a.tiles = (int)ceilDiv(vocab, few ? kFewColumns : k.tile);
-  a.stats = static_cast<float *>(work);
+  auto kernelFor = [&](size_t n, bool fetch) { return kernelOf(productOf(tokens, n, d, 1, 1, 1).tile, tokens, n, fetch, true); };
+  Lays lays;
+  if (b.lay)
+    lays.add(x, ldx, w + b.stats, tokens, d, 2);
+  XentArgs a{};
+  a.targets = targets, a.target_i64 = targetType == HCAMD_I64, a.vocab = (int)vocab;
+  const bool fetch = fetchable(x, ldx, d, 2, b.lay) &&
+                     (b.lay ? fetchable(w, padCols(d), d, 2, true) : fetchable(weight, ldw, d, 2, false));
+  for (size_t v0 = 0; v0 < vocab; v0 += b.piece) {
+    const size_t n = std::min(b.piece, vocab - v0);
+    a.tiles += (int)ceilDiv(n, few ? kFewColumns : kernelFor(n, fetch).tile);
+  }
+  a.stats = reinterpret_cast<float *>(w);
   a.zt = a.stats + tokens * a.tiles * 2;
   char name[64];
-  std::snprintf(name, sizeof(name), "hcamd_xent_stats_%s_%s", typeName(elemType), few ? few : k.suffix);
-  const size_t groups = few ? a.tiles : groupsOf(k, ceilDiv(tokens, k.tile) * a.tiles, 1, a.mma.half_from);
-  if (c.launch("xent", name, a, groups, 1, 1, few ? 512 : k.threads))
-    return 1;
+  for (size_t v0 = 0; v0 < vocab; v0 += b.piece) {
+    const size_t n = std::min(b.piece, vocab - v0);
+    const void *rows = static_cast<const char *>(weight) + v0 * ldw * 2;
+    size_t ldr = ldw;
+    if (b.lay) {
+      lays.add(rows, ldr, w + b.stats + layBytes(tokens, d, 2), n, d, 2);
+      if (lays.launch(c, 2))
+        return 1;
+    }
+    const Kernel k = kernelFor(n, fetch);
+    const size_t tiles = ceilDiv(n, few ? kFewColumns : k.tile);
+    a.mma.a[0] = x, a.mma.lda[0] = ldx, a.mma.b[0] = rows, a.mma.ldb[0] = ldr;
+    a.mma.M = (int)tokens, a.mma.N = (int)n, a.mma.K = (int)d, a.mma.segments = a.mma.splits = 1;
+    a.v0 = (int)v0;
+    std::snprintf(name, sizeof(name), "hcamd_xent_stats_%s_%s", typeName(elemType), few ? few : k.suffix);
+    const size_t groups = few ? tiles : groupsOf(k, ceilDiv(tokens, k.tile) * tiles, 1, a.mma.half_from);
+    if (c.launch("xent", name, a, groups, 1, 1, few ? 512 : k.threads))
+      return 1;
+    a.tile0 += (int)tiles;
+  }
   XentRowsArgs r{a.stats, a.zt, targets, a.target_i64, loss, lse, (uint32_t)tokens, (uint32_t)vocab,
                  (uint32_t)a.tiles};
   return c.launch("xent", "hcamd_xent_rows", r, ceilDiv(tokens, 4));
@@ -611,9 +715,10 @@ int hcamdLaunchLinearCrossEntropy(OlQueue q, int elemType, const void *x, size_t
 
 namespace {
 // the workspace of the backward pass: the factor, p of a piece, the partial sums of dx,
-// the partial sums of a piece's dW, the rows of x that take part
+// the partial sums of a piece's dW, the rows of x that take part, a copy of the piece's
+// rows of W
 struct XentBack {
-  size_t piece, ldp, p, dx, dw, live, bytes;
+  size_t piece, ldp, p, dx, dw, live, lay, bytes;
   Product px, pw;
 };
 XentBack xentBack(size_t tokens, size_t d, size_t vocab, size_t piece) {
@@ -631,7 +736,8 @@ XentBack xentBack(size_t tokens, size_t d, size_t vocab, size_t piece) {
   b.dx = alignUp((size_t)b.px.splits * tokens * padCols(d) * 4, 256);
   b.dw = partialBytes(b.pw, b.piece, d);
   b.live = alignUp(tokens * padCols(d) * 2, 256);
-  b.bytes = 256 + b.p + b.dx + b.dw + b.live;
+  b.lay = 256 + b.p + b.dx + b.dw + b.live;
+  b.bytes = b.lay + (laidOut(tokens, d, 2) ? layBytes(b.piece, d, 2) : 0);
   return b;
 }
 } // namespace
@@ -667,6 +773,7 @@ int hcamdLaunchLinearCrossEntropyBackward(OlQueue q, int elemType, const void *x
   char name[64];
   float *factor = reinterpret_cast<float *>(w);
   const void *live = w + 256 + b.p + b.dx + b.dw;
+  const bool lay = laidOut(tokens, d, 2);
   if (tokens) {
     XentPrepareArgs a{};
     a.x = x, a.targets = targets, a.grad_loss = gradLoss, a.target_i64 = targetType == HCAMD_I64;
@@ -675,32 +782,42 @@ int hcamdLaunchLinearCrossEntropyBackward(OlQueue q, int elemType, const void *x
     a.rows = (uint32_t)tokens, a.cols = (uint32_t)d, a.vocab = (uint32_t)vocab;
     if (c.launch("xent", "hcamd_xent_factor", a, 1, 1, 1, 1024))
       return 1;
-    if (gradWeight && c.launch("xent", "hcamd_xent_live", a,
+    if ((gradWeight || lay) && c.launch("xent", "hcamd_xent_live", a,
                                std::min<size_t>(ceilDiv(tokens * ceilDiv(d, 8), 256), 4096)))
       return 1;
   }
+  if (lay) // (the logits of rows that take no part are not looked at)
+    x = live, ldx = padCols(d);
   const float *undo = tokens ? factor + 1 : nullptr;
   float *dx = reinterpret_cast<float *>(w + 256 + b.p);
   Folds folds;
   for (size_t v0 = 0; v0 < vocab; v0 += b.piece) {
     const size_t n = std::min(b.piece, vocab - v0);
-    const char *rows = static_cast<const char *>(weight) + v0 * ldw * 2;
+    const void *rows = static_cast<const char *>(weight) + v0 * ldw * 2;
+    size_t ldr = ldw;
+    if (lay) {
+      Lays l;
+      l.add(rows, ldr, w + b.lay, n, d, 2);
+      if (l.launch(c, 2))
+        return 1;
+    }
     XentArgs a{};
-    a.mma.a[0] = x, a.mma.lda[0] = ldx, a.mma.b[0] = rows, a.mma.ldb[0] = ldw;
+    a.mma.a[0] = x, a.mma.lda[0] = ldx, a.mma.b[0] = rows, a.mma.ldb[0] = ldr;
     a.mma.M = (int)tokens, a.mma.N = (int)n, a.mma.K = (int)d, a.mma.segments = a.mma.splits = 1;
     a.targets = targets, a.target_i64 = targetType == HCAMD_I64, a.v0 = (int)v0, a.vocab = (int)vocab;
     a.lse = lse, a.grad_loss = gradLoss, a.factor = factor, a.p = w + 256, a.ldp = b.ldp;
-    Kernel k = kernelOf(productOf(tokens, n, d, 1, 1, 1).tile, tokens, n, fetchable(x, ldx, d, 2, false) && fetchable(rows, ldw, d, 2, false), true);
+    Kernel k = kernelOf(productOf(tokens, n, d, 1, 1, 1).tile, tokens, n,
+                        fetchable(x, ldx, d, 2, lay) && fetchable(rows, ldr, d, 2, lay), true);
     std::snprintf(name, sizeof(name), "hcamd_xent_p_%s_%s", typeName(elemType), k.suffix);
     size_t groups = groupsOf(k, ceilDiv(tokens, k.tile) * ceilDiv(n, k.tile), 1, a.mma.half_from);
     if (tokens && c.launch("xent", name, a, groups, 1, 1, k.threads))
       return 1;
     if (gradX) {
       StoreArgs s{};
-      s.mma.a[0] = a.p, s.mma.lda[0] = b.ldp, s.mma.b[0] = rows, s.mma.ldb[0] = ldw;
+      s.mma.a[0] = a.p, s.mma.lda[0] = b.ldp, s.mma.b[0] = rows, s.mma.ldb[0] = ldr;
       s.mma.M = (int)tokens, s.mma.N = (int)d, s.mma.K = (int)n, s.mma.segments = 1, s.mma.splits = b.px.splits;
       s.partial = dx, s.ldp = padCols(d), s.accumulate = v0 != 0;
-      k = kernelOf(b.px.tile, tokens, d, fetchable(rows, ldw, d, 2, false), true);
+      k = kernelOf(b.px.tile, tokens, d, fetchable(rows, ldr, d, 2, lay), true);
       std::snprintf(name, sizeof(name), "hcamd_product_nn_%s_%s", typeName(elemType), k.suffix);
       groups = groupsOf(k, ceilDiv(tokens, k.tile) * ceilDiv(d, k.tile), b.px.splits, s.mma.half_from);
       if (c.launch("ffn", name, s, groups, b.px.splits, 1, k.threads))

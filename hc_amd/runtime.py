@@ -181,11 +181,12 @@ hcamdAddRmsNormBackwardWorkspace = _sig(_rt, "hcamdAddRmsNormBackwardWorkspace",
 hcamdLaunchAddRmsNormBackward = _sig(_rt, "hcamdLaunchAddRmsNormBackward", _int, _vp, _int, _vp, _sz, _vp, _sz,
                                      _vp, _int, _vp, _vp, _sz, _vp, _sz, _vp, _sz, _sz, _vp, _sz)
 hcamdLaunchGatedFfn = _sig(_rt, "hcamdLaunchGatedFfn", _int, _vp, _int, _vp, _sz, _vp, _vp, _sz, _vp, _vp, _sz, _vp,
-                           _int, _vp, _int, _sz, _vp, _sz, _vp, _sz, _sz, _sz, _sz)
+                           _int, _vp, _int, _sz, _vp, _sz, _vp, _sz, _sz, _sz, _sz, _vp, _sz)
+hcamdGatedFfnWorkspace = _sig(_rt, "hcamdGatedFfnWorkspace", _sz, _int, _sz, _sz, _sz)
 hcamdGatedFfnBackwardWorkspace = _sig(_rt, "hcamdGatedFfnBackwardWorkspace", _sz, _sz, _sz, _sz)
 hcamdLaunchGatedFfnBackward = _sig(_rt, "hcamdLaunchGatedFfnBackward", _int, _vp, _int, *[_vp, _sz] * 6, _int,
                                    *[_vp, _sz] * 3, _sz, _sz, _sz, _vp, _sz)
-hcamdLinearCrossEntropyWorkspace = _sig(_rt, "hcamdLinearCrossEntropyWorkspace", _sz, _sz, _sz)
+hcamdLinearCrossEntropyWorkspace = _sig(_rt, "hcamdLinearCrossEntropyWorkspace", _sz, _sz, _sz, _sz)
 hcamdLaunchLinearCrossEntropy = _sig(_rt, "hcamdLaunchLinearCrossEntropy", _int, _vp, _int, _vp, _sz, _vp, _sz, _vp,
                                      _int, _vp, _vp, _sz, _sz, _sz, _vp, _sz)
 hcamdLinearCrossEntropyBackwardWorkspace = _sig(_rt, "hcamdLinearCrossEntropyBackwardWorkspace", _sz, _sz, _sz, _sz,
@@ -1189,7 +1190,8 @@ def _activation(name: str) -> int:
 def plan_gated_ffn(x, w_gate, w_up, out, activation: str = "silu", gate=None, up=None, scales=None) -> Plan:
     """out = act(x @ w_gate.T) * (x @ w_up.T) (see hcamdLaunchGatedFfn): x [T, d], weights [f, d], out
     [T, f], fp16 or bf16; `gate` and `up` [T, f] receive the two products for the backward pass.
-    int8 operands take scales = (x_scale [T], gate_scale [f], up_scale [f]) and an fp16 or bf16 out."""
+    int8 operands take scales = (x_scale [T], gate_scale [f], up_scale [f]) and an fp16 or bf16 out.
+    A workspace, where the sizes need one, is allocated here, once, with the plan."""
     ctx = _ctx_of(x, w_gate, w_up, out)
     mx = _Operand(x, "x", (F16, BF16, I8))
     mg = _Operand(w_gate, "w_gate", (mx.type,))
@@ -1204,10 +1206,13 @@ def plan_gated_ffn(x, w_gate, w_up, out, activation: str = "silu", gate=None, up
     xs, gs, us = scales if scales is not None else (None, None, None)
     vx, vg, vu = (_Vector(xs, "x_scale", t, (F32,)), _Vector(gs, "gate_scale", f, (F32,)),
                   _Vector(us, "up_scale", f, (F32,)))
+    need = hcamdGatedFfnWorkspace(mx.type, t, d, f)
+    work = _workspace(need, ctx)
     return Plan(ctx, hcamdLaunchGatedFfn,
                 (ctx.queue, mx.type, mx.ptr, mx.ld, vx.ptr, mg.ptr, mg.ld, vg.ptr, mu.ptr, mu.ld, vu.ptr,
-                 _activation(activation), mo.ptr, mo.type, mo.ld, sg.ptr, sg.ld, su.ptr, su.ld, t, d, f),
-                "hcamdLaunchGatedFfn", (x, w_gate, w_up, out, gate, up, scales))
+                 _activation(activation), mo.ptr, mo.type, mo.ld, sg.ptr, sg.ld, su.ptr, su.ld, t, d, f,
+                 work.ptr if work else None, need), "hcamdLaunchGatedFfn",
+                (x, w_gate, w_up, out, gate, up, scales, work))
 
 
 def plan_gated_ffn_backward(grad_out, x, w_gate, w_up, gate, up, grad_x=None, grad_w_gate=None, grad_w_up=None,
@@ -1247,7 +1252,7 @@ def plan_linear_cross_entropy(x, weight, targets, loss, lse) -> Plan:
         raise HcRuntimeError(f"weight: rows of {mw.cols}, expected {mx.cols}")
     tg = _Vector(targets, "targets", mx.rows, (I32, I64))
     lo, ls = _Vector(loss, "loss", mx.rows, (F32,)), _Vector(lse, "lse", mx.rows, (F32,))
-    need = hcamdLinearCrossEntropyWorkspace(mx.rows, mw.rows)
+    need = hcamdLinearCrossEntropyWorkspace(mx.rows, mx.cols, mw.rows)
     work = _workspace(need, ctx)
     return Plan(ctx, hcamdLaunchLinearCrossEntropy,
                 (ctx.queue, mx.type, mx.ptr, mx.ld, mw.ptr, mw.ld, tg.ptr, tg.type, lo.ptr, ls.ptr, mx.rows, mx.cols,

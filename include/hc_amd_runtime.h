@@ -824,7 +824,8 @@ const char *hcamdLastKernelName(void) HCAMD_NOEXCEPT;
  * into a graph once the same call has run before (the first one on a device loads
  * the kernel's code object).  Matrices are row-major with unit inner stride; leading dimensions in
  * elements; pointers need the alignment of their elements only (16 bytes and
- * leading dimensions to match take the fast kernels).  Element types are
+ * leading dimensions to match take the fast kernels; rows of other lengths are copied into the
+ * workspace where that pays).  Element types are
  * HCAMD_F32 / F16 / BF16 / I8 where an operator says so.  A workspace is the
  * caller's, 256-byte aligned, at least the size its function names, its contents
  * meaningless before and after; calls that may overlap in time (two queues, two
@@ -864,10 +865,12 @@ int hcamdLaunchAddRmsNormBackward(OlQueue q, int elemType, const void *gradOut, 
  * hcamdLaunchQuantizeF16I8 and the 8-bit output above make), outType F16 or BF16;
  * gate and up must be null.  GELU is the tanh form. */
 enum HcamdActivation { HCAMD_SILU = 0, HCAMD_GELU = 1 };
+size_t hcamdGatedFfnWorkspace(int elemType, size_t tokens, size_t d, size_t f) HCAMD_NOEXCEPT;
 int hcamdLaunchGatedFfn(OlQueue q, int elemType, const void *x, size_t ldx, const float *xScale, const void *wGate,
                         size_t ldwg, const float *gateScale, const void *wUp, size_t ldwu, const float *upScale,
                         int activation, void *out, int outType, size_t ldo, void *gate, size_t ldgate, void *up,
-                        size_t ldup, size_t tokens, size_t d, size_t f) HCAMD_NOEXCEPT;
+                        size_t ldup, size_t tokens, size_t d, size_t f, void *work,
+                        size_t workBytes) HCAMD_NOEXCEPT;
 /* Its backward pass from the stored gate and up (F16 / BF16): dg = gradOut * up *
  * act'(gate) and du = gradOut * act(gate), each rounded to elemType, then gradX = dg Wg +
  * du Wu, gradWGate = dg' x, gradWUp = du' x, summed in fp32.  Gradients that are
@@ -884,7 +887,7 @@ int hcamdLaunchGatedFfnBackward(OlQueue q, int elemType, const void *gradOut, si
  * fp32 and never stored): lse = log(sum(exp(z))) and loss = lse - z[target] per row.
  * targets: I32 or I64; a negative one takes its row out (loss 0), one of vocab or
  * more is an error that shows as a loss of NaN. */
-size_t hcamdLinearCrossEntropyWorkspace(size_t tokens, size_t vocab) HCAMD_NOEXCEPT;
+size_t hcamdLinearCrossEntropyWorkspace(size_t tokens, size_t d, size_t vocab) HCAMD_NOEXCEPT;
 int hcamdLaunchLinearCrossEntropy(OlQueue q, int elemType, const void *x, size_t ldx, const void *weight, size_t ldw,
                                   const void *targets, int targetType, float *loss, float *lse, size_t tokens,
                                   size_t d, size_t vocab, void *work, size_t workBytes) HCAMD_NOEXCEPT;

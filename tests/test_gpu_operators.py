@@ -1032,3 +1032,40 @@ def test_nothing_is_allocated_by_a_launch():
         for p in plans:
             p.launch(sync=True)
     assert free_bytes() == before
+
+
+# ---------------------------------------------------------------------------
+# many tokens with rows that are no multiple of 16 bytes: copied into the workspace
+# ---------------------------------------------------------------------------
+LAID = [(768, 9, 130), (801, 1003, 300), (1000, 63, 777), (1500, 530, 136), (2049, 1, 264)]
+
+
+@pytest.mark.parametrize("layout", ["dense", "strided", "odd"])
+@pytest.mark.parametrize("shape", LAID, ids=str)
+@pytest.mark.parametrize("ty", ["f16", "bf16"])
+def test_block_with_copied_rows(ty, shape, layout):
+    assert rt.hcamdGatedFfnWorkspace(TYPES[ty] == torch.float16 and rt.F16 or rt.BF16, *shape) > 0
+    test_gated_ffn(ty, shape, layout)
+    test_gated_ffn_backward(ty, shape, layout)
+
+
+@pytest.mark.parametrize("layout", ["dense", "strided", "odd"])
+@pytest.mark.parametrize("shape", LAID + [(900, 1000, 200)], ids=str)
+def test_block_int8_with_copied_rows(shape, layout):
+    assert rt.hcamdGatedFfnWorkspace(rt.I8, *shape) > 0
+    test_gated_ffn_int8("bf16", shape, layout)
+
+
+# (the last two: several pieces of the weight in the forward pass, the last one of 4 and of 904 rows)
+@pytest.mark.parametrize("layout", ["dense", "strided", "odd"])
+@pytest.mark.parametrize("shape", LAID + [(900, 515, 60), (769, 16385, 4100), (770, 16401, 9096)], ids=str)
+@pytest.mark.parametrize("ty", ["f16", "bf16"])
+def test_cross_entropy_with_copied_rows(ty, shape, layout):
+    test_linear_cross_entropy(ty, shape, layout)
+    if shape[1] < 2000:
+        test_linear_cross_entropy_backward(ty, shape, layout)
+
+
+@pytest.mark.parametrize("ty", ["f16", "bf16"])
+def test_cross_entropy_with_copied_rows_padding_holds_anything(ty):
+    test_linear_cross_entropy_padding_holds_anything(ty, (800, 263, 520))

@@ -110,8 +110,8 @@ def norm_back(q, ty=F16, g=P, gw=None, wt=F32, rows=2, cols=8, work=None, have=0
     return rt.hcamdLaunchAddRmsNormBackward(q, ty, g, 8, P, 8, None, wt, rstd, None, 8, P, 8, gw, rows, cols, work, have)
 
 
-def ffn(q, ty=F16, x=P, ldx=8, xs=None, act=0, ot=F16, gate=None, t=2, d=8, f=4, out=P, wu=P):
-    return rt.hcamdLaunchGatedFfn(q, ty, x, ldx, xs, P, 1 << 18, xs, wu, 1 << 18, xs, act, out, ot, 4, gate, 4, None, 4, t, d, f)
+def ffn(q, ty=F16, x=P, ldx=8, xs=None, act=0, ot=F16, gate=None, t=2, d=8, f=4, out=P, wu=P, work=None, have=0):
+    return rt.hcamdLaunchGatedFfn(q, ty, x, ldx, xs, P, 1 << 18, xs, wu, 1 << 18, xs, act, out, ot, 4, gate, 4, None, 4, t, d, f, work, have)
 
 
 def ffn_back(q, ty=F16, g=P, x=P, w=P, gx=P, work=None, have=0, t=2, d=8, f=4, act=0):
@@ -148,7 +148,8 @@ ENTRIES = [
     ("output type 6", ffn, dict(ty=I8, xs=P, ot=I8)), ("out is null", ffn, dict(out=None)), ("w_up is null", ffn, dict(wu=None)),
     ("element type 6", ffn_back, dict(ty=I8)), ("grad_out is null", ffn_back, dict(g=None)), ("x is null", ffn_back, dict(x=None)),
     ("w_gate is null", ffn_back, dict(w=None)), ("empty dimension", ffn_back, dict(f=0)), ("workspace of 0 bytes", ffn_back, {}),
-    ("activation -1", ffn_back, dict(act=-1)),
+    ("workspace of 0 bytes", ffn, dict(t=800, d=7)), ("aligned to 256", ffn, dict(t=800, d=7, work=P + 16, have=1 << 20)),
+    ("workspace of 0 bytes", ffn, dict(ty=I8, xs=P, t=800, ldx=16, d=9)), ("activation -1", ffn_back, dict(act=-1)),
     ("element type 0", ce, dict(ty=F32)), ("target type 0", ce, dict(tt=F32)), ("targets is null", ce, dict(targets=None)),
     ("targets is not aligned", ce, dict(targets=P + 4)), ("empty dimension", ce, dict(v=0)), ("workspace of 0 bytes", ce, {}),
     ("loss is null", ce, dict(loss=None)),
