@@ -31,6 +31,7 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef __attribute__((address_space(3))) s16x4 *lds_s16x4_ptr;
+typedef const __attribute__((address_space(1))) u32x4_u *global_u32x4_ptr;
 
 template <class E> struct MmaType {
   using acc = f32x4;
@@ -108,19 +109,23 @@ struct Tile {
 
 // ---------------------------------------------------------------------------
 // General kernel body: any sizes, leading dimensions and alignment.  128 x 128
-// tile, four waves of 64 x 64, panels through registers (unaligned 16-byte
-// loads, element loads where a chunk crosses an edge), two LDS stages, one
-// barrier per k tile.  (Loads two k tiles ahead cost more registers than they hide:
-// 1038 -> 1483 us for the gated block of 4096 x 4096 x 11264.)  GATED: the N panel holds 32 rows of b[0], then the same 32
-// of b[1], alternating, so that a wave's blocks j and j + 2 are the two
-// projections of the same outputs.
+// tile, four waves of 64 x 64, panels through registers in unaligned 16-byte pieces,
+// two tiles of k ahead, two LDS stages, one barrier per k tile.  Every piece is one load
+// whatever it crosses: one that reaches past the end of its row is fetched that much
+// earlier and shifted into place on its way to LDS, rows and k past the end are those of
+// the last one, and what lies past K is stored as zeros.  So a k-fast operand has a
+// piece of k at least, or rows padded with zeros to one, and a k-slow operand likewise
+// (their padding may hold anything).  No load stands in a branch: the compiler would
+// wait there for all of them.
+// GATED: the N panel holds 32 rows of b[0], then the same 32 of b[1], alternating, so that
+// a wave's blocks j and j + 2 are the two projections of the same outputs.
 // ---------------------------------------------------------------------------
 template <class E, Layout LA, Layout LB, bool GATED, class Init, class Epilogue>
 __device__ __forceinline__ void mma_general(const MmaArgs &g, int wg, unsigned char *lds, Init &&init,
                                             Epilogue &&epilogue) {
   using T = MmaType<E>;
   constexpr int BM = 128, BN = 128, BNO = GATED ? BN / 2 : BN;
-  constexpr int kPanel = 128 * 128, kStage = 2 * kPanel;
+  constexpr int kPanel = 128 * 128, kStage = 2 * kPanel, kChunk = T::kChunk;
   static_assert(sizeof(E) == 2 || (LA == kKFast && LB == kKFast), "transposed reads are for 16-bit elements");
   int tm, tn;
   tile_of(wg, (g.M + BM - 1) / BM, (g.N + BNO - 1) / BNO, tm, tn);
@@ -130,56 +135,75 @@ __device__ __forceinline__ void mma_general(const MmaArgs &g, int wg, unsigned c
   int kt0, kt1;
   split_of(all, g.splits, kt0, kt1);
 
-  // This thread's four pieces of each panel: their address at k tile 0 of a segment
-  // (rows past the end read the last one, their results are not stored).  Tiles whose
-  // pieces all exist in full are fetched without a question; in the last k tile, and in
-  // edge tiles of k-slow operands, every piece asks how much of it exists.
-  u32x4 ra[4], rb[4];
-  const E *pa[4], *pb[4];
-  int segment = -1;
+  // This thread's four pieces of a panel.  k-fast: chunk tid % 8 of rows tid / 8 + 32 i;
+  // k-slow: columns tid % 16 * 8 .. + 7 of k tid / 16 + 16 i.
   // (a k-slow operand's last tile begins 128 rows before its end, where it has as many)
   const Tile tile = {LA == kKSlow && g.M >= BM ? min(tm * BM, g.M - BM) : tm * BM,
                      LB == kKSlow && g.N >= BN ? min(tn * BNO, g.N - BN) : tn * BNO, tm * BM, tn * BNO, tn};
-  const bool edge = (LA == kKSlow && g.M < BM) || (LB == kKSlow && g.N < BN);
+  const int chunk = tid % 8 * kChunk, last_chunk = max(g.K - kChunk, 0), column = tid % 16 * 8, slow_k = tid / 16;
+  // columns that a narrow k-slow operand's pieces are fetched early by
+  const int early_a = LA == kKSlow ? max(tile.m0 + column - max(g.M - 8, 0), 0) : 0;
+  const int early_b = LB == kKSlow ? max(tile.n0 + column - max(g.N - 8, 0), 0) : 0;
+  const bool narrow = (LA == kKSlow && g.M < BM) || (LB == kKSlow && g.N < BN);
+  constexpr int kAhead = LA == kKFast && LB == kKFast ? 2 : 1;
+  u32x4 ra[kAhead][4], rb[kAhead][4];
+  const E *pa[4], *pb[4]; // k-fast: the rows; k-slow: the pieces at k tile 0
+  size_t lda = 0, ldb = 0;
+  int segment = -1;
   auto aim = [&](int seg) {
+    lda = seg ? g.lda[1] : g.lda[0], ldb = seg ? g.ldb[1] : g.ldb[0];
+    const E *a = static_cast<const E *>(seg ? g.a[1] : g.a[0]), *b = static_cast<const E *>(seg ? g.b[1] : g.b[0]);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int id = tid + i * 256;
       if constexpr (LA == kKFast)
-        pa[i] = static_cast<const E *>(g.a[seg]) + (size_t)min(tm * BM + id / 8, g.M - 1) * g.lda[seg] + id % 8 * T::kChunk;
+        pa[i] = a + (size_t)min(tile.m0 + tid / 8 + 32 * i, g.M - 1) * lda;
       else
-        pa[i] = static_cast<const E *>(g.a[seg]) + (size_t)(id / 16) * g.lda[seg] + tile.m0 + id % 16 * 8;
-      if constexpr (LB == kKFast) {
-        const int r = id / 8, which = GATED ? r / 32 % 2 : seg;
-        const int n = min(GATED ? tn * BNO + r / 64 * 32 + r % 32 : tn * BN + r, g.N - 1);
-        pb[i] = static_cast<const E *>(g.b[which]) + (size_t)n * g.ldb[which] + id % 8 * T::kChunk;
+        pa[i] = a + (size_t)(slow_k + 16 * i) * lda + (tile.m0 + column - early_a);
+      if constexpr (GATED) {
+        const int r = tid / 8 + 32 * i, n = min(tile.n0 + i / 2 * 32 + r % 32, g.N - 1);
+        pb[i] = static_cast<const E *>(i % 2 ? g.b[1] : g.b[0]) + (size_t)n * (i % 2 ? g.ldb[1] : g.ldb[0]);
+      } else if constexpr (LB == kKFast) {
+        pb[i] = b + (size_t)min(tile.n0 + tid / 8 + 32 * i, g.N - 1) * ldb;
       } else {
-        pb[i] = static_cast<const E *>(g.b[seg]) + (size_t)(id / 16) * g.ldb[seg] + tile.n0 + id % 16 * 8;
+        pb[i] = b + (size_t)(slow_k + 16 * i) * ldb + (tile.n0 + column - early_b);
       }
     }
     segment = seg;
   };
-  auto load = [&](int kt) {
-    const int seg = kt >= tiles_k ? 1 : 0;
-    const int k0 = (kt - seg * tiles_k) * T::kBK;
-    if (seg != segment)
-      aim(seg);
-    const size_t step_a = LA == kKFast ? (size_t)k0 : k0 * g.lda[seg], step_b = LB == kKFast ? (size_t)k0 : k0 * g.ldb[seg];
-    if (k0 + T::kBK <= g.K && !edge) {
+  auto begin_of = [&](int kt) { return (kt >= tiles_k ? kt - tiles_k : kt) * T::kBK; };
+  auto load = [&](int kt, auto set) {
+    constexpr int S = decltype(set)::value;
+    if ((kt >= tiles_k ? 1 : 0) != segment)
+      aim(kt >= tiles_k ? 1 : 0);
+    const int k0 = begin_of(kt), at = min(k0 + chunk, last_chunk);
+    size_t qa[4], qb[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      qa[i] = LA == kKFast ? (size_t)at : k0 * lda;
+      qb[i] = LB == kKFast ? (size_t)at : k0 * ldb;
+    }
+    if ((LA == kKSlow || LB == kKSlow) && k0 + T::kBK > g.K) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        ra[i] = *reinterpret_cast<const u32x4_u *>(pa[i] + step_a);
-        rb[i] = *reinterpret_cast<const u32x4_u *>(pb[i] + step_b);
+        const size_t past = max(k0 + slow_k + 16 * i - (g.K - 1), 0);
+        if (LA == kKSlow)
+          qa[i] -= past * lda;
+        if (LB == kKSlow)
+          qb[i] -= past * ldb;
       }
-      return;
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int id = tid + i * 256, fast = g.K - k0 - id % 8 * T::kChunk, slow = k0 + id / 16;
-      const int m = tile.m0 + id % 16 * 8, n = tile.n0 + id % 16 * 8;
-      ra[i] = load_chunk(pa[i] + step_a, LA == kKFast ? fast : slow < g.K ? g.M - m : 0, LA == kKFast ? g.K - fast : m);
-      rb[i] = load_chunk(pb[i] + step_b, LB == kKFast ? fast : slow < g.K ? g.N - n : 0, LB == kKFast ? g.K - fast : n);
+      ra[S][i] = *(global_u32x4_ptr)(pa[i] + qa[i]);
+      rb[S][i] = *(global_u32x4_ptr)(pb[i] + qb[i]);
     }
+  };
+  // what was fetched early moves into place, what lies past K becomes zero
+  auto place = [&](Layout l, u32x4 v, int k0, int i, int early) {
+    const int by = l == kKFast ? max(k0 + chunk - last_chunk, 0) : early;
+    const bool none = l == kKFast ? by >= kChunk : k0 + slow_k + 16 * i >= g.K;
+    v = shift_down(v, min(by, kChunk - 1) * (int)sizeof(E));
+    return none ? u32x4{0u, 0u, 0u, 0u} : v;
   };
   auto offset = [&](Layout l, int id) {
     if (l == kKFast)
@@ -187,43 +211,66 @@ __device__ __forceinline__ void mma_general(const MmaArgs &g, int wg, unsigned c
     const int k = id / 16, pos = id % 16;
     return k * 256 + (((pos / 2) ^ slow_swizzle(k)) * 32) + pos % 2 * 16;
   };
-  auto store = [&](int buf) {
+  auto store = [&](int kt, int buf, auto set) {
+    constexpr int S = decltype(set)::value;
+    const int k0 = begin_of(kt);
+    if (narrow || k0 + T::kBK > g.K) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        ra[S][i] = place(LA, ra[S][i], k0, i, early_a);
+        rb[S][i] = place(LB, rb[S][i], k0, i, early_b);
+      }
+    }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      *reinterpret_cast<u32x4 *>(lds + buf * kStage + offset(LA, tid + i * 256)) = ra[i];
-      *reinterpret_cast<u32x4 *>(lds + buf * kStage + kPanel + offset(LB, tid + i * 256)) = rb[i];
+      *reinterpret_cast<u32x4 *>(lds + buf * kStage + offset(LA, tid + i * 256)) = ra[S][i];
+      *reinterpret_cast<u32x4 *>(lds + buf * kStage + kPanel + offset(LB, tid + i * 256)) = rb[S][i];
     }
   };
 
   typename T::acc acc[4][4] = {};
   init(acc, tile, wave_m, wave_n, lane);
-  if (kt0 < kt1) {
-    load(kt0);
-    store(0);
-    __syncthreads();
-    for (int kt = kt0; kt < kt1; ++kt) {
-      const int buf = (kt - kt0) & 1;
-      if (kt + 1 < kt1)
-        load(kt + 1);
-      const unsigned char *pa = lds + buf * kStage, *pb = pa + kPanel;
+  using Set0 = std::integral_constant<int, 0>;
+  using Set1 = std::integral_constant<int, kAhead - 1>;
+  // tile kt lies in stage `buf`, its registers (set `own`) are free, tile kt + 1 is in set
+  // `next` (past the last tile: the last one again, which nothing reads)
+  auto tile_step = [&](int kt, int buf, auto own, auto next) {
+    if constexpr (kAhead == 2)
+      load(min(kt + 2, kt1 - 1), own);
+    else if (kt + 1 < kt1)
+      load(kt + 1, own);
+    const unsigned char *pa = lds + buf * kStage, *pb = pa + kPanel;
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        u32x4 fa[4], fb[4];
+    for (int h = 0; h < 2; ++h) {
+      u32x4 fa[4], fb[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          fa[i] = read_operand<LA, 128>(pa, wave_m + i * 16, h, lane);
-          fb[i] = read_operand<LB, 128>(pb, wave_n + i * 16, h, lane);
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            acc[i][j] = mma16<E>(fb[j], fa[i], acc[i][j]);
+      for (int i = 0; i < 4; ++i) {
+        fa[i] = read_operand<LA, 128>(pa, wave_m + i * 16, h, lane);
+        fb[i] = read_operand<LB, 128>(pb, wave_n + i * 16, h, lane);
       }
-      if (kt + 1 < kt1)
-        store(buf ^ 1);
-      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          acc[i][j] = mma16<E>(fb[j], fa[i], acc[i][j]);
     }
+    if (kAhead == 2 || kt + 1 < kt1)
+      store(min(kt + 1, kt1 - 1), buf ^ 1, next);
+    __syncthreads();
+  };
+  if (kt0 < kt1) {
+    load(kt0, Set0{});
+    if constexpr (kAhead == 2)
+      load(min(kt0 + 1, kt1 - 1), Set1{});
+    store(kt0, 0, Set0{});
+    __syncthreads();
+    int kt = kt0;
+    for (; kt + 1 < kt1; kt += 2) {
+      tile_step(kt, 0, Set0{}, Set1{});
+      tile_step(kt + 1, 1, Set1{}, Set0{});
+    }
+    if (kt < kt1)
+      tile_step(kt, 0, Set0{}, Set1{});
   }
   epilogue(acc, tile, wave_m, wave_n, lane, lds);
 }

@@ -158,13 +158,13 @@ template <class E, int MB, int NB, int U, bool ODD> __device__ __forceinline__ v
       sum += __shfl_xor(sum, o);
     if (m >= a.mma.M)
       continue;
-    const int64_t t = target_of(a.targets, a.target_i64, m) - n0;
+    const int64_t t = target_of(a.targets, a.target_i64, m) - a.v0 - n0;
 #pragma unroll
     for (int j = 0; j < NB; ++j)
       if (t == n + j * 16 && n + j * 16 < left)
         a.zt[m] = z[j];
     if (n == 0) {
-      float *cell = a.stats + ((size_t)m * a.tiles + blockIdx.x) * 2;
+      float *cell = a.stats + ((size_t)m * a.tiles + a.tile0 + blockIdx.x) * 2;
       cell[0] = most;
       cell[1] = sum;
     }

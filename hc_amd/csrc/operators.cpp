@@ -182,9 +182,15 @@ constexpr size_t kFewColumns = 64; // of the loss to a workgroup
 
 // Products over rows whose length is not a multiple of 16 bytes.  The general kernel reads
 // them as they lie; with enough tokens a copy in rows that the pipelined kernels can fetch
-// costs less than those kernels gain.
-constexpr size_t kLayTokens = 768;
-bool laidOut(size_t tokens, size_t d, size_t bytes) { return tokens >= kLayTokens && d * bytes % 16 != 0; }
+// costs less than those kernels gain.  A backward pass reads its copies twice.  (us, as
+// they lie / copied: block 500 x 2231 x 5001 bf16 forward 52 / 62, backward 127 / 112;
+// 1000 x 2231 x 5001 103 / 75 and 200 / 170; 333 x 4085 x 11001 backward 310 / 316; loss
+// 500 x 1025 x 50021 121 / 108 and 389 / 317, 300 x 1001 x 20001 backward 109 / 113.)
+// Rows shorter than a piece are always copied: the general kernel reads whole pieces.
+enum Pass { kForward, kBackward };
+bool laidOut(Pass pass, size_t tokens, size_t d, size_t bytes) {
+  return d * bytes < 16 || (tokens >= (pass == kForward ? 768 : 384) && d * bytes % 16 != 0);
+}
 size_t layBytes(size_t rows, size_t d, size_t bytes) { return alignUp(rows * alignUp(d * bytes, 16), 256); }
 // The copies of a call, one launch for up to three of them.
 struct Lays {
@@ -405,7 +411,7 @@ size_t hcamdGatedFfnWorkspace(int elemType, size_t tokens, size_t d, size_t f) n
   if (d == 0 || f == 0 || tokens > kMaxDim || d > kMaxDim || f > kMaxDim)
     return 0;
   const size_t e = elemBytes(elemType);
-  return laidOut(tokens, d, e) ? layBytes(tokens, d, e) + 2 * layBytes(f, d, e) : 0;
+  return laidOut(kForward, tokens, d, e) ? layBytes(tokens, d, e) + 2 * layBytes(f, d, e) : 0;
 }
 
 int hcamdLaunchGatedFfn(OlQueue q, int elemType, const void *x, size_t ldx, const float *xScale, const void *wGate,
@@ -448,7 +454,7 @@ int hcamdLaunchGatedFfn(OlQueue q, int elemType, const void *x, size_t ldx, cons
   }
   if (c.work(work, workBytes, hcamdGatedFfnWorkspace(elemType, tokens, d, f)))
     return 1;
-  const bool lay = laidOut(tokens, d, e);
+  const bool lay = laidOut(kForward, tokens, d, e);
   if (lay) {
     char *w = static_cast<char *>(work);
     Lays l;
@@ -496,7 +502,7 @@ FfnBack ffnBack(size_t tokens, size_t d, size_t f) {
   b.dx = partialBytes(b.px, tokens, d);
   b.dw = partialBytes(b.pw, f, d);
   b.lay = 2 * b.dg + b.dx + 2 * b.dw;
-  b.bytes = b.lay + (laidOut(tokens, d, 2) ? layBytes(tokens, d, 2) + 2 * layBytes(f, d, 2) : 0);
+  b.bytes = b.lay + (laidOut(kBackward, tokens, d, 2) ? layBytes(tokens, d, 2) + 2 * layBytes(f, d, 2) : 0);
   return b;
 }
 } // namespace
@@ -550,7 +556,7 @@ int hcamdLaunchGatedFfnBackward(OlQueue q, int elemType, const void *gradOut, si
   std::snprintf(name, sizeof(name), "hcamd_gated_back_%s", typeName(elemType));
   if (tokens && c.launch("ffn", name, e, std::min<size_t>(ceilDiv(tokens * ceilDiv(f, 8), 256), 8192)))
     return 1;
-  const bool lay = laidOut(tokens, d, 2);
+  const bool lay = laidOut(kBackward, tokens, d, 2);
   if (lay) {
     char *to = w + b.lay;
     Lays l;
@@ -640,7 +646,7 @@ struct XentFront {
 };
 XentFront xentFront(size_t tokens, size_t d, size_t vocab) {
   XentFront b;
-  b.lay = laidOut(tokens, d, 2);
+  b.lay = laidOut(kForward, tokens, d, 2);
   b.stats = tokens * ceilDiv(vocab, statsCols(tokens)) * 8 + tokens * 4;
   b.piece = vocab;
   b.bytes = b.stats;
@@ -737,7 +743,7 @@ XentBack xentBack(size_t tokens, size_t d, size_t vocab, size_t piece) {
   b.dw = partialBytes(b.pw, b.piece, d);
   b.live = alignUp(tokens * padCols(d) * 2, 256);
   b.lay = 256 + b.p + b.dx + b.dw + b.live;
-  b.bytes = b.lay + (laidOut(tokens, d, 2) ? layBytes(b.piece, d, 2) : 0);
+  b.bytes = b.lay + (laidOut(kBackward, tokens, d, 2) ? layBytes(b.piece, d, 2) : 0);
   return b;
 }
 } // namespace
@@ -773,7 +779,7 @@ int hcamdLaunchLinearCrossEntropyBackward(OlQueue q, int elemType, const void *x
   char name[64];
   float *factor = reinterpret_cast<float *>(w);
   const void *live = w + 256 + b.p + b.dx + b.dw;
-  const bool lay = laidOut(tokens, d, 2);
+  const bool lay = laidOut(kBackward, tokens, d, 2);
   if (tokens) {
     XentPrepareArgs a{};
     a.x = x, a.targets = targets, a.grad_loss = gradLoss, a.target_i64 = targetType == HCAMD_I64;

@@ -1069,3 +1069,51 @@ def test_cross_entropy_with_copied_rows(ty, shape, layout):
 @pytest.mark.parametrize("ty", ["f16", "bf16"])
 def test_cross_entropy_with_copied_rows_padding_holds_anything(ty):
     test_linear_cross_entropy_padding_holds_anything(ty, (800, 263, 520))
+
+
+# ---------------------------------------------------------------------------
+# dimensions shorter than a 16-byte piece, at more tokens than one pass over the weights takes
+# ---------------------------------------------------------------------------
+NARROW = [(64, 5, 40), (100, 7, 300), (200, 3, 9), (300, 64, 5), (300, 200, 1), (130, 137, 7), (40, 1, 1), (400, 11, 3), (133, 8, 8)]
+
+
+@pytest.mark.parametrize("layout", ["dense", "strided", "odd"])
+@pytest.mark.parametrize("shape", NARROW, ids=str)
+@pytest.mark.parametrize("ty", ["f16", "bf16"])
+def test_narrow_dimensions(ty, shape, layout):
+    test_gated_ffn(ty, shape, layout)
+    test_gated_ffn_backward(ty, shape, layout)
+    test_gated_ffn_int8(ty, shape, layout)
+    test_linear_cross_entropy(ty, shape, layout)
+    test_linear_cross_entropy_backward(ty, shape, layout)
+
+
+@pytest.mark.parametrize("t", [5, 40, 300, 800])
+@pytest.mark.parametrize("d", [3, 9, 100, 517])
+def test_operands_end_with_their_memory(t, d):
+    """Operands whose last element is the last of its allocation, rows with NaN between them: nothing around a row
+    changes a result."""
+    f, k = 77, torch.bfloat16
+
+    def last(x, pad):
+        wide = torch.full((x.shape[0], x.shape[1] + pad), float("nan"), device="cuda", dtype=x.dtype)
+        wide[:, pad:] = x
+        return wide[:, pad:]
+    x, wg, wu = ffn_inputs(t, d, f, k)
+    dh = dev(normal(8, t, f), k)
+    targets = (torch.arange(t) % f).cuda()
+    results = []
+    for pad in (0, 3):
+        xs, a, b, g = (last(v, pad) for v in (x, wg, wu, dh))
+        out, gate, up = (empty(t, f, ty=k) for _ in range(3))
+        gx, gg, gu, cx, cw = empty(t, d, ty=k), empty(f, d, ty=k), empty(f, d, ty=k), empty(t, d, ty=k), empty(f, d, ty=k)
+        rt.gated_ffn(xs, a, b, out, gate=gate, up=up)
+        rt.gated_ffn_backward(g, xs, a, b, gate, up, gx, gg, gu)
+        loss, lse = empty(t, ty=torch.float32), empty(t, ty=torch.float32)
+        rt.linear_cross_entropy(xs, a, targets, loss, lse)
+        rt.linear_cross_entropy_backward(xs, a, targets, lse, torch.ones(t, device="cuda"), cx, cw)
+        results.append((out, gate, up, gx, gg, gu, loss, lse, cx, cw))
+    # the two runs may take different kernels, which add in different orders: a stored value then differs by one step of
+    # its type at most (2^-7), and a gradient made of stored gate, up, dg and du by as much again of the largest
+    for p, q in zip(*results):
+        assert bool(torch.isfinite(q).all()) and torch.allclose(p.float(), q.float(), rtol=2 ** -6, atol=2 ** -6 * float(p.abs().max()))
