@@ -233,6 +233,41 @@ template <class E, int B> __device__ __forceinline__ void p_tile(const XentArgs 
       });
 }
 
+// Few tokens, as in the forward pass: one pass over the piece's rows of the weight, which
+// the tiles feed from too few workgroups (8 tokens, 32000 x 4096 bf16: 90 us in tiles).
+template <class E, int MB, int NB, int U, bool ODD> __device__ __forceinline__ void p_few(const XentArgs &a) {
+  __shared__ __attribute__((aligned(16))) unsigned char lds[skinny_lds<MB, NB>()];
+  const int n0 = blockIdx.x * (NB * 16), N = a.mma.N;
+  mma_skinny<E, MB, NB, U, ODD>(
+      a.mma,
+      [&](int j) {
+        const int n = min(n0 + j * 16 + (int)threadIdx.x % 16, N - 1);
+        return static_cast<const E *>(a.mma.b[0]) + (size_t)n * a.mma.ldb[0];
+      },
+      lds);
+  const f32x4 *cells = reinterpret_cast<const f32x4 *>(lds);
+  const float factor = *a.factor;
+  for (int c = threadIdx.x; c < MB * 16 * NB * 4; c += 512) { // four columns of a row
+    const int m = c / (NB * 4), quad = c % (NB * 4), n = n0 + quad * 4;
+    if (m >= a.mma.M || n >= N)
+      continue;
+    const int64_t t = target_of(a.targets, a.target_i64, m);
+    const bool live = t >= 0 && t < a.vocab;
+    f32x4 v = cells[(quad / 4 * MB + m / 16) * 64 + quad % 4 * 16 + m % 16];
+    const float g = live ? a.grad_loss[m] * factor : 0.0f, lse = a.lse[m];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float p = __expf(v[e] - lse) - (t == a.v0 + n + e ? 1.0f : 0.0f);
+      v[e] = live && n + e < N ? p * g : 0.0f;
+    }
+    const int padded = (N + 7) & ~7;
+    E *row = static_cast<E *>(a.p) + (size_t)m * a.ldp;
+    store4(row, n, 0, padded, v);
+    if (n + 4 >= N && n + 4 < padded)
+      store4(row, n + 4, 0, padded, f32x4{0.0f, 0.0f, 0.0f, 0.0f});
+  }
+}
+
 // one wave per row joins the tiles' statistics
 __device__ __forceinline__ void rows_join(const XentRowsArgs &a) {
   const int lane = threadIdx.x % kWave;
@@ -328,6 +363,18 @@ HCAMD_XENT(f16, _Float16)
   }                                                                                                       \
   extern "C" __global__ __launch_bounds__(512) void hcamd_xent_stats_##SUFFIX##_s32odd(XentArgs a) {      \
     stats_few<E, 2, 4, 2, true>(a);                                                                       \
+  }                                                                                                       \
+  extern "C" __global__ __launch_bounds__(512) void hcamd_xent_p_##SUFFIX##_s16(XentArgs a) {             \
+    p_few<E, 1, 4, 2, false>(a);                                                                          \
+  }                                                                                                       \
+  extern "C" __global__ __launch_bounds__(512) void hcamd_xent_p_##SUFFIX##_s32(XentArgs a) {             \
+    p_few<E, 2, 4, 2, false>(a);                                                                          \
+  }                                                                                                       \
+  extern "C" __global__ __launch_bounds__(512) void hcamd_xent_p_##SUFFIX##_s16odd(XentArgs a) {          \
+    p_few<E, 1, 4, 2, true>(a);                                                                           \
+  }                                                                                                       \
+  extern "C" __global__ __launch_bounds__(512) void hcamd_xent_p_##SUFFIX##_s32odd(XentArgs a) {          \
+    p_few<E, 2, 4, 2, true>(a);                                                                           \
   }
 HCAMD_XENT_FEW(bf16, __bf16)
 HCAMD_XENT_FEW(f16, _Float16)

@@ -183,9 +183,10 @@ constexpr size_t kFewColumns = 64; // of the loss to a workgroup
 // Products over rows whose length is not a multiple of 16 bytes.  The general kernel reads
 // them as they lie; with enough tokens a copy in rows that the pipelined kernels can fetch
 // costs less than those kernels gain.  A backward pass reads its copies twice.  (us, as
-// they lie / copied: block 500 x 2231 x 5001 bf16 forward 52 / 62, backward 127 / 112;
-// 1000 x 2231 x 5001 103 / 75 and 200 / 170; 333 x 4085 x 11001 backward 310 / 316; loss
-// 500 x 1025 x 50021 121 / 108 and 389 / 317, 300 x 1001 x 20001 backward 109 / 113.)
+// they lie / copied: block 500 x 2231 x 5001 bf16 forward 55 / 63, backward 121 / 111;
+// 700 x 1001 x 2731 forward 29 / 32; 1000 x 2231 x 5001 83 / 75 and 202 / 169; 333 x 4085 x
+// 11001 backward 300 / 309; loss 500 x 1025 x 50021 111 / 106 and 382 / 310, 300 x 1001 x
+// 20001 backward 111 / 112.)
 // Rows shorter than a piece are always copied: the general kernel reads whole pieces.
 enum Pass { kForward, kBackward };
 bool laidOut(Pass pass, size_t tokens, size_t d, size_t bytes) {
@@ -814,9 +815,11 @@ int hcamdLaunchLinearCrossEntropyBackward(OlQueue q, int elemType, const void *x
     a.lse = lse, a.grad_loss = gradLoss, a.factor = factor, a.p = w + 256, a.ldp = b.ldp;
     Kernel k = kernelOf(productOf(tokens, n, d, 1, 1, 1).tile, tokens, n,
                         fetchable(x, ldx, d, 2, lay) && fetchable(rows, ldr, d, 2, lay), true);
-    std::snprintf(name, sizeof(name), "hcamd_xent_p_%s_%s", typeName(elemType), k.suffix);
-    size_t groups = groupsOf(k, ceilDiv(tokens, k.tile) * ceilDiv(n, k.tile), 1, a.mma.half_from);
-    if (tokens && c.launch("xent", name, a, groups, 1, 1, k.threads))
+    const char *few = fewOf(tokens, oddRows(x, ldx, 2) || oddRows(rows, ldr, 2));
+    std::snprintf(name, sizeof(name), "hcamd_xent_p_%s_%s", typeName(elemType), few ? few : k.suffix);
+    size_t groups = few ? ceilDiv(n, kFewColumns)
+                        : groupsOf(k, ceilDiv(tokens, k.tile) * ceilDiv(n, k.tile), 1, a.mma.half_from);
+    if (tokens && c.launch("xent", name, a, groups, 1, 1, few ? 512 : k.threads))
       return 1;
     if (gradX) {
       StoreArgs s{};
