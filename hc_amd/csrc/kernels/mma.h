@@ -652,22 +652,30 @@ __device__ __forceinline__ void mma_skinny(const MmaArgs &g, R &&row_of, unsigne
       sa[i] = (uint32_t)(reinterpret_cast<uintptr_t>(pa[i]) & 3) * 8;
   }
   u32x4 fb[NB][U], fa[MB][U];
-  uint32_t eb[NB][U], ea[MB][U]; // ODD: the words behind
-  auto fetch = [&](const E *p, uint32_t bits, u32x4 &v, uint32_t &extra) {
+  uint32_t eb[NB], ea[MB]; // ODD: the words behind the last pieces
+  auto fetch = [&](const E *p, uint32_t bits, u32x4 &v, uint32_t &last, bool is_last) {
     if constexpr (ODD) {
       typedef u32x4 u32x4_w __attribute__((aligned(4)));
       const uint32_t *w = reinterpret_cast<const uint32_t *>(reinterpret_cast<uintptr_t>(p) & ~(uintptr_t)3);
       v = *reinterpret_cast<const u32x4_w *>(w);
-      extra = 0;
-      if (bits)
-        extra = w[4];
+      if (is_last) {
+        last = 0;
+        if (bits && lane >= 48)
+          last = w[4];
+      }
     } else {
       v = *reinterpret_cast<const u32x4_u *>(p);
     }
   };
-  auto place = [](const u32x4 &v, uint32_t extra, uint32_t bits) {
+  // the word behind a piece is the first one of the next piece of its row, which the lane 16
+  // further holds, or lane - 48 in the next u
+  auto place = [&](const u32x4 (&f)[U], int u, uint32_t last, uint32_t bits) {
+    const u32x4 &v = f[u];
     if constexpr (!ODD)
       return v;
+    const uint32_t give = u + 1 < U && lane < 16 ? f[u + 1 < U ? u + 1 : u][0] : v[0];
+    const uint32_t got = (uint32_t)__builtin_amdgcn_ds_bpermute((lane + 16) % kWave * 4, (int)give);
+    const uint32_t extra = u + 1 == U && lane >= 48 ? last : got;
     return u32x4{__builtin_amdgcn_alignbit(v[1], v[0], bits), __builtin_amdgcn_alignbit(v[2], v[1], bits),
                  __builtin_amdgcn_alignbit(v[3], v[2], bits), __builtin_amdgcn_alignbit(extra, v[3], bits)};
   };
@@ -677,10 +685,10 @@ __device__ __forceinline__ void mma_skinny(const MmaArgs &g, R &&row_of, unsigne
     for (int u = 0; u < U; ++u) {
 #pragma unroll
       for (int j = 0; j < NB; ++j)
-        fetch(pb[j] + k + u * kStep, sb[j], fb[j][u], eb[j][u]);
+        fetch(pb[j] + k + u * kStep, sb[j], fb[j][u], eb[j], u == U - 1);
 #pragma unroll
       for (int i = 0; i < MB; ++i)
-        fetch(pa[i] + k + u * kStep, sa[i], fa[i][u], ea[i][u]);
+        fetch(pa[i] + k + u * kStep, sa[i], fa[i][u], ea[i], u == U - 1);
     }
   };
   auto multiply = [&](const u32x4 (&b)[NB][U], const u32x4 (&a)[MB][U]) {
@@ -701,10 +709,10 @@ __device__ __forceinline__ void mma_skinny(const MmaArgs &g, R &&row_of, unsigne
     for (int u = 0; u < U; ++u) {
 #pragma unroll
       for (int j = 0; j < NB; ++j)
-        b[j][u] = place(fb[j][u], eb[j][u], sb[j]);
+        b[j][u] = place(fb[j], u, eb[j], sb[j]);
 #pragma unroll
       for (int i = 0; i < MB; ++i)
-        a[i][u] = place(fa[i][u], ea[i][u], sa[i]);
+        a[i][u] = place(fa[i], u, ea[i], sa[i]);
     }
     if (block + 8 < blocks)
       request(block + 8);
