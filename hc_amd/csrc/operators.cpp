@@ -66,6 +66,24 @@ struct Call {
         return 1;
     return 0;
   }
+  // outputs that begin where another one or an input does
+  int apart(std::initializer_list<const void *> outputs, std::initializer_list<const void *> inputs) const {
+    for (auto o = outputs.begin(); o != outputs.end(); ++o) {
+      if (!*o)
+        continue;
+      for (auto p = outputs.begin(); p != o; ++p)
+        if (*p == *o)
+          return fail("two outputs are one buffer");
+      for (const void *i : inputs)
+        if (i == *o)
+          return fail("an output is an input's buffer");
+    }
+    return 0;
+  }
+  // an output that may be this input, row for row
+  int inPlace(const void *out, size_t ldo, const void *in, size_t ldi, size_t rows) const {
+    return out && out == in && ldo != ldi && rows > 1 ? fail("in place with another leading dimension") : 0;
+  }
   int work(const void *work, size_t have, size_t need) const {
     if (need == 0)
       return 0;
@@ -325,6 +343,11 @@ int hcamdLaunchAddRmsNorm(OlQueue q, int elemType, const void *x, size_t ldx, co
     return 1;
   if (outType == HCAMD_I8 ? c.check({"scale", scale, rows, 1, rows, 4}) : scale != nullptr)
     return outType == HCAMD_I8 ? 1 : c.fail("a scale needs an int8 output");
+  if (c.apart({out, summed, scale, rstd}, {weight}) || c.apart({scale, rstd}, {x, residual}) ||
+      (outType != elemType && c.apart({out}, {x, residual})) || c.inPlace(out, ldo, x, ldx, rows) ||
+      c.inPlace(out, ldo, residual, ldr, rows) || c.inPlace(summed, lds, x, ldx, rows) ||
+      c.inPlace(summed, lds, residual, ldr, rows))
+    return 1;
   NormArgs a{};
   a.x = x, a.residual = residual, a.weight = weight, a.summed = summed, a.out = out, a.scale = scale, a.rstd = rstd;
   a.ldx = ldx, a.ldr = ldr, a.lds = lds, a.ldo = ldo;
@@ -383,6 +406,9 @@ int hcamdLaunchAddRmsNormBackward(OlQueue q, int elemType, const void *gradOut, 
   char name[64];
   if (gradWeight && c.work(work, workBytes, hcamdAddRmsNormBackwardWorkspace(rows, cols)))
     return 1;
+  if (rows && (c.apart({gradIn, gradWeight}, {summed, weight, rstd}) || c.apart({gradWeight}, {gradOut, gradSummed}) ||
+               c.inPlace(gradIn, ldgi, gradOut, ldg, rows) || c.inPlace(gradIn, ldgi, gradSummed, ldgs, rows)))
+    return 1;
   if (k.general) {
     // the weight's gradient first: grad_in may be grad_out
     a.band = (uint32_t)ceilDiv(rows, std::max<size_t>(lines, 1));
@@ -435,8 +461,8 @@ int hcamdLaunchGatedFfn(OlQueue q, int elemType, const void *x, size_t ldx, cons
     return 0;
   if (d == 0)
     return c.fail("the inner dimension must be at least 1");
-  if (i8 && d > 131072)
-    return c.fail("an inner dimension of %zu (int8 sums are exact up to 131072)", d);
+  if (i8 && d >= 131072) // 2^17 products of 2^14 would be 2^31
+    return c.fail("an inner dimension of %zu (int8 sums are exact below 131072)", d);
   const size_t e = elemBytes(elemType), oe = elemBytes(outType);
   if (c.checkAll({{"x", x, ldx, tokens, d, e}, {"w_gate", wGate, ldwg, f, d, e}, {"w_up", wUp, ldwu, f, d, e},
                   {"out", out, ldo, tokens, f, oe}}))
@@ -453,7 +479,8 @@ int hcamdLaunchGatedFfn(OlQueue q, int elemType, const void *x, size_t ldx, cons
     if ((gate && c.check({"gate", gate, ldgate, tokens, f, oe})) || (up && c.check({"up", up, ldup, tokens, f, oe})))
       return 1;
   }
-  if (c.work(work, workBytes, hcamdGatedFfnWorkspace(elemType, tokens, d, f)))
+  if (c.work(work, workBytes, hcamdGatedFfnWorkspace(elemType, tokens, d, f)) ||
+      c.apart({out, gate, up}, {x, wGate, wUp, xScale, gateScale, upScale}))
     return 1;
   const bool lay = laidOut(kForward, tokens, d, e);
   if (lay) {
@@ -544,7 +571,8 @@ int hcamdLaunchGatedFfnBackward(OlQueue q, int elemType, const void *gradOut, si
       (gradWUp && c.check({"grad_w_up", gradWUp, ldgwu, f, d, 2})))
     return 1;
   const FfnBack b = ffnBack(tokens, d, f);
-  if (tokens && c.work(work, workBytes, b.bytes))
+  if ((tokens && c.work(work, workBytes, b.bytes)) ||
+      c.apart({gradX, gradWGate, gradWUp}, {gradOut, x, wGate, wUp, gate, up}))
     return 1;
   if (!gradX && !gradWGate && !gradWUp)
     return 0;
@@ -676,7 +704,7 @@ int hcamdLaunchLinearCrossEntropy(OlQueue q, int elemType, const void *x, size_t
     return 0;
   const XentFront b = xentFront(tokens, d, vocab);
   if (c.checkAll({{"loss", loss, tokens, 1, tokens, 4}, {"lse", lse, tokens, 1, tokens, 4}}) ||
-      c.work(work, workBytes, b.bytes))
+      c.work(work, workBytes, b.bytes) || c.apart({loss, lse}, {x, weight, targets}))
     return 1;
   char *w = static_cast<char *>(work);
   const char *few = fewOf(tokens, oddRows(x, ldx, 2) || oddRows(weight, ldw, 2));
@@ -772,7 +800,8 @@ int hcamdLaunchLinearCrossEntropyBackward(OlQueue q, int elemType, const void *x
       (gradWeight && c.check({"grad_weight", gradWeight, ldgw, vocab, d, 2})))
     return 1;
   const XentBack b = xentBack(tokens, d, vocab, piece);
-  if (tokens && c.work(work, workBytes, b.bytes))
+  if ((tokens && c.work(work, workBytes, b.bytes)) ||
+      c.apart({gradX, gradWeight}, {x, weight, targets, lse, gradLoss}))
     return 1;
   if (!gradX && !gradWeight)
     return 0;

@@ -1303,6 +1303,10 @@ def plan_clip_grad_norm(grads, outs, norm, max_norm: float) -> Plan:
         if not mg.is_contiguous() or not mo.is_contiguous():
             raise HcRuntimeError(f"clip_grad_norm: tensor {i} must be contiguous")
         table[i].in_, table[i].out, table[i].count, table[i].type = mg.ptr, mo.ptr, mg.size, tg
+    owner = {t.out: i for i, t in enumerate(table[:len(grads)]) if t.count}
+    for i, t in enumerate(table[:len(grads)]):
+        if t.count and (owner[t.out] != i or owner.get(t.in_, i) != i):
+            raise HcRuntimeError(f"clip_grad_norm: tensor {i}: its output is written twice, or is another tensor's input")
     nv = _Vector(norm, "norm", 1, (F32,))
     need = hcamdClipGradNormWorkspace(len(grads))
     work = _workspace(need, ctx)

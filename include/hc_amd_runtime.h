@@ -830,7 +830,7 @@ const char *hcamdLastKernelName(void) HCAMD_NOEXCEPT;
  * caller's, 256-byte aligned, at least the size its function names, its contents
  * meaningless before and after; calls that may overlap in time (two queues, two
  * captured graphs) need one each.  Outputs must not overlap inputs or each other
- * unless stated.  Every result is the same in every run: no atomics.
+ * unless stated; those that begin at one address are refused.  Every result is the same in every run: no atomics.
  */
 
 /* h = x + residual, rounded to elemType; y = h / sqrt(mean(h^2) + eps) * weight
@@ -860,7 +860,7 @@ int hcamdLaunchAddRmsNormBackward(OlQueue q, int elemType, const void *gradOut, 
 /* The gated half of a feed-forward block: out = act(x Wg') * (x Wu').  x is
  * tokens x d, wGate and wUp are f x d, out is tokens x f.  elemType F16 / BF16:
  * fp32 sums, out in elemType; gate and up (may be null) receive x Wg' and x Wu' for
- * the backward pass.  elemType I8: whole sums (d at most 131072), the operands
+ * the backward pass.  elemType I8: whole sums (d below 131072), the operands
  * stand for x[t] * xScale[t], wGate[j] * gateScale[j], wUp[j] * upScale[j] (what
  * hcamdLaunchQuantizeF16I8 and the 8-bit output above make), outType F16 or BF16;
  * gate and up must be null.  GELU is the tanh form. */
@@ -906,7 +906,8 @@ int hcamdLaunchLinearCrossEntropyBackward(OlQueue q, int elemType, const void *x
 
 /* norm[0] = sqrt of the sum of squares over all tensors (summed in fp64), out = in *
  * min(1, maxNorm / (norm + 1e-6)) for each, in fp32 and rounded to the tensor's type
- * (F32, F16, BF16, types may mix; contiguous; count 0 allowed).  out may be in. */
+ * (F32, F16, BF16, types may mix; contiguous; count 0 allowed).  out may be in of the same
+ * tensor. */
 typedef struct HcamdClipTensor {
   const void *in;
   void *out;

@@ -1117,3 +1117,50 @@ def test_operands_end_with_their_memory(t, d):
     # its type at most (2^-7), and a gradient made of stored gate, up, dg and du by as much again of the largest
     for p, q in zip(*results):
         assert bool(torch.isfinite(q).all()) and torch.allclose(p.float(), q.float(), rtol=2 ** -6, atol=2 ** -6 * float(p.abs().max()))
+
+
+def test_copied_rows_captured_and_replayed():
+    """The copies are part of the recorded work: new contents of the operands are seen by every replay."""
+    ctx = rt.default_context()
+    k, t, d, f = torch.bfloat16, 800, 131, 77
+    x, wg, wu, dh = dev(normal(1, t, d), k), dev(normal(2, f, d), k), dev(normal(3, f, d), k), dev(normal(4, t, f), k)
+    targets, g = (torch.arange(t) % f).cuda(), torch.full((t,), 1 / t, device="cuda")
+    out, gate, up = (empty(t, f, ty=k) for _ in range(3))
+    gx, gg, gu, cx, cw = empty(t, d, ty=k), empty(f, d, ty=k), empty(f, d, ty=k), empty(t, d, ty=k), empty(f, d, ty=k)
+    loss, lse = empty(t, ty=torch.float32), empty(t, ty=torch.float32)
+    outs = [out, gate, up, gx, gg, gu, loss, lse, cx, cw]
+    plans = [rt.plan_gated_ffn(x, wg, wu, out, gate=gate, up=up),
+             rt.plan_gated_ffn_backward(dh, x, wg, wu, gate, up, gx, gg, gu),
+             rt.plan_linear_cross_entropy(x, wg, targets, loss, lse),
+             rt.plan_linear_cross_entropy_backward(x, wg, targets, lse, g, cx, cw, piece=40)]
+    for p in plans:
+        p.launch(sync=True)
+    graph = Graph(ctx, lambda: [p.launch() for p in plans])
+    for turn in range(3):
+        x.copy_(dev(normal(50 + turn, t, d), k))
+        wg.copy_(dev(normal(60 + turn, f, d), k))
+        torch.cuda.synchronize()
+        for p in plans:
+            p.launch(sync=True)
+        want = [o.clone() for o in outs]
+        for o in outs:
+            o.fill_(1)
+        torch.cuda.synchronize()
+        graph.replay()
+        ctx.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(outs, want)), turn
+    graph.close()
+
+
+def test_one_tensor_twice_is_refused():
+    a, b, norm = torch.ones(8, device="cuda"), torch.ones(8, device="cuda"), empty(1, ty=torch.float32)
+    for grads, outs in (([a, a], [a, a]), ([a, b], [b, a]), ([a, b], [a, a])):
+        with pytest.raises(rt.HcRuntimeError, match="written twice"):
+            rt.plan_clip_grad_norm(grads, outs, norm, 1.0)
+    c = torch.empty_like(a)
+    rt.clip_grad_norm([a, a], [c, torch.empty_like(a)], norm, 1.0)          # one gradient counted twice, two outputs
+    assert torch.allclose(c, a / 4, rtol=1e-5)
+    x = torch.ones(4, 16, device="cuda", dtype=torch.float16)
+    with pytest.raises(rt.HcRuntimeError, match="two outputs are one buffer"):
+        y = torch.empty_like(x)
+        rt.add_rms_norm(x, None, None, y, summed=y)

@@ -171,6 +171,44 @@ def test_entry_points_refuse(k):
     assert len(q.messages) == 1 and match in q.messages[0], q.messages
 
 
+Q = [P + (k << 24) for k in range(1, 9)]    # addresses apart from P and from each other
+ALIASES = [
+    ("two outputs", lambda q: norm(q, out=P, summed=P)),
+    ("two outputs", lambda q: norm(q, ot=I8, out=Q[0], scale=Q[1], rstd=Q[1])),
+    ("an output is an input", lambda q: norm(q, x=P, ot=I8, out=P, scale=Q[1])),
+    ("an output is an input", lambda q: norm(q, x=Q[0], w=Q[1], out=Q[1])),
+    ("in place with another", lambda q: norm(q, x=P, out=P, ldo=16)),
+    ("in place with another", lambda q: norm(q, x=P, ldx=16, out=Q[0], summed=P)),
+    ("an output is an input", lambda q: norm_back(q, gw=None)),              # grad_in is summed
+    ("two outputs", lambda q: rt.hcamdLaunchGatedFfn(q, F16, P, 8, None, Q[0], 8, None, Q[1], 8, None, 0, Q[2], F16, 4,
+                                                     Q[3], 4, Q[3], 4, 2, 8, 4, None, 0)),
+    ("an output is an input", lambda q: rt.hcamdLaunchGatedFfn(q, F16, P, 8, None, Q[0], 8, None, Q[1], 8, None, 0, P, F16, 8,
+                                                               None, 8, None, 8, 2, 8, 8, None, 0)),
+    ("an output is an input", lambda q: rt.hcamdLaunchGatedFfnBackward(q, F16, Q[0], 4, P, 8, Q[1], 8, Q[2], 8, Q[3], 4, Q[4], 4,
+                                                                       0, P, 8, None, 8, Q[5], 8, 2, 8, 4, Q[6], 1 << 20)),
+    ("two outputs", lambda q: rt.hcamdLaunchGatedFfnBackward(q, F16, Q[0], 4, P, 8, Q[1], 8, Q[2], 8, Q[3], 4, Q[4], 4, 0, None,
+                                                             8, Q[5], 8, Q[5], 8, 2, 8, 4, Q[6], 1 << 20)),
+    ("two outputs", lambda q: rt.hcamdLaunchLinearCrossEntropy(q, F16, Q[0], 8, Q[1], 8, Q[2], I64, P, P, 2, 8, 5, Q[3], 1 << 20)),
+    ("an output is an input", lambda q: rt.hcamdLaunchLinearCrossEntropyBackward(
+        q, F16, Q[0], 8, Q[1], 8, Q[2], I64, Q[3], Q[4], None, 8, Q[1], 8, 2, 8, 5, 0, Q[5], 1 << 20)),
+]
+
+
+@pytest.mark.parametrize("k", range(len(ALIASES)))
+def test_shared_buffers_are_refused(k):
+    match, call = ALIASES[k]
+    q = FakeQueue()
+    assert call(q.ptr) == 1
+    assert len(q.messages) == 1 and match in q.messages[0], q.messages
+
+
+def test_int8_sums_stay_below_their_limit():
+    """131071 products of (-128)^2 fit 32 bits, one more does not."""
+    q = FakeQueue()
+    assert 131071 * 128 * 128 < 2 ** 31 <= 131072 * 128 * 128
+    assert ffn(q.ptr, ty=I8, xs=P, d=131072, ldx=1 << 18) == 1 and "below 131072" in q.messages[0]
+
+
 def test_nothing_to_do_is_no_error():
     q = FakeQueue()
     assert norm(q.ptr, rows=0, x=None, out=None) == 0
