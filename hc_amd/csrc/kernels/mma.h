@@ -109,14 +109,20 @@ struct Tile {
 
 // ---------------------------------------------------------------------------
 // General kernel body: any sizes, leading dimensions and alignment.  128 x 128
-// tile, four waves of 64 x 64, panels through registers in unaligned 16-byte pieces,
-// two tiles of k ahead, two LDS stages, one barrier per k tile.  Every piece is one load
+// tile, four waves of 64 x 64, panels through registers in unaligned 16-byte pieces, two
+// LDS stages, one barrier per k tile.  Panels of k-fast operands are requested two k tiles
+// ahead, others one (the gradient of the weights over 100 tokens has two k tiles in all:
+// 4001 x 9001 bf16 87 us one ahead, 147 us two ahead).  Every piece is one load
 // whatever it crosses: one that reaches past the end of its row is fetched that much
 // earlier and shifted into place on its way to LDS, rows and k past the end are those of
 // the last one, and what lies past K is stored as zeros.  So a k-fast operand has a
 // piece of k at least, or rows padded with zeros to one, and a k-slow operand likewise
 // (their padding may hold anything).  No load stands in a branch: the compiler would
 // wait there for all of them.
+// Bound by the path through registers and LDS (a tile moves 32 KiB into LDS and 64 KiB out
+// of it for 512 cycles of MFMA): 4000 x 11000 x 4088 bf16 both projections 0.82 PFLOP/s
+// forward where the pipelined kernel reaches 1.2; small products by the latency of their
+// k tiles, 0.8 us each.
 // GATED: the N panel holds 32 rows of b[0], then the same 32 of b[1], alternating, so that
 // a wave's blocks j and j + 2 are the two projections of the same outputs.
 // ---------------------------------------------------------------------------
@@ -283,7 +289,7 @@ __device__ __forceinline__ void mma_general(const MmaArgs &g, int wg, unsigned c
 //     consumed.
 //   * A tile is two halves of k.  While the MFMAs of one half run, the operands of
 //     the next are read from LDS into a second register set, one fenced slot per
-//     MFMA in hand order: reads over the first RS MFMAs, loads every LS-th.
+//     MFMA in hand order (the slots are worked out below).
 //   * One barrier per tile, in front of its second half: there this wave's loads
 //     of the next tile have landed and its reads of this tile are done.
 //   * Edges: the last tile of a row or column of tiles begins BM rows (BN columns)
@@ -295,6 +301,13 @@ __device__ __forceinline__ void mma_general(const MmaArgs &g, int wg, unsigned c
 //     readable elements up to there (the library's own buffers).
 // A load's address is a lane part, held in a register for the whole loop, plus a
 // scalar part; from tile to tile only the base of the buffer descriptor moves.
+// Bound by the matrix cores: they are busy 69 % of the cycles with two k-fast operands, 64 %
+// with one k-slow operand, 57 % with two (whose reads are two of 8 bytes and must not
+// stand behind loads into LDS); the clock gives way under the load as it does for a
+// plain product.  256 x 256 tiles over 4096 x 4096 x 11264 bf16: both projections 600 us
+// (1.26 PFLOP/s), dx 590 us, dW 645 us; 2000 x 4096 x 11264 int8 170 us (2.17 POP/s).  For
+// 2048 cycles of MFMA a tile's eight waves of 128 x 64 read 192 KiB from LDS; four waves of
+// 128 x 128 would read a third less, but spill (dx 700 -> 1007 us).
 // ---------------------------------------------------------------------------
 constexpr int waitcnt_imm(int vmcnt, int lgkmcnt) {
   return (vmcnt & 0xf) | ((vmcnt >> 4) << 14) | (7 << 4) | ((lgkmcnt & 0xf) << 8);
@@ -619,10 +632,13 @@ __device__ __forceinline__ void mma_tiles(const MmaArgs &g, int tile, int half_f
 // meet in LDS.  Any size and alignment: rows past the end are read from the last one and
 // not stored, pieces that cross K go element by element.
 //   row_of(j): this lane's row lane % 16 of block j
+// Bound by the weights' bytes: 5.3 TB/s over 2 x 11264 x 4096 bf16 for one token.
 // ODD: rows that do not all begin at a multiple of 4 bytes.  Loads of 16 bytes run at full
-// speed from such addresses only (odd rows of bf16, 60000 x 2231: 2.4 TB/s as they lie), so
-// a piece is fetched from the 4-byte word its first element lies in, with the word that
-// holds its last bytes, and shifted into place.  Both words hold an element of the piece.
+// speed from such addresses only, so a piece is fetched from the 4-byte word its first
+// element lies in and shifted into place.  The word behind it is the first one of the
+// row's next piece, which another lane holds; the last lanes of a block load it, and it
+// holds an element of their piece.  (One token, 60000 x 2231 bf16: 113 us as the rows lie, 74 us
+// so; 11264 x 4095 both projections 3.8 TB/s.)
 // The result lies in LDS as float or int [NB][MB][256], element (m, n) of a block at
 // ((n / 4) * 16 + m) * 4 + n % 4.
 // ---------------------------------------------------------------------------
