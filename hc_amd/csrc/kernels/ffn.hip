@@ -107,7 +107,7 @@ __device__ __forceinline__ void gated_epilogue(const GatedArgs &a, typename MmaT
 template <class E> __device__ __forceinline__ void gated_general(const GatedArgs &a) {
   __shared__ __attribute__((aligned(1024))) unsigned char lds[4 * 128 * 128];
   mma_general<E, kKFast, kKFast, true>(
-      a.mma, blockIdx.x, lds, FromZero{},
+      a.mma, blockIdx.x, 0, lds, FromZero{},
       [&](auto &acc, const Tile &t, int wave_m, int wave_n, int lane, unsigned char *) {
         gated_epilogue<E, 4, 4, false>(a, acc, t, t.m0 + wave_m, t.n0 + wave_n / 2, lane, nullptr);
       });
@@ -115,7 +115,7 @@ template <class E> __device__ __forceinline__ void gated_general(const GatedArgs
 template <class E, int B> __device__ __forceinline__ void gated_tile(const GatedArgs &a) {
   __shared__ __attribute__((aligned(1024))) unsigned char lds[pipelined_lds<B>()];
   mma_tiles<E, kKFast, kKFast, true, B>(
-      a.mma, blockIdx.x, a.mma.half_from, lds, FromZero{},
+      a.mma, blockIdx.x, 0, a.mma.half_from, lds, FromZero{},
       [&](auto &acc, const Tile &t, int wave_m, int wave_n, int lane, unsigned char *l) {
         constexpr int MI = sizeof(acc) / sizeof(acc[0]), NI = sizeof(acc[0]) / sizeof(acc[0][0]);
         gated_epilogue<E, MI, NI, true>(a, acc, t, t.m0 + wave_m, t.n0 + wave_n / 2, lane,
@@ -198,29 +198,29 @@ template <class E> __device__ __forceinline__ void gated_back(const GatedBackArg
 }
 
 // a product that is stored; `tile` counts its workgroups
-template <class E, Layout LA, Layout LB> __device__ __forceinline__ void product_general(const StoreArgs &s, int tile) {
-  __shared__ __attribute__((aligned(1024))) unsigned char lds[4 * 128 * 128];
+template <class E, Layout LA, Layout LB>
+__device__ __forceinline__ void product_general(const StoreArgs &s, int tile, int split, unsigned char *lds) {
   mma_general<E, LA, LB, false>(
-      s.mma, tile, lds,
+      s.mma, tile, split, lds,
       [&](auto &acc, const Tile &t, int wave_m, int wave_n, int lane) {
-        begin_tile<4, 4>(s, acc, t.m0 + wave_m, t.n0 + wave_n, lane);
+        begin_tile<4, 4>(s, acc, t.m0 + wave_m, t.n0 + wave_n, lane, split);
       },
       [&](auto &acc, const Tile &t, int wave_m, int wave_n, int lane, unsigned char *) {
-        store_tile<E, 4, 4, false>(s, acc, t, t.m0 + wave_m, t.n0 + wave_n, lane, nullptr);
+        store_tile<E, 4, 4, false>(s, acc, t, t.m0 + wave_m, t.n0 + wave_n, lane, split, nullptr);
       });
 }
 template <class E, Layout LA, Layout LB, int B>
-__device__ __forceinline__ void product_tile(const StoreArgs &s, int tile, int half_from) {
-  __shared__ __attribute__((aligned(1024))) unsigned char lds[pipelined_lds<B>()];
+__device__ __forceinline__ void product_tile(const StoreArgs &s, int tile, int split, int half_from,
+                                             unsigned char *lds) {
   mma_tiles<E, LA, LB, false, B>(
-      s.mma, tile, half_from, lds,
+      s.mma, tile, split, half_from, lds,
       [&](auto &acc, const Tile &t, int wave_m, int wave_n, int lane) {
         constexpr int MI = sizeof(acc) / sizeof(acc[0]), NI = sizeof(acc[0]) / sizeof(acc[0][0]);
-        begin_tile<MI, NI>(s, acc, t.m0 + wave_m, t.n0 + wave_n, lane);
+        begin_tile<MI, NI>(s, acc, t.m0 + wave_m, t.n0 + wave_n, lane, split);
       },
       [&](auto &acc, const Tile &t, int wave_m, int wave_n, int lane, unsigned char *l) {
         constexpr int MI = sizeof(acc) / sizeof(acc[0]), NI = sizeof(acc[0]) / sizeof(acc[0][0]);
-        store_tile<E, MI, NI, true>(s, acc, t, t.m0 + wave_m, t.n0 + wave_n, lane,
+        store_tile<E, MI, NI, true>(s, acc, t, t.m0 + wave_m, t.n0 + wave_n, lane, split,
                                     l + threadIdx.x / kWave * (MI * NI * 512));
       });
 }
@@ -229,14 +229,37 @@ __device__ __forceinline__ void product_tile(const StoreArgs &s, int tile, int h
 struct OfPair {
   int which, tile, half_from;
 };
-__device__ __forceinline__ OfPair of_pair(const PairStoreArgs &a) {
-  const int wg = blockIdx.x, from = a.p[0].mma.half_from;
+__device__ __forceinline__ OfPair of_pair(const PairStoreArgs &a, int wg) {
+  const int from = a.p[0].mma.half_from;
   const int tile = wg < from ? wg : from + (wg - from) / 2; // among the tiles of both
   const int which = tile >= a.tiles ? 1 : 0, first = which * a.tiles;
   // the product's own count, with its half tiles from half_from on
   const int half_from = max(0, min(from - first, a.tiles));
   const int own = tile - first;
   return {which, own < half_from ? own : half_from + 2 * (own - half_from) + (wg - from) % 2, half_from};
+}
+
+// The products of a backward pass with 128 x 128 tiles in one launch, dx's workgroups first:
+// alone neither of them fills the card for long (333 x 1001 x 2731 fp16: 20 and 18.5 us one
+// after the other).
+template <class E, bool PIPELINED> __device__ __forceinline__ void products(const ProductsArgs &a) {
+  __shared__ __attribute__((aligned(1024))) unsigned char lds[4 * 128 * 128];
+  static_assert(pipelined_lds<128>() == sizeof(lds), "");
+  const int first = a.nn_groups * a.nn.mma.splits, wg = blockIdx.x;
+  if (wg < first) {
+    const int split = __builtin_amdgcn_readfirstlane(wg / a.nn_groups), tile = wg - split * a.nn_groups;
+    if constexpr (PIPELINED)
+      product_tile<E, kKFast, kKSlow, 128>(a.nn, tile, split, 0, lds);
+    else
+      product_general<E, kKFast, kKSlow>(a.nn, tile, split, lds);
+  } else {
+    const int split = __builtin_amdgcn_readfirstlane((wg - first) / a.tn_groups);
+    const OfPair o = of_pair(a.tn, wg - first - split * a.tn_groups);
+    if constexpr (PIPELINED)
+      product_tile<E, kKSlow, kKSlow, 128>(a.tn.p[o.which], o.tile, split, 0, lds);
+    else
+      product_general<E, kKSlow, kKSlow>(a.tn.p[o.which], o.tile, split, lds);
+  }
 }
 
 // the partial sums of the splits, added in the order of the splits, four columns a lane
@@ -318,26 +341,20 @@ HCAMD_FFN_FEW(i8, int8_t)
   extern "C" __global__ __launch_bounds__(256) void hcamd_gated_back_##SUFFIX(GatedBackArgs a) {          \
     gated_back<E>(a);                                                                                     \
   }                                                                                                       \
-  extern "C" __global__ __launch_bounds__(256) void hcamd_product_nn_##SUFFIX##_general(StoreArgs a) {    \
-    product_general<E, kKFast, kKSlow>(a, blockIdx.x);                                                                                   \
+  extern "C" __global__ __launch_bounds__(256) void hcamd_products_##SUFFIX##_general(ProductsArgs a) {   \
+    products<E, false>(a);                                                                                \
   }                                                                                                       \
-  extern "C" __global__ __launch_bounds__(256) void hcamd_product_tn_##SUFFIX##_general(PairStoreArgs a) { \
-    const OfPair o = of_pair(a);                                                                          \
-    product_general<E, kKSlow, kKSlow>(a.p[o.which], o.tile);                                                                                     \
+  extern "C" __global__ __launch_bounds__(256) void hcamd_products_##SUFFIX##_t128(ProductsArgs a) {      \
+    products<E, true>(a);                                                                                 \
   }                                                                                                       \
   extern "C" __global__ __launch_bounds__(512) void hcamd_product_nn_##SUFFIX##_t256(StoreArgs a) {       \
-    product_tile<E, kKFast, kKSlow, 256>(a, blockIdx.x, a.mma.half_from);                                                        \
-  }                                                                                                       \
-  extern "C" __global__ __launch_bounds__(256) void hcamd_product_nn_##SUFFIX##_t128(StoreArgs a) {       \
-    product_tile<E, kKFast, kKSlow, 128>(a, blockIdx.x, 0);                                                        \
+    __shared__ __attribute__((aligned(1024))) unsigned char lds[pipelined_lds<256>()];                    \
+    product_tile<E, kKFast, kKSlow, 256>(a, blockIdx.x, blockIdx.y, a.mma.half_from, lds);                \
   }                                                                                                       \
   extern "C" __global__ __launch_bounds__(512) void hcamd_product_tn_##SUFFIX##_t256(PairStoreArgs a) {   \
-    const OfPair o = of_pair(a);                                                                          \
-    product_tile<E, kKSlow, kKSlow, 256>(a.p[o.which], o.tile, o.half_from);                                          \
-  }                                                                                                       \
-  extern "C" __global__ __launch_bounds__(256) void hcamd_product_tn_##SUFFIX##_t128(PairStoreArgs a) {   \
-    const OfPair o = of_pair(a);                                                                          \
-    product_tile<E, kKSlow, kKSlow, 128>(a.p[o.which], o.tile, o.half_from);                                          \
+    __shared__ __attribute__((aligned(1024))) unsigned char lds[pipelined_lds<256>()];                    \
+    const OfPair o = of_pair(a, blockIdx.x);                                                              \
+    product_tile<E, kKSlow, kKSlow, 256>(a.p[o.which], o.tile, blockIdx.y, o.half_from, lds);             \
   }                                                                                                       \
   extern "C" __global__ __launch_bounds__(256) void hcamd_fold_##SUFFIX(FoldJobs a) { fold<E>(a.job[blockIdx.y]); }
 HCAMD_FFN_BACK(bf16, __bf16)

@@ -72,9 +72,9 @@ __device__ __forceinline__ void tile_of(int wg, int tiles_m, int tiles_n, int &t
   tn = __builtin_amdgcn_readfirstlane(in / rows);
 }
 
-// the k tiles [kt0, kt1) of this workgroup's split
-__device__ __forceinline__ void split_of(int all, int splits, int &kt0, int &kt1) {
-  const int split = blockIdx.y, each = all / splits, more = all % splits;
+// the k tiles [kt0, kt1) of a split
+__device__ __forceinline__ void split_of(int all, int split, int splits, int &kt0, int &kt1) {
+  const int each = all / splits, more = all % splits;
   kt0 = __builtin_amdgcn_readfirstlane(split * each + min(split, more));
   kt1 = __builtin_amdgcn_readfirstlane(kt0 + each + (split < more ? 1 : 0));
 }
@@ -127,7 +127,7 @@ struct Tile {
 // a wave's blocks j and j + 2 are the two projections of the same outputs.
 // ---------------------------------------------------------------------------
 template <class E, Layout LA, Layout LB, bool GATED, class Init, class Epilogue>
-__device__ __forceinline__ void mma_general(const MmaArgs &g, int wg, unsigned char *lds, Init &&init,
+__device__ __forceinline__ void mma_general(const MmaArgs &g, int wg, int split, unsigned char *lds, Init &&init,
                                             Epilogue &&epilogue) {
   using T = MmaType<E>;
   constexpr int BM = 128, BN = 128, BNO = GATED ? BN / 2 : BN;
@@ -139,7 +139,7 @@ __device__ __forceinline__ void mma_general(const MmaArgs &g, int wg, unsigned c
   const int wave_m = wave / 2 * 64, wave_n = wave % 2 * 64;
   const int tiles_k = (g.K + T::kBK - 1) / T::kBK, all = tiles_k * g.segments;
   int kt0, kt1;
-  split_of(all, g.splits, kt0, kt1);
+  split_of(all, split, g.splits, kt0, kt1);
 
   // This thread's four pieces of a panel.  k-fast: chunk tid % 8 of rows tid / 8 + 32 i;
   // k-slow: columns tid % 16 * 8 .. + 7 of k tid / 16 + 16 i.
@@ -318,7 +318,7 @@ typedef __attribute__((address_space(3))) void *lds_void_ptr;
 template <int B> constexpr int pipelined_lds() { return 4 * B * 128; }
 
 template <class E, Layout LA, Layout LB, bool GATED, int BM, int BN, int WM, int WN, class Init, class Epilogue>
-__device__ __forceinline__ void mma_pipelined(const MmaArgs &g, int m_lo, int tn, unsigned char *lds, Init &&init,
+__device__ __forceinline__ void mma_pipelined(const MmaArgs &g, int m_lo, int tn, int split, unsigned char *lds, Init &&init,
                                               Epilogue &&epilogue) {
   using T = MmaType<E>;
   constexpr int kWaves = WM * WN, kWaveM = BM / WM, kWaveN = BN / WN;
@@ -361,7 +361,7 @@ __device__ __forceinline__ void mma_pipelined(const MmaArgs &g, int m_lo, int tn
   const int wave_m = wave / WN * kWaveM, wave_n = wave % WN * kWaveN;
   const int tiles_k = (g.K + T::kBK - 1) / T::kBK, all = tiles_k * g.segments;
   int kt0, kt1;
-  split_of(all, g.splits, kt0, kt1);
+  split_of(all, split, g.splits, kt0, kt1);
   const int steps = kt1 - kt0;
   // valid k of the last tile of a segment: elements (k-slow), 16-byte chunks (k-fast)
   const int tail_k = g.K - (tiles_k - 1) * T::kBK;
@@ -602,23 +602,23 @@ __device__ __forceinline__ void mma_pipelined(const MmaArgs &g, int m_lo, int tn
 // card then takes half as long (4096 x 11264 outputs of the gated block: 5.5 rounds
 // instead of 6).  `tile` counts the launch's workgroups from this product's first.
 template <class E, Layout LA, Layout LB, bool GATED, int B, class Init, class Epilogue>
-__device__ __forceinline__ void mma_tiles(const MmaArgs &g, int tile, int half_from, unsigned char *lds, Init &&init,
+__device__ __forceinline__ void mma_tiles(const MmaArgs &g, int tile, int split, int half_from, unsigned char *lds, Init &&init,
                                           Epilogue &&epilogue) {
   constexpr int BNO = GATED ? B / 2 : B;
   const int tiles_m = (g.M + B - 1) / B, tiles_n = (g.N + BNO - 1) / BNO;
   int tm, tn;
   if constexpr (B == 128) {
     tile_of(tile, tiles_m, tiles_n, tm, tn);
-    mma_pipelined<E, LA, LB, GATED, 128, 128, 2, 2>(g, tm * 128, tn, lds, init, epilogue);
+    mma_pipelined<E, LA, LB, GATED, 128, 128, 2, 2>(g, tm * 128, tn, split, lds, init, epilogue);
   } else {
     if (tile < half_from) {
       tile_of(tile, tiles_m, tiles_n, tm, tn);
-      mma_pipelined<E, LA, LB, GATED, 256, 256, 2, 4>(g, tm * 256, tn, lds, init, epilogue);
+      mma_pipelined<E, LA, LB, GATED, 256, 256, 2, 4>(g, tm * 256, tn, split, lds, init, epilogue);
     } else {
       tile_of(half_from + (tile - half_from) / 2, tiles_m, tiles_n, tm, tn);
       const int m_lo = tm * 256 + (tile - half_from) % 2 * 128;
       if (m_lo < g.M)
-        mma_pipelined<E, LA, LB, GATED, 128, 256, 2, 4>(g, m_lo, tn, lds, init, epilogue);
+        mma_pipelined<E, LA, LB, GATED, 128, 256, 2, 4>(g, m_lo, tn, split, lds, init, epilogue);
     }
   }
 }
@@ -854,14 +854,14 @@ __device__ __forceinline__ void store_direct(O *out, size_t ld, int m0, int n0, 
 // or not as a whole)
 template <class E, int MI, int NI, bool LDS>
 __device__ __forceinline__ void store_tile(const StoreArgs &s, f32x4 (&acc)[MI][NI], const Tile &t, int m0, int n0,
-                                           int lane, unsigned char *mine) {
+                                           int lane, int split, unsigned char *mine) {
   if (s.partial && !LDS) {
-    store_direct<float, MI, NI>(s.partial + (size_t)blockIdx.y * s.mma.M * s.ldp, s.ldp, m0, n0,
+    store_direct<float, MI, NI>(s.partial + (size_t)split * s.mma.M * s.ldp, s.ldp, m0, n0,
                                 Window{t.m_lo, s.mma.M, t.n_lo, s.mma.N}, lane, [&](int i, int j) { return acc[i][j]; });
     return;
   }
   if (s.partial) {
-    float *base = s.partial + (size_t)blockIdx.y * s.mma.M * s.ldp + n0 + lane / 16 * 4;
+    float *base = s.partial + (size_t)split * s.mma.M * s.ldp + n0 + lane / 16 * 4;
     const int left = s.mma.N - n0 - lane / 16 * 4, skip = t.n_lo - n0 - lane / 16 * 4;
 #pragma unroll
     for (int i = 0; i < MI; ++i) {
@@ -885,11 +885,11 @@ __device__ __forceinline__ void store_tile(const StoreArgs &s, f32x4 (&acc)[MI][
 }
 // what the sums begin with: zero, or the partial sums of the calls before
 template <int MI, int NI>
-__device__ __forceinline__ void begin_tile(const StoreArgs &s, f32x4 (&acc)[MI][NI], int m0, int n0, int lane) {
+__device__ __forceinline__ void begin_tile(const StoreArgs &s, f32x4 (&acc)[MI][NI], int m0, int n0, int lane, int split) {
   if (!s.accumulate)
     return;
   typedef f32x4 f32x4_u __attribute__((aligned(4)));
-  const float *base = s.partial + (size_t)blockIdx.y * s.mma.M * s.ldp;
+  const float *base = s.partial + (size_t)split * s.mma.M * s.ldp;
 #pragma unroll
   for (int i = 0; i < MI; ++i) {
     const float *row = base + (size_t)min(m0 + i * 16 + lane % 16, s.mma.M - 1) * s.ldp;

@@ -69,6 +69,11 @@ struct PairStoreArgs { // two products of one shape, one after the other in grid
   StoreArgs p[2];
   int tiles; // of one of them
 };
+struct ProductsArgs { // dx and dW of a backward pass; workgroups of one split of each, 0: not wanted
+  StoreArgs nn;
+  PairStoreArgs tn;
+  int nn_groups, tn_groups;
+};
 struct FoldArgs { // out = sum over splits of partial (* *undo)
   const float *partial;
   void *out;

@@ -107,7 +107,7 @@ __device__ __forceinline__ void tile_stats(const XentArgs &a, f32x4 (&acc)[MI][N
 template <class E> __device__ __forceinline__ void stats_general(const XentArgs &a) {
   __shared__ __attribute__((aligned(1024))) unsigned char lds[4 * 128 * 128];
   mma_general<E, kKFast, kKFast, false>(
-      a.mma, blockIdx.x, lds, FromZero{},
+      a.mma, blockIdx.x, 0, lds, FromZero{},
       [&](auto &acc, const Tile &t, int wave_m, int wave_n, int lane, unsigned char *l) {
         // (the main loop ends with a barrier: its stages are free)
         tile_stats<4, 4, 2, 128, 128>(a, acc, t, wave_m, wave_n, lane, reinterpret_cast<float *>(l));
@@ -117,7 +117,7 @@ template <class E> __device__ __forceinline__ void stats_general(const XentArgs 
 template <class E, int B> __device__ __forceinline__ void stats_tile(const XentArgs &a) {
   __shared__ __attribute__((aligned(1024))) unsigned char lds[pipelined_lds<B>()];
   mma_tiles<E, kKFast, kKFast, false, B>(
-      a.mma, blockIdx.x, a.mma.half_from, lds, FromZero{},
+      a.mma, blockIdx.x, 0, a.mma.half_from, lds, FromZero{},
       [&](auto &acc, const Tile &t, int wave_m, int wave_n, int lane, unsigned char *l) {
         constexpr int MI = sizeof(acc) / sizeof(acc[0]), NI = sizeof(acc[0]) / sizeof(acc[0][0]);
         constexpr int WN = B / (NI * 16), BM = MI * 16 * 2;
@@ -220,7 +220,7 @@ __device__ __forceinline__ void tile_p(const XentArgs &a, f32x4 (&acc)[MI][NI], 
 template <class E> __device__ __forceinline__ void p_general(const XentArgs &a) {
   __shared__ __attribute__((aligned(1024))) unsigned char lds[4 * 128 * 128];
   mma_general<E, kKFast, kKFast, false>(
-      a.mma, blockIdx.x, lds, FromZero{},
+      a.mma, blockIdx.x, 0, lds, FromZero{},
       [&](auto &acc, const Tile &t, int wave_m, int wave_n, int lane, unsigned char *) {
         tile_p<E, 4, 4, false>(a, acc, t, t.m0 + wave_m, t.n0 + wave_n, lane, nullptr);
       });
@@ -228,7 +228,7 @@ template <class E> __device__ __forceinline__ void p_general(const XentArgs &a) 
 template <class E, int B> __device__ __forceinline__ void p_tile(const XentArgs &a) {
   __shared__ __attribute__((aligned(1024))) unsigned char lds[pipelined_lds<B>()];
   mma_tiles<E, kKFast, kKFast, false, B>(
-      a.mma, blockIdx.x, a.mma.half_from, lds, FromZero{},
+      a.mma, blockIdx.x, 0, a.mma.half_from, lds, FromZero{},
       [&](auto &acc, const Tile &t, int wave_m, int wave_n, int lane, unsigned char *l) {
         constexpr int MI = sizeof(acc) / sizeof(acc[0]), NI = sizeof(acc[0]) / sizeof(acc[0][0]);
         tile_p<E, MI, NI, true>(a, acc, t, t.m0 + wave_m, t.n0 + wave_n, lane,
@@ -300,7 +300,7 @@ __device__ __forceinline__ void rows_join(const XentRowsArgs &a) {
 // the usual grad_loss, one value for every live row, the -1 at a target is then
 // represented exactly, where -grad_loss itself would carry one and the same rounding
 // error into every row's largest entry; and fp16 keeps the small p of a large
-// vocabulary above its subnormals.  One workgroup.
+// vocabulary above its subnormals.  The first workgroup.
 __device__ __forceinline__ void p_factor(const XentPrepareArgs &a) {
   __shared__ float slots[16];
   float most = 0.0f;
@@ -317,12 +317,12 @@ __device__ __forceinline__ void p_factor(const XentPrepareArgs &a) {
 
 // x as the weight's gradient takes it: rows that take no part are zeros, so that
 // whatever stands in them (padding, NaN) meets no zero of p in a product; rows are
-// padded to pieces of 8.
+// padded to pieces of 8.  The other workgroups.
 template <class E> __device__ __forceinline__ void live_rows(const XentPrepareArgs &a) {
   const uint32_t pieces = (a.cols + 7) / 8;
   const uint64_t total = (uint64_t)a.rows * pieces;
-  for (uint64_t id = (uint64_t)blockIdx.x * blockDim.x + threadIdx.x; id < total;
-       id += (uint64_t)gridDim.x * blockDim.x) {
+  for (uint64_t id = (uint64_t)(blockIdx.x - 1) * blockDim.x + threadIdx.x; id < total;
+       id += (uint64_t)(gridDim.x - 1) * blockDim.x) {
     const uint32_t r = (uint32_t)(id / pieces), c = (uint32_t)(id % pieces) * 8;
     u32x4 v = {0u, 0u, 0u, 0u};
     if (takes_part(a.targets, a.target_i64, r, a.vocab))
@@ -382,6 +382,10 @@ HCAMD_XENT(f16, _Float16)
 HCAMD_XENT_FEW(bf16, __bf16)
 HCAMD_XENT_FEW(f16, _Float16)
 extern "C" __global__ __launch_bounds__(256) void hcamd_xent_rows(XentRowsArgs a) { rows_join(a); }
-extern "C" __global__ __launch_bounds__(1024) void hcamd_xent_factor(XentPrepareArgs a) { p_factor(a); }
-// (a copy of 16-bit values: one kernel for both types)
-extern "C" __global__ __launch_bounds__(256) void hcamd_xent_live(XentPrepareArgs a) { live_rows<uint16_t>(a); }
+// (live rows are a copy of 16-bit values: one kernel for both types)
+extern "C" __global__ __launch_bounds__(1024) void hcamd_xent_prepare(XentPrepareArgs a) {
+  if (blockIdx.x == 0)
+    p_factor(a);
+  else
+    live_rows<uint16_t>(a);
+}

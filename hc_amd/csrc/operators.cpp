@@ -248,6 +248,37 @@ struct Folds {
   }
 };
 
+// The products of a backward pass.  With 128 x 128 tiles both go in one launch.
+struct Products {
+  ProductsArgs args{};
+  Kernel nn{}, tn{};
+  size_t gn = 0, gt = 0; // workgroups of one split of each
+  int launch(const Call &c, int type) {
+    char name[64];
+    const size_t sn = args.nn.mma.splits, st = args.tn.p[0].mma.splits;
+    const bool together = gn && gt && nn.tile == 128 && tn.tile == 128 && !std::strcmp(nn.suffix, tn.suffix);
+    for (int k = together ? 1 : 0; k < 2; ++k) {
+      const Kernel &kernel = k ? tn : nn;
+      if (!(k ? gt : gn))
+        continue;
+      if (kernel.tile == 256) {
+        std::snprintf(name, sizeof(name), "hcamd_product_%s_%s_t256", k ? "tn" : "nn", typeName(type));
+        if (k ? c.launch("ffn", name, args.tn, gt, st, 1, 512) : c.launch("ffn", name, args.nn, gn, sn, 1, 512))
+          return 1;
+        continue;
+      }
+      const size_t n = together || !k ? gn : 0, t = together || k ? gt : 0;
+      if (n > 0x7fffff || t > 0x7fffff)
+        return c.fail("%zu workgroups", std::max(n, t));
+      args.nn_groups = (int)n, args.tn_groups = (int)t;
+      std::snprintf(name, sizeof(name), "hcamd_products_%s_%s", typeName(type), kernel.suffix);
+      if (c.launch("ffn", name, args, n * sn + t * st))
+        return 1;
+    }
+    return 0;
+  }
+};
+
 bool dimsOk(const Call &c, size_t a, size_t b, size_t d) {
   if (a > kMaxDim || b > kMaxDim || d > kMaxDim) {
     c.fail("a dimension exceeds 2^31 - 256");
@@ -599,24 +630,23 @@ int hcamdLaunchGatedFfnBackward(OlQueue q, int elemType, const void *gradOut, si
       return 1;
   }
   Folds folds;
+  Products products;
   if (gradX) {
-    StoreArgs s{};
+    StoreArgs &s = products.args.nn;
     s.mma.a[0] = e.dgate, s.mma.a[1] = e.dup, s.mma.lda[0] = s.mma.lda[1] = b.ldd;
     s.mma.b[0] = wGate, s.mma.b[1] = wUp, s.mma.ldb[0] = ldwg, s.mma.ldb[1] = ldwu;
     s.mma.M = (int)tokens, s.mma.N = (int)d, s.mma.K = (int)f, s.mma.segments = 2, s.mma.splits = b.px.splits;
     s.out = gradX, s.ldo = ldgx, s.ldp = padCols(d);
     s.partial = b.dx ? reinterpret_cast<float *>(w + 2 * b.dg) : nullptr;
-    const Kernel k = kernelOf(b.px.tile, tokens, d, fetchable(wGate, ldwg, d, 2, lay) && fetchable(wUp, ldwu, d, 2, lay),
-                              true);
-    std::snprintf(name, sizeof(name), "hcamd_product_nn_%s_%s", typeName(elemType), k.suffix);
-    const size_t groups = groupsOf(k, ceilDiv(tokens, k.tile) * ceilDiv(d, k.tile), b.px.splits, s.mma.half_from);
-    if (c.launch("ffn", name, s, groups, b.px.splits, 1, k.threads))
-      return 1;
+    products.nn = kernelOf(b.px.tile, tokens, d, fetchable(wGate, ldwg, d, 2, lay) && fetchable(wUp, ldwu, d, 2, lay),
+                           true);
+    products.gn = groupsOf(products.nn, ceilDiv(tokens, products.nn.tile) * ceilDiv(d, products.nn.tile),
+                                            b.px.splits, s.mma.half_from);
     if (s.partial)
       folds.add({s.partial, gradX, s.ldp, ldgx, (uint32_t)tokens, (uint32_t)d, (uint32_t)b.px.splits, nullptr});
   }
   if (gradWGate || gradWUp) {
-    PairStoreArgs s{};
+    PairStoreArgs &s = products.args.tn;
     size_t n = 0;
     for (int k = 0; k < 2; ++k) {
       void *to = k ? gradWUp : gradWGate;
@@ -630,16 +660,15 @@ int hcamdLaunchGatedFfnBackward(OlQueue q, int elemType, const void *gradOut, si
       t.partial = b.dw ? reinterpret_cast<float *>(w + 2 * b.dg + b.dx + n * b.dw) : nullptr;
       ++n;
     }
-    const Kernel k = kernelOf(b.pw.tile, f, d, fetchable(x, ldx, d, 2, lay), false);
-    std::snprintf(name, sizeof(name), "hcamd_product_tn_%s_%s", typeName(elemType), k.suffix);
-    s.tiles = (int)(ceilDiv(f, k.tile) * ceilDiv(d, k.tile));
-    const size_t groups = groupsOf(k, s.tiles * n, b.pw.splits, s.p[0].mma.half_from);
-    if (c.launch("ffn", name, s, groups, b.pw.splits, 1, k.threads))
-      return 1;
+    products.tn = kernelOf(b.pw.tile, f, d, fetchable(x, ldx, d, 2, lay), false);
+    s.tiles = (int)(ceilDiv(f, products.tn.tile) * ceilDiv(d, products.tn.tile));
+    products.gt = groupsOf(products.tn, s.tiles * n, b.pw.splits, s.p[0].mma.half_from);
     for (size_t k = 0; b.dw && k < n; ++k)
       folds.add({s.p[k].partial, s.p[k].out, s.p[k].ldp, s.p[k].ldo, (uint32_t)f, (uint32_t)d, (uint32_t)b.pw.splits,
                  nullptr});
   }
+  if (products.launch(c, elemType))
+    return 1;
   return folds.launch(c, elemType);
 }
 
@@ -816,10 +845,8 @@ int hcamdLaunchLinearCrossEntropyBackward(OlQueue q, int elemType, const void *x
     a.top = elemType == HCAMD_F16 ? 0x1p15f : 1.0f, a.factor = factor;
     a.live_x = const_cast<void *>(live), a.ldx = ldx, a.ldl = padCols(d);
     a.rows = (uint32_t)tokens, a.cols = (uint32_t)d, a.vocab = (uint32_t)vocab;
-    if (c.launch("xent", "hcamd_xent_factor", a, 1, 1, 1, 1024))
-      return 1;
-    if ((gradWeight || lay) && c.launch("xent", "hcamd_xent_live", a,
-                               std::min<size_t>(ceilDiv(tokens * ceilDiv(d, 8), 256), 4096)))
+    const size_t rest = gradWeight || lay ? std::min<size_t>(ceilDiv(tokens * ceilDiv(d, 8), 1024), 1024) : 0;
+    if (c.launch("xent", "hcamd_xent_prepare", a, 1 + rest, 1, 1, 1024))
       return 1;
   }
   if (lay) // (the logits of rows that take no part are not looked at)
@@ -842,41 +869,38 @@ int hcamdLaunchLinearCrossEntropyBackward(OlQueue q, int elemType, const void *x
     a.mma.M = (int)tokens, a.mma.N = (int)n, a.mma.K = (int)d, a.mma.segments = a.mma.splits = 1;
     a.targets = targets, a.target_i64 = targetType == HCAMD_I64, a.v0 = (int)v0, a.vocab = (int)vocab;
     a.lse = lse, a.grad_loss = gradLoss, a.factor = factor, a.p = w + 256, a.ldp = b.ldp;
-    Kernel k = kernelOf(productOf(tokens, n, d, 1, 1, 1).tile, tokens, n,
+    const Kernel k = kernelOf(productOf(tokens, n, d, 1, 1, 1).tile, tokens, n,
                         fetchable(x, ldx, d, 2, lay) && fetchable(rows, ldr, d, 2, lay), true);
     const char *few = fewOf(tokens, oddRows(x, ldx, 2) || oddRows(rows, ldr, 2));
     std::snprintf(name, sizeof(name), "hcamd_xent_p_%s_%s", typeName(elemType), few ? few : k.suffix);
-    size_t groups = few ? ceilDiv(n, kFewColumns)
+    const size_t groups = few ? ceilDiv(n, kFewColumns)
                         : groupsOf(k, ceilDiv(tokens, k.tile) * ceilDiv(n, k.tile), 1, a.mma.half_from);
     if (tokens && c.launch("xent", name, a, groups, 1, 1, few ? 512 : k.threads))
       return 1;
+    Products products;
     if (gradX) {
-      StoreArgs s{};
+      StoreArgs &s = products.args.nn;
       s.mma.a[0] = a.p, s.mma.lda[0] = b.ldp, s.mma.b[0] = rows, s.mma.ldb[0] = ldr;
       s.mma.M = (int)tokens, s.mma.N = (int)d, s.mma.K = (int)n, s.mma.segments = 1, s.mma.splits = b.px.splits;
       s.partial = dx, s.ldp = padCols(d), s.accumulate = v0 != 0;
-      k = kernelOf(b.px.tile, tokens, d, fetchable(rows, ldr, d, 2, lay), true);
-      std::snprintf(name, sizeof(name), "hcamd_product_nn_%s_%s", typeName(elemType), k.suffix);
-      groups = groupsOf(k, ceilDiv(tokens, k.tile) * ceilDiv(d, k.tile), b.px.splits, s.mma.half_from);
-      if (c.launch("ffn", name, s, groups, b.px.splits, 1, k.threads))
-        return 1;
+      products.nn = kernelOf(b.px.tile, tokens, d, fetchable(rows, ldr, d, 2, lay), true);
+      products.gn = groupsOf(
+          products.nn, ceilDiv(tokens, products.nn.tile) * ceilDiv(d, products.nn.tile), b.px.splits, s.mma.half_from);
     }
     if (gradWeight) {
-      PairStoreArgs s{};
-      StoreArgs &t = s.p[0];
+      StoreArgs &t = products.args.tn.p[0];
       t.mma.a[0] = a.p, t.mma.lda[0] = b.ldp, t.mma.b[0] = live, t.mma.ldb[0] = padCols(d);
       t.mma.M = (int)n, t.mma.N = (int)d, t.mma.K = (int)tokens, t.mma.segments = 1, t.mma.splits = b.pw.splits;
       t.out = static_cast<char *>(gradWeight) + v0 * ldgw * 2, t.ldo = ldgw, t.undo = undo;
       t.partial = b.dw ? reinterpret_cast<float *>(w + 256 + b.p + b.dx) : nullptr, t.ldp = padCols(d);
-      k = kernelOf(b.pw.tile, n, d, fetchable(live, padCols(d), d, 2, true), false);
-      std::snprintf(name, sizeof(name), "hcamd_product_tn_%s_%s", typeName(elemType), k.suffix);
-      s.tiles = (int)(ceilDiv(n, k.tile) * ceilDiv(d, k.tile));
-      groups = groupsOf(k, s.tiles, b.pw.splits, t.mma.half_from);
-      if (c.launch("ffn", name, s, groups, b.pw.splits, 1, k.threads))
-        return 1;
+      products.tn = kernelOf(b.pw.tile, n, d, fetchable(live, padCols(d), d, 2, true), false);
+      products.args.tn.tiles = (int)(ceilDiv(n, products.tn.tile) * ceilDiv(d, products.tn.tile));
+      products.gt = groupsOf(products.tn, products.args.tn.tiles, b.pw.splits, t.mma.half_from);
       if (b.dw)
         folds.add({t.partial, t.out, t.ldp, ldgw, (uint32_t)n, (uint32_t)d, (uint32_t)b.pw.splits, undo});
     }
+    if (products.launch(c, elemType))
+      return 1;
     if (gradX && v0 + n == vocab)
       folds.add({dx, gradX, padCols(d), ldgx, (uint32_t)tokens, (uint32_t)d, (uint32_t)b.px.splits, undo});
     if (folds.launch(c, elemType)) // (the next piece writes the partial sums of dW again)
