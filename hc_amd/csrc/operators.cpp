@@ -256,6 +256,9 @@ struct Products {
   int launch(const Call &c, int type) {
     char name[64];
     const size_t sn = args.nn.mma.splits, st = args.tn.p[0].mma.splits;
+    const bool resident = gn * sn + gt * st <= 2 * kUnits; // all at once: one launch beats the faster kernel
+    if (gn && gt && nn.tile == 128 && tn.tile == 128 && resident && std::strcmp(nn.suffix, tn.suffix))
+      nn.suffix = tn.suffix = "general";
     const bool together = gn && gt && nn.tile == 128 && tn.tile == 128 && !std::strcmp(nn.suffix, tn.suffix);
     for (int k = together ? 1 : 0; k < 2; ++k) {
       const Kernel &kernel = k ? tn : nn;
