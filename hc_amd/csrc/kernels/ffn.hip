@@ -321,22 +321,21 @@ template <class E> __device__ __forceinline__ void lay_out(const LayArgs &a) {
 HCAMD_FFN(bf16, __bf16)
 HCAMD_FFN(f16, _Float16)
 HCAMD_FFN(i8, int8_t)
-#define HCAMD_FFN_FEW(SUFFIX, E)                                                                          \
-  extern "C" __global__ __launch_bounds__(512) void hcamd_gated_##SUFFIX##_s16(GatedArgs a) {             \
-    gated_few<E, 1, 2, 4, false>(a);                                                                      \
+#define HCAMD_FFN_FEW(SUFFIX, E, ROWS, NB, U)                                                             \
+  extern "C" __global__ __launch_bounds__(512) void hcamd_gated_##SUFFIX##_s##ROWS(GatedArgs a) {         \
+    gated_few<E, ROWS / 16, NB, U, false>(a);                                                             \
   }                                                                                                       \
-  extern "C" __global__ __launch_bounds__(512) void hcamd_gated_##SUFFIX##_s32(GatedArgs a) {             \
-    gated_few<E, 2, 2, 4, false>(a);                                                                      \
-  }                                                                                                       \
-  extern "C" __global__ __launch_bounds__(512) void hcamd_gated_##SUFFIX##_s16odd(GatedArgs a) {          \
-    gated_few<E, 1, 2, 4, true>(a);                                                                       \
-  }                                                                                                       \
-  extern "C" __global__ __launch_bounds__(512) void hcamd_gated_##SUFFIX##_s32odd(GatedArgs a) {          \
-    gated_few<E, 2, 2, 4, true>(a);                                                                       \
+  extern "C" __global__ __launch_bounds__(512) void hcamd_gated_##SUFFIX##_s##ROWS##odd(GatedArgs a) {    \
+    gated_few<E, ROWS / 16, NB, U, true>(a);                                                              \
   }
-HCAMD_FFN_FEW(bf16, __bf16)
-HCAMD_FFN_FEW(f16, _Float16)
-HCAMD_FFN_FEW(i8, int8_t)
+#define HCAMD_FFN_FEWS(SUFFIX, E)                                                                         \
+  HCAMD_FFN_FEW(SUFFIX, E, 16, 2, 4)                                                                      \
+  HCAMD_FFN_FEW(SUFFIX, E, 32, 2, 4)                                                                      \
+  HCAMD_FFN_FEW(SUFFIX, E, 64, 2, 2)                                                                      \
+  HCAMD_FFN_FEW(SUFFIX, E, 128, 2, 1)
+HCAMD_FFN_FEWS(bf16, __bf16)
+HCAMD_FFN_FEWS(f16, _Float16)
+HCAMD_FFN_FEWS(i8, int8_t)
 #define HCAMD_FFN_BACK(SUFFIX, E)                                                                         \
   extern "C" __global__ __launch_bounds__(256) void hcamd_gated_back_##SUFFIX(GatedBackArgs a) {          \
     gated_back<E>(a);                                                                                     \

@@ -877,7 +877,18 @@ __device__ __forceinline__ void store_tile(const StoreArgs &s, f32x4 (&acc)[MI][
   }
   const Window w = {t.m_lo, s.mma.M, t.n_lo, s.mma.N};
   const float by = s.undo ? *s.undo : 1.0f;
-  auto value = [&](int i, int j) { return acc[i][j] * by; };
+  // (the product is an fp32 value before it is rounded to the type: folded into the conversion
+  // it would be rounded once in some kernels and twice in others)
+  auto value = [&](int i, int j) {
+    f32x4 v = acc[i][j] * by;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      float x = v[e];
+      asm volatile("" : "+v"(x));
+      v[e] = x;
+    }
+    return v;
+  };
   if constexpr (LDS)
     store_block<E, MI, NI>(mine, static_cast<E *>(s.out), s.ldo, m0, n0, w, lane, value);
   else

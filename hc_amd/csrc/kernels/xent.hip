@@ -354,33 +354,27 @@ template <class E> __device__ __forceinline__ void live_rows(const XentPrepareAr
   }
 HCAMD_XENT(bf16, __bf16)
 HCAMD_XENT(f16, _Float16)
-#define HCAMD_XENT_FEW(SUFFIX, E)                                                                         \
-  extern "C" __global__ __launch_bounds__(512) void hcamd_xent_stats_##SUFFIX##_s16(XentArgs a) {         \
-    stats_few<E, 1, 4, 2, false>(a);                                                                      \
+#define HCAMD_XENT_FEW(SUFFIX, E, ROWS, NB, U)                                                            \
+  extern "C" __global__ __launch_bounds__(512) void hcamd_xent_stats_##SUFFIX##_s##ROWS(XentArgs a) {     \
+    stats_few<E, ROWS / 16, NB, U, false>(a);                                                             \
   }                                                                                                       \
-  extern "C" __global__ __launch_bounds__(512) void hcamd_xent_stats_##SUFFIX##_s32(XentArgs a) {         \
-    stats_few<E, 2, 4, 2, false>(a);                                                                      \
+  extern "C" __global__ __launch_bounds__(512) void hcamd_xent_stats_##SUFFIX##_s##ROWS##odd(XentArgs a) { \
+    stats_few<E, ROWS / 16, NB, U, true>(a);                                                              \
   }                                                                                                       \
-  extern "C" __global__ __launch_bounds__(512) void hcamd_xent_stats_##SUFFIX##_s16odd(XentArgs a) {      \
-    stats_few<E, 1, 4, 2, true>(a);                                                                       \
+  extern "C" __global__ __launch_bounds__(512) void hcamd_xent_p_##SUFFIX##_s##ROWS(XentArgs a) {         \
+    p_few<E, ROWS / 16, NB, U, false>(a);                                                                 \
   }                                                                                                       \
-  extern "C" __global__ __launch_bounds__(512) void hcamd_xent_stats_##SUFFIX##_s32odd(XentArgs a) {      \
-    stats_few<E, 2, 4, 2, true>(a);                                                                       \
-  }                                                                                                       \
-  extern "C" __global__ __launch_bounds__(512) void hcamd_xent_p_##SUFFIX##_s16(XentArgs a) {             \
-    p_few<E, 1, 4, 2, false>(a);                                                                          \
-  }                                                                                                       \
-  extern "C" __global__ __launch_bounds__(512) void hcamd_xent_p_##SUFFIX##_s32(XentArgs a) {             \
-    p_few<E, 2, 4, 2, false>(a);                                                                          \
-  }                                                                                                       \
-  extern "C" __global__ __launch_bounds__(512) void hcamd_xent_p_##SUFFIX##_s16odd(XentArgs a) {          \
-    p_few<E, 1, 4, 2, true>(a);                                                                           \
-  }                                                                                                       \
-  extern "C" __global__ __launch_bounds__(512) void hcamd_xent_p_##SUFFIX##_s32odd(XentArgs a) {          \
-    p_few<E, 2, 4, 2, true>(a);                                                                           \
+  extern "C" __global__ __launch_bounds__(512) void hcamd_xent_p_##SUFFIX##_s##ROWS##odd(XentArgs a) {    \
+    p_few<E, ROWS / 16, NB, U, true>(a);                                                                  \
   }
-HCAMD_XENT_FEW(bf16, __bf16)
-HCAMD_XENT_FEW(f16, _Float16)
+HCAMD_XENT_FEW(bf16, __bf16, 16, 4, 2)
+HCAMD_XENT_FEW(bf16, __bf16, 32, 4, 2)
+HCAMD_XENT_FEW(bf16, __bf16, 64, 2, 2)
+HCAMD_XENT_FEW(bf16, __bf16, 128, 2, 1)
+HCAMD_XENT_FEW(f16, _Float16, 16, 4, 2)
+HCAMD_XENT_FEW(f16, _Float16, 32, 4, 2)
+HCAMD_XENT_FEW(f16, _Float16, 64, 2, 2)
+HCAMD_XENT_FEW(f16, _Float16, 128, 2, 1)
 extern "C" __global__ __launch_bounds__(256) void hcamd_xent_rows(XentRowsArgs a) { rows_join(a); }
 // (live rows are a copy of 16-bit values: one kernel for both types)
 extern "C" __global__ __launch_bounds__(1024) void hcamd_xent_prepare(XentPrepareArgs a) {

@@ -185,18 +185,36 @@ size_t groupsOf(const Kernel &k, size_t tiles, int splits, int &halfFrom) {
   return halves ? tiles + rem : tiles;
 }
 
-// Up to 32 tokens the forward products are one pass over the weights, which the tiled
-// kernels feed from too few workgroups (one token, 2 x 11264 x 4096 bf16: 36 us against
-// 65 us; 48 tokens: 67 us against 65 us).  Null: not for this many tokens.
-constexpr size_t kFewTokens = 32;
-const char *fewOf(size_t tokens, bool odd) {
+// Few tokens: the products with the weights as one pass over them.  Up to 32 tokens always:
+// the tiles feed that pass from too few workgroups (one token, 2 x 11264 x 4096 bf16: 35 us
+// against 65 us).  Up to 128 where it is estimated to take less time: its workgroups read
+// every token's row again, altogether 8.4 TB/s (a workgroup at most 36 KB a us, odd rows
+// 1.6 times as long), the tiles take 0.66 us for each k tile while they are few, half as
+// much again from odd rows.  (64 x 1000 x 2000 bf16 12 us in tiles, 5.9 us so; 64 x 2232 x 5000 31
+// / 22; 100 x 2232 x 5000 32 / 33; 64 x 4096 x 11264 47 / 69; loss 64 x 1001 x 1500 24 / 12,
+// 64 x 1000 x 20000 22 / 24.)  Null: in tiles.
+// rows: of the weights, 32 to a workgroup; k: elements of a row; tileGroups: workgroups in
+// 128 x 128 tiles.
+constexpr size_t kFewTokens = 32, kMostFewTokens = 128;
+const char *fewOf(size_t tokens, size_t rows, size_t k, size_t bytes, size_t tileGroups, bool odd) {
   const int v = hcamdInternalVariant("mma");
-  if (tokens > kFewTokens || (v >= 1 && v <= 3))
+  if (tokens > kMostFewTokens || (v >= 1 && v <= 3))
     return nullptr;
-  return odd ? (tokens <= 16 ? "s16odd" : "s32odd") : tokens <= 16 ? "s16" : "s32";
+  if (tokens > kFewTokens && v != 4) {
+    const double groups = (double)ceilDiv(rows, 32), share = (tokens <= 64 ? 96.0 : 160.0) * k * bytes;
+    const double few = 3.5 * std::max(1.0, groups / (2 * kUnits)) +
+                       (odd ? 1.6 : 1.0) * std::max(groups * share / 8.4e6, share / 3.6e4);
+    const double tiles = (odd ? 1.5 : 1.0) * 1.65 * roundsOf(128, tileGroups) * (ceilDiv(k * bytes, 128) + 3.0);
+    if (few >= tiles)
+      return nullptr;
+  }
+  return tokens <= 16   ? (odd ? "s16odd" : "s16")
+         : tokens <= 32 ? (odd ? "s32odd" : "s32")
+         : tokens <= 64 ? (odd ? "s64odd" : "s64")
+                        : (odd ? "s128odd" : "s128");
 }
 constexpr size_t kFewOutputs = 16; // of the gated block to a workgroup
-constexpr size_t kFewColumns = 64; // of the loss to a workgroup
+size_t fewColumns(size_t tokens) { return tokens <= kFewTokens ? 64 : 32; } // of the loss to a workgroup
 
 // Products over rows whose length is not a multiple of 16 bytes.  The general kernel reads
 // them as they lie; with enough tokens a copy in rows that the pipelined kernels can fetch
@@ -534,7 +552,7 @@ int hcamdLaunchGatedFfn(OlQueue q, int elemType, const void *x, size_t ldx, cons
   a.out = out, a.gate = gate, a.up = up, a.ldo = ldo, a.ldgate = ldgate, a.ldup = ldup;
   a.activation = activation, a.out_f16 = outType == HCAMD_F16;
   char name[64];
-  if (const char *few = fewOf(tokens, oddRows(x, ldx, e) || oddRows(wGate, ldwg, e) || oddRows(wUp, ldwu, e))) {
+  if (const char *few = fewOf(tokens, 2 * f, d, e, ceilDiv(f, 64), oddRows(x, ldx, e) || oddRows(wGate, ldwg, e) || oddRows(wUp, ldwu, e))) {
     std::snprintf(name, sizeof(name), "hcamd_gated_%s_%s", typeName(elemType), few);
     return c.launch("ffn", name, a, ceilDiv(f, kFewOutputs), 1, 1, 512);
   }
@@ -680,7 +698,7 @@ int hcamdLaunchGatedFfnBackward(OlQueue q, int elemType, const void *gradOut, si
 // ===========================================================================
 namespace {
 // columns of the narrowest statistics tile
-size_t statsCols(size_t tokens) { return tokens <= kFewTokens ? kFewColumns : 128; }
+size_t statsCols(size_t tokens) { return tokens <= kMostFewTokens ? fewColumns(tokens) : 128; }
 int xentCommon(const Call &c, int elemType, const void *x, size_t ldx, const void *weight, size_t ldw,
                const void *targets, int targetType, size_t tokens, size_t d, size_t vocab) {
   if (!half16(elemType))
@@ -739,7 +757,7 @@ int hcamdLaunchLinearCrossEntropy(OlQueue q, int elemType, const void *x, size_t
       c.work(work, workBytes, b.bytes) || c.apart({loss, lse}, {x, weight, targets}))
     return 1;
   char *w = static_cast<char *>(work);
-  const char *few = fewOf(tokens, oddRows(x, ldx, 2) || oddRows(weight, ldw, 2));
+  const char *few = fewOf(tokens, vocab, d, 2, ceilDiv(vocab, 128), oddRows(x, ldx, 2) || oddRows(weight, ldw, 2));
   auto kernelFor = [&](size_t n, bool fetch) { return kernelOf(productOf(tokens, n, d, 1, 1, 1).tile, tokens, n, fetch, true); };
   Lays lays;
   if (b.lay)
@@ -750,7 +768,7 @@ int hcamdLaunchLinearCrossEntropy(OlQueue q, int elemType, const void *x, size_t
                      (b.lay ? fetchable(w, padCols(d), d, 2, true) : fetchable(weight, ldw, d, 2, false));
   for (size_t v0 = 0; v0 < vocab; v0 += b.piece) {
     const size_t n = std::min(b.piece, vocab - v0);
-    a.tiles += (int)ceilDiv(n, few ? kFewColumns : kernelFor(n, fetch).tile);
+    a.tiles += (int)ceilDiv(n, few ? fewColumns(tokens) : kernelFor(n, fetch).tile);
   }
   a.stats = reinterpret_cast<float *>(w);
   a.zt = a.stats + tokens * a.tiles * 2;
@@ -765,7 +783,7 @@ int hcamdLaunchLinearCrossEntropy(OlQueue q, int elemType, const void *x, size_t
         return 1;
     }
     const Kernel k = kernelFor(n, fetch);
-    const size_t tiles = ceilDiv(n, few ? kFewColumns : k.tile);
+    const size_t tiles = ceilDiv(n, few ? fewColumns(tokens) : k.tile);
     a.mma.a[0] = x, a.mma.lda[0] = ldx, a.mma.b[0] = rows, a.mma.ldb[0] = ldr;
     a.mma.M = (int)tokens, a.mma.N = (int)n, a.mma.K = (int)d, a.mma.segments = a.mma.splits = 1;
     a.v0 = (int)v0;
@@ -874,9 +892,9 @@ int hcamdLaunchLinearCrossEntropyBackward(OlQueue q, int elemType, const void *x
     a.lse = lse, a.grad_loss = gradLoss, a.factor = factor, a.p = w + 256, a.ldp = b.ldp;
     const Kernel k = kernelOf(productOf(tokens, n, d, 1, 1, 1).tile, tokens, n,
                         fetchable(x, ldx, d, 2, lay) && fetchable(rows, ldr, d, 2, lay), true);
-    const char *few = fewOf(tokens, oddRows(x, ldx, 2) || oddRows(rows, ldr, 2));
+    const char *few = fewOf(tokens, n, d, 2, ceilDiv(n, 128), oddRows(x, ldx, 2) || oddRows(rows, ldr, 2));
     std::snprintf(name, sizeof(name), "hcamd_xent_p_%s_%s", typeName(elemType), few ? few : k.suffix);
-    const size_t groups = few ? ceilDiv(n, kFewColumns)
+    const size_t groups = few ? ceilDiv(n, fewColumns(tokens))
                         : groupsOf(k, ceilDiv(tokens, k.tile) * ceilDiv(n, k.tile), 1, a.mma.half_from);
     if (tokens && c.launch("xent", name, a, groups, 1, 1, few ? 512 : k.threads))
       return 1;

@@ -1164,3 +1164,23 @@ def test_one_tensor_twice_is_refused():
     with pytest.raises(rt.HcRuntimeError, match="two outputs are one buffer"):
         y = torch.empty_like(x)
         rt.add_rms_norm(x, None, None, y, summed=y)
+
+
+# ---------------------------------------------------------------------------
+# one pass over the weights for as many tokens as it takes
+# ---------------------------------------------------------------------------
+FEW = [(33, 64, 40), (48, 333, 97), (64, 136, 130), (65, 1001, 77), (100, 9, 300), (127, 264, 520), (128, 2000, 33), (90, 40, 1)]
+
+
+@pytest.mark.parametrize("layout", ["dense", "strided", "odd"])
+@pytest.mark.parametrize("shape", FEW, ids=str)
+def test_up_to_128_tokens_in_one_pass(shape, layout):
+    rt.set_variant("mma", 4)
+    try:
+        for ty in ("f16", "bf16"):
+            test_gated_ffn(ty, shape, layout)
+            test_linear_cross_entropy(ty, shape, layout)
+            test_linear_cross_entropy_backward(ty, shape, layout)
+            test_gated_ffn_int8(ty, shape, layout)
+    finally:
+        rt.set_variant("mma", 0)
