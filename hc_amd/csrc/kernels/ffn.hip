@@ -104,12 +104,12 @@ __device__ __forceinline__ void gated_epilogue(const GatedArgs &a, typename MmaT
   }
 }
 
-template <class E> __device__ __forceinline__ void gated_general(const GatedArgs &a) {
-  __shared__ __attribute__((aligned(1024))) unsigned char lds[4 * 128 * 128];
-  mma_general<E, kKFast, kKFast, true>(
+template <class E, int BM> __device__ __forceinline__ void gated_general(const GatedArgs &a) {
+  __shared__ __attribute__((aligned(1024))) unsigned char lds[2 * (BM + 128) * 128];
+  mma_general<E, kKFast, kKFast, true, BM>(
       a.mma, blockIdx.x, 0, lds, FromZero{},
       [&](auto &acc, const Tile &t, int wave_m, int wave_n, int lane, unsigned char *) {
-        gated_epilogue<E, 4, 4, false>(a, acc, t, t.m0 + wave_m, t.n0 + wave_n / 2, lane, nullptr);
+        gated_epilogue<E, BM / 32, 4, false>(a, acc, t, t.m0 + wave_m, t.n0 + wave_n / 2, lane, nullptr);
       });
 }
 template <class E, int B> __device__ __forceinline__ void gated_tile(const GatedArgs &a) {
@@ -200,7 +200,7 @@ template <class E> __device__ __forceinline__ void gated_back(const GatedBackArg
 // a product that is stored; `tile` counts its workgroups
 template <class E, Layout LA, Layout LB>
 __device__ __forceinline__ void product_general(const StoreArgs &s, int tile, int split, unsigned char *lds) {
-  mma_general<E, LA, LB, false>(
+  mma_general<E, LA, LB, false, 128>(
       s.mma, tile, split, lds,
       [&](auto &acc, const Tile &t, int wave_m, int wave_n, int lane) {
         begin_tile<4, 4>(s, acc, t.m0 + wave_m, t.n0 + wave_n, lane, split);
@@ -310,7 +310,10 @@ template <class E> __device__ __forceinline__ void lay_out(const LayArgs &a) {
 
 #define HCAMD_FFN(SUFFIX, E)                                                                              \
   extern "C" __global__ __launch_bounds__(256) void hcamd_gated_##SUFFIX##_general(GatedArgs a) {         \
-    gated_general<E>(a);                                                                                  \
+    gated_general<E, 128>(a);                                                                             \
+  }                                                                                                       \
+  extern "C" __global__ __launch_bounds__(256) void hcamd_gated_##SUFFIX##_half(GatedArgs a) {            \
+    gated_general<E, 64>(a);                                                                              \
   }                                                                                                       \
   extern "C" __global__ __launch_bounds__(512) void hcamd_gated_##SUFFIX##_t256(GatedArgs a) {            \
     gated_tile<E, 256>(a);                                                                          \

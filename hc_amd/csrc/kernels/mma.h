@@ -126,17 +126,18 @@ struct Tile {
 // GATED: the N panel holds 32 rows of b[0], then the same 32 of b[1], alternating, so that
 // a wave's blocks j and j + 2 are the two projections of the same outputs.
 // ---------------------------------------------------------------------------
-template <class E, Layout LA, Layout LB, bool GATED, class Init, class Epilogue>
+template <class E, Layout LA, Layout LB, bool GATED, int BM, class Init, class Epilogue>
 __device__ __forceinline__ void mma_general(const MmaArgs &g, int wg, int split, unsigned char *lds, Init &&init,
                                             Epilogue &&epilogue) {
   using T = MmaType<E>;
-  constexpr int BM = 128, BN = 128, BNO = GATED ? BN / 2 : BN;
-  constexpr int kPanel = 128 * 128, kStage = 2 * kPanel, kChunk = T::kChunk;
+  constexpr int BN = 128, BNO = GATED ? BN / 2 : BN;
+  constexpr int kPanel = BM * 128, kStage = kPanel + BN * 128, kA = BM / 32, kMI = BM / 32, kChunk = T::kChunk;
+  static_assert(BM == 128 || LA == kKFast, "a k-slow panel is 128 wide");
   static_assert(sizeof(E) == 2 || (LA == kKFast && LB == kKFast), "transposed reads are for 16-bit elements");
   int tm, tn;
   tile_of(wg, (g.M + BM - 1) / BM, (g.N + BNO - 1) / BNO, tm, tn);
   const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
-  const int wave_m = wave / 2 * 64, wave_n = wave % 2 * 64;
+  const int wave_m = wave / 2 * (BM / 2), wave_n = wave % 2 * 64;
   const int tiles_k = (g.K + T::kBK - 1) / T::kBK, all = tiles_k * g.segments;
   int kt0, kt1;
   split_of(all, split, g.splits, kt0, kt1);
@@ -152,19 +153,22 @@ __device__ __forceinline__ void mma_general(const MmaArgs &g, int wg, int split,
   const int early_b = LB == kKSlow ? max(tile.n0 + column - max(g.N - 8, 0), 0) : 0;
   const bool narrow = (LA == kKSlow && g.M < BM) || (LB == kKSlow && g.N < BN);
   constexpr int kAhead = LA == kKFast && LB == kKFast ? 2 : 1;
-  u32x4 ra[kAhead][4], rb[kAhead][4];
-  const E *pa[4], *pb[4]; // k-fast: the rows; k-slow: the pieces at k tile 0
+  u32x4 ra[kAhead][kA], rb[kAhead][4];
+  const E *pa[kA], *pb[4]; // k-fast: the rows; k-slow: the pieces at k tile 0
   size_t lda = 0, ldb = 0;
   int segment = -1;
   auto aim = [&](int seg) {
     lda = seg ? g.lda[1] : g.lda[0], ldb = seg ? g.ldb[1] : g.ldb[0];
     const E *a = static_cast<const E *>(seg ? g.a[1] : g.a[0]), *b = static_cast<const E *>(seg ? g.b[1] : g.b[0]);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < kA; ++i) {
       if constexpr (LA == kKFast)
         pa[i] = a + (size_t)min(tile.m0 + tid / 8 + 32 * i, g.M - 1) * lda;
       else
         pa[i] = a + (size_t)(slow_k + 16 * i) * lda + (tile.m0 + column - early_a);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
       if constexpr (GATED) {
         const int r = tid / 8 + 32 * i, n = min(tile.n0 + i / 2 * 32 + r % 32, g.N - 1);
         pb[i] = static_cast<const E *>(i % 2 ? g.b[1] : g.b[0]) + (size_t)n * (i % 2 ? g.ldb[1] : g.ldb[0]);
@@ -182,27 +186,29 @@ __device__ __forceinline__ void mma_general(const MmaArgs &g, int wg, int split,
     if ((kt >= tiles_k ? 1 : 0) != segment)
       aim(kt >= tiles_k ? 1 : 0);
     const int k0 = begin_of(kt), at = min(k0 + chunk, last_chunk);
-    size_t qa[4], qb[4];
+    size_t qa[kA], qb[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < kA; ++i)
       qa[i] = LA == kKFast ? (size_t)at : k0 * lda;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
       qb[i] = LB == kKFast ? (size_t)at : k0 * ldb;
-    }
     if ((LA == kKSlow || LB == kKSlow) && k0 + T::kBK > g.K) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const size_t past = max(k0 + slow_k + 16 * i - (g.K - 1), 0);
-        if (LA == kKSlow)
+        if constexpr (LA == kKSlow)
           qa[i] -= past * lda;
-        if (LB == kKSlow)
+        if constexpr (LB == kKSlow)
           qb[i] -= past * ldb;
       }
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < kA; ++i)
       ra[S][i] = *(global_u32x4_ptr)(pa[i] + qa[i]);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
       rb[S][i] = *(global_u32x4_ptr)(pb[i] + qb[i]);
-    }
   };
   // what was fetched early moves into place, what lies past K becomes zero
   auto place = [&](Layout l, u32x4 v, int k0, int i, int early) {
@@ -222,19 +228,21 @@ __device__ __forceinline__ void mma_general(const MmaArgs &g, int wg, int split,
     const int k0 = begin_of(kt);
     if (narrow || k0 + T::kBK > g.K) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
+      for (int i = 0; i < kA; ++i)
         ra[S][i] = place(LA, ra[S][i], k0, i, early_a);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
         rb[S][i] = place(LB, rb[S][i], k0, i, early_b);
-      }
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < kA; ++i)
       *reinterpret_cast<u32x4 *>(lds + buf * kStage + offset(LA, tid + i * 256)) = ra[S][i];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
       *reinterpret_cast<u32x4 *>(lds + buf * kStage + kPanel + offset(LB, tid + i * 256)) = rb[S][i];
-    }
   };
 
-  typename T::acc acc[4][4] = {};
+  typename T::acc acc[kMI][4] = {};
   init(acc, tile, wave_m, wave_n, lane);
   using Set0 = std::integral_constant<int, 0>;
   using Set1 = std::integral_constant<int, kAhead - 1>;
@@ -248,14 +256,15 @@ __device__ __forceinline__ void mma_general(const MmaArgs &g, int wg, int split,
     const unsigned char *pa = lds + buf * kStage, *pb = pa + kPanel;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      u32x4 fa[4], fb[4];
+      u32x4 fa[kMI], fb[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        fa[i] = read_operand<LA, 128>(pa, wave_m + i * 16, h, lane);
-        fb[i] = read_operand<LB, 128>(pb, wave_n + i * 16, h, lane);
-      }
+      for (int i = 0; i < kMI; ++i)
+        fa[i] = read_operand<LA, BM>(pa, wave_m + i * 16, h, lane);
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+      for (int j = 0; j < 4; ++j)
+        fb[j] = read_operand<LB, BN>(pb, wave_n + j * 16, h, lane);
+#pragma unroll
+      for (int i = 0; i < kMI; ++i)
 #pragma unroll
         for (int j = 0; j < 4; ++j)
           acc[i][j] = mma16<E>(fb[j], fa[i], acc[i][j]);

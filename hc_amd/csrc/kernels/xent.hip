@@ -104,13 +104,13 @@ __device__ __forceinline__ void tile_stats(const XentArgs &a, f32x4 (&acc)[MI][N
   }
 }
 
-template <class E> __device__ __forceinline__ void stats_general(const XentArgs &a) {
-  __shared__ __attribute__((aligned(1024))) unsigned char lds[4 * 128 * 128];
-  mma_general<E, kKFast, kKFast, false>(
+template <class E, int BM> __device__ __forceinline__ void stats_general(const XentArgs &a) {
+  __shared__ __attribute__((aligned(1024))) unsigned char lds[2 * (BM + 128) * 128];
+  mma_general<E, kKFast, kKFast, false, BM>(
       a.mma, blockIdx.x, 0, lds, FromZero{},
       [&](auto &acc, const Tile &t, int wave_m, int wave_n, int lane, unsigned char *l) {
         // (the main loop ends with a barrier: its stages are free)
-        tile_stats<4, 4, 2, 128, 128>(a, acc, t, wave_m, wave_n, lane, reinterpret_cast<float *>(l));
+        tile_stats<BM / 32, 4, 2, BM, 128>(a, acc, t, wave_m, wave_n, lane, reinterpret_cast<float *>(l));
       });
 }
 
@@ -217,12 +217,12 @@ __device__ __forceinline__ void tile_p(const XentArgs &a, f32x4 (&acc)[MI][NI], 
     store_direct<E, MI, NI>(static_cast<E *>(a.p), a.ldp, m0, n0, w, lane, value);
 }
 
-template <class E> __device__ __forceinline__ void p_general(const XentArgs &a) {
-  __shared__ __attribute__((aligned(1024))) unsigned char lds[4 * 128 * 128];
-  mma_general<E, kKFast, kKFast, false>(
+template <class E, int BM> __device__ __forceinline__ void p_general(const XentArgs &a) {
+  __shared__ __attribute__((aligned(1024))) unsigned char lds[2 * (BM + 128) * 128];
+  mma_general<E, kKFast, kKFast, false, BM>(
       a.mma, blockIdx.x, 0, lds, FromZero{},
       [&](auto &acc, const Tile &t, int wave_m, int wave_n, int lane, unsigned char *) {
-        tile_p<E, 4, 4, false>(a, acc, t, t.m0 + wave_m, t.n0 + wave_n, lane, nullptr);
+        tile_p<E, BM / 32, 4, false>(a, acc, t, t.m0 + wave_m, t.n0 + wave_n, lane, nullptr);
       });
 }
 template <class E, int B> __device__ __forceinline__ void p_tile(const XentArgs &a) {
@@ -335,11 +335,17 @@ template <class E> __device__ __forceinline__ void live_rows(const XentPrepareAr
 
 #define HCAMD_XENT(SUFFIX, E)                                                                             \
   extern "C" __global__ __launch_bounds__(256) void hcamd_xent_stats_##SUFFIX##_general(XentArgs a) {     \
-    stats_general<E>(a);                                                                                  \
-  }                                                                                                       \
+    stats_general<E, 128>(a);  \
+  }  \
+  extern "C" __global__ __launch_bounds__(256) void hcamd_xent_stats_##SUFFIX##_half(XentArgs a) {  \
+    stats_general<E, 64>(a);  \
+  }  \
   extern "C" __global__ __launch_bounds__(256) void hcamd_xent_p_##SUFFIX##_general(XentArgs a) {         \
-    p_general<E>(a);                                                                                      \
-  }                                                                                                       \
+    p_general<E, 128>(a);  \
+  }  \
+  extern "C" __global__ __launch_bounds__(256) void hcamd_xent_p_##SUFFIX##_half(XentArgs a) {  \
+    p_general<E, 64>(a);  \
+  }  \
   extern "C" __global__ __launch_bounds__(512) void hcamd_xent_stats_##SUFFIX##_t256(XentArgs a) {        \
     stats_tile<E, 256>(a);                                                                          \
   }                                                                                                       \

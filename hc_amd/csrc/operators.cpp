@@ -114,6 +114,7 @@ constexpr size_t kUnits = 256;
 struct Product {
   int tile; // 256 or 128
   int splits;
+  double groups, steps, fold, cost; // of the model: workgroups, k tiles of each, folding, all
 };
 size_t padCols(size_t n) { return alignUp(n, 8); }
 // units of time of `groups` workgroups that each hold one tile's share of k
@@ -125,14 +126,15 @@ double roundsOf(int tile, size_t groups) {
   const size_t rem = groups % kUnits;
   return (double)(groups / kUnits) + (rem == 0 ? 0.0 : rem <= kUnits / 2 ? 0.55 : 1.0);
 }
-// `products` of one shape in one launch; maxSplits 1: the k of a tile stays with one workgroup
-Product productOf(size_t m, size_t n, size_t k, int segments, size_t products, size_t maxSplits) {
+// `products` of one shape in one launch; maxSplits 1: the k of a tile stays with one
+// workgroup; only: this tile size (0: either)
+Product productOf(size_t m, size_t n, size_t k, int segments, size_t products, size_t maxSplits, int only = 0) {
   const int v = hcamdInternalVariant("mma");
   const size_t kTiles = ceilDiv(k, (size_t)64) * segments;
-  Product best{128, 1};
-  double least = 1e300;
+  Product best{128, 1, 0, 0, 0, 1e300};
   for (int tile : {128, 256}) {
-    if ((tile == 256 && (m < 256 || n < 256 || v == 2)) || (tile == 128 && v == 3 && m >= 256 && n >= 256))
+    if ((tile == 256 && (m < 256 || n < 256 || v == 2)) || (tile == 128 && v == 3 && m >= 256 && n >= 256) ||
+        (only && tile != only))
       continue;
     const size_t tiles = ceilDiv(m, tile) * ceilDiv(n, tile) * products;
     for (size_t s = 1; s <= maxSplits && (s == 1 || kTiles / s >= 4); s *= 2) {
@@ -141,12 +143,24 @@ Product productOf(size_t m, size_t n, size_t k, int segments, size_t products, s
         break;
       // (split tiles are not halved)
       const double rounds = s > 1 && tile == 256 ? (double)ceilDiv(tiles * s, kUnits) : roundsOf(tile, tiles * s);
-      const double cost = rounds * ((double)ceilDiv(kTiles, s) + 3.0) + (s > 1 ? (2 * bytes / 8e12 * 1e6 + 5.0) / 1.65 : 0.0);
-      if (cost < least)
-        least = cost, best = {tile, (int)s};
+      const double steps = (double)ceilDiv(kTiles, s) + 3.0, fold = s > 1 ? (2 * bytes / 8e12 * 1e6 + 5.0) / 1.65 : 0.0;
+      if (rounds * steps + fold < best.cost)
+        best = {tile, (int)s, (double)(tiles * s), steps, fold, rounds * steps + fold};
     }
   }
   return best;
+}
+// dx and dW: with 128 x 128 tiles they go in one launch, which saves 2.4 units and lets either
+// fill the places that the other leaves, for as long as the card holds most of them at once
+// (us apart / together: loss 300 x 1000 x 5000 bf16 backward, 704 workgroups 45 / 38; 300 x
+// 1000 x 20000, 1640 of them 100 / 91; block 1000 x 2224 x 5000, 2016 of them 155 / 168).
+void pairOf(Product &dx, Product &dw, const Product &dx128, const Product &dw128) {
+  const double work = dx128.groups * dx128.steps + dw128.groups * dw128.steps;
+  const double together = std::max(0.64 / (2 * kUnits) * work, 0.64 * std::max(dx128.steps, dw128.steps)) +
+                          dx128.fold + dw128.fold;
+  if (hcamdInternalVariant("mma") == 0 && dx128.groups + dw128.groups <= 3.5 * 2 * kUnits &&
+      together < dx.cost + dw.cost + 2.4)
+    dx = dx128, dw = dw128;
 }
 constexpr size_t kMaxSplits = 64;
 size_t partialBytes(const Product &p, size_t m, size_t n) {
@@ -167,14 +181,26 @@ struct Kernel {
   const char *suffix;
   size_t threads;
   int tile;
+  int rows; // of a tile
 };
 // (fewM: a k-fast A may have fewer rows than the tile)
 Kernel kernelOf(int tile, size_t m, size_t n, bool fetch, bool fewM) {
   if (!fetch || hcamdInternalVariant("mma") == 1 || (m < 128 && !fewM) || n < 128)
-    return {"general", 256, 128};
+    return {"general", 256, 128, 128};
   if (tile == 256 && m >= 256 && n >= 256)
-    return {"t256", 512, 256};
-  return {"t128", 256, 128};
+    return {"t256", 512, 256, 256};
+  return {"t128", 256, 128, 128};
+}
+// A product with weights, whose tiles take as many columns as there are: while 64 x 128 tiles
+// fill the card no more than once they take less time than 128 x 128 ones on half of it (48
+// tokens, 2 x 11264 x 4096 bf16: 30 us against 43 us; 500 x 1001 x 1001 fp16 13 against 19;
+// where they need a second round 333 x 1001 x 2731 21 against 18.4).
+Kernel forwardKernel(size_t m, size_t n, size_t k, bool fetch) {
+  Kernel kernel = kernelOf(productOf(m, n, k, 1, 1, 1).tile, m, n, fetch, true);
+  const int v = hcamdInternalVariant("mma");
+  if ((v == 0 && kernel.tile == 128 && ceilDiv(m, 64) * ceilDiv(n, 128) <= kUnits) || v == 5)
+    kernel = {"half", 256, 128, 64};
+  return kernel;
 }
 // The workgroups of `tiles` tiles: a last round of 256 x 256 tiles that fills at most half
 // the card is worked in halves, from `halfFrom` on.
@@ -189,10 +215,10 @@ size_t groupsOf(const Kernel &k, size_t tiles, int splits, int &halfFrom) {
 // the tiles feed that pass from too few workgroups (one token, 2 x 11264 x 4096 bf16: 35 us
 // against 65 us).  Up to 128 where it is estimated to take less time: its workgroups read
 // every token's row again, altogether 8.4 TB/s (a workgroup at most 36 KB a us, odd rows
-// 1.6 times as long), the tiles take 0.66 us for each k tile while they are few, half as
-// much again from odd rows.  (64 x 1000 x 2000 bf16 12 us in tiles, 5.9 us so; 64 x 2232 x 5000 31
-// / 22; 100 x 2232 x 5000 32 / 33; 64 x 4096 x 11264 47 / 69; loss 64 x 1001 x 1500 24 / 12,
-// 64 x 1000 x 20000 22 / 24.)  Null: in tiles.
+// 1.6 times as long), the tiles take 0.42 us for each k tile while 64 x 128 ones fit the
+// card, 0.66 us while 128 x 128 ones do, more from odd rows.  (In tiles / so: 64 x 1000 x 2000
+// bf16 11 / 5.9 us; 100 x 1001 x 2001 13 / 12; 64 x 2232 x 5000 19 / 22; 64 x 4096 x 11264 31 / 69;
+// loss 64 x 1001 x 1500 17 / 12, 64 x 1000 x 20000 22 / 24.)  Null: in tiles.
 // rows: of the weights, 32 to a workgroup; k: elements of a row; tileGroups: workgroups in
 // 128 x 128 tiles.
 constexpr size_t kFewTokens = 32, kMostFewTokens = 128;
@@ -204,7 +230,10 @@ const char *fewOf(size_t tokens, size_t rows, size_t k, size_t bytes, size_t til
     const double groups = (double)ceilDiv(rows, 32), share = (tokens <= 64 ? 96.0 : 160.0) * k * bytes;
     const double few = 3.5 * std::max(1.0, groups / (2 * kUnits)) +
                        (odd ? 1.6 : 1.0) * std::max(groups * share / 8.4e6, share / 3.6e4);
-    const double tiles = (odd ? 1.5 : 1.0) * 1.65 * roundsOf(128, tileGroups) * (ceilDiv(k * bytes, 128) + 3.0);
+    const double kTiles = (double)ceilDiv(k * bytes, 128);
+    const double tiles = ceilDiv(tokens, 64) * tileGroups <= kUnits
+                             ? 4.0 + (odd ? 0.55 : 0.42) * kTiles
+                             : (odd ? 1.5 : 1.0) * 1.65 * roundsOf(128, tileGroups) * (kTiles + 3.0);
     if (few >= tiles)
       return nullptr;
   }
@@ -557,12 +586,11 @@ int hcamdLaunchGatedFfn(OlQueue q, int elemType, const void *x, size_t ldx, cons
     return c.launch("ffn", name, a, ceilDiv(f, kFewOutputs), 1, 1, 512);
   }
   // (a tile of outputs takes twice its columns of the two weight matrices)
-  const Kernel k = kernelOf(productOf(tokens, 2 * f, i8 ? d / 2 : d, 1, 1, 1).tile, tokens, 2 * f,
-                            fetchable(x, ldx, d, e, lay) && fetchable(wGate, ldwg, d, e, lay) &&
-                                fetchable(wUp, ldwu, d, e, lay),
-                            true);
+  const Kernel k = forwardKernel(tokens, 2 * f, i8 ? d / 2 : d,
+                                 fetchable(x, ldx, d, e, lay) && fetchable(wGate, ldwg, d, e, lay) &&
+                                     fetchable(wUp, ldwu, d, e, lay));
   std::snprintf(name, sizeof(name), "hcamd_gated_%s_%s", typeName(elemType), k.suffix);
-  const size_t groups = groupsOf(k, ceilDiv(tokens, k.tile) * ceilDiv(f, k.tile / 2), 1, a.mma.half_from);
+  const size_t groups = groupsOf(k, ceilDiv(tokens, k.rows) * ceilDiv(f, k.tile / 2), 1, a.mma.half_from);
   return c.launch("ffn", name, a, groups, 1, 1, k.threads);
 }
 
@@ -579,6 +607,7 @@ FfnBack ffnBack(size_t tokens, size_t d, size_t f) {
   b.dg = alignUp(tokens * b.ldd * 2, 256);
   b.px = productOf(tokens, d, f, 2, 1, kMaxSplits);
   b.pw = productOf(f, d, tokens, 1, 2, kMaxSplits);
+  pairOf(b.px, b.pw, productOf(tokens, d, f, 2, 1, kMaxSplits, 128), productOf(f, d, tokens, 1, 2, kMaxSplits, 128));
   b.dx = partialBytes(b.px, tokens, d);
   b.dw = partialBytes(b.pw, f, d);
   b.lay = 2 * b.dg + b.dx + 2 * b.dw;
@@ -758,7 +787,6 @@ int hcamdLaunchLinearCrossEntropy(OlQueue q, int elemType, const void *x, size_t
     return 1;
   char *w = static_cast<char *>(work);
   const char *few = fewOf(tokens, vocab, d, 2, ceilDiv(vocab, 128), oddRows(x, ldx, 2) || oddRows(weight, ldw, 2));
-  auto kernelFor = [&](size_t n, bool fetch) { return kernelOf(productOf(tokens, n, d, 1, 1, 1).tile, tokens, n, fetch, true); };
   Lays lays;
   if (b.lay)
     lays.add(x, ldx, w + b.stats, tokens, d, 2);
@@ -768,7 +796,7 @@ int hcamdLaunchLinearCrossEntropy(OlQueue q, int elemType, const void *x, size_t
                      (b.lay ? fetchable(w, padCols(d), d, 2, true) : fetchable(weight, ldw, d, 2, false));
   for (size_t v0 = 0; v0 < vocab; v0 += b.piece) {
     const size_t n = std::min(b.piece, vocab - v0);
-    a.tiles += (int)ceilDiv(n, few ? fewColumns(tokens) : kernelFor(n, fetch).tile);
+    a.tiles += (int)ceilDiv(n, few ? fewColumns(tokens) : forwardKernel(tokens, n, d, fetch).tile);
   }
   a.stats = reinterpret_cast<float *>(w);
   a.zt = a.stats + tokens * a.tiles * 2;
@@ -782,13 +810,13 @@ int hcamdLaunchLinearCrossEntropy(OlQueue q, int elemType, const void *x, size_t
       if (lays.launch(c, 2))
         return 1;
     }
-    const Kernel k = kernelFor(n, fetch);
+    const Kernel k = forwardKernel(tokens, n, d, fetch);
     const size_t tiles = ceilDiv(n, few ? fewColumns(tokens) : k.tile);
     a.mma.a[0] = x, a.mma.lda[0] = ldx, a.mma.b[0] = rows, a.mma.ldb[0] = ldr;
     a.mma.M = (int)tokens, a.mma.N = (int)n, a.mma.K = (int)d, a.mma.segments = a.mma.splits = 1;
     a.v0 = (int)v0;
     std::snprintf(name, sizeof(name), "hcamd_xent_stats_%s_%s", typeName(elemType), few ? few : k.suffix);
-    const size_t groups = few ? tiles : groupsOf(k, ceilDiv(tokens, k.tile) * tiles, 1, a.mma.half_from);
+    const size_t groups = few ? tiles : groupsOf(k, ceilDiv(tokens, k.rows) * tiles, 1, a.mma.half_from);
     if (c.launch("xent", name, a, groups, 1, 1, few ? 512 : k.threads))
       return 1;
     a.tile0 += (int)tiles;
@@ -818,6 +846,8 @@ XentBack xentBack(size_t tokens, size_t d, size_t vocab, size_t piece) {
   b.p = alignUp(tokens * b.ldp * 2, 256);
   b.px = productOf(tokens, d, b.piece, 1, 1, kMaxSplits);
   b.pw = productOf(b.piece, d, tokens, 1, 1, kMaxSplits);
+  pairOf(b.px, b.pw, productOf(tokens, d, b.piece, 1, 1, kMaxSplits, 128),
+         productOf(b.piece, d, tokens, 1, 1, kMaxSplits, 128));
   b.dx = alignUp((size_t)b.px.splits * tokens * padCols(d) * 4, 256);
   b.dw = partialBytes(b.pw, b.piece, d);
   b.live = alignUp(tokens * padCols(d) * 2, 256);
@@ -890,12 +920,11 @@ int hcamdLaunchLinearCrossEntropyBackward(OlQueue q, int elemType, const void *x
     a.mma.M = (int)tokens, a.mma.N = (int)n, a.mma.K = (int)d, a.mma.segments = a.mma.splits = 1;
     a.targets = targets, a.target_i64 = targetType == HCAMD_I64, a.v0 = (int)v0, a.vocab = (int)vocab;
     a.lse = lse, a.grad_loss = gradLoss, a.factor = factor, a.p = w + 256, a.ldp = b.ldp;
-    const Kernel k = kernelOf(productOf(tokens, n, d, 1, 1, 1).tile, tokens, n,
-                        fetchable(x, ldx, d, 2, lay) && fetchable(rows, ldr, d, 2, lay), true);
+    const Kernel k = forwardKernel(tokens, n, d, fetchable(x, ldx, d, 2, lay) && fetchable(rows, ldr, d, 2, lay));
     const char *few = fewOf(tokens, n, d, 2, ceilDiv(n, 128), oddRows(x, ldx, 2) || oddRows(rows, ldr, 2));
     std::snprintf(name, sizeof(name), "hcamd_xent_p_%s_%s", typeName(elemType), few ? few : k.suffix);
     const size_t groups = few ? ceilDiv(n, fewColumns(tokens))
-                        : groupsOf(k, ceilDiv(tokens, k.tile) * ceilDiv(n, k.tile), 1, a.mma.half_from);
+                        : groupsOf(k, ceilDiv(tokens, k.rows) * ceilDiv(n, k.tile), 1, a.mma.half_from);
     if (tokens && c.launch("xent", name, a, groups, 1, 1, few ? 512 : k.threads))
       return 1;
     Products products;

@@ -1184,3 +1184,17 @@ def test_up_to_128_tokens_in_one_pass(shape, layout):
             test_gated_ffn_int8(ty, shape, layout)
     finally:
         rt.set_variant("mma", 0)
+
+
+@pytest.mark.parametrize("layout", ["dense", "odd"])
+@pytest.mark.parametrize("shape", FEW + [(257, 200, 264), (300, 328, 391), (513, 640, 520)], ids=str)
+def test_tiles_of_64_rows(shape, layout):
+    rt.set_variant("mma", 5)
+    try:
+        for ty in ("f16", "bf16"):
+            test_gated_ffn(ty, shape, layout)
+            test_linear_cross_entropy(ty, shape, layout)
+            test_linear_cross_entropy_backward(ty, shape, layout)
+            test_gated_ffn_int8(ty, shape, layout)
+    finally:
+        rt.set_variant("mma", 0)
