@@ -124,9 +124,9 @@ template <class E, int B> __device__ __forceinline__ void gated_tile(const Gated
 }
 
 // Few tokens: one pass over the weights; a workgroup holds NB * 8 outputs' rows of both
-// (blocks j and j + NB / 2 belong together).  NB 2, U 4: 36 us for one token and 50 us for
-// 32 over 2 x 11264 x 4096 bf16 (5.1 and 3.7 TB/s); NB 4, U 2: 47 and 54 us, half as
-// many workgroups.
+// (blocks j and j + NB / 2 belong together).  NB 2, U 4: 35 us for one token and 48 us for
+// 32 over 2 x 11264 x 4096 bf16 (5.3 and 3.8 TB/s); NB 4, U 2: 47 and 54 us, half as
+// many workgroups.  Beyond 32 tokens fewer pieces of k are under way (U 2, 1): registers.
 template <class E, class O, int MB, int NB, int U, bool ODD>
 __device__ __forceinline__ void gated_skinny(const GatedArgs &a, unsigned char *lds) {
   constexpr int H = NB / 2;

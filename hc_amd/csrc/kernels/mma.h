@@ -633,7 +633,7 @@ __device__ __forceinline__ void mma_tiles(const MmaArgs &g, int tile, int split,
 }
 
 // ---------------------------------------------------------------------------
-// Few tokens: M <= 16 * MB rows of A against NB blocks of sixteen rows of B, for
+// Few tokens (which of them: the launcher's estimate): M <= 16 * MB rows of A against NB blocks of sixteen rows of B, for
 // products that are one pass over B.  Eight waves share the k of the tile; each reads B and A straight into
 // MFMA operand registers (sixteen rows, 64 consecutive bytes of a row per four lanes;
 // which k a lane holds does not matter as long as both operands agree), the next block

@@ -126,8 +126,8 @@ template <class E, int B> __device__ __forceinline__ void stats_tile(const XentA
 }
 
 // Few tokens: one pass over the weight, NB * 16 of its rows a workgroup.  NB 4, U 2: 57 us
-// for one token and 61 us for 32 over 32000 x 4096 bf16 with the joining (4.6 and 4.3
-// TB/s); NB 2, U 4: 65 and 85 us (x is read once per workgroup).
+// for one token and 62 us for 32 over 32000 x 4096 bf16 with the joining (4.6 and 4.3
+// TB/s); NB 2, U 4: 65 and 85 us (x is read once per workgroup).  Beyond 32 tokens NB 2: LDS.
 template <class E, int MB, int NB, int U, bool ODD> __device__ __forceinline__ void stats_few(const XentArgs &a) {
   __shared__ __attribute__((aligned(16))) unsigned char lds[skinny_lds<MB, NB>()];
   const int n0 = blockIdx.x * (NB * 16), left = a.mma.N - n0;

@@ -176,7 +176,9 @@ bool fetchable(const void *p, size_t ld, size_t along, size_t bytes, bool padded
   return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % piece == 0 && (padded || along % piece == 0) &&
          ld * bytes < ((size_t)1 << 23);
 }
-// The kernel of a product: "general", "t128" or "t256", and its workgroups.
+// The kernel of a product: "general", "half" (the same with 64 rows), "t128" or "t256".  The
+// variant family "mma" (0: by size) asks for one of them where the operands allow it: 1
+// general, 2 t128, 3 t256, 4 one pass over the weights up to 128 tokens, 5 half (forward).
 struct Kernel {
   const char *suffix;
   size_t threads;
@@ -224,7 +226,7 @@ size_t groupsOf(const Kernel &k, size_t tiles, int splits, int &halfFrom) {
 constexpr size_t kFewTokens = 32, kMostFewTokens = 128;
 const char *fewOf(size_t tokens, size_t rows, size_t k, size_t bytes, size_t tileGroups, bool odd) {
   const int v = hcamdInternalVariant("mma");
-  if (tokens > kMostFewTokens || (v >= 1 && v <= 3))
+  if (tokens > kMostFewTokens || (v >= 1 && v <= 3) || v == 5)
     return nullptr;
   if (tokens > kFewTokens && v != 4) {
     const double groups = (double)ceilDiv(rows, 32), share = (tokens <= 64 ? 96.0 : 160.0) * k * bytes;
