@@ -136,10 +136,10 @@ template <class T, class W> __device__ __forceinline__ void back_general(const N
 // consecutive bytes.  A workgroup of T lanes walks groups of T / TPR rows; the weight
 // stays in registers, the pieces of the next rows are requested before the sums of the
 // present ones are joined.
-// Bound by memory: 8192 x 4096 bf16 forward with sum 49 us (5.4 TB/s), backward 47 us (5.7
+// Bound by memory: 8192 x 4096 bf16 forward with sum 46 us (5.8 TB/s), backward 47 us (5.7
 // TB/s); 16384 x 4096 fp16 to 8 bits 94 us (5.0 TB/s; the rounding's arithmetic shows).  Rows
 // that begin at odd addresses go in unaligned pieces: 16384 x 4095 bf16 forward 133 us (4.0
-// TB/s), to 8 bits 120 us, backward 114 us.  Four rows: 5 us, the latency of a launch.
+// TB/s), to 8 bits 120 us, backward 114 us.  Four rows: 4 us, the latency of a launch.
 // ---------------------------------------------------------------------------
 template <class T> constexpr int kPiece = 16 / (int)sizeof(T);
 template <class T> using Piece __attribute__((ext_vector_type(kPiece<T>))) = T;
@@ -459,13 +459,15 @@ HCAMD_NORM(float, f32)
 HCAMD_NORM(_Float16, f16)
 HCAMD_NORM(__bf16, bf16)
 
+#define HCAMD_NORM_I8(T, NAME, TPR, VPT, THREADS)                                                          \
+  extern "C" __global__ __launch_bounds__(THREADS) void hcamd_rmsnorm_##NAME##_i8_r##TPR##v##VPT(NormArgs a) { \
+    norm_rows<T, TPR, VPT, THREADS, true>(a);                                                              \
+  }
 #define HCAMD_NORM_ROWS(T, NAME, TPR, VPT, THREADS)                                                        \
   extern "C" __global__ __launch_bounds__(THREADS) void hcamd_rmsnorm_##NAME##_r##TPR##v##VPT(NormArgs a) { \
     norm_rows<T, TPR, VPT, THREADS, false>(a);                                                             \
   }                                                                                                        \
-  extern "C" __global__ __launch_bounds__(THREADS) void hcamd_rmsnorm_##NAME##_i8_r##TPR##v##VPT(NormArgs a) { \
-    norm_rows<T, TPR, VPT, THREADS, true>(a);                                                              \
-  }
+  HCAMD_NORM_I8(T, NAME, TPR, VPT, THREADS)
 #define HCAMD_NORM_BACK(T, NAME, TPR, VPT, THREADS)                                                        \
   extern "C" __global__ __launch_bounds__(THREADS) void hcamd_rmsnorm_back_##NAME##_r##TPR##v##VPT(NormBackArgs a) { \
     back_rows<T, TPR, VPT, THREADS>(a);                                                                    \
@@ -476,16 +478,18 @@ HCAMD_NORM(__bf16, bf16)
 #define HCAMD_NORM_SHORT(T, NAME)                                                                          \
   HCAMD_NORM_BOTH(T, NAME, 64, 1, 256)                                                                     \
   HCAMD_NORM_BOTH(T, NAME, 64, 2, 256)                                                                     \
-  HCAMD_NORM_BOTH(T, NAME, 256, 1, 256)                                                                    \
-  HCAMD_NORM_BOTH(T, NAME, 256, 2, 256)
+  HCAMD_NORM_BOTH(T, NAME, 256, 1, 256)
 #define HCAMD_NORM_16(T, NAME)                                                                             \
   HCAMD_NORM_SHORT(T, NAME)                                                                                \
+  HCAMD_NORM_I8(T, NAME, 256, 2, 256)                                                                      \
+  HCAMD_NORM_BOTH(T, NAME, 512, 1, 512)                                                                    \
   HCAMD_NORM_ROWS(T, NAME, 1024, 1, 1024)                                                                  \
   HCAMD_NORM_BACK(T, NAME, 512, 2, 512)                                                                    \
   HCAMD_NORM_BOTH(T, NAME, 1024, 2, 1024)
 HCAMD_NORM_16(__bf16, bf16)
 HCAMD_NORM_16(_Float16, f16)
 HCAMD_NORM_SHORT(float, f32)
+HCAMD_NORM_BOTH(float, f32, 256, 2, 256)
 HCAMD_NORM_BOTH(float, f32, 256, 4, 256)
 HCAMD_NORM_BOTH(float, f32, 512, 4, 512)
 HCAMD_NORM_BOTH(float, f32, 1024, 4, 1024)

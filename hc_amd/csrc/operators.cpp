@@ -343,17 +343,21 @@ bool dimsOk(const Call &c, size_t a, size_t b, size_t d) {
 
 namespace {
 // The kernel of a row length: as many lanes a row and 16-byte pieces a lane as hold it.  A
-// wave to a row needs no barrier; longer rows take more lanes.  Beyond 512 pieces 16-bit
-// rows, whose values take twice their size in registers, do better with 1024 lanes than
-// with more pieces to a lane (4096 x 8192 bf16: 45 us forward against 51 us, 50 against 58 us
-// in 8 bits; the backward pass 58 us with 512 lanes, 62 us with 1024), fp32 rows do not.
+// wave to a row needs no barrier; longer rows take more lanes.  16-bit rows, whose values take
+// twice their size in registers, do better with more lanes than with more pieces to a lane
+// (4096 x 8192 bf16 with 1024 lanes: 45 us forward against 51 us, 50 against 58 us in 8 bits; the
+// backward pass 58 us with 512 lanes, 62 us with 1024), fp32 rows do not.  From 257 to 512
+// pieces too (8192 x 4096: 43 against 46 us, 4 rows 3.6 against 4.3), but many 8-bit rows do not
+// (8192 x 3001 49 against 43 us; 512 x 3001 6.3 against 7.3), and from 65 to 128 pieces only
+// up to 1024 rows forward (512 x 1000 3.6 against 4.5 us, 2000 x 1000 5.9 against 5.5).
 // Rows beyond 1024 lanes x 2 pieces (fp32: x 4) are read twice by the general kernel.
+enum RowPass { kRowForward, kRowTo8Bits, kRowBackward };
 struct RowKernel {
   const char *suffix;
   size_t lanes, threads;
   bool general;
 };
-RowKernel rowKernel(int type, size_t cols, bool back) {
+RowKernel rowKernel(int type, size_t rows, size_t cols, RowPass pass) {
   struct Entry {
     size_t pieces;
     RowKernel kernel;
@@ -370,6 +374,11 @@ RowKernel rowKernel(int type, size_t cols, bool back) {
   const size_t need = ceilDiv(cols, 16 / elemBytes(type));
   if (hcamdInternalVariant("rmsnorm") == 1)
     return {"general", 256, 256, true};
+  const bool half = type != HCAMD_F32;
+  if (half && pass != kRowBackward && rows <= 4 * kUnits && need > 64 && need <= 128)
+    return shortRows[2].kernel;
+  if (half && need > 256 && need <= 512 && (pass != kRowTo8Bits || rows <= 2 * kUnits))
+    return {"r512v1", 512, 512, false};
   for (const Entry &e : shortRows)
     if (need <= e.pieces)
       return e.kernel;
@@ -378,7 +387,7 @@ RowKernel rowKernel(int type, size_t cols, bool back) {
       if (need <= e.pieces)
         return e.kernel;
   } else {
-    for (const Entry &e : back ? back16 : forward16)
+    for (const Entry &e : pass == kRowBackward ? back16 : forward16)
       if (need <= e.pieces)
         return e.kernel;
   }
@@ -436,7 +445,7 @@ int hcamdLaunchAddRmsNorm(OlQueue q, int elemType, const void *x, size_t ldx, co
   a.ldx = ldx, a.ldr = ldr, a.lds = lds, a.ldo = ldo;
   a.rows = (uint32_t)rows, a.cols = (uint32_t)cols, a.eps = eps;
   a.weight_f32 = !weight || weightType == HCAMD_F32;
-  const RowKernel k = rowKernel(elemType, cols, false);
+  const RowKernel k = rowKernel(elemType, rows, cols, outType == HCAMD_I8 ? kRowTo8Bits : kRowForward);
   char name[64];
   std::snprintf(name, sizeof(name), "hcamd_rmsnorm_%s%s_%s", typeName(elemType), outType == HCAMD_I8 ? "_i8" : "",
                 k.suffix);
@@ -484,7 +493,7 @@ int hcamdLaunchAddRmsNormBackward(OlQueue q, int elemType, const void *gradOut, 
   a.grad_in = gradIn, a.grad_weight = gradWeight, a.partial = static_cast<float *>(work);
   a.ldg = ldg, a.ldh = lds, a.ldgs = ldgs, a.ldgi = ldgi;
   a.rows = (uint32_t)rows, a.cols = (uint32_t)cols, a.weight_f32 = weightType == HCAMD_F32;
-  const RowKernel k = rowKernel(elemType, cols, true);
+  const RowKernel k = rowKernel(elemType, rows, cols, kRowBackward);
   const size_t lines = normBands(rows);
   char name[64];
   if (gradWeight && c.work(work, workBytes, hcamdAddRmsNormBackwardWorkspace(rows, cols)))

@@ -1198,3 +1198,12 @@ def test_tiles_of_64_rows(shape, layout):
             test_gated_ffn_int8(ty, shape, layout)
     finally:
         rt.set_variant("mma", 0)
+
+
+@pytest.mark.parametrize("layout", ["dense", "odd", "bare"])
+@pytest.mark.parametrize("shape", [(3, 520), (700, 1016), (1030, 1000), (3, 2056), (600, 2057), (5, 4095), (520, 4096)], ids=str)
+@pytest.mark.parametrize("ty", TYPES)
+def test_row_kernels_on_both_sides_of_their_limits(ty, shape, layout):
+    test_add_rms_norm(ty, shape, layout)
+    test_add_rms_norm_int8(ty, shape, layout)
+    test_add_rms_norm_backward(ty, shape, layout)
