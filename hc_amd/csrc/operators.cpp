@@ -900,7 +900,7 @@ int hcamdLaunchLinearCrossEntropyBackward(OlQueue q, int elemType, const void *x
   char name[64];
   float *factor = reinterpret_cast<float *>(w);
   const void *live = w + 256 + b.p + b.dx + b.dw;
-  const bool lay = laidOut(kBackward, tokens, d, 2);
+  const bool lay = tokens && laidOut(kBackward, tokens, d, 2); // (without tokens there is no workspace, and nothing to read)
   if (tokens) {
     XentPrepareArgs a{};
     a.x = x, a.targets = targets, a.grad_loss = gradLoss, a.target_i64 = targetType == HCAMD_I64;
