@@ -677,7 +677,7 @@ int hcamdLaunchGatedFfnBackward(OlQueue q, int elemType, const void *gradOut, si
   std::snprintf(name, sizeof(name), "hcamd_gated_back_%s", typeName(elemType));
   if (tokens && c.launch("ffn", name, e, std::min<size_t>(ceilDiv(tokens * ceilDiv(f, 8), 256), 8192)))
     return 1;
-  const bool lay = laidOut(kBackward, tokens, d, 2);
+  const bool lay = tokens && laidOut(kBackward, tokens, d, 2);
   if (lay) {
     char *to = w + b.lay;
     Lays l;

@@ -25,3 +25,16 @@ def test_cross_entropy_backward_without_tokens(ty, d):
     rt.linear_cross_entropy_backward(x, w, targets, none, none, torch.empty_like(x), gw)
     assert not bool(gw.any())
     rt.linear_cross_entropy_backward(x, w, targets, none, none, grad_x=torch.empty_like(x))
+
+
+@pytest.mark.parametrize("d", [1, 5, 7, 8, 13, 200])
+@pytest.mark.parametrize("ty", ["f16", "bf16"])
+def test_gated_ffn_backward_without_tokens(ty, d):
+    """No rows: the weights' gradients are zeros, whatever the length of their rows."""
+    f, k = 40, TYPES[ty]
+    x, z = torch.empty(0, d, device="cuda", dtype=k), torch.empty(0, f, device="cuda", dtype=k)
+    w = dev(normal(1, f, d), k)
+    gg, gu = empty(f, d, ty=k), empty(f, d, ty=k)
+    rt.gated_ffn_backward(z, x, w, w, z, z, torch.empty_like(x), gg, gu)
+    assert not bool(gg.any()) and not bool(gu.any())
+    rt.gated_ffn_backward(z, x, w, w, z, z, grad_x=torch.empty_like(x))
