@@ -168,7 +168,8 @@ size_t partialBytes(const Product &p, size_t m, size_t n) {
 }
 
 // Whether the pipelined kernels can fetch an operand: 16-byte pieces, offsets inside a
-// tile below 2^31.  `along` is its extent in the direction that runs through memory
+// tile (of up to 256 rows, in 32 bits) below 2^31: asked for every operand, the library's own
+// too, whose rows are as long as the block is wide or a piece of the vocabulary.  `along` is its extent in the direction that runs through memory
 // (k for a k-fast operand, its rows for a k-slow one); the library's own buffers are
 // padded there.
 bool fetchable(const void *p, size_t ld, size_t along, size_t bytes, bool padded) {
@@ -699,7 +700,9 @@ int hcamdLaunchGatedFfnBackward(OlQueue q, int elemType, const void *gradOut, si
     s.mma.M = (int)tokens, s.mma.N = (int)d, s.mma.K = (int)f, s.mma.segments = 2, s.mma.splits = b.px.splits;
     s.out = gradX, s.ldo = ldgx, s.ldp = padCols(d);
     s.partial = b.dx ? reinterpret_cast<float *>(w + 2 * b.dg) : nullptr;
-    products.nn = kernelOf(b.px.tile, tokens, d, fetchable(wGate, ldwg, d, 2, lay) && fetchable(wUp, ldwu, d, 2, lay),
+    products.nn = kernelOf(b.px.tile, tokens, d,
+                           fetchable(w, b.ldd, f, 2, true) && fetchable(wGate, ldwg, d, 2, lay) &&
+                               fetchable(wUp, ldwu, d, 2, lay),
                            true);
     products.gn = groupsOf(products.nn, ceilDiv(tokens, products.nn.tile) * ceilDiv(d, products.nn.tile),
                                             b.px.splits, s.mma.half_from);
@@ -721,7 +724,7 @@ int hcamdLaunchGatedFfnBackward(OlQueue q, int elemType, const void *gradOut, si
       t.partial = b.dw ? reinterpret_cast<float *>(w + 2 * b.dg + b.dx + n * b.dw) : nullptr;
       ++n;
     }
-    products.tn = kernelOf(b.pw.tile, f, d, fetchable(x, ldx, d, 2, lay), false);
+    products.tn = kernelOf(b.pw.tile, f, d, fetchable(w, b.ldd, f, 2, true) && fetchable(x, ldx, d, 2, lay), false);
     s.tiles = (int)(ceilDiv(f, products.tn.tile) * ceilDiv(d, products.tn.tile));
     products.gt = groupsOf(products.tn, s.tiles * n, b.pw.splits, s.p[0].mma.half_from);
     for (size_t k = 0; b.dw && k < n; ++k)
@@ -944,7 +947,8 @@ int hcamdLaunchLinearCrossEntropyBackward(OlQueue q, int elemType, const void *x
       s.mma.a[0] = a.p, s.mma.lda[0] = b.ldp, s.mma.b[0] = rows, s.mma.ldb[0] = ldr;
       s.mma.M = (int)tokens, s.mma.N = (int)d, s.mma.K = (int)n, s.mma.segments = 1, s.mma.splits = b.px.splits;
       s.partial = dx, s.ldp = padCols(d), s.accumulate = v0 != 0;
-      products.nn = kernelOf(b.px.tile, tokens, d, fetchable(rows, ldr, d, 2, lay), true);
+      products.nn = kernelOf(b.px.tile, tokens, d, fetchable(a.p, b.ldp, n, 2, true) && fetchable(rows, ldr, d, 2, lay),
+                             true);
       products.gn = groupsOf(
           products.nn, ceilDiv(tokens, products.nn.tile) * ceilDiv(d, products.nn.tile), b.px.splits, s.mma.half_from);
     }
@@ -954,7 +958,8 @@ int hcamdLaunchLinearCrossEntropyBackward(OlQueue q, int elemType, const void *x
       t.mma.M = (int)n, t.mma.N = (int)d, t.mma.K = (int)tokens, t.mma.segments = 1, t.mma.splits = b.pw.splits;
       t.out = static_cast<char *>(gradWeight) + v0 * ldgw * 2, t.ldo = ldgw, t.undo = undo;
       t.partial = b.dw ? reinterpret_cast<float *>(w + 256 + b.p + b.dx) : nullptr, t.ldp = padCols(d);
-      products.tn = kernelOf(b.pw.tile, n, d, fetchable(live, padCols(d), d, 2, true), false);
+      products.tn = kernelOf(b.pw.tile, n, d,
+                             fetchable(a.p, b.ldp, n, 2, true) && fetchable(live, padCols(d), d, 2, true), false);
       products.args.tn.tiles = (int)(ceilDiv(n, products.tn.tile) * ceilDiv(d, products.tn.tile));
       products.gt = groupsOf(products.tn, products.args.tn.tiles, b.pw.splits, t.mma.half_from);
       if (b.dw)

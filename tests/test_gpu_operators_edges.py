@@ -38,3 +38,85 @@ def test_gated_ffn_backward_without_tokens(ty, d):
     rt.gated_ffn_backward(z, x, w, w, z, z, torch.empty_like(x), gg, gu)
     assert not bool(gg.any()) and not bool(gu.any())
     rt.gated_ffn_backward(z, x, w, w, z, z, grad_x=torch.empty_like(x))
+
+
+def far_columns(n):
+    """A few of n columns: both ends, and around the places where 32-bit byte offsets of 16-bit rows end."""
+    at = [0, 1, 7, n // 3, n // 2 + 1, (1 << 22) - 1, 1 << 22, (1 << 22) + 5, n - 9, n - 8, n - 1]
+    return torch.tensor(sorted({c for c in at if 0 <= c < n}))
+
+
+# (the largest 16-bit rows whose 255th, 127th starts within 2^31 bytes hold 4.2 and 8.4 million values)
+@pytest.mark.parametrize("shape", [(128, 128, 8_500_003), (256, 256, 4_300_000)], ids=str)
+def test_block_backward_of_extreme_width(shape):
+    """Pre-activation gradients whose rows lie more than 2^31 bytes apart in all: everything but a few columns is
+    zero, so that the result is a short sum."""
+    t, d, f = shape
+    k = torch.bfloat16
+    at = far_columns(f)
+    n = len(at)
+    vals = {name: dev(normal(i, t, n), k) for i, name in enumerate(("dh", "gate", "up"))}
+    rows = {name: dev(normal(10 + i, n, d), k) for i, name in enumerate(("wg", "wu"))}
+    x = dev(normal(20, t, d), k)
+    dh, gate, up = (torch.zeros(t, f, device="cuda", dtype=k) for _ in range(3))
+    wg, wu, gg, gu = (torch.zeros(f, d, device="cuda", dtype=k) for _ in range(4))
+    for whole, name in ((dh, "dh"), (gate, "gate"), (up, "up")):
+        whole[:, at.cuda()] = vals[name]
+    wg[at.cuda()], wu[at.cuda()] = rows["wg"], rows["wu"]
+    gx = empty(t, d, ty=k)
+    rt.gated_ffn_backward(dh, x, wg, wu, gate, up, gx, gg, gu)
+    a, da = act_reference("silu", f64(vals["gate"]))
+    dg, du = f64(vals["dh"]) * f64(vals["up"]) * da, f64(vals["dh"]) * a
+    edg = dg.abs() * half(k) + 40 * U * (f64(vals["dh"]) * f64(vals["up"])).abs() + tiny(k)
+    edu = du.abs() * half(k) + 40 * U * f64(vals["dh"]).abs() + tiny(k)
+    gd, ud, xd = f64(rows["wg"]), f64(rows["wu"]), f64(x)
+    # (2 n + 2 terms that are not zero, and one addition each for at most 64 partial sums)
+    want, sums = dg @ gd + du @ ud, (4 * n + 130) * U * (dg.abs() @ gd.abs() + du.abs() @ ud.abs())
+    near(gx, want, want.abs() * half(k) + 1.01 * (edg @ gd.abs() + edu @ ud.abs() + sums) + tiny(k), "grad_x")
+    for got, p, ep, name in ((gg, dg, edg, "grad_w_gate"), (gu, du, edu, "grad_w_up")):
+        want = p.t() @ xd
+        near(got[at.cuda()], want, want.abs() * half(k) + 1.01 * (ep.t() @ xd.abs() + 2 * t * U * (p.abs().t() @ xd.abs())) + tiny(k), name)
+        got[at.cuda()] = 0
+        assert not bool(got.any()), name
+
+
+def test_cross_entropy_backward_of_an_extreme_piece():
+    """One piece of the vocabulary whose rows of p lie more than 2^31 bytes apart in all; the weight is zero but for
+    a few rows, so that dx is a short sum and every other row of dW is one and the same."""
+    t, d, v = 128, 128, 8_500_003
+    k = torch.bfloat16
+    at = far_columns(v)
+    n = len(at)
+    x, rows = dev(normal(1, t, d), k), dev(normal(2, n, d) * 0.3, k)
+    w, gw = torch.zeros(v, d, device="cuda", dtype=k), torch.full((v, d), 77.0, device="cuda", dtype=k)
+    w[at.cuda()] = rows
+    hit = torch.arange(t) % n
+    targets = at[hit].cuda()
+    loss, lse = empty(t, ty=torch.float32), empty(t, ty=torch.float32)
+    rt.linear_cross_entropy(x, w, targets, loss, lse)
+    z = f64(x) @ f64(rows).t()
+    want_lse = (z.exp().sum(1) + (v - n)).log()
+    # z is a sum of d products; an exponential's argument is off by a few u of itself on top
+    ez = 2 * d * U * (f64(x).abs() @ f64(rows).abs().t()) + 16 * U * (z.abs() + want_lse[:, None])
+    # a sum of v terms by tiles, of at most 32 additions each, joined by 64 lanes with v / 32 / 64 additions each
+    share = ((z - want_lse[:, None]).exp() * ez).sum(1)
+    near(lse, want_lse, 1.1 * share + (v / 2048 + 80) * U + want_lse.abs() * 4 * U, "lse")
+    gx = empty(t, d, ty=k)
+    grad = torch.full((t,), 1.0, device="cuda")
+    rt.linear_cross_entropy_backward(x, w, targets, lse, grad, gx, gw, piece=v)
+    p = (z - f64(lse)[:, None]).exp()
+    ep = 1.1 * p * (ez + 8 * U)
+    p[torch.arange(t), hit] -= 1
+    ep += (p.abs() + ep) * half(k) + 2 * U + tiny(k)      # (the subtraction, the rounding to the type)
+    rd, xd = f64(rows), f64(x)
+    want = p @ rd
+    near(gx, want, want.abs() * half(k) + 1.01 * (ep @ rd.abs() + (2 * n + 130) * U * (p.abs() @ rd.abs())) + tiny(k), "grad_x")
+    want = p.t() @ xd
+    near(gw[at.cuda()], want, want.abs() * half(k) + 1.01 * (ep.t() @ xd.abs() + 2 * t * U * (p.abs().t() @ xd.abs())) + tiny(k), "grad_weight")
+    other = torch.ones(v, dtype=torch.bool)
+    other[at] = False
+    first = gw[2]
+    assert bool((gw[other.cuda()] == first).all())
+    p0 = (-f64(lse)).exp()
+    want = p0 @ xd
+    near(first, want, want.abs() * half(k) + 1.01 * ((p0 * (half(k) + 300 * U)) @ xd.abs()) + tiny(k), "the other rows")
