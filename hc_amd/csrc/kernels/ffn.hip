@@ -7,7 +7,8 @@
 // is stored.  4 T D F operations.
 // Backward, from the stored pre-activations g and u:
 //   dg = dh u act'(g), du = dh act(g)        element by element, rounded to the
-//                                            element type as matrix operands
+//                                            element type as matrix operands (fp16:
+//                                            scaled by a power of two first)
 //   dx = dg Wg + du Wu                        one product, k runs through both pairs
 //   dWg = dg' x, dWu = du' x                  one launch, both operands k-slow
 #include "mma.h"
@@ -170,10 +171,9 @@ template <class E, int MB, int NB, int U, bool ODD> __device__ __forceinline__ v
   }
 }
 
-// pre-activation gradients: a workgroup walks rows, eight elements a lane.  The
-// destination is the library's own, its rows padded to a multiple of 8.  Bound by memory:
-// 4096 x 11264 bf16 84 us (5.5 TB/s).
-template <class E> __device__ __forceinline__ void gated_back(const GatedBackArgs &a) {
+// f(row, first column, dg, du) for this lane's eights of pre-activation gradients, in fp32
+// (zeros past the end of a row)
+template <class E, class F> __device__ __forceinline__ void each_gated_back(const GatedBackArgs &a, F &&f) {
   const uint32_t chunks = (a.cols + 7) / 8;
   const uint64_t total = (uint64_t)a.rows * chunks;
   for (uint64_t id = (uint64_t)blockIdx.x * blockDim.x + threadIdx.x; id < total;
@@ -184,17 +184,68 @@ template <class E> __device__ __forceinline__ void gated_back(const GatedBackArg
     const ex8 dh = __builtin_bit_cast(ex8, load_chunk(static_cast<const E *>(a.grad_out) + (size_t)r * a.ldg + c, valid, (int)c));
     const ex8 g = __builtin_bit_cast(ex8, load_chunk(static_cast<const E *>(a.gate) + (size_t)r * a.ldgate + c, valid, (int)c));
     const ex8 u = __builtin_bit_cast(ex8, load_chunk(static_cast<const E *>(a.up) + (size_t)r * a.ldup + c, valid, (int)c));
-    ex8 dg, du;
+    float dg[8], du[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      float f, df;
-      activate_both(a.activation, (float)g[e], f, df);
-      dg[e] = (E)((float)dh[e] * (float)u[e] * df);
-      du[e] = (E)((float)dh[e] * f);
+      float act, dact;
+      activate_both(a.activation, (float)g[e], act, dact);
+      dg[e] = (float)dh[e] * (float)u[e] * dact;
+      du[e] = (float)dh[e] * act;
     }
-    *reinterpret_cast<ex8 *>(static_cast<E *>(a.dgate) + (size_t)r * a.ldd + c) = dg;
-    *reinterpret_cast<ex8 *>(static_cast<E *>(a.dup) + (size_t)r * a.ldd + c) = du;
+    f(r, c, dg, du);
   }
+}
+
+// fp16 holds 40 binary places, of which the lowest ten lack precision, and dg and du are products of
+// values that may stand anywhere in them: rounded as they are, those of a gradient of 1e-6
+// would keep four bits, and those of one of 3e4 overflow and meet other terms as NaN.  So they are scaled by the power of two that
+// brings the largest of them to 2^14 .. 2^15, and the products undo it in fp32 (exactly: a block
+// whose dg and du are normal numbers has the results it would have unscaled).  One more launch
+// reads the operands for that maximum.
+__device__ __forceinline__ void gated_back_most(const GatedBackArgs &a) {
+  __shared__ float slots[4];
+  float most = 0.0f;
+  each_gated_back<_Float16>(a, [&](uint32_t, uint32_t, const float *dg, const float *du) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      most = fmaxf(most, fmaxf(__builtin_fabsf(dg[e]), __builtin_fabsf(du[e]))); // (of a NaN and a number: the number)
+  });
+  most = group_reduce<MaxOp, 4>(most, slots);
+  if (threadIdx.x == 0)
+    a.most[blockIdx.x] = most;
+}
+// that power of two; 1 where the largest is zero or infinite (which it then stays)
+__device__ __forceinline__ float gated_back_scale(const GatedBackArgs &a) {
+  __shared__ float slots[4];
+  float most = 0.0f;
+  for (uint32_t i = threadIdx.x; i < a.mosts; i += 256)
+    most = fmaxf(most, a.most[i]);
+  most = group_reduce<MaxOp, 4>(most, slots);
+  const int exponent = (int)(__builtin_bit_cast(uint32_t, most) >> 23) - 127; // (at most 33: products of fp16 values)
+  const int by = most > 0.0f && most < INFINITY ? min(14 - exponent, 100) : 0;
+  if (blockIdx.x == 0 && threadIdx.x == 0)
+    *a.undo = __builtin_bit_cast(float, (uint32_t)(127 - by) << 23);
+  return __builtin_bit_cast(float, (uint32_t)(127 + by) << 23);
+}
+
+// pre-activation gradients: a workgroup walks rows, eight elements a lane.  The
+// destination is the library's own, its rows padded to a multiple of 8.  Bound by memory:
+// 4096 x 11264 bf16 84 us (5.5 TB/s).
+template <class E> __device__ __forceinline__ void gated_back(const GatedBackArgs &a) {
+  float by = 1.0f;
+  if constexpr (std::is_same<E, _Float16>::value)
+    by = gated_back_scale(a);
+  each_gated_back<E>(a, [&](uint32_t r, uint32_t c, const float *dg, const float *du) {
+    typedef E ex8 __attribute__((ext_vector_type(8)));
+    ex8 vg, vu;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      vg[e] = (E)(dg[e] * by);
+      vu[e] = (E)(du[e] * by);
+    }
+    *reinterpret_cast<ex8 *>(static_cast<E *>(a.dgate) + (size_t)r * a.ldd + c) = vg;
+    *reinterpret_cast<ex8 *>(static_cast<E *>(a.dup) + (size_t)r * a.ldd + c) = vu;
+  });
 }
 
 // a product that is stored; `tile` counts its workgroups
@@ -361,6 +412,7 @@ HCAMD_FFN_FEWS(i8, int8_t)
   extern "C" __global__ __launch_bounds__(256) void hcamd_fold_##SUFFIX(FoldJobs a) { fold<E>(a.job[blockIdx.y]); }
 HCAMD_FFN_BACK(bf16, __bf16)
 HCAMD_FFN_BACK(f16, _Float16)
+extern "C" __global__ __launch_bounds__(256) void hcamd_gated_back_most_f16(GatedBackArgs a) { gated_back_most(a); }
 // (copies: one kernel for both 16-bit types)
 extern "C" __global__ __launch_bounds__(256) void hcamd_lay_out_2(LayJobs a) { lay_out<uint16_t>(a.job[blockIdx.y]); }
 extern "C" __global__ __launch_bounds__(256) void hcamd_lay_out_1(LayJobs a) { lay_out<uint8_t>(a.job[blockIdx.y]); }

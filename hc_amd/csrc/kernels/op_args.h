@@ -53,6 +53,10 @@ struct GatedBackArgs { // pre-activation gradients, element by element
   size_t ldg, ldgate, ldup, ldd;
   uint32_t rows, cols;
   int activation;
+  // fp16: the largest magnitude each workgroup of a launch before this one has met, and what
+  // undoes the scaling that follows from them (written by the first workgroup)
+  float *most, *undo;
+  uint32_t mosts;
 };
 
 // a product whose result is stored: in the element type (`out`), or as fp32

@@ -607,8 +607,10 @@ int hcamdLaunchGatedFfn(OlQueue q, int elemType, const void *x, size_t ldx, cons
 }
 
 namespace {
-// the workspace of the backward pass: dg, du, then the partial sums of dx, then of
-// the two weight gradients, then the copies of x, Wg and Wu
+// the workspace of the backward pass: fp16's scaling (what undoes it, the maxima it comes from), dg,
+// du, then the partial sums of dx, then of the two weight gradients, then the copies of x, Wg
+// and Wu
+constexpr size_t kMosts = 1024, kFfnBackHead = 256 + kMosts * 4;
 struct FfnBack {
   size_t ldd, dg, dx, dw, lay, bytes;
   Product px, pw;
@@ -623,7 +625,8 @@ FfnBack ffnBack(size_t tokens, size_t d, size_t f) {
   b.dx = partialBytes(b.px, tokens, d);
   b.dw = partialBytes(b.pw, f, d);
   b.lay = 2 * b.dg + b.dx + 2 * b.dw;
-  b.bytes = b.lay + (laidOut(kBackward, tokens, d, 2) ? layBytes(tokens, d, 2) + 2 * layBytes(f, d, 2) : 0);
+  b.bytes = kFfnBackHead + b.lay +
+            (laidOut(kBackward, tokens, d, 2) ? layBytes(tokens, d, 2) + 2 * layBytes(f, d, 2) : 0);
   return b;
 }
 } // namespace
@@ -669,14 +672,20 @@ int hcamdLaunchGatedFfnBackward(OlQueue q, int elemType, const void *gradOut, si
     return 1;
   if (!gradX && !gradWGate && !gradWUp)
     return 0;
-  char *w = static_cast<char *>(work);
+  char *w = static_cast<char *>(work) + kFfnBackHead;
   char name[64];
   GatedBackArgs e{};
+  e.undo = static_cast<float *>(work), e.most = e.undo + 64;
+  const float *undo = tokens && elemType == HCAMD_F16 ? e.undo : nullptr;
   e.grad_out = gradOut, e.gate = gate, e.up = up, e.dgate = w, e.dup = w + b.dg;
   e.ldg = ldg, e.ldgate = ldgate, e.ldup = ldup, e.ldd = b.ldd;
   e.rows = (uint32_t)tokens, e.cols = (uint32_t)f, e.activation = activation;
+  const size_t eights = ceilDiv(tokens * ceilDiv(f, 8), 256);
+  e.mosts = (uint32_t)std::min(eights, kMosts);
+  if (undo && c.launch("ffn", "hcamd_gated_back_most_f16", e, e.mosts))
+    return 1;
   std::snprintf(name, sizeof(name), "hcamd_gated_back_%s", typeName(elemType));
-  if (tokens && c.launch("ffn", name, e, std::min<size_t>(ceilDiv(tokens * ceilDiv(f, 8), 256), 8192)))
+  if (tokens && c.launch("ffn", name, e, std::min<size_t>(eights, 8192)))
     return 1;
   const bool lay = tokens && laidOut(kBackward, tokens, d, 2);
   if (lay) {
@@ -698,7 +707,7 @@ int hcamdLaunchGatedFfnBackward(OlQueue q, int elemType, const void *gradOut, si
     s.mma.a[0] = e.dgate, s.mma.a[1] = e.dup, s.mma.lda[0] = s.mma.lda[1] = b.ldd;
     s.mma.b[0] = wGate, s.mma.b[1] = wUp, s.mma.ldb[0] = ldwg, s.mma.ldb[1] = ldwu;
     s.mma.M = (int)tokens, s.mma.N = (int)d, s.mma.K = (int)f, s.mma.segments = 2, s.mma.splits = b.px.splits;
-    s.out = gradX, s.ldo = ldgx, s.ldp = padCols(d);
+    s.out = gradX, s.ldo = ldgx, s.ldp = padCols(d), s.undo = undo;
     s.partial = b.dx ? reinterpret_cast<float *>(w + 2 * b.dg) : nullptr;
     products.nn = kernelOf(b.px.tile, tokens, d,
                            fetchable(w, b.ldd, f, 2, true) && fetchable(wGate, ldwg, d, 2, lay) &&
@@ -707,7 +716,7 @@ int hcamdLaunchGatedFfnBackward(OlQueue q, int elemType, const void *gradOut, si
     products.gn = groupsOf(products.nn, ceilDiv(tokens, products.nn.tile) * ceilDiv(d, products.nn.tile),
                                             b.px.splits, s.mma.half_from);
     if (s.partial)
-      folds.add({s.partial, gradX, s.ldp, ldgx, (uint32_t)tokens, (uint32_t)d, (uint32_t)b.px.splits, nullptr});
+      folds.add({s.partial, gradX, s.ldp, ldgx, (uint32_t)tokens, (uint32_t)d, (uint32_t)b.px.splits, undo});
   }
   if (gradWGate || gradWUp) {
     PairStoreArgs &s = products.args.tn;
@@ -720,7 +729,7 @@ int hcamdLaunchGatedFfnBackward(OlQueue q, int elemType, const void *gradOut, si
       t.mma.a[0] = k ? e.dup : e.dgate, t.mma.lda[0] = b.ldd;
       t.mma.b[0] = x, t.mma.ldb[0] = ldx;
       t.mma.M = (int)f, t.mma.N = (int)d, t.mma.K = (int)tokens, t.mma.segments = 1, t.mma.splits = b.pw.splits;
-      t.out = to, t.ldo = k ? ldgwu : ldgwg, t.ldp = padCols(d);
+      t.out = to, t.ldo = k ? ldgwu : ldgwg, t.ldp = padCols(d), t.undo = undo;
       t.partial = b.dw ? reinterpret_cast<float *>(w + 2 * b.dg + b.dx + n * b.dw) : nullptr;
       ++n;
     }
@@ -729,7 +738,7 @@ int hcamdLaunchGatedFfnBackward(OlQueue q, int elemType, const void *gradOut, si
     products.gt = groupsOf(products.tn, s.tiles * n, b.pw.splits, s.p[0].mma.half_from);
     for (size_t k = 0; b.dw && k < n; ++k)
       folds.add({s.p[k].partial, s.p[k].out, s.p[k].ldp, s.p[k].ldo, (uint32_t)f, (uint32_t)d, (uint32_t)b.pw.splits,
-                 nullptr});
+                 undo});
   }
   if (products.launch(c, elemType))
     return 1;

@@ -872,7 +872,8 @@ int hcamdLaunchGatedFfn(OlQueue q, int elemType, const void *x, size_t ldx, cons
                         size_t ldup, size_t tokens, size_t d, size_t f, void *work,
                         size_t workBytes) HCAMD_NOEXCEPT;
 /* Its backward pass from the stored gate and up (F16 / BF16): dg = gradOut * up *
- * act'(gate) and du = gradOut * act(gate), each rounded to elemType, then gradX = dg Wg +
+ * act'(gate) and du = gradOut * act(gate), each rounded to elemType (F16: scaled by a power of
+ * two that brings the largest to 2^14 .. 2^15, which the results undo), then gradX = dg Wg +
  * du Wu, gradWGate = dg' x, gradWUp = du' x, summed in fp32.  Gradients that are
  * null are not computed (x, wGate and wUp may be null where only others need them).
  * Without tokens the weights' gradients are zeros. */

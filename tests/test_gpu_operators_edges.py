@@ -120,3 +120,54 @@ def test_cross_entropy_backward_of_an_extreme_piece():
     p0 = (-f64(lse)).exp()
     want = p0 @ xd
     near(first, want, want.abs() * half(k) + 1.01 * ((p0 * (half(k) + 300 * U)) @ xd.abs()) + tiny(k), "the other rows")
+
+
+@pytest.mark.parametrize("layout", ["dense", "odd"])
+@pytest.mark.parametrize("size", [1e-6, 1e-4, 3e4])
+@pytest.mark.parametrize("shape", [(5, 40, 24), (129, 65, 77), (512, 256, 512), (700, 520, 640)], ids=str)
+def test_block_backward_gradients_at_the_ends_of_fp16(shape, size, layout):
+    """Gradients whose products with the activations leave fp16's normal numbers on either side: dg and du keep their
+    relative precision, and nothing becomes infinite that the results can hold."""
+    t, d, f = shape
+    k = torch.float16
+    kind = "gelu" if layout == "odd" else "silu"
+    by = 0.01 if size > 1 else 1.0                      # (results of large gradients stay below 65504)
+    x, wg, wu = dev(normal(1, t, d) * by, k), dev(normal(2, f, d) * by * d ** -0.5, k), dev(normal(3, f, d) * by * d ** -0.5, k)
+    gate, up = dev(normal(5, t, f), k), dev(normal(6, t, f), k)
+    dh = dev((normal(7, t, f) * size).clamp(-6e4, 6e4), k)
+    pad, off = (3, 1) if layout == "odd" else (0, 0)
+    gx = strided(empty(t, d, ty=k), pad, off)
+    gg, gu = (strided(empty(f, d, ty=k), pad, off) for _ in range(2))
+    rt.gated_ffn_backward(*[strided(v, pad, off) for v in (dh, x, wg, wu, gate, up)], gx, gg, gu, activation=kind)
+    a, da = act_reference(kind, f64(gate))
+    dg, du = f64(dh) * f64(up) * da, f64(dh) * a
+    # the largest of them is scaled to 2^14 at least: half a subnormal step is then that part of it
+    low = tiny(k) * 2.0 ** -14 * max(dg.abs().max(), du.abs().max())
+    edg = dg.abs() * half(k) + 40 * U * (f64(dh) * f64(up)).abs() + low
+    edu = du.abs() * half(k) + 40 * U * f64(dh).abs() + low
+    xd, gd, ud = f64(x), f64(wg), f64(wu)
+    want = dg @ gd + du @ ud
+    assert want.abs().max() < 65000
+    sums = 4 * f * U * (dg.abs() @ gd.abs() + du.abs() @ ud.abs())
+    near(gx, want, want.abs() * half(k) + 1.01 * (edg @ gd.abs() + edu @ ud.abs() + sums) + tiny(k), "grad_x")
+    for got, p, ep, name in ((gg, dg, edg, "grad_w_gate"), (gu, du, edu, "grad_w_up")):
+        want = p.t() @ xd
+        assert want.abs().max() < 65000
+        near(got, want, want.abs() * half(k) + 1.01 * (ep.t() @ xd.abs() + 2 * t * U * (p.abs().t() @ xd.abs())) + tiny(k), name)
+
+
+def test_block_backward_fp16_that_is_zero_or_not_finite():
+    """Gradients that are all zero; one that is infinite or NaN reaches its own row and column only."""
+    t, d, f = 40, 64, 96
+    k = torch.float16
+    x, w = dev(normal(1, t, d), k), dev(normal(2, f, d) * 0.1, k)
+    gate, up = dev(normal(3, t, f), k), dev(normal(4, t, f), k)
+    for bad in (0.0, float("inf"), float("nan")):
+        dh = torch.zeros(t, f, device="cuda", dtype=k)
+        dh[5, 7] = bad
+        gx, gg, gu = (torch.full_like(v, 77.0) for v in (x, w, w))
+        rt.gated_ffn_backward(dh, x, w, w, gate, up, gx, gg, gu)
+        for o, row in ((gx, 5), (gg, 7), (gu, 7)):
+            assert bool(torch.isfinite(o[row]).any()) == (bad == 0.0)
+            o[row] = 0
+            assert not bool(o.any())
