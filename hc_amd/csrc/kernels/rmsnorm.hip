@@ -38,6 +38,12 @@ __device__ __forceinline__ int8_t quantise(float h, float w, float per, double m
   return !(__builtin_fabsf(t - q) <= 0.5f - 0x1p-14f) ? quantise64(h, w, most) : (int8_t)q;
 }
 
+// rstd * most / 127; NaN for a row that is not finite, 0 for one of zeros (whose rstd is
+// infinite where eps is 0)
+__device__ __forceinline__ float scale_of(double most, float rstd) {
+  return !(most < (double)INFINITY) ? __builtin_nanf("") : most > 0.0 ? (float)(most * rstd / 127.0) : 0.0f;
+}
+
 template <class T, class W> struct Row {
   const T *x, *r;
   const W *w;
@@ -100,7 +106,7 @@ template <class T, class W, bool I8> __device__ __forceinline__ void norm_genera
       if (a.rstd)
         a.rstd[row] = rstd;
       if constexpr (I8)
-        a.scale[row] = most < (double)INFINITY ? (float)(most * rstd / 127.0) : __builtin_nanf("");
+        a.scale[row] = scale_of(most, rstd);
     }
     __syncthreads(); // the slots are used again
   }
@@ -249,7 +255,7 @@ __device__ __forceinline__ void norm_rows(const NormArgs &a) {
       if (a.rstd)
         a.rstd[row] = rstd;
       if constexpr (I8)
-        a.scale[row] = most < (double)INFINITY ? (float)(most * rstd / 127.0) : __builtin_nanf("");
+        a.scale[row] = scale_of(most, rstd);
     }
     const bool usable = most > 0.0 && most < (double)INFINITY;
     const float per = most > 0x1p-60 && most < 0x1p60 ? 127.0f / (float)most : __builtin_nanf("");

@@ -171,3 +171,16 @@ def test_block_backward_fp16_that_is_zero_or_not_finite():
             assert bool(torch.isfinite(o[row]).any()) == (bad == 0.0)
             o[row] = 0
             assert not bool(o.any())
+
+
+@pytest.mark.parametrize("cols", [1, 100, 4096, 20000])
+@pytest.mark.parametrize("ty", TYPES)
+def test_a_row_of_zeros_has_scale_0_without_eps(ty, cols):
+    x = dev(normal(1, 4, cols), TYPES[ty])
+    x[1] = 0
+    w = torch.ones(cols, device="cuda")
+    for weight, zeros in ((w, [1]), (w * 0, [0, 1, 2, 3])):
+        q, scale = torch.full((4, cols), 55, device="cuda", dtype=torch.int8), empty(4, ty=torch.float32)
+        rt.add_rms_norm(x, None, weight, q, eps=0.0, scale=scale)
+        assert [r for r in range(4) if float(scale[r]) == 0.0] == zeros, scale
+        assert not bool(q[zeros].any()) and bool(torch.isfinite(scale).all())
