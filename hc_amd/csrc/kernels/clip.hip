@@ -2,8 +2,8 @@
 //   norm = sqrt(sum of squares over all tensors), out = in * min(1, max_norm / (norm + 1e-6)).
 // Two launches (per 64 tensors, which travel in the kernel arguments): partial sums of
 // squares per workgroup, then every workgroup adds all partial sums in their order and
-// scales its share.  Sums are held in 64 bits: no overflow of large fp32 gradients, and
-// the result does not depend on how the tensors are cut.
+// scales its share.  Sums, the norm and the factor are held in 64 bits: no overflow of large
+// fp32 gradients, and the result does not depend on how the tensors are cut.
 // Bound by memory: no element can be stored before the last has been read, so the tensors are
 // read twice.  60 tensors of 0.8 GB: 160 us for the sums (5 TB/s), 278 us for the scaling
 // (5.8 TB/s); 12 small ones 3.5 + 4 us, two launches.
@@ -70,12 +70,12 @@ template <class T> __device__ __forceinline__ double chunk_squares(const void *i
   return sum;
 }
 template <class T>
-__device__ __forceinline__ void chunk_scale(const void *in, void *out, uint64_t first, int n, float by) {
+__device__ __forceinline__ void chunk_scale(const void *in, void *out, uint64_t first, int n, float pre, float by) {
   T *to = static_cast<T *>(out) + first;
   each_piece(static_cast<const T *>(in) + first, n, [&](Piece<T> v, int at, int valid) {
 #pragma unroll
     for (int e = 0; e < kPiece<T>; ++e)
-      v[e] = (T)((float)v[e] * by);
+      v[e] = (T)((float)v[e] * pre * by);
     store_chunk(to + at, __builtin_bit_cast(u32x4, v), valid);
   });
 }
@@ -107,12 +107,15 @@ __device__ __forceinline__ void scale(const ClipArgs &a) {
   double sum = 0.0;
   for (uint32_t i = threadIdx.x; i < a.cells; i += 256)
     sum += a.partial[i];
-  const float norm = (float)__builtin_sqrt(group_sum64(sum, slots));
+  const double norm = __builtin_sqrt(group_sum64(sum, slots));
   // (a NaN norm gives a NaN factor, an infinite one 0)
-  float factor = a.max_norm / (norm + 1e-6f);
-  factor = factor > 1.0f ? 1.0f : factor;
+  double factor = (double)a.max_norm / (norm + 1e-6);
+  factor = factor > 1.0 ? 1.0 : factor;
+  // a factor near or below fp32's smallest normal numbers goes in two steps, the first a power
+  // of two
+  const float pre = factor < 0x1p-64 ? 0x1p-64f : 1.0f, by = (float)(factor < 0x1p-64 ? factor * 0x1p64 : factor);
   if (blockIdx.x == 0 && threadIdx.x == 0)
-    *a.norm = norm;
+    *a.norm = (float)norm;
   // from the last chunk to the first: what the sums read last is still in the
   // memory-side cache
   const uint32_t chunks = a.first_chunk[a.tensors];
@@ -121,11 +124,11 @@ __device__ __forceinline__ void scale(const ClipArgs &a) {
     uint64_t first;
     const int n = chunk_of(a, chunk, t, first);
     if (a.type[t] == 0)
-      chunk_scale<float>(a.in[t], a.out[t], first, n, factor);
+      chunk_scale<float>(a.in[t], a.out[t], first, n, pre, by);
     else if (a.type[t] == 1)
-      chunk_scale<_Float16>(a.in[t], a.out[t], first, n, factor);
+      chunk_scale<_Float16>(a.in[t], a.out[t], first, n, pre, by);
     else
-      chunk_scale<__bf16>(a.in[t], a.out[t], first, n, factor);
+      chunk_scale<__bf16>(a.in[t], a.out[t], first, n, pre, by);
   }
 }
 

@@ -905,8 +905,9 @@ int hcamdLaunchLinearCrossEntropyBackward(OlQueue q, int elemType, const void *x
                                           size_t ldgw, size_t tokens, size_t d, size_t vocab, size_t piece,
                                           void *work, size_t workBytes) HCAMD_NOEXCEPT;
 
-/* norm[0] = sqrt of the sum of squares over all tensors (summed in fp64), out = in *
- * min(1, maxNorm / (norm + 1e-6)) for each, in fp32 and rounded to the tensor's type
+/* norm[0] = sqrt of the sum of squares over all tensors (summed in fp64; infinite where it leaves
+ * fp32), out = in * min(1, maxNorm / (norm + 1e-6)) for each, the factor from the norm in
+ * fp64, the product in fp32 and rounded to the tensor's type
  * (F32, F16, BF16, types may mix; contiguous; count 0 allowed).  out may be in of the same
  * tensor. */
 typedef struct HcamdClipTensor {

@@ -184,3 +184,22 @@ def test_a_row_of_zeros_has_scale_0_without_eps(ty, cols):
         rt.add_rms_norm(x, None, weight, q, eps=0.0, scale=scale)
         assert [r for r in range(4) if float(scale[r]) == 0.0] == zeros, scale
         assert not bool(q[zeros].any()) and bool(torch.isfinite(scale).all())
+
+
+@pytest.mark.parametrize("most", [1.0, 1e30])
+@pytest.mark.parametrize("size", [1e18, 1e37, 3e38])
+@pytest.mark.parametrize("ty", ["f32", "bf16"])
+def test_clip_of_gradients_whose_norm_leaves_fp32(ty, size, most):
+    """Finite gradients are scaled to the norm asked for, also where their norm is beyond fp32 or the factor below its
+    normal numbers.  The factor is off by 3 u (64 bits, rounded once), the product by one more."""
+    k = TYPES[ty]
+    g = [dev(torch.full((n,), size) * (1 - 0.5 * torch.rand(n, generator=torch.Generator().manual_seed(n))), k) for n in (100, 4099, 3)]
+    g.append(dev(torch.tensor([1.0, 1e-30, 0.0]), torch.float32))
+    out, norm = [torch.empty_like(v) for v in g], empty(1, ty=torch.float32)
+    rt.clip_grad_norm(g, out, norm, most)
+    total = float(sum(f64(v).square().sum() for v in g).sqrt())
+    near(norm, torch.tensor([total]).double().float().double(), total * U if total < 3e38 else 0.0) if total < 3e38 else None
+    assert total < 3e38 or bool(torch.isinf(norm).all())
+    for v, o in zip(g, out):
+        want = f64(v) * min(1.0, most / (total + 1e-6))
+        near(o, want, want.abs() * (4 * U + (half(k) if v.dtype == k else 0)) + tiny(torch.float32), "clipped")
