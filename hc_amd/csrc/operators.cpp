@@ -9,6 +9,9 @@
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
+#include <functional>
+#include <utility>
+#include <vector>
 
 using namespace hcamd;
 
@@ -995,6 +998,32 @@ size_t clipChunk(size_t elems) { return elems >= ((size_t)16 << 20) ? 16384 : 40
 size_t clipGroups(size_t chunks, size_t all) {
   return std::max<size_t>(1, std::min(chunks, all <= kClipCells ? chunks : chunks * kClipCells / all));
 }
+// Every clipped tensor is written once, over nothing that another workgroup reads: an output is
+// neither another one nor another tensor's input, and the norm is none of them.
+int clipApart(const Call &c, const HcamdClipTensor *tensors, size_t count, const float *norm) {
+  std::vector<std::pair<const void *, size_t>> outs; // by address, with the tensor's index
+  outs.reserve(count);
+  for (size_t i = 0; i < count; ++i)
+    if (tensors[i].count)
+      outs.emplace_back(tensors[i].out, i);
+  const std::less<const void *> below;
+  std::sort(outs.begin(), outs.end(), [&](const auto &a, const auto &b) { return below(a.first, b.first); });
+  for (size_t i = 1; i < outs.size(); ++i)
+    if (outs[i].first == outs[i - 1].first)
+      return c.fail("tensor %zu: two outputs are one buffer", std::max(outs[i].second, outs[i - 1].second));
+  for (size_t i = 0; i < count; ++i) {
+    const HcamdClipTensor &t = tensors[i];
+    if (!t.count)
+      continue;
+    if (t.in == norm || t.out == norm)
+      return c.fail("tensor %zu: the norm is a tensor's buffer", i);
+    const auto at = std::lower_bound(outs.begin(), outs.end(), t.in,
+                                     [&](const auto &o, const void *p) { return below(o.first, p); });
+    if (at != outs.end() && at->first == t.in && at->second != i)
+      return c.fail("tensor %zu: an output is another tensor's input", i);
+  }
+  return 0;
+}
 } // namespace
 
 size_t hcamdClipGradNormWorkspace(size_t tensors) noexcept { return (kClipCells + ceilDiv(tensors, kClipTensors)) * 8; }
@@ -1021,6 +1050,12 @@ int hcamdLaunchClipGradNorm(OlQueue q, const HcamdClipTensor *tensors, size_t co
                     c.check({"a clipped tensor", t.out, t.count, 1, t.count, elemBytes(t.type)})))
       return 1;
     elems += t.count;
+  }
+  try {
+    if (clipApart(c, tensors, count, norm))
+      return 1;
+  } catch (...) {
+    return c.fail("out of host memory");
   }
   const size_t chunk = clipChunk(elems);
   for (size_t i = 0; i < count; ++i)

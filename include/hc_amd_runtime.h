@@ -909,7 +909,7 @@ int hcamdLaunchLinearCrossEntropyBackward(OlQueue q, int elemType, const void *x
  * fp32), out = in * min(1, maxNorm / (norm + 1e-6)) for each, the factor from the norm in
  * fp64, the product in fp32 and rounded to the tensor's type
  * (F32, F16, BF16, types may mix; contiguous; count 0 allowed).  out may be in of the same
- * tensor. */
+ * tensor; one that is another tensor's in or out, or norm, is refused. */
 typedef struct HcamdClipTensor {
   const void *in;
   void *out;
