@@ -1351,13 +1351,17 @@ def add_rms_norm(x, residual, weight, out, eps: float = 1e-6, summed=None, scale
 
 
 def add_rms_norm_backward(grad_out, summed, weight, rstd, grad_in, grad_weight=None, grad_summed=None) -> None:
-    # (calls that bring a workspace of their own always wait: it goes with the plan)
+    # (calls that bring a workspace of their own wait: it goes with the plan)
     plan_add_rms_norm_backward(grad_out, summed, weight, rstd, grad_in, grad_weight, grad_summed).launch(sync=True)
 
 
 def gated_ffn(x, w_gate, w_up, out, activation: str = "silu", gate=None, up=None, scales=None,
               sync: bool = True) -> None:
-    plan_gated_ffn(x, w_gate, w_up, out, activation, gate, up, scales).launch(sync)
+    """gated_ffn as one call.  sync=False returns once it is enqueued, unless its sizes need a workspace
+    (rows that are no multiple of 16 bytes): that goes with the plan, so the call waits.  To enqueue
+    those too, keep a plan_gated_ffn."""
+    plan = plan_gated_ffn(x, w_gate, w_up, out, activation, gate, up, scales)
+    plan.launch(sync or plan.keep[-1] is not None)
 
 
 def gated_ffn_backward(grad_out, x, w_gate, w_up, gate, up, grad_x=None, grad_w_gate=None, grad_w_up=None,

@@ -203,3 +203,30 @@ def test_clip_of_gradients_whose_norm_leaves_fp32(ty, size, most):
     for v, o in zip(g, out):
         want = f64(v) * min(1.0, most / (total + 1e-6))
         near(o, want, want.abs() * (4 * U + (half(k) if v.dtype == k else 0)) + tiny(torch.float32), "clipped")
+
+
+def test_a_workspace_outlives_the_kernels_that_use_it(monkeypatch):
+    """sync=False of a call that brings a workspace of its own waits all the same; one without does not."""
+    events = []
+
+    class Watched(rt.DeviceArray):
+        def free(self):
+            if getattr(self, "ptr", None):
+                events.append("free")
+            super().free()
+
+    monkeypatch.setattr(rt, "_workspace", lambda n, ctx: Watched((n,), np.uint8, ctx) if n else None)
+    inner = rt.Context.synchronize
+    monkeypatch.setattr(rt.Context, "synchronize", lambda self: (events.append("wait"), inner(self))[1])
+    k = torch.float16
+    for (t, d, f), want in (((800, 33, 40), ["wait", "free"]), ((3, 5, 16), ["wait", "free"]), ((3, 64, 16), [])):
+        x, wg, wu = dev(normal(1, t, d), k), dev(normal(2, f, d), k), dev(normal(3, f, d), k)
+        out = empty(t, f, ty=k)
+        torch.cuda.synchronize()
+        events.clear()
+        rt.gated_ffn(x, wg, wu, out, sync=False)
+        assert events == want, (t, d, f)
+        rt.default_context().synchronize()
+        a, _ = act_reference("silu", f64(x) @ f64(wg).t())
+        want_out = a * (f64(x) @ f64(wu).t())
+        assert float((f64(out) - want_out).norm() / want_out.norm()) < 4 * half(k)
