@@ -328,7 +328,7 @@ template <class E> __device__ __forceinline__ void fold(const FoldArgs &a) {
 #pragma unroll 4
     for (uint32_t s = 1; s < a.splits; ++s)
       v += *reinterpret_cast<const f32x4 *>(from + (size_t)s * a.rows * a.ldp);
-    store4<E>(static_cast<E *>(a.out) + (size_t)r * a.ldo, (int)c, 0, (int)a.cols, v * by);
+    store4<E>(static_cast<E *>(a.out) + (size_t)r * a.ldo, (int)c, 0, (int)a.cols, times(v, by));
   }
 }
 

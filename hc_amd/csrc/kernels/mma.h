@@ -858,6 +858,19 @@ __device__ __forceinline__ void store_direct(O *out, size_t ld, int m0, int n0, 
   }
 }
 
+// v * by as fp32 values, before they are rounded to a type: folded into the conversion the
+// product would be rounded once in some kernels and twice in others.
+__device__ __forceinline__ f32x4 times(f32x4 v, float by) {
+  v *= by;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    float x = v[e];
+    asm volatile("" : "+v"(x));
+    v[e] = x;
+  }
+  return v;
+}
+
 // C to `out` (element type) or `partial` (fp32; its rows are padded to a multiple of 8
 // and the pipelined kernels' tiles begin at multiples of 8, so four columns are stored
 // or not as a whole)
@@ -886,18 +899,7 @@ __device__ __forceinline__ void store_tile(const StoreArgs &s, f32x4 (&acc)[MI][
   }
   const Window w = {t.m_lo, s.mma.M, t.n_lo, s.mma.N};
   const float by = s.undo ? *s.undo : 1.0f;
-  // (the product is an fp32 value before it is rounded to the type: folded into the conversion
-  // it would be rounded once in some kernels and twice in others)
-  auto value = [&](int i, int j) {
-    f32x4 v = acc[i][j] * by;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      float x = v[e];
-      asm volatile("" : "+v"(x));
-      v[e] = x;
-    }
-    return v;
-  };
+  auto value = [&](int i, int j) { return times(acc[i][j], by); };
   if constexpr (LDS)
     store_block<E, MI, NI>(mine, static_cast<E *>(s.out), s.ldo, m0, n0, w, lane, value);
   else

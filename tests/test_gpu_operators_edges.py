@@ -230,3 +230,33 @@ def test_a_workspace_outlives_the_kernels_that_use_it(monkeypatch):
         a, _ = act_reference("silu", f64(x) @ f64(wg).t())
         want_out = a * (f64(x) @ f64(wu).t())
         assert float((f64(out) - want_out).norm() / want_out.norm()) < 4 * half(k)
+
+
+def test_results_are_rounded_alike_with_and_without_partial_sums():
+    """The loss's gradients are fp32 values before they are rounded to the type, also those that partial sums are
+    folded into.  With a weight of zeros every p is one 16-bit value, and the rows of x are such that the sums of
+    a column are its own number: the result is known to the bit."""
+    t, d, v = 4096, 1024, 1000
+    k = torch.float16
+    w = torch.zeros(v, d, device="cuda", dtype=k)
+    targets = torch.zeros(t, device="cuda", dtype=torch.int64)
+    lse = torch.full((t,), float(np.log(np.float32(v))), device="cuda")
+    gw = torch.empty_like(w)
+    x = torch.zeros(t, d, dtype=k)
+    for bit in range(10):                               # in different parts of the sum over the tokens
+        x[bit * 400] = (torch.arange(d) >> bit & 1) * 2.0 ** bit
+    x = x.cuda()
+    # p in 16 bits, from a gradient that nothing has to be undone for but a power of two
+    rt.linear_cross_entropy_backward(x, w, targets, lse, torch.ones(t, device="cuda"), None, gw)
+    p = float(f64(gw[1, 1])) * 2.0 ** 15
+    assert p == float(np.float16(p)) and 30 < p < 35
+    sums = p * np.arange(d)                             # 21 bits: exact in fp32 and as sums
+    # gradients for which rounding in one step and in two differ somewhere, both known exactly in 64 bits
+    tried = np.random.default_rng(1).uniform(0.01, 5, 4000).astype(np.float32)
+    once = sums * (tried / np.float32(2.0 ** 15)).astype(np.float64)[:, None]
+    twice = once.astype(np.float32).astype(np.float16)
+    chosen = np.flatnonzero((once.astype(np.float16) != twice).any(1))[:8]
+    assert len(chosen) == 8
+    for i in chosen:
+        rt.linear_cross_entropy_backward(x, w, targets, lse, torch.full((t,), float(tried[i]), device="cuda"), None, gw)
+        assert np.array_equal(gw[1].cpu().numpy(), twice[i]), tried[i]
