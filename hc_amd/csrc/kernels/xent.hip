@@ -29,6 +29,11 @@ __device__ __forceinline__ bool takes_part(const void *targets, int is64, size_t
 // The products dominate: 4096 x 4096 x 131072 bf16 forward 3.2 ms (1.37 PFLOP/s), backward a
 // piece of 16384 rows p 453 us, dx 452 us, dW 478 us.
 
+// What is subtracted before the exponentials: the largest value, or 0 where that is infinite.  The terms
+// of a row of -infinities are then 0, +infinity gives an infinite sum (its difference with itself
+// would be NaN), and a NaN, which no maximum takes, makes the sum NaN.
+__device__ __forceinline__ float subtracted(float most) { return __builtin_fabsf(most) == INFINITY ? 0.0f : most; }
+
 // per-row statistics of a tile: lanes l, l + 16, l + 32, l + 48 hold one row's
 // columns; WN waves share the row and meet in LDS
 template <int MI, int NI, int WN, int BM, int BN>
@@ -69,8 +74,7 @@ __device__ __forceinline__ void tile_stats(const XentArgs &a, f32x4 (&acc)[MI][N
         most = fmaxf(most, acc[i][j][e]);
     most = fmaxf(most, __shfl_xor(most, 16));
     most = fmaxf(most, __shfl_xor(most, 32));
-    // a row of -infinities: subtract 0, every term is then 0
-    const float from = most == -INFINITY ? 0.0f : most;
+    const float from = subtracted(most);
     float sum = 0.0f;
 #pragma unroll
     for (int j = 0; j < NI; ++j)
@@ -93,7 +97,7 @@ __device__ __forceinline__ void tile_stats(const XentArgs &a, f32x4 (&acc)[MI][N
 #pragma unroll
     for (int w = 1; w < WN; ++w)
       most = fmaxf(most, slot_m[w * BM + r]);
-    const float from = most == -INFINITY ? 0.0f : most;
+    const float from = subtracted(most);
     float sum = 0.0f;
 #pragma unroll
     for (int w = 0; w < WN; ++w)
@@ -151,7 +155,7 @@ template <class E, int MB, int NB, int U, bool ODD> __device__ __forceinline__ v
 #pragma unroll
     for (int o = 8; o > 0; o >>= 1)
       most = fmaxf(most, __shfl_xor(most, o));
-    const float from = most == -INFINITY ? 0.0f : most;
+    const float from = subtracted(most);
     float sum = 0.0f;
 #pragma unroll
     for (int j = 0; j < NB; ++j)
@@ -282,7 +286,7 @@ __device__ __forceinline__ void rows_join(const XentRowsArgs &a) {
   for (uint32_t t = lane; t < a.tiles; t += kWave)
     most = fmaxf(most, cells[t][0]);
   most = wave_reduce<MaxOp>(most);
-  const float from = most == -INFINITY ? 0.0f : most;
+  const float from = subtracted(most);
   float sum = 0.0f;
   for (uint32_t t = lane; t < a.tiles; t += kWave)
     sum += cells[t][1] * __expf(cells[t][0] - from);

@@ -260,3 +260,24 @@ def test_results_are_rounded_alike_with_and_without_partial_sums():
     for i in chosen:
         rt.linear_cross_entropy_backward(x, w, targets, lse, torch.full((t,), float(tried[i]), device="cuda"), None, gw)
         assert np.array_equal(gw[1].cpu().numpy(), twice[i]), tried[i]
+
+
+@pytest.mark.parametrize("t", [1, 20, 100, 300])
+def test_loss_of_infinite_logits(t):
+    """An infinite logit: the log-sum-exp is infinite (or, all being -infinity, minus that), not NaN."""
+    d, v, k = 64, 1031, torch.bfloat16
+    x, w = torch.zeros(t, d, device="cuda", dtype=k), torch.zeros(v, d, device="cuda", dtype=k)
+    x[:, 0], x[:, 1] = 3e38, 1
+    w[:, 1] = dev(normal(1, v), k)
+    w[777, 0] = 3e38                                    # column 777: +infinity
+    targets = torch.zeros(t, device="cuda", dtype=torch.int64)
+    loss, lse = empty(t, ty=torch.float32), empty(t, ty=torch.float32)
+    rt.linear_cross_entropy(x, w, targets, loss, lse)
+    assert bool((lse == float("inf")).all()) and bool((loss == float("inf")).all()), (lse[:3], loss[:3])
+    w[777, 0] = -3e38                                   # -infinity: its term is 0
+    rt.linear_cross_entropy(x, w, targets, loss, lse)
+    z = f64(x[:1, 1:]) @ f64(w[:, 1:]).t()
+    z[0, 777] = -float("inf")
+    want = torch.logsumexp(z, 1).expand(t)
+    near(lse, want, 200 * U * want.abs(), "lse")
+    near(loss, want - z[0, 0], 200 * U * (want.abs() + z[0, 0].abs()), "loss")
