@@ -281,3 +281,22 @@ def test_loss_of_infinite_logits(t):
     want = torch.logsumexp(z, 1).expand(t)
     near(lse, want, 200 * U * want.abs(), "lse")
     near(loss, want - z[0, 0], 200 * U * (want.abs() + z[0, 0].abs()), "loss")
+
+
+@pytest.mark.parametrize("shape", [(1, 64, 40), (33, 333, 97), (130, 129, 200), (300, 1024, 257), (513, 640, 520), (800, 33, 40)], ids=str)
+def test_gated_ffn_int8_gelu(shape):
+    t, d, f = shape
+    k = torch.bfloat16
+    g = torch.Generator().manual_seed(9)
+    x, wg, wu = (torch.randint(-127, 128, s, generator=g).to(torch.int8) for s in ((t, d), (f, d), (f, d)))
+    xs, gs, us = (0.5 + torch.rand(n, generator=g) for n in (t, f, f))
+    gs, us, xs = gs * 0.02, us * 0.02, xs * 0.02 / d ** 0.5
+    out = empty(t, f, ty=k)
+    rt.gated_ffn(x.cuda(), wg.cuda(), wu.cuda(), out, activation="gelu", scales=(xs.cuda(), gs.cuda(), us.cuda()))
+    gg = (x.double() @ wg.double().t()) * xs.double()[:, None] * gs.double()
+    uu = (x.double() @ wu.double().t()) * xs.double()[:, None] * us.double()
+    a, _ = act_reference("gelu", gg)
+    # the sums are exact; a conversion and two products each; the exponential's argument, 1.6 (g + 0.045 g^3), is
+    # off by some 8 u of itself
+    want = a * uu
+    near(out, want, want.abs() * (half(k) + 12 * U) + 24 * U * (gg.abs() + gg * gg + 0.08 * gg ** 4) * uu.abs() + tiny(k), "out")
