@@ -46,6 +46,12 @@ __device__ __forceinline__ void activate_both(int kind, float x, float &f, float
   df = p == 0.0f ? s : s + x * dt * p;
 }
 
+// gate and up are rounded to the element type: half the bytes to keep and to read again, and dg
+// and du, which come from them, are rounded all the same, being matrix operands.  The gradients
+// are thereby 1.8 times as far from the exact ones as a single rounding at the end would leave
+// them (bf16 0.0030 of their size against 0.0017, fp16 0.00037 against 0.00021): of the added
+// squares gate and up bring 56 %, dg and du 44 %.
+//
 // the outputs of a wave: blocks j and j + NI / 2 are the two projections of the same
 // columns.  LDS: through the wave's region `mine`, else straight from registers
 template <class E, class O, int MI, int NI, bool LDS>
@@ -201,7 +207,7 @@ template <class E, class F> __device__ __forceinline__ void each_gated_back(cons
 // would keep four bits, and those of one of 3e4 overflow and meet other terms as NaN.  So they are scaled by the power of two that
 // brings the largest of them to 2^14 .. 2^15, and the products undo it in fp32 (exactly: a block
 // whose dg and du are normal numbers has the results it would have unscaled).  One more launch
-// reads the operands for that maximum.
+// reads the operands for that maximum (333 x 2731 4 us, 4096 x 11264 76 us).
 __device__ __forceinline__ void gated_back_most(const GatedBackArgs &a) {
   __shared__ float slots[4];
   float most = 0.0f;

@@ -310,11 +310,12 @@ __device__ __forceinline__ void mma_general(const MmaArgs &g, int wg, int split,
 //     readable elements up to there (the library's own buffers).
 // A load's address is a lane part, held in a register for the whole loop, plus a
 // scalar part; from tile to tile only the base of the buffer descriptor moves.
-// Bound by the matrix cores: they are busy 69 % of the cycles with two k-fast operands, 64 %
-// with one k-slow operand, 57 % with two (whose reads are two of 8 bytes and must not
+// Bound by the matrix cores: they are busy 66 % of the cycles with two k-fast operands, 58 %
+// with one k-slow operand, 54 % with two (whose reads are two of 8 bytes and must not
 // stand behind loads into LDS); the clock gives way under the load as it does for a
-// plain product.  256 x 256 tiles over 4096 x 4096 x 11264 bf16: both projections 600 us
-// (1.26 PFLOP/s), dx 590 us, dW 645 us; 2000 x 4096 x 11264 int8 170 us (2.17 POP/s).  For
+// plain product.  256 x 256 tiles over 4096 x 4096 x 11264 bf16: both projections and their
+// storing 601 us (1.26 PFLOP/s), dx 590 us, dW 645 us; 2000 x 4096 x 11264 int8 168 us (2.19
+// POP/s).  For
 // 2048 cycles of MFMA a tile's eight waves of 128 x 64 read 192 KiB from LDS; four waves of
 // 128 x 128 would read a third less, but spill (dx 700 -> 1007 us).
 // ---------------------------------------------------------------------------

@@ -303,7 +303,8 @@ __device__ __forceinline__ void rows_join(const XentRowsArgs &a) {
 // products, factor[1]: the largest |grad_loss| becomes 1 (bf16) or 2^15 (fp16).  With
 // the usual grad_loss, one value for every live row, the -1 at a target is then
 // represented exactly, where -grad_loss itself would carry one and the same rounding
-// error into every row's largest entry; and fp16 keeps the small p of a large
+// error into every row's largest entry (gradients that differ from row to row are rounded
+// there, each by itself); and fp16 keeps the small p of a large
 // vocabulary above its subnormals.  The first workgroup.
 __device__ __forceinline__ void p_factor(const XentPrepareArgs &a) {
   __shared__ float slots[16];

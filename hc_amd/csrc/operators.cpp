@@ -108,7 +108,8 @@ struct Call {
 
 // ---- tiled products -----------------------------------------------------------
 // Tile and splits of a product, from its shape alone (a workspace is sized before any
-// pointer is seen): the cheapest by a model of the card's 256 compute units.  Its unit is
+// pointer is seen): the cheapest by a model of the card's 256 compute units (with fewer of
+// them the choice is less good, the results are the same).  Its unit is
 // what a 256 x 256 tile takes for one k tile, 1.65 us at the 1.3 PFLOP/s those kernels
 // reach; measured beside it: two 128 x 128 tiles on a unit 0.64, one alone 0.4, half a
 // 256 x 256 tile 0.55; a tile's beginning and end cost about three k tiles; fp32 partial

@@ -800,12 +800,13 @@ int hcamdLaunchGemmF16(OlQueue q, const void *a, size_t lda, const void *bt,
  * "fma", "softmax", "quantize", "gemm", "copy", "map", "rows", "cols", "stream", "norm"
  * (lanes to a row in the normalisation kernels: 1 twice, 2 half as many), "gather"
  * (block shape), "gather_fuse" (groups per workgroup; read by
- * hcamdGatherGemmCreate).
+ * hcamdGatherGemmCreate), "rmsnorm" (1: rows read twice) and "mma" (tiles of the
+ * language-model products: 1 to 5; a workspace is sized for the variant in force).
  * Process-wide, guarded by a lock.  Returns 1 for an unknown family, and for
  * the numbers of the measurement builds of the "gemm" family (17..22, 26, 28..34:
  * most of them leave something other than the product in C) unless the library was built with them
  * (hc_amd_bench.h).  Every variant a default build accepts computes the same
- * result as variant 0. */
+ * result as variant 0 ("rmsnorm" and "mma": but for the order of fp32 sums). */
 int hcamdSetVariant(const char *family, int variant) HCAMD_NOEXCEPT;
 /* The same choice for the calling thread only: it takes precedence over
  * hcamdSetVariant for launches made by this thread and is invisible to others
@@ -840,7 +841,9 @@ const char *hcamdLastKernelName(void) HCAMD_NOEXCEPT;
  * outType elemType: out = y.  outType HCAMD_I8: out = q = rint(127 v / most), half
  * to even, v = h * weight, most = max |v| over the row, and scale[row] =
  * rstd * most / 127, so that q * scale stands for y; a row of zeros has q = 0 and
- * scale 0, a row with a value that is not finite q = 0 and scale NaN.
+ * scale 0 whatever eps is, a row with a value that is not finite q = 0 and scale NaN.
+ * Squares are fp32: where mean(h^2) leaves its range (|h| from about 1.8e19), rstd, y
+ * and scale are 0.
  * summed and out may be x or residual (same leading dimension). */
 int hcamdLaunchAddRmsNorm(OlQueue q, int elemType, const void *x, size_t ldx, const void *residual, size_t ldr,
                           const void *weight, int weightType, float eps, void *summed, size_t lds, void *out,
