@@ -204,10 +204,10 @@ template <class E, class F> __device__ __forceinline__ void each_gated_back(cons
 
 // fp16 holds 40 binary places, of which the lowest ten lack precision, and dg and du are products of
 // values that may stand anywhere in them: rounded as they are, those of a gradient of 1e-6
-// would keep four bits, and those of one of 3e4 overflow and meet other terms as NaN.  So they are scaled by the power of two that
-// brings the largest of them to 2^14 .. 2^15, and the products undo it in fp32 (exactly: a block
-// whose dg and du are normal numbers has the results it would have unscaled).  One more launch
-// reads the operands for that maximum (333 x 2731 4 us, 4096 x 11264 76 us).
+// would keep four bits, and those of one of 3e4 overflow and meet other terms as NaN.  So they
+// are scaled by the power of two that brings the largest of them to 2^14 .. 2^15, and the
+// products undo it in fp32 (exactly: a block whose dg and du are normal numbers below 2^15 has
+// the results it would have unscaled).  One more launch reads the operands for that maximum (333 x 2731 4 us, 4096 x 11264 76 us).
 __device__ __forceinline__ void gated_back_most(const GatedBackArgs &a) {
   __shared__ float slots[4];
   float most = 0.0f;

@@ -315,9 +315,8 @@ __device__ __forceinline__ void mma_general(const MmaArgs &g, int wg, int split,
 // stand behind loads into LDS); the clock gives way under the load as it does for a
 // plain product.  256 x 256 tiles over 4096 x 4096 x 11264 bf16: both projections and their
 // storing 601 us (1.26 PFLOP/s), dx 590 us, dW 645 us; 2000 x 4096 x 11264 int8 168 us (2.19
-// POP/s).  For
-// 2048 cycles of MFMA a tile's eight waves of 128 x 64 read 192 KiB from LDS; four waves of
-// 128 x 128 would read a third less, but spill (dx 700 -> 1007 us).
+// POP/s).  For 2048 cycles of MFMA a tile's eight waves of 128 x 64 read 192 KiB from LDS;
+// four waves of 128 x 128 would read a third less, but spill (dx 700 -> 1007 us).
 // ---------------------------------------------------------------------------
 constexpr int waitcnt_imm(int vmcnt, int lgkmcnt) {
   return (vmcnt & 0xf) | ((vmcnt >> 4) << 14) | (7 << 4) | ((lgkmcnt & 0xf) << 8);

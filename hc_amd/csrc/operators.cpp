@@ -173,9 +173,9 @@ size_t partialBytes(const Product &p, size_t m, size_t n) {
 
 // Whether the pipelined kernels can fetch an operand: 16-byte pieces, offsets inside a
 // tile (of up to 256 rows, in 32 bits) below 2^31: asked for every operand, the library's own
-// too, whose rows are as long as the block is wide or a piece of the vocabulary.  `along` is its extent in the direction that runs through memory
-// (k for a k-fast operand, its rows for a k-slow one); the library's own buffers are
-// padded there.
+// too, whose rows are as long as the block is wide or a piece of the vocabulary.  `along` is
+// its extent in the direction that runs through memory (k for a k-fast operand, its rows
+// for a k-slow one); the library's own buffers are padded there.
 bool fetchable(const void *p, size_t ld, size_t along, size_t bytes, bool padded) {
   const size_t piece = 16 / bytes;
   return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % piece == 0 && (padded || along % piece == 0) &&
